@@ -7,6 +7,9 @@ exports the reference engine's MoE entry points under their own names and signat
 bind it in place of the CPU libraries, plus `draco_b200_*` extensions (whole-layer forward on
 a token batch, routing only, activation mode, weight registry).
 
+`decoder` has the operators of a decoder layer around the MoE FFN for torch CUDA tensors: block planning, the 4-bit
+paged KV cache, attention over it, and the residual RMS norm with 8-bit output.
+
 This module is the Python face of that library, mirroring how the reference's drivers call
 it (`src/qwen35_engine.py:92-131`, `src/qwen35_prefill.py:65-83`, `src/k2_engine.py:97-106`):
 `lib()` returns the ctypes handle with every signature declared, and a few helpers wrap the
@@ -59,6 +62,31 @@ class M6MoeP(ct.Structure):
                 ("norm_w", ct.c_int), ("w_scale", ct.c_float), ("inter", ct.c_int), ("n_in", ct.c_int),
                 ("n_out", ct.c_int), ("sh_g", _vp), ("sh_u", _vp), ("sh_d", _vp), ("csg", ct.c_int),
                 ("csu", ct.c_int), ("csd", ct.c_int), ("sh_ff", ct.c_int), ("scratch", _f)]
+
+
+class DracoKV4Cache(ct.Structure):
+    """Layout of `DracoKV4Cache` in include/draco_moe_b200.h."""
+    _fields_ = [("pages", _vp), ("n_pages", ct.c_int), ("page_size", ct.c_int), ("n_kv_heads", ct.c_int),
+                ("head_dim", ct.c_int)]
+
+
+class DracoKV4Attention(ct.Structure):
+    """Layout of `DracoKV4Attention` in include/draco_moe_b200.h."""
+    _fields_ = [("q", _vp), ("out", _vp), ("lse", _vp), ("q_token_stride", ct.c_long), ("q_head_stride", ct.c_long),
+                ("out_token_stride", ct.c_long), ("out_head_stride", ct.c_long), ("dtype", ct.c_int),
+                ("n_heads", ct.c_int), ("n_req", ct.c_int), ("n_tokens", ct.c_int), ("cu_q", _vp), ("seq_len", _vp),
+                ("block_table", _vp), ("table_stride", ct.c_long), ("table_width", ct.c_int), ("max_q_len", ct.c_int),
+                ("max_seq_len", ct.c_int), ("scale", ct.c_float), ("window", ct.c_int), ("sinks", ct.c_int), ("workspace", _vp),
+                ("workspace_bytes", ct.c_size_t)]
+
+
+class DracoNormQ8(ct.Structure):
+    """Layout of `DracoNormQ8` in include/draco_moe_b200.h."""
+    _fields_ = [("x", _vp), ("residual", _vp), ("weight", _vp), ("h", _vp), ("y", _vp), ("codes", _vp),
+                ("scales", _vp), ("x_stride", ct.c_long), ("residual_stride", ct.c_long), ("h_stride", ct.c_long),
+                ("y_stride", ct.c_long), ("codes_stride", ct.c_long), ("scales_stride", ct.c_long),
+                ("dtype", ct.c_int), ("fmt", ct.c_int), ("n_rows", ct.c_int), ("hidden", ct.c_int),
+                ("group", ct.c_int), ("eps", ct.c_float)]
 
 
 # name: (argtypes, restype) -- the reference drivers' own ctypes signatures where they exist
@@ -123,6 +151,16 @@ _SIGS = {
     "draco_b200_q8k_quantize": ([_f, ct.c_int, _f, _i8, _i16], ct.c_int),
     "draco_b200_q8k_block_dots": ([ct.c_int, _u8, ct.c_int, ct.c_int, _i8, _i16, _i32], ct.c_int),
     "draco_b200_gemv_q8k": ([ct.c_int, _u8, ct.c_int, ct.c_int, _i8, _f, _i16, _f], ct.c_int),
+    "draco_b200_plan_blocks": ([_vp, _vp, ct.c_int, ct.c_int, _vp, ct.c_long, ct.c_int, _vp, ct.c_int, _vp, ct.c_int,
+                                _vp, _vp, _vp, _vp, _vp, _vp, _vp], ct.c_int),
+    "draco_b200_kv4_page_bytes": ([ct.c_int, ct.c_int, ct.c_int], ct.c_size_t),
+    "draco_b200_kv4_append": ([ct.POINTER(DracoKV4Cache), ct.c_int, _vp, ct.c_long, ct.c_long, _vp, ct.c_long,
+                               ct.c_long, _vp, ct.c_int, _vp], ct.c_int),
+    "draco_b200_kv4_read": ([ct.POINTER(DracoKV4Cache), ct.c_int, _vp, ct.c_long, ct.c_long, _vp, ct.c_long,
+                             ct.c_long, _vp, ct.c_int, _vp], ct.c_int),
+    "draco_b200_kv4_attention_workspace": ([ct.POINTER(DracoKV4Cache), ct.POINTER(DracoKV4Attention)], ct.c_size_t),
+    "draco_b200_kv4_attention": ([ct.POINTER(DracoKV4Cache), ct.POINTER(DracoKV4Attention), _vp], ct.c_int),
+    "draco_b200_rmsnorm_q8": ([ct.POINTER(DracoNormQ8), _vp], ct.c_int),
 }
 
 _LIB = None

@@ -33,7 +33,8 @@ def nvcc() -> str:
 
 
 def _headers():
-    return glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(ROOT, "include", "*.h"))
+    return [h for d, p in ((CSRC, "*.cuh"), (CSRC, "*.h"), (os.path.join(ROOT, "include"), "*.h"))
+            for h in glob.glob(os.path.join(d, p))]
 
 
 def build(verbose: bool = False, extra_flags=()) -> str:

@@ -7,6 +7,7 @@
 // text.  Weights arrive as the caller's addresses; host ranges are copied to device memory
 // once, on first use, and found again by address on later calls.
 #include "../../include/draco_moe_b200.h"
+#include "abi.h"
 #include "kernels.cuh"
 #include "tc_gemm.cuh"
 
@@ -1422,6 +1423,16 @@ int stage_in(Ctx* c, cudaStream_t s, size_t off, const T* h, size_t n) {
 }  // namespace
 
 // ===================================== Part 1 ==========================================
+// for the entry points outside this file (abi.h)
+namespace draco {
+void abi_error(const char* text) { g_err = text; }
+void abi_count(int kernels) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    g_launches += kernels;
+}
+bool abi_device_ptr(const void* p) { return is_device_ptr(p); }
+}  // namespace draco
+
 extern "C" {
 
 void m6_granite_moe(const float* x0, const uint64_t* ptrs, const int* codes, const float* gate_inp, int n_exp,

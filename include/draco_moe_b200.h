@@ -3,7 +3,8 @@
  * Part 1 re-exports the reference engine's MoE entry points with their exact signatures and
  * argument meaning, so the reference's numpy/ctypes drivers bind this library instead of the
  * CPU one.  Each declaration cites the reference interface it replaces (paths inside the
- * reference project).  Part 2 adds entry points the reference has no counterpart for.
+ * reference project).  Part 2 adds entry points the reference has no counterpart for, part 3 the
+ * operators of a decoder layer around the MoE FFN (4-bit paged KV cache, attention, norm).
  *
  * Common behaviour:
  *   - Weights are addressed by the caller's pointers, as in the reference (host virtual
@@ -329,6 +330,99 @@ int draco_b200_q8k_block_dots(int code, const uint8_t* W, int rows, int n_in, co
                               const int16_t* bsums, int32_t* out2);
 int draco_b200_gemv_q8k(int code, const uint8_t* W, int rows, int n_in, const int8_t* q,
                         const float* d, const int16_t* bsums, float* y);
+
+/* ============================ Part 3: decoder-layer operators ============================
+ *
+ * What a decoder layer needs around the MoE FFN on the same GPU: page allocation and slot maps, a 4-bit paged KV cache,
+ * attention over it, and the residual RMS norm with 8-bit output.  No counterpart in the reference.  All pointers are
+ * device memory; every call is asynchronous on `stream` (null: the legacy default stream), allocates nothing, keeps
+ * nothing between calls and can be captured in a CUDA graph.  Returns 0, -1 (arguments; nothing was launched) or
+ * -3 (CUDA error), with the text in draco_b200_last_error().  Element types (dtype): 0 fp32, 1 fp16, 2 bf16. */
+
+/* Block tables and slot maps from the requests' lengths, for n_req (<= 16384) requests, in one launch.
+ * Request r has ctx_len[r] tokens in the cache and gets new_len[r] more (negative values count as 0).  It holds
+ * ceil(ctx/page_size) pages, in the first entries of its row of block_table ([n_req] rows, table_stride entries apart,
+ * table_width usable), and takes the pages that it lacks from the end of free_pages[0 .. *n_free) in request order;
+ * their ids are written to its row, the rest of the table is left as it is.  A request whose pages the list no longer
+ * has, counting those of every request before it, or which a row cannot hold, is refused: no page, slots -1.
+ *   cu_new[n_req+1]   tokens before each request;    seq_len[r]   ctx + new, or ctx where refused
+ *   slots, positions [max_tokens]   for token i of request r (at cu_new[r] + i): position ctx + i, and slot
+ *                     page * page_size + position % page_size; -1 for tokens of refused requests (slots) and past the
+ *                     last token (both).  Tokens past max_tokens are not written, their pages are.
+ *   n_free_out        pages left;   refused   number of refused requests
+ * free_len is the length of free_pages.  slots and positions must be 16-byte aligned; no output may overlap an input
+ * (the table, which is both, apart). */
+int draco_b200_plan_blocks(const int* ctx_len, const int* new_len, int n_req, int page_size, int* block_table,
+                           long table_stride, int table_width, const int* free_pages, int free_len, const int* n_free,
+                           int max_tokens, int* cu_new, int* seq_len, int* slots, int* positions, int* n_free_out,
+                           int* refused, void* stream);
+
+/* A paged KV cache in 4 bits: pages [n_pages][n_kv_heads][page_size / 16] tiles of 16 tokens, 20 * head_dim bytes each
+ * (the tile's layout: csrc/kv4.cuh).  Groups of 32 channels of a token share an fp16 scale and an fp16 offset:
+ *   K = s * c + m, s = fp16((max - min) / 15), m = fp16(min), c = clamp(rint((x - m) / s), 0, 15)
+ *   V = s * (c - 8) + m, m = fp16(min + 8 s), c = clamp(rint((x - m) / s) + 8, 0, 15)
+ * (1 / s as one rounded reciprocal, everything in fp32).  Scale and offset saturate at fp16's range; a group with a
+ * value that is not finite is stored as NaN.  page_size is a multiple of 16, head_dim 64, 128 or 256, pages 16-byte
+ * aligned, n_pages * page_size < 2^31.  A slot is page * page_size + token of the page. */
+typedef struct DracoKV4Cache {
+    void* pages;
+    int n_pages, page_size, n_kv_heads, head_dim;
+} DracoKV4Cache;
+/* bytes of one page (0: not a shape of the cache) */
+size_t draco_b200_kv4_page_bytes(int page_size, int n_kv_heads, int head_dim);
+/* Quantise k and v ([n_tokens][n_kv_heads][head_dim], strides in elements, channels contiguous) into the given slots;
+ * slots outside the cache are skipped.  No slot may be given twice. */
+int draco_b200_kv4_append(const DracoKV4Cache* cache, int dtype, const void* k, long k_token_stride,
+                          long k_head_stride, const void* v, long v_token_stride, long v_head_stride,
+                          const int* slots, int n_tokens, void* stream);
+/* The values that the given slots hold, as rows of the same kind; zeros for slots outside the cache. */
+int draco_b200_kv4_read(const DracoKV4Cache* cache, int dtype, void* k, long k_token_stride, long k_head_stride,
+                        void* v, long v_token_stride, long v_head_stride, const int* slots, int n_tokens,
+                        void* stream);
+
+/* Attention of ragged queries over the cache.  Request r's queries are tokens cu_q[r] .. cu_q[r+1] of q, the last ones
+ * of its seq_len[r] cached tokens: query i has position p = seq_len - q_len + i and sees the keys j <= p with
+ * window == 0 or p - j < window or j < sinks.  Query head h reads kv head h / (n_heads / n_kv_heads).
+ *   out = softmax(scale * q . k) . v, zeros where nothing is seen; lse (optional, [n_tokens][n_heads]) its natural log
+ *   of the sum of exponentials, -infinity where nothing is seen.
+ * block_table: n_req rows of table_width entries, table_stride entries apart; lengths beyond a row (or 2^30) are cut to it, entries
+ * outside the cache count as not seen.  max_q_len and max_seq_len (host values) bound the requests' lengths: queries past max_q_len get
+ * no output, a longer sequence only runs slower.  workspace: draco_b200_kv4_attention_workspace() bytes, 16-byte
+ * aligned, any content; calls that may overlap on the GPU need workspaces of their own. */
+typedef struct DracoKV4Attention {
+    const void* q;
+    void* out;
+    float* lse;
+    long q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+    int dtype, n_heads, n_req, n_tokens;
+    const int *cu_q, *seq_len, *block_table;
+    long table_stride;
+    int table_width, max_q_len, max_seq_len;
+    float scale;
+    int window, sinks;
+    void* workspace;
+    size_t workspace_bytes;
+} DracoKV4Attention;
+size_t draco_b200_kv4_attention_workspace(const DracoKV4Cache* cache, const DracoKV4Attention* args);
+int draco_b200_kv4_attention(const DracoKV4Cache* cache, const DracoKV4Attention* args, void* stream);
+
+/* Residual addition, RMS norm and 8-bit output, row by row (hidden values each, row strides in elements):
+ *   h = x + residual rounded to dtype (h and residual given together; h may be residual or x), h = x without one
+ *   rstd = 1 / sqrt(mean(h^2) + eps);  y = h * rstd * weight (y optional; weight fp32)
+ *   codes, per group of u = h * weight with a = max |u|:  fmt 0: int8 rint(u * (127 / a)), fmt 1: e4m3(u * (448 / a))
+ *   scales[row][group] = a / 127 (or 448) * rstd, so that code * scale is the normalised value
+ * group: 32, 64, 128, 256 or 0 (one scale a row), dividing hidden.  A group with a < 2^-100 has code and scale 0, one
+ * with an infinity or NaN a NaN scale. */
+typedef struct DracoNormQ8 {
+    const void *x, *residual;
+    const float* weight;
+    void *h, *y, *codes;
+    float* scales;
+    long x_stride, residual_stride, h_stride, y_stride, codes_stride, scales_stride;
+    int dtype, fmt, n_rows, hidden, group;
+    float eps;
+} DracoNormQ8;
+int draco_b200_rmsnorm_q8(const DracoNormQ8* args, void* stream);
 
 #ifdef __cplusplus
 }
