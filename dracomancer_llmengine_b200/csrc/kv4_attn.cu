@@ -4,18 +4,28 @@
 //   o = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * q . k_j - max),   over the keys j that the query at position p
 //   (= seq_len - q_len + i) sees:  j <= p  and  (window == 0  or  p - j < window  or  j < sinks)
 //
-// Rows: the queries of one kv head (q_len * heads / kv_heads of them, token-major) in blocks of 8.  A block of rows
-// walks the visible tiles of 16 tokens once, with the running maximum and sum of the softmax.
+// Rows: the queries of one kv head (q_len * heads / kv_heads of them, token-major) in blocks of 8 or 16.  A block of rows
+// walks the visible tiles of 16 tokens once, with a running maximum and sum of the softmax.
 //
-// Arithmetic, on mma.m16n8k16 (fp16 operands, fp32 sums).  Its 16 operand rows are the 8 query rows twice: their high
-// and their low fp16 halves (x = hi + lo / 2048, 22 bits), so that fp32 queries and weights keep fp32-like precision at
-// the price of rows that a decode step would leave empty.
+// Arithmetic, on mma.m16n8k16 (fp16 operands, fp32 sums), transposed: tokens (scores) and channels (output) are the 16
+// rows of the product, the 8 query rows its columns, so that a single token with up to 8 heads per kv head fills it.
 //   scores: q . k = sum over groups g of s_g * (q . codes)_g + m_g * sum(q)_g.  A code's four bits are used as they are,
 //     as an fp16 subnormal (c * 2^-24, or 16 c * 2^-24 for the odd nibbles, against q / 16): one AND per two codes.
 //     Group sums come out of the products unscaled and are scaled in fp32; the offsets are one small product more.
-//   output: sum_t p_t v_t = sum_t (p_t s_tg) (c - 8) + sum_t p_t m_tg: the weights are scaled in fp32, per group, then
-//     split in two halves; codes become c - 8 (or 16 (c - 8), undone at the end) by OR-ing in the exponent of 1024 and
-//     subtracting.  Queries are scaled to |q| <= 1 by a power of two per row before the split.
+//     Queries are scaled to |q| <= 1 by a power of two per row first (16-bit queries then are exact in fp16); their
+//     sums have a high and a low half in every type, so the scores, and with them lse, keep fp32 precision.
+//   output: sum_t p_t v_t = sum_t (p_t s_tg / 2) (2 c - 15) + sum_t p_t (m_tg - s_tg / 2): the weights take the scales,
+//     codes become (2 c - 15) * 2^-10 in one multiply-add.  They are centred because the sums run over the whole context:
+//     uncentred ones would grow with its length, cancel against the offsets' sum, and lose the result's low bits.
+// Precision of the operands, by the type of queries and output:
+//   fp32  queries and weights are split in two halves (x = hi + lo / 2048, 22 bits), the low halves take 8 columns more;
+//         codes of K are made normal numbers (c * 2^-9): with subnormal ones the sums of a product are aligned ten bits
+//         too high, which showed as 1e-6 of the result (2^-14 of a code; measured 1.1e-6 against 0.5e-6 without)
+//   fp16  weights are scaled in fp32 and rounded to fp16 once, as the output will be
+//   bf16  weights are rounded to fp16 and scaled there (2^-11 twice, an eighth of the output's own rounding)
+//
+// The running maximum is raised only when a score exceeds it by more than 3 (log2): weights stay below 8, and most tiles
+// need neither the reduction over tokens nor the rescaling of the sums.
 //
 // Memory: a warp owns every kWarps-th tile of its split and copies tiles (20 D bytes, contiguous) into its own ring of
 // stages with cp.async, page ids fetched 32 tiles at a time.  The long axis is split over blocks when rows are few; a
@@ -23,13 +33,22 @@
 #include "kv4.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace draco {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStages = 4;
-constexpr int kRows = 8;
+// What a variant of the kernel takes per block: NT columns of 8 (queries, or their two halves)
+template <int D, int NT>
+struct Shape {
+    static constexpr int kStages = D == 256 ? 3 : 4;                      // of a warp's ring
+    static constexpr bool kQInSmem = D == 256 && NT == 2;                 // 64 registers a lane otherwise
+    static constexpr int kBlocks = D == 64 ? (NT == 1 ? 5 : 4) : D == 128 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2);
+};
+constexpr uint32_t kTwo15 = 0x78007800u;   // 2^15, 2^15 in fp16
+constexpr float kNone = -1e30f;     // maximum of a row that has seen nothing
+constexpr float kSlack = 3.f;       // log2 of the largest weight
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLoScale = 2048.f, kLoInv = 1.f / 2048.f;
@@ -37,23 +56,34 @@ constexpr float kLoScale = 2048.f, kLoInv = 1.f / 2048.f;
 struct Args {
     Kv4Attn a;
     int tiles_per_split, n_splits, row_blocks, group;   // group: query heads of a kv head
+    int block_rows;
     bool wide_q, wide_o;
-    float* part;        // [unit][split][8][D] sums, relative to the split's maximum
-    float2* ml;         // [unit][split][8] maximum (log2 domain) and sum
+    float* part;        // [unit][split][block_rows][D] sums, relative to the split's maximum
+    float2* ml;         // [unit][split][block_rows] maximum (log2 domain) and sum
 };
 
-__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                      uint32_t b1) {
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
+                                      float c1, float c2, float c3) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
-__device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    mma16(d, a, b0, b1, d[0], d[1], d[2], d[3]);
+}
+// d = a b with k = 8
+__device__ __forceinline__ void mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
     asm volatile(
-        "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(b0));
+        "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
+}
+// 8 x 8 matrix of halves: lane (r, q) has row r, columns 2 q and 2 q + 1 before, column r, rows 2 q and 2 q + 1 after
+__device__ __forceinline__ uint32_t transpose(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -72,16 +102,22 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
     lo = pack((a - f.x) * kLoScale, (b - f.y) * kLoScale);
 }
 __device__ __forceinline__ float2 halves(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-// (w & mask) | 1024's exponent, minus `base`: two centred codes
-template <uint32_t MASK>
-__device__ __forceinline__ uint32_t centred(uint32_t w, uint32_t base) {
-    uint32_t t;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(t) : "r"(w), "n"(MASK), "r"(0x64006400u));   // (w & MASK) | 0x6400...
-    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&t), *reinterpret_cast<const __half2*>(&base));
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    const __half2 d = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&d);
 }
-constexpr uint32_t kBase1 = 0x64086408u;    // 1032, 1032
-constexpr uint32_t kBase16 = 0x64806480u;   // 1152, 1152
+// two codes as subnormals (c * 2^-24, odd nibbles 16 c * 2^-24) to (2 c - 15) * 2^-10 (2^-6); exact
+__device__ __forceinline__ uint32_t centred(uint32_t codes, bool odd) {
+    const __half2 k = __float2half2_rn(32768.f), o = __float2half2_rn(odd ? -15.f / 64.f : -15.f / 1024.f);
+    const __half2 d = __hfma2(*reinterpret_cast<const __half2*>(&codes), k, o);
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+// a word's halves that are infinite or NaN set to 0
+__device__ __forceinline__ uint32_t finite2(uint32_t z) {
+    if ((z & 0x7c00u) == 0x7c00u) z &= 0xffff0000u;
+    if ((z & 0x7c000000u) == 0x7c000000u) z &= 0xffffu;
+    return z;
+}
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
@@ -124,11 +160,11 @@ __device__ __forceinline__ bool span_of(const Args& x, int req, int rb, Span& s)
     s.q0 = max(s.q0, 0);
     s.q_len = q1 - s.q0;
     const int rows = s.q_len * x.group;
-    if (rb * kRows >= rows) return false;
+    if (rb * x.block_rows >= rows) return false;
     const long cap = min((long)a.table_width * a.cache.page_size, 1l << 30);
     s.seq = (int)min((long)max(a.seq_len[req], 0), cap);
-    s.p_lo = s.seq - s.q_len + rb * kRows / x.group;
-    s.p_hi = s.seq - s.q_len + min(rb * kRows + kRows - 1, rows - 1) / x.group;
+    s.p_lo = s.seq - s.q_len + rb * x.block_rows / x.group;
+    s.p_hi = s.seq - s.q_len + (min((rb + 1) * x.block_rows, rows) - 1) / x.group;
     s.head = s.first = s.n = 0;
     if (s.p_hi < 0) return true;   // nothing before any query: no tile
     const int last = s.p_hi / kKvTile;
@@ -140,12 +176,17 @@ __device__ __forceinline__ bool span_of(const Args& x, int req, int rb, Span& s)
     return true;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32, D == 256 ? 2 : 3) attend_kernel(const Args x) {
+// NT columns of 8: 8 NT query rows, or (SPLIT) the high and low halves of 8
+template <typename T, int D, int NT, bool SPLIT>
+__global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_kernel(const Args x) {
+    using S = Shape<D, NT>;
     constexpr int NG = D / kKvGroup;
+    constexpr int kStages = S::kStages;
     constexpr int kTileB = kv4_tile_bytes(D);
     constexpr int kChunks = kTileB / 16;
-    constexpr bool kQInSmem = D == 256;   // its fragments would take 64 registers a lane
+    constexpr int ET = SPLIT ? 1 : NT;          // columns of 8 query rows
+    constexpr int kRows = 8 * ET;
+    constexpr bool kFp16 = sizeof(T) == 2 && !SPLIT && std::is_same<T, __half>::value;
     extern __shared__ __align__(16) uint8_t smem[];
     const Kv4Attn& a = x.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r8 = lane >> 2, q4 = lane & 3;
@@ -162,38 +203,41 @@ __global__ void __launch_bounds__(kWarps * 32, D == 256 ? 2 : 3) attend_kernel(c
     uint8_t* ring = smem + warp * kStages * kTileB;
     const int* table = a.table + (long)req * a.table_stride;
     const int tiles_per_page = a.cache.page_size / kKvTile;
-    const size_t head_bytes = (size_t)tiles_per_page * kTileB;
 
-    // this warp's tiles: idx = begin + warp + kWarps * i, i < count; 32 page ids at a time, one per lane
+    // this warp's tiles: idx = begin + warp + kWarps * i, i < count; where 32 of them lie (tile ordinal in the cache, or
+    // -1 for a page outside it), one per lane
     const int mine = begin + warp;
     const int count = mine < end ? (end - mine + kWarps - 1) / kWarps : 0;
     auto tile_of = [&](int i) {
         const int idx = mine + kWarps * i;
         return idx < sp.head ? idx : sp.first + idx - sp.head;
     };
-    auto fetch_ids = [&](int i0) {
+    auto fetch = [&](int i0) {
         const int i = i0 + lane;
         if (i >= count) return -1;
-        const int page = table[tile_of(i) / tiles_per_page];
-        return page < a.cache.n_pages ? page : -1;
+        const int tile = tile_of(i), p = tile / tiles_per_page, page = table[p];
+        if (page < 0 || page >= a.cache.n_pages) return -1;
+        return (page * a.cache.n_kv_heads + kvh) * tiles_per_page + (tile - p * tiles_per_page);
     };
-    int ids = fetch_ids(0), ids_next = fetch_ids(32);
-    auto issue = [&](int i) {   // copy tile i into its stage; a page id outside the cache copies nothing
+    int where = fetch(0), where_next = fetch(32);
+    uint32_t there = 0;   // bit j: the tile issued j calls ago has a page
+    const uint8_t* src0 = a.cache.pages + lane * 16;
+    uint8_t* dst0 = ring + lane * 16;
+    auto issue = [&](int i) {   // copy tile i into its stage
+        there <<= 1;
         if (i < count) {
             if ((i & 31) == 0 && i) {
-                ids = ids_next;
-                ids_next = fetch_ids(i + 32);
+                where = where_next;
+                where_next = fetch(i + 32);
             }
-            const int page = __shfl_sync(0xffffffffu, ids, i & 31);
-            if (page >= 0) {
-                const int tile = tile_of(i);
-                const uint8_t* src = a.cache.pages + ((size_t)page * a.cache.n_kv_heads + kvh) * head_bytes +
-                                     (size_t)(tile % tiles_per_page) * kTileB;
-                uint8_t* dst = ring + (i % kStages) * kTileB;
+            const int at = __shfl_sync(0xffffffffu, where, i & 31);
+            if (at >= 0) {
+                there |= 1;
+                const uint8_t* src = src0 + (size_t)at * kTileB;
+                uint8_t* dst = dst0 + (i % kStages) * kTileB;
 #pragma unroll
                 for (int c = 0; c < (kChunks + 31) / 32; c++)
-                    if (kChunks % 32 == 0 || c * 32 + lane < kChunks)
-                        cp_async16(dst + (c * 32 + lane) * 16, src + (c * 32 + lane) * 16);
+                    if (kChunks % 32 == 0 || c * 32 + lane < kChunks) cp_async16(dst + c * 512, src + c * 512);
             }
         }
         cp_commit();
@@ -201,18 +245,18 @@ __global__ void __launch_bounds__(kWarps * 32, D == 256 ? 2 : 3) attend_kernel(c
 #pragma unroll
     for (int i = 0; i < kStages - 1; i++) issue(i);
 
-    // ---- the rows' queries as operand fragments, scaled by a power of two ----
-    const int rows = sp.q_len * x.group;
-    const int row = rb * kRows + r8;
-    const bool has_row = row < rows;
-    const int tok = has_row ? row / x.group : 0;
-    const int head = kvh * x.group + (has_row ? row % x.group : 0);
-    const int my_p = sp.seq - sp.q_len + tok;
-    uint32_t* q_sm = reinterpret_cast<uint32_t*>(smem + kWarps * kStages * kTileB);   // [NG][2][32 lanes][4]
-    uint32_t qf[kQInSmem ? 1 : NG][8];
-    uint32_t qs_hi = 0, qs_lo = 0;
-    float qk;
-    {
+    // ---- the rows' queries as operand fragments: lane (r8, q4) has channels g*32 + q4*8 .. + 7 of row r8 (+ 8) ----
+    const int rows = sp.q_len * x.group, row0 = rb * kRows;
+    uint32_t* q_sm = reinterpret_cast<uint32_t*>(smem + kWarps * kStages * kTileB);   // [NG][NT][32 lanes][4]
+    uint32_t qf[S::kQInSmem ? 1 : NG][NT][4];    // two steps of 16 channels, two registers each
+    uint32_t qs[2][NT];                          // sums of groups 2 q4, 2 q4 + 1 of row r8: [high | low half]
+    float qk[ET][2];                             // score to log2 units, for the rows of this lane's sums: 2 q4, 2 q4 + 1
+    int pos_of[ET][2];
+#pragma unroll
+    for (int e = 0; e < ET; e++) {
+        const int row = row0 + e * 8 + r8;
+        const bool has_row = row < rows;
+        const int tok = has_row ? row / x.group : 0, head = kvh * x.group + (has_row ? row % x.group : 0);
         const T* q = (const T*)a.q + (long)(sp.q0 + tok) * a.q_tok + (long)head * a.q_head + q4 * 8;
         float v[NG][8];
         float top = 0.f;
@@ -228,14 +272,21 @@ __global__ void __launch_bounds__(kWarps * 32, D == 256 ? 2 : 3) attend_kernel(c
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // the power of two above the largest magnitude; zero, subnormal and huge rows keep a finite factor
-        int e = (int)((__float_as_uint(top) >> 23) & 255) - 126;
-        e = min(max(e, -120), 120);
-        const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
-        qk = a.scale * kLog2e * up;
+        int ex = (int)((__float_as_uint(top) >> 23) & 255) - 126;
+        ex = min(max(ex, -120), 120);
+        const float down = __uint_as_float((uint32_t)(127 - ex) << 23), up = __uint_as_float((uint32_t)(127 + ex) << 23);
+        const float my_qk = a.scale * kLog2e * up;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            qk[e][j] = __shfl_sync(0xffffffffu, my_qk, (2 * q4 + j) * 4);
+            pos_of[e][j] = sp.seq - sp.q_len + (row0 + e * 8 + 2 * q4 + j) / x.group;
+        }
+        qs[0][e] = qs[1][e] = 0;
+        if constexpr (SPLIT) qs[0][1] = qs[1][1] = 0;
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             float t = 0.f;
-            uint32_t f[8];
+            uint32_t hi[4], lo[4];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 v[g][j] *= down;
@@ -243,198 +294,315 @@ __global__ void __launch_bounds__(kWarps * 32, D == 256 ? 2 : 3) attend_kernel(c
             }
 #pragma unroll
             for (int st = 0; st < 2; st++) {
-                split2(v[g][2 * st], v[g][2 * st + 4], f[4 * st], f[4 * st + 1]);
-                split2(v[g][2 * st + 1] * 0.0625f, v[g][2 * st + 5] * 0.0625f, f[4 * st + 2], f[4 * st + 3]);
+                split2(v[g][2 * st], v[g][2 * st + 4], hi[2 * st], lo[2 * st]);
+                split2(v[g][2 * st + 1] * 0.0625f, v[g][2 * st + 5] * 0.0625f, hi[2 * st + 1], lo[2 * st + 1]);
             }
-            if constexpr (kQInSmem) {
+            if constexpr (S::kQInSmem) {
                 if (warp == 0) {
-                    reinterpret_cast<uint4*>(q_sm)[(g * 2) * 32 + lane] = make_uint4(f[0], f[1], f[2], f[3]);
-                    reinterpret_cast<uint4*>(q_sm)[(g * 2 + 1) * 32 + lane] = make_uint4(f[4], f[5], f[6], f[7]);
+                    reinterpret_cast<uint4*>(q_sm)[(g * NT + e) * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if constexpr (SPLIT)
+                        reinterpret_cast<uint4*>(q_sm)[(g * NT + 1) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; j++) qf[g][j] = f[j];
+                for (int j = 0; j < 4; j++) {
+                    qf[g][e][j] = hi[j];
+                    if constexpr (SPLIT) qf[g][1][j] = lo[j];
+                }
             }
             t += __shfl_xor_sync(0xffffffffu, t, 1);
             t += __shfl_xor_sync(0xffffffffu, t, 2);
-            // operand of the offsets' product: column k = g of row r8 lies in lane q4 = g / 2
-            uint32_t hi, lo;
-            split2(t, 0.f, hi, lo);
+            uint32_t th, tl;
+            split2(t, 0.f, th, tl);
             if (q4 == g / 2) {
-                qs_hi |= (hi & 0xffffu) << (16 * (g & 1));
-                qs_lo |= (lo & 0xffffu) << (16 * (g & 1));
+                qs[0][e] |= (th & 0xffffu) << (16 * (g & 1));
+                qs[1][e] |= (tl & 0xffffu) << (16 * (g & 1));
             }
         }
-        if constexpr (kQInSmem) __syncthreads();
     }
+    if constexpr (S::kQInSmem) __syncthreads();
 
-    float acc[NG][4][4];
-    float zacc[4] = {0.f, 0.f, 0.f, 0.f};
+    float acc[NT][NG][2][4];      // channels g*32 + r8*4 + {0, 1 | 2, 3} x rows 2 q4, 2 q4 + 1
+    float zacc[NT][4];            // group r8 x rows 2 q4, 2 q4 + 1 (the last two are not used)
+    float m[ET][2], l[ET][2];
 #pragma unroll
-    for (int g = 0; g < NG; g++)
+    for (int n = 0; n < NT; n++) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int j = 0; j < 4; j++) zacc[n][j] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; j++) acc[g][i][j] = 0.f;
-    float m = -INFINITY, l = 0.f;
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) acc[n][g][j >> 2][j & 3] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < ET; e++) m[e][0] = m[e][1] = kNone, l[e][0] = l[e][1] = 0.f;
+    const int odd_shift = (r8 & 1) * 16;
 
-    int cur_ids = 0;
     for (int i = 0; i < count; i++) {
-        if ((i & 31) == 0) cur_ids = i == 0 ? ids : fetch_ids(i);
-        const bool there = __shfl_sync(0xffffffffu, cur_ids, i & 31) >= 0;
         cp_wait<kStages - 2>();
         __syncwarp();
         issue(i + kStages - 1);   // into the stage that the previous step finished with (the barrier above)
-        if (!there) continue;
+        if (!((there >> (kStages - 1)) & 1)) continue;
         const uint8_t* t = ring + (i % kStages) * kTileB;
         const int base = tile_of(i) * kKvTile;
 
-        // ---- scores of 8 rows x 16 tokens ----
-        float sc[4];   // tokens 2 q4, 2 q4 + 1, 8 + 2 q4, 8 + 2 q4 + 1 of row r8
+        // ---- scores: tokens r8, r8 + 8 x rows 2 q4, 2 q4 + 1 of each column ----
+        float sc[ET][4];
+        {
+            uint32_t w0[NG], w1[NG], k0[NG], k1[NG];
+            load_words<NG>(t + (r8 * 4 + q4) * NG * 4, w0);
+            load_words<NG>(t + ((r8 + 8) * 4 + q4) * NG * 4, w1);
+            load_words<NG>(t + kv4_off_ks(D) + (r8 >> 1) * NG * 4, k0);
+            load_words<NG>(t + kv4_off_ks(D) + ((r8 >> 1) + 4) * NG * 4, k1);
+            uint32_t m0 = 0, m1 = 0;
+            if (2 * q4 < NG) {
+                m0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_km(D) + (r8 * NG + 2 * q4) * 2);
+                m1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_km(D) + ((r8 + 8) * NG + 2 * q4) * 2);
+            }
+            float s[ET][4];
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            uint32_t w[NG], ks[NG];
-            load_words<NG>(t + ((j * 8 + r8) * 4 + q4) * NG * 4, w);
-            load_words<NG>(t + kv4_off_ks(D) + (j * 4 + q4) * NG * 4, ks);
-            float s0 = 0.f, s1 = 0.f;
+            for (int e = 0; e < ET; e++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) s[e][j] = 0.f;
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                uint32_t f[8];
-                if constexpr (kQInSmem) {
-                    load_words<4>(q_sm + ((g * 2) * 32 + lane) * 4, *reinterpret_cast<uint32_t(*)[4]>(f));
-                    load_words<4>(q_sm + ((g * 2 + 1) * 32 + lane) * 4, *reinterpret_cast<uint32_t(*)[4]>(f + 4));
-                } else {
+                const uint32_t x0 = w0[g] >> 8, x1 = w1[g] >> 8;
+                uint32_t c0[4] = {w0[g] & 0x000f000fu, w1[g] & 0x000f000fu, w0[g] & 0x00f000f0u, w1[g] & 0x00f000f0u};
+                uint32_t c1[4] = {x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u};
+                if constexpr (SPLIT) {
 #pragma unroll
-                    for (int k = 0; k < 8; k++) f[k] = qf[g][k];
+                    for (int j = 0; j < 4; j++) c0[j] = mul2(c0[j], kTwo15), c1[j] = mul2(c1[j], kTwo15);
                 }
-                const uint32_t w8 = w[g] >> 8;
-                mma16(c, f[0], f[1], f[2], f[3], w[g] & 0x000f000fu, w[g] & 0x00f000f0u);
-                mma16(c, f[4], f[5], f[6], f[7], w8 & 0x000f000fu, w8 & 0x00f000f0u);
-                const float2 s = halves(ks[g]);
-                s0 = fmaf(s.x, fmaf(c[2], kLoInv, c[0]), s0);
-                s1 = fmaf(s.y, fmaf(c[3], kLoInv, c[1]), s1);
+                float c[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    uint32_t f[4];
+                    if constexpr (S::kQInSmem) {
+                        load_words<4>(q_sm + ((g * NT + n) * 32 + lane) * 4, f);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) f[j] = qf[g][n][j];
+                    }
+                    mma16(c[n], c0, f[0], f[1], 0.f, 0.f, 0.f, 0.f);
+                    mma16(c[n], c1, f[2], f[3]);
+                }
+                const float s0 = __half2float(__ushort_as_half((uint16_t)(k0[g] >> odd_shift)));
+                const float s1 = __half2float(__ushort_as_half((uint16_t)(k1[g] >> odd_shift)));
+#pragma unroll
+                for (int e = 0; e < ET; e++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float d = SPLIT ? fmaf(c[NT - 1][j], kLoInv, c[e][j]) : c[e][j];
+                        s[e][j] = fmaf(j < 2 ? s0 : s1, d, s[e][j]);
+                    }
             }
-            uint32_t km = 0;
-            if (2 * q4 < NG) km = *reinterpret_cast<const uint32_t*>(t + kv4_off_km(D) + ((j * 8 + r8) * NG + 2 * q4) * 2);
-            float z[4] = {0.f, 0.f, 0.f, 0.f};
-            mma8(z, qs_hi, qs_lo, km);
-            sc[2 * j] = fmaf(s0, 16777216.f, fmaf(z[2], kLoInv, z[0])) * qk;
-            sc[2 * j + 1] = fmaf(s1, 16777216.f, fmaf(z[3], kLoInv, z[1])) * qk;
+#pragma unroll
+            for (int e = 0; e < ET; e++) {
+                float z[4];
+                mma8(z, m0, m1, qs[0][e]);
+                float y[4];
+                mma8(y, m0, m1, qs[1][e]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) z[j] = fmaf(y[j], kLoInv, z[j]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) sc[e][j] = fmaf(s[e][j], SPLIT ? 512.f : 16777216.f, z[j]);
+            }
         }
 
-        // ---- masks: only tiles that some row sees in part ----
-        const bool part_mask = base + kKvTile - 1 > sp.p_lo ||
-                               (a.window > 0 && base <= sp.p_hi - a.window && base + kKvTile > a.sinks);
-        if (part_mask) {
+        // ---- exponents relative to the running maximum; masks only where some row sees a part of the tile ----
+        const bool part = base + kKvTile - 1 > sp.p_lo ||
+                          (a.window > 0 && base <= sp.p_hi - a.window && base + kKvTile > a.sinks);
+        float ex[ET][4];
+        auto exponents = [&]() {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int pos = base + (j >> 1) * 8 + 2 * q4 + (j & 1);
-                const bool sees = pos <= my_p && (a.window <= 0 || pos > my_p - a.window || pos < a.sinks);
-                if (!sees) sc[j] = -INFINITY;
+            for (int e = 0; e < ET; e++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) ex[e][j] = fmaf(sc[e][j], qk[e][j & 1], -m[e][j & 1]);
+            if (part) {
+#pragma unroll
+                for (int e = 0; e < ET; e++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int pos = base + r8 + (j >> 1) * 8, p = pos_of[e][j & 1];
+                        if (pos > p || (a.window > 0 && pos <= p - a.window && pos >= a.sinks)) ex[e][j] = -INFINITY;
+                    }
+            }
+        };
+        exponents();
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < ET; e++) top = fmaxf(top, fmaxf(fmaxf(ex[e][0], ex[e][1]), fmaxf(ex[e][2], ex[e][3])));
+        if (__any_sync(0xffffffffu, top > kSlack)) {
+#pragma unroll
+            for (int e = 0; e < ET; e++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    float now = fmaxf(ex[e][j] == -INFINITY ? -INFINITY : sc[e][j] * qk[e][j],
+                                      ex[e][j + 2] == -INFINITY ? -INFINITY : sc[e][j + 2] * qk[e][j]);
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+                    now = fmaxf(m[e][j], now);
+                    const float f = ex2(m[e][j] - now);
+                    m[e][j] = now;
+                    l[e][j] *= f;
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        if (!SPLIT && n != e) continue;
+                        zacc[n][j] *= f;
+#pragma unroll
+                        for (int g = 0; g < NG; g++) {
+                            acc[n][g][0][j] *= f;
+                            acc[n][g][0][j + 2] *= f;
+                            acc[n][g][1][j] *= f;
+                            acc[n][g][1][j + 2] *= f;
+                        }
+                    }
+                }
+            exponents();
+        }
+
+        // ---- weights, to the layout of the second product: row r8 x tokens 2 q4, + 1 (lo: of 16) and 2 q4 + 8, + 9 ----
+        uint32_t ph[ET][2], pl[ET][2];
+#pragma unroll
+        for (int e = 0; e < ET; e++) {
+            float p[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) p[j] = ex2(ex[e][j]);
+            l[e][0] += p[0] + p[2];
+            l[e][1] += p[1] + p[3];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if constexpr (SPLIT || kFp16) {
+                    split2(p[2 * h], p[2 * h + 1], ph[e][h], pl[e][h]);
+                    pl[e][h] = transpose(pl[e][h]);
+                } else {
+                    ph[e][h] = pack(p[2 * h], p[2 * h + 1]);
+                }
+                ph[e][h] = transpose(ph[e][h]);
             }
         }
 
-        // ---- running maximum and weights ----
-        float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if (__any_sync(0xffffffffu, top > m)) {
-            const float up = fmaxf(m, top);
-            const float f = up == -INFINITY ? 1.f : ex2(m - up);
-            m = up;
-            l *= f;
-#pragma unroll
-            for (int g = 0; g < NG; g++)
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[g][k][j] *= f;
-#pragma unroll
-            for (int j = 0; j < 4; j++) zacc[j] *= f;
-        }
-        const float mm = m == -INFINITY ? 0.f : m;
-        float p[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) p[j] = ex2(sc[j] - mm);
-        l += (p[0] + p[1]) + (p[2] + p[3]);
-
-        // ---- offsets of V, then its codes, group by group ----
-        {
-            uint32_t h0, l0, h1, l1, z0 = 0, z1 = 0;
-            split2(p[0], p[1], h0, l0);
-            split2(p[2], p[3], h1, l1);
-            if (r8 < NG) {
-                z0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vm(D) + (q4 * NG + r8) * 4);
-                z1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vm(D) + ((q4 + 4) * NG + r8) * 4);
-            }
-            if (part_mask) {
-                // a hidden token's bytes may hold anything: infinities and NaN must not meet its weight of zero.  A
-                // stored token that is not finite has a NaN scale too, which reaches the rows that do see it below.
-                auto clean = [](uint32_t z) {
-                    if ((z & 0x7c00u) == 0x7c00u) z &= 0xffff0000u;
-                    if ((z & 0x7c000000u) == 0x7c000000u) z &= 0xffffu;
-                    return z;
-                };
-                z0 = clean(z0);
-                z1 = clean(z1);
-            }
-            mma16(zacc, h0, l0, h1, l1, z0, z1);
-        }
+        // ---- output: scales into the weights, codes of V, offsets ----
         uint32_t v0[NG], v1[NG], s0[NG], s1[NG];
         load_words<NG>(t + kv4_off_vc(D) + (q4 * 8 + r8) * NG * 4, v0);
         load_words<NG>(t + kv4_off_vc(D) + ((q4 + 4) * 8 + r8) * NG * 4, v1);
         load_words<NG>(t + kv4_off_vs(D) + q4 * NG * 4, s0);
         load_words<NG>(t + kv4_off_vs(D) + (q4 + 4) * NG * 4, s1);
+        {
+            uint32_t z0 = 0, z1 = 0, y0 = 0, y1 = 0;
+            if (r8 < NG) {
+                z0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vm(D) + (q4 * NG + r8) * 4);
+                z1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vm(D) + ((q4 + 4) * NG + r8) * 4);
+                y0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vs(D) + (q4 * NG + r8) * 4);
+                y1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vs(D) + ((q4 + 4) * NG + r8) * 4);
+            }
+            if (part) {
+                // a hidden token's bytes may hold anything: infinities and NaN must not meet its weight of zero.  A stored
+                // token that is not finite has a NaN scale, which still reaches the rows that do see it below.
+                z0 = finite2(z0), z1 = finite2(z1), y0 = finite2(y0), y1 = finite2(y1);
+            }
+            const uint32_t za[4] = {z0, z0, z1, z1}, ya[4] = {y0, y0, y1, y1};   // rows 8 .. 15: not used
+#pragma unroll
+            for (int e = 0; e < ET; e++) {
+                const uint32_t minus_half = 0xb800b800u;
+                mma16(zacc[e], za, ph[e][0], ph[e][1]);
+                mma16(zacc[e], ya, mul2(ph[e][0], minus_half), mul2(ph[e][1], minus_half));
+                if constexpr (SPLIT) {
+                    mma16(zacc[1], za, pl[e][0], pl[e][1]);
+                    mma16(zacc[1], ya, mul2(pl[e][0], minus_half), mul2(pl[e][1], minus_half));
+                }
+            }
+        }
+        uint32_t b[NT][NG][2];
+#pragma unroll
+        for (int e = 0; e < ET; e++) {
+            uint32_t u0[NG], u1[NG];   // the scales, 0 where a weight is: they may not be finite
+#pragma unroll
+            for (int g = 0; g < NG; g++) u0[g] = s0[g], u1[g] = s1[g];
+            if (part) {
+                const uint32_t any0 = SPLIT || kFp16 ? ph[e][0] | pl[e][0] : ph[e][0];
+                const uint32_t any1 = SPLIT || kFp16 ? ph[e][1] | pl[e][1] : ph[e][1];
+                const uint32_t k0 = (any0 & 0x7fffu ? 0xffffu : 0u) | (any0 & 0x7fff0000u ? 0xffff0000u : 0u);
+                const uint32_t k1 = (any1 & 0x7fffu ? 0xffffu : 0u) | (any1 & 0x7fff0000u ? 0xffff0000u : 0u);
+#pragma unroll
+                for (int g = 0; g < NG; g++) u0[g] &= k0, u1[g] &= k1;
+            }
+            if constexpr (SPLIT || kFp16) {
+                const float2 h0 = halves(ph[e][0]), h1 = halves(ph[e][1]), l0 = halves(pl[e][0]), l1 = halves(pl[e][1]);
+                const float p0 = fmaf(l0.x, kLoInv, h0.x), p1 = fmaf(l0.y, kLoInv, h0.y);
+                const float p2 = fmaf(l1.x, kLoInv, h1.x), p3 = fmaf(l1.y, kLoInv, h1.y);
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const float2 a0 = halves(u0[g]), a1 = halves(u1[g]);
+                    if constexpr (SPLIT) {
+                        split2(p0 * a0.x, p1 * a0.y, b[0][g][0], b[NT - 1][g][0]);
+                        split2(p2 * a1.x, p3 * a1.y, b[0][g][1], b[NT - 1][g][1]);
+                    } else {
+                        b[e][g][0] = pack(p0 * a0.x, p1 * a0.y);
+                        b[e][g][1] = pack(p2 * a1.x, p3 * a1.y);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    b[e][g][0] = mul2(ph[e][0], u0[g]);
+                    b[e][g][1] = mul2(ph[e][1], u1[g]);
+                }
+            }
+        }
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            const float2 a0 = halves(s0[g]), a1 = halves(s1[g]);
-            float w0 = p[0] * a0.x, w1 = p[1] * a0.y, w2 = p[2] * a1.x, w3 = p[3] * a1.y;
-            if (part_mask) {
-                w0 = p[0] == 0.f ? 0.f : w0;
-                w1 = p[1] == 0.f ? 0.f : w1;
-                w2 = p[2] == 0.f ? 0.f : w2;
-                w3 = p[3] == 0.f ? 0.f : w3;
-            }
-            uint32_t h0, l0, h1, l1;
-            split2(w0, w1, h0, l0);
-            split2(w2, w3, h1, l1);
             const uint32_t x0 = v0[g] >> 8, x1 = v1[g] >> 8;
-            mma16(acc[g][0], h0, l0, h1, l1, centred<0x000f000fu>(v0[g], kBase1), centred<0x000f000fu>(v1[g], kBase1));
-            mma16(acc[g][1], h0, l0, h1, l1, centred<0x00f000f0u>(v0[g], kBase16), centred<0x00f000f0u>(v1[g], kBase16));
-            mma16(acc[g][2], h0, l0, h1, l1, centred<0x000f000fu>(x0, kBase1), centred<0x000f000fu>(x1, kBase1));
-            mma16(acc[g][3], h0, l0, h1, l1, centred<0x00f000f0u>(x0, kBase16), centred<0x00f000f0u>(x1, kBase16));
+            const uint32_t c0[4] = {centred(v0[g] & 0x000f000fu, false), centred(v0[g] & 0x00f000f0u, true),
+                                    centred(v1[g] & 0x000f000fu, false), centred(v1[g] & 0x00f000f0u, true)};
+            const uint32_t c1[4] = {centred(x0 & 0x000f000fu, false), centred(x0 & 0x00f000f0u, true),
+                                    centred(x1 & 0x000f000fu, false), centred(x1 & 0x00f000f0u, true)};
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                mma16(acc[n][g][0], c0, b[n][g][0], b[n][g][1]);
+                mma16(acc[n][g][1], c1, b[n][g][0], b[n][g][1]);
+            }
         }
     }
     cp_wait<0>();
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
+#pragma unroll
+    for (int e = 0; e < ET; e++)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) l[e][j] += __shfl_xor_sync(0xffffffffu, l[e][j], o);
 
     // ---- join the warps: their rows meet in shared memory (over the finished ring) ----
     __syncthreads();
-    float* s_o = reinterpret_cast<float*>(smem);                                   // [kWarps][8][D]
-    float2* s_ml = reinterpret_cast<float2*>(smem + kWarps * kRows * D * 4);       // [kWarps][8]
-    const float zl0 = fmaf(zacc[2], kLoInv, zacc[0]), zl1 = fmaf(zacc[3], kLoInv, zacc[1]);   // groups 2 q4, 2 q4 + 1
+    float* s_o = reinterpret_cast<float*>(smem);                                   // [kWarps][kRows][D]
+    float2* s_ml = reinterpret_cast<float2*>(smem + kWarps * kRows * D * 4);       // [kWarps][kRows]
 #pragma unroll
-    for (int g = 0; g < NG; g++) {
-        const float ze = __shfl_sync(0xffffffffu, (g & 1) ? zl1 : zl0, (lane & ~3) | (g >> 1));
-        float o[8];
+    for (int e = 0; e < ET; e++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float f = i & 1 ? 0.0625f : 1.f;
-            o[i] = fmaf(fmaf(acc[g][i][2], kLoInv, acc[g][i][0]), f, ze);
-            o[4 + i] = fmaf(fmaf(acc[g][i][3], kLoInv, acc[g][i][1]), f, ze);
+        for (int j = 0; j < 2; j++) {
+            const int rr = warp * kRows + e * 8 + 2 * q4 + j;
+            const float z = SPLIT ? fmaf(zacc[NT - 1][j], kLoInv, zacc[e][j]) : zacc[e][j];
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const float zg = __shfl_sync(0xffffffffu, z, g * 4 + q4);
+                float o[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {   // channel g*32 + r8*4 + k
+                    const float v = SPLIT ? fmaf(acc[NT - 1][g][k >> 1][j + 2 * (k & 1)], kLoInv, acc[e][g][k >> 1][j + 2 * (k & 1)])
+                                          : acc[e][g][k >> 1][j + 2 * (k & 1)];
+                    o[k] = fmaf(v, k & 1 ? 32.f : 512.f, zg);
+                }
+                *reinterpret_cast<float4*>(s_o + rr * D + g * kKvGroup + r8 * 4) = make_float4(o[0], o[1], o[2], o[3]);
+            }
+            if (r8 == 0) s_ml[rr] = make_float2(m[e][j], l[e][j]);
         }
-        float4* d = reinterpret_cast<float4*>(s_o + (warp * kRows + r8) * D + g * kKvGroup + q4 * 8);
-        d[0] = make_float4(o[0], o[1], o[2], o[3]);
-        d[1] = make_float4(o[4], o[5], o[6], o[7]);
-    }
-    if (q4 == 0) s_ml[warp * kRows + r8] = make_float2(m, l);
     __syncthreads();
     const long unit = ((long)req * a.cache.n_kv_heads + kvh) * x.row_blocks + rb;
     for (int i = tid; i < kRows * D / 4; i += kWarps * 32) {
         const int rr = i / (D / 4), c4 = i % (D / 4);
-        float mx = -INFINITY;
+        const int rw = row0 + rr;
+        if (rw >= rows) break;
+        float mx = kNone;
 #pragma unroll
         for (int w = 0; w < kWarps; w++) mx = fmaxf(mx, s_ml[w * kRows + rr].x);
         float sum = 0.f;
@@ -442,13 +610,11 @@ __global__ void __launch_bounds__(kWarps * 32, D == 256 ? 2 : 3) attend_kernel(c
 #pragma unroll
         for (int w = 0; w < kWarps; w++) {
             const float2 ml = s_ml[w * kRows + rr];
-            const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - mx);
+            const float f = ex2(ml.x - mx);
             sum = fmaf(ml.y, f, sum);
             const float4 v = reinterpret_cast<const float4*>(s_o + (w * kRows + rr) * D)[c4];
             o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
         }
-        const int rw = rb * kRows + rr;
-        if (rw >= rows) continue;
         if (active == 1) {
             const int tk = sp.q0 + rw / x.group, hd = kvh * x.group + rw % x.group;
             const float n = sum == 0.f ? 0.f : 1.f / sum;
@@ -458,7 +624,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 256 ? 2 : 3) attend_kernel(c
                 if constexpr (sizeof(T) == 4) {
                     *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
                 } else {
-                    T e[4] = {from_f<T>(f[0]), from_f<T>(f[1]), from_f<T>(f[2]), from_f<T>(f[3])};
+                    const T e[4] = {from_f<T>(f[0]), from_f<T>(f[1]), from_f<T>(f[2]), from_f<T>(f[3])};
                     *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(e);
                 }
             } else {
@@ -477,8 +643,10 @@ __global__ void __launch_bounds__(kWarps * 32, D == 256 ? 2 : 3) attend_kernel(c
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join_kernel(const Args x) {
     const Kv4Attn& a = x.a;
-    const int rr = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rb = blockIdx.x % x.row_blocks, kvh = blockIdx.x / x.row_blocks, req = blockIdx.y;
+    const int lane = threadIdx.x & 31, kRows = x.block_rows;
+    const int unit_row = blockIdx.x * 8 + (threadIdx.x >> 5);       // row of (kv head, row block)
+    const int rr = unit_row % kRows, ub = unit_row / kRows;
+    const int rb = ub % x.row_blocks, kvh = ub / x.row_blocks, req = blockIdx.y;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     Span sp;
     if (!span_of(x, req, rb, sp)) return;
@@ -487,7 +655,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Args x) {
     if (active == 1 || rw >= sp.q_len * x.group) return;
     const long unit = ((long)req * a.cache.n_kv_heads + kvh) * x.row_blocks + rb;
     const long at = unit * x.n_splits * kRows + rr;
-    float mx = -INFINITY;
+    float mx = kNone;
     for (int s = lane; s < active; s += 32) mx = fmaxf(mx, x.ml[at + (long)s * kRows].x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -498,7 +666,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Args x) {
 #pragma unroll 4
     for (int s = 0; s < active; s++) {
         const float2 ml = x.ml[at + (long)s * kRows];
-        const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - mx);
+        const float f = ex2(ml.x - mx);
         sum = fmaf(ml.y, f, sum);
         const float* v = x.part + (at + (long)s * kRows) * D + lane * kPer;
         float t[kPer];
@@ -515,33 +683,44 @@ __global__ void __launch_bounds__(256) join_kernel(const Args x) {
     if (a.lse && lane == 0) a.lse[(long)tk * a.n_heads + hd] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
-// How the long axis is split.  Blocks of at least 8 tiles (128 tokens), and about four times as many blocks as the GPU
-// holds at once: ragged lengths then even out, and the partial rows stay a few per cent of the cache bytes.
+// How the rows are blocked and the long axis is split.  Blocks of 16 rows where 16-bit queries have more than 8 (a tile's
+// codes are then unpacked for twice the rows).  Splits of at least 8 tiles (128 tokens), and about four times as many
+// blocks as the GPU holds at once: ragged lengths then even out, and the partial rows stay a few per cent of the cache bytes.
 void plan(const Kv4Attn& a, Args& x) {
     x.group = a.n_heads / a.cache.n_kv_heads;
-    x.row_blocks = (int)(((long)a.max_q * x.group + kRows - 1) / kRows);
+    const long rows = (long)a.max_q * x.group;
+    x.block_rows = a.dtype != kF32 && rows > 8 ? 16 : 8;
+    x.row_blocks = (int)((rows + x.block_rows - 1) / x.block_rows);
     const int tiles = std::max(1, (a.max_seq + kKvTile - 1) / kKvTile);
     int span = tiles;
     if (a.window > 0)   // the widest walk of one row block
-        span = (int)std::min<long>(tiles, ((long)a.window + std::min(a.max_q, kRows / x.group + 2)) / kKvTile + 2 +
+        span = (int)std::min<long>(tiles, ((long)a.window + std::min(a.max_q, x.block_rows / x.group + 2)) / kKvTile + 2 +
                                               ((long)a.sinks + kKvTile - 1) / kKvTile);
     const long units = (long)a.n_req * a.cache.n_kv_heads * x.row_blocks;
-    const long want = std::max<long>(1, 148L * 3 * 4 / units);
+    const long want = std::max<long>(1, 148L * 4 * 4 / units);
     const long per = std::max<long>(8, (span + want - 1) / want);
     x.tiles_per_split = (int)per;
     x.n_splits = (int)((span + per - 1) / per);
 }
 
+template <typename T, int D, int NT, bool SPLIT>
+void run_nt(const Args& x, cudaStream_t s) {
+    using S = Shape<D, NT>;
+    const int rows = SPLIT ? 8 : 8 * NT;
+    const int smem = std::max(kWarps * S::kStages * kv4_tile_bytes(D), kWarps * rows * (D * 4 + 8)) +
+                     (S::kQInSmem ? D / kKvGroup * NT * 32 * 16 : 0);
+    cudaFuncSetAttribute(attend_kernel<T, D, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const dim3 grid((unsigned)(x.n_splits * x.a.cache.n_kv_heads * x.row_blocks), (unsigned)x.a.n_req);
+    attend_kernel<T, D, NT, SPLIT><<<grid, kWarps * 32, smem, s>>>(x);
+}
 template <typename T, int D>
 void run(const Args& x, cudaStream_t s) {
-    const int smem = std::max(kWarps * kStages * kv4_tile_bytes(D), kWarps * kRows * D * 4 + kWarps * kRows * 8) +
-                     (D == 256 ? D / kKvGroup * 2 * 32 * 16 : 0);
-    cudaFuncSetAttribute(attend_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    const dim3 grid((unsigned)(x.n_splits * x.a.cache.n_kv_heads * x.row_blocks), (unsigned)x.a.n_req);
-    attend_kernel<T, D><<<grid, kWarps * 32, smem, s>>>(x);
+    if constexpr (sizeof(T) == 4) run_nt<T, D, 2, true>(x, s);
+    else if (x.block_rows == 16) run_nt<T, D, 2, false>(x, s);
+    else run_nt<T, D, 1, false>(x, s);
     if (x.n_splits == 1) return;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(x.a.cache.n_kv_heads * x.row_blocks), (unsigned)x.a.n_req);
+    cfg.gridDim = dim3((unsigned)(x.a.cache.n_kv_heads * x.row_blocks * x.block_rows / 8), (unsigned)x.a.n_req);
     cfg.blockDim = dim3(256);
     cfg.stream = s;
     cudaLaunchAttribute at{};
@@ -559,7 +738,7 @@ void run_d(const Args& x, cudaStream_t s) {
 }
 
 size_t part_bytes(const Kv4Attn& a, const Args& x) {
-    return (size_t)a.n_req * a.cache.n_kv_heads * x.row_blocks * x.n_splits * kRows * sizeof(float) * a.cache.head_dim;
+    return (size_t)a.n_req * a.cache.n_kv_heads * x.row_blocks * x.n_splits * x.block_rows * sizeof(float) * a.cache.head_dim;
 }
 
 }  // namespace
