@@ -27,9 +27,14 @@
 // The running maximum is raised only when a score exceeds it by more than 3 (log2): weights stay below 8, and most tiles
 // need neither the reduction over tokens nor the rescaling of the sums.
 //
-// Memory: a warp owns every kWarps-th tile of its split and copies tiles (20 D bytes, contiguous) into its own ring of
-// stages with cp.async, page ids fetched 32 tiles at a time.  The long axis is split over blocks when rows are few; a
-// second kernel joins the splits' partial sums (fixed order: results do not depend on timing).
+// Memory: a warp owns every kWarps-th tile of its block's run and copies tiles (20 D bytes, contiguous) into its own ring
+// of stages with cp.async, page ids fetched 32 tiles at a time.
+//
+// Work: a unit is a block of rows of one request and kv head.  Where every request is one block of rows (decode), the
+// tiles of all units form one sequence, cut into as many equal runs as the GPU holds blocks; a run crosses units, and a
+// unit that lies in several runs is joined by a second kernel from at most two partial sums per block.  Every block finds
+// its run itself, by a scan of the lengths.  Otherwise (chunks, or more requests than that scan takes) a block takes one
+// unit, or a split of it where units are few.  Sums are joined in a fixed order: results do not depend on timing.
 #include "kv4.cuh"
 
 #include <algorithm>
@@ -53,13 +58,33 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLoScale = 2048.f, kLoInv = 1.f / 2048.f;
 
+// n / d for 0 <= n < 2^31 by one high product: m = floor(2^(31 + l) / d) + 1 with 2^l >= d
+struct Div {
+    uint32_t m, s;
+    int d;
+};
+Div make_div(int d) {
+    int l = 0;
+    while ((1l << l) < d) l++;
+    return Div{d == 1 ? 0u : (uint32_t)(((uint64_t)1 << (31 + l)) / (uint32_t)d + 1), (uint32_t)(d == 1 ? 0 : l - 1), d};
+}
+__device__ __forceinline__ int operator/(int n, const Div& v) {
+    return v.d == 1 ? n : (int)(__umulhi((uint32_t)n, v.m) >> v.s);
+}
+
 struct Args {
     Kv4Attn a;
-    int tiles_per_split, n_splits, row_blocks, group;   // group: query heads of a kv head
-    int block_rows;
+    int row_blocks, block_rows;
+    int runs;                               // blocks of the run form (0: a block per unit and split)
+    int tiles_per_split, n_splits;          // of the other form
+    Div group;          // query heads of a kv head
+    Div page_tiles;     // tiles of a page
     bool wide_q, wide_o;
-    float* part;        // [unit][split][block_rows][D] sums, relative to the split's maximum
-    float2* ml;         // [unit][split][block_rows] maximum (log2 domain) and sum
+    // partial sums, relative to their own maximum, in slots of block_rows rows: [unit][split], or two for each run (of a
+    // unit that began in an earlier run, and of one that begins in it)
+    float* part;        // [slot][block_rows][D]
+    float2* ml;         // [slot][block_rows] maximum (log2 domain) and sum
+    int* before;        // [n_req + 1] tiles of one kv head before each request (run form; for the join)
 };
 
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
@@ -119,8 +144,10 @@ __device__ __forceinline__ uint32_t finite2(uint32_t z) {
     return z;
 }
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+// 16 bytes, of which the first `n` are read and the rest are zeros
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+                 "r"(n)
                  : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -159,14 +186,15 @@ __device__ __forceinline__ bool span_of(const Args& x, int req, int rb, Span& s)
     const int q1 = min(a.cu_q[req + 1], a.n_tokens);
     s.q0 = max(s.q0, 0);
     s.q_len = q1 - s.q0;
-    const int rows = s.q_len * x.group;
+    const int rows = s.q_len * x.group.d;
     if (rb * x.block_rows >= rows) return false;
     const long cap = min((long)a.table_width * a.cache.page_size, 1l << 30);
     s.seq = (int)min((long)max(a.seq_len[req], 0), cap);
     s.p_lo = s.seq - s.q_len + rb * x.block_rows / x.group;
     s.p_hi = s.seq - s.q_len + (min((rb + 1) * x.block_rows, rows) - 1) / x.group;
-    s.head = s.first = s.n = 0;
-    if (s.p_hi < 0) return true;   // nothing before any query: no tile
+    s.head = s.first = 0;
+    s.n = 1;
+    if (s.p_hi < 0) return true;   // nothing before any query: one tile, hidden from all of them
     const int last = s.p_hi / kKvTile;
     if (a.window > 0 && s.p_lo - a.window + 1 > 0) {
         s.first = (s.p_lo - a.window + 1) / kKvTile;
@@ -174,6 +202,39 @@ __device__ __forceinline__ bool span_of(const Args& x, int req, int rb, Span& s)
     }
     s.n = s.head + last - s.first + 1;
     return true;
+}
+
+constexpr int kRunReqs = 1024;      // requests that a block scans
+constexpr int kRunMin = 8;          // tiles of a run: two for each warp
+
+// tiles of a run, of `total`
+__device__ __forceinline__ int run_tiles(long total, int runs) { return (int)max((long)kRunMin, (total + runs - 1) / runs); }
+
+// before[r] = tiles of one kv head in the requests before r, for the whole block
+__device__ __forceinline__ void scan_requests(const Args& x, int* before) {
+    __shared__ int s_warp[kWarps];
+    const int tid = threadIdx.x, lane = tid & 31, n = x.a.n_req;
+    const int per = (n + kWarps * 32 - 1) / (kWarps * 32), lo = min(n, tid * per), hi = min(n, lo + per);
+    int sum = 0;
+    for (int r = lo; r < hi; r++) {
+        Span sp;
+        const int t = span_of(x, r, 0, sp) ? sp.n : 0;
+        before[r + 1] = t;
+        sum += t;
+    }
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+    }
+    if (lane == 31) s_warp[tid >> 5] = inc;
+    if (tid == 0) before[0] = 0;
+    __syncthreads();
+    int at = inc - sum;
+    for (int w = 0; w < tid >> 5; w++) at += s_warp[w];
+    for (int r = lo; r < hi; r++) before[r + 1] = at += before[r + 1];
+    __syncthreads();
 }
 
 // NT columns of 8: 8 NT query rows, or (SPLIT) the high and low halves of 8
@@ -190,452 +251,492 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_ker
     extern __shared__ __align__(16) uint8_t smem[];
     const Kv4Attn& a = x.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r8 = lane >> 2, q4 = lane & 3;
-    // the row blocks of one split are neighbours: they read the same tiles
-    const int rb = blockIdx.x % x.row_blocks, rest = blockIdx.x / x.row_blocks;
-    const int split = rest % x.n_splits, kvh = rest / x.n_splits, req = blockIdx.y;
+    __shared__ int s_before[kRunReqs + 1];
+    // the segment: tiles [begin, end) of a unit, and where its sums go if it is not the whole unit
+    int rb = 0, kvh, req, begin, end;
+    long slot, left = 0;      // left: tiles of the run behind this segment
     Span sp;
-    if (!span_of(x, req, rb, sp)) return;
-    const int active = min(x.n_splits, max(1, (sp.n + x.tiles_per_split - 1) / x.tiles_per_split));
-    if (split >= active) return;
-    const int begin = split * x.tiles_per_split;
-    const int end = split == x.n_splits - 1 ? sp.n : min(sp.n, begin + x.tiles_per_split);
-
-    uint8_t* ring = smem + warp * kStages * kTileB;
-    const int* table = a.table + (long)req * a.table_stride;
-    const int tiles_per_page = a.cache.page_size / kKvTile;
-
-    // this warp's tiles: idx = begin + warp + kWarps * i, i < count; where 32 of them lie (tile ordinal in the cache, or
-    // -1 for a page outside it), one per lane
-    const int mine = begin + warp;
-    const int count = mine < end ? (end - mine + kWarps - 1) / kWarps : 0;
-    auto tile_of = [&](int i) {
-        const int idx = mine + kWarps * i;
-        return idx < sp.head ? idx : sp.first + idx - sp.head;
-    };
-    auto fetch = [&](int i0) {
-        const int i = i0 + lane;
-        if (i >= count) return -1;
-        const int tile = tile_of(i), p = tile / tiles_per_page, page = table[p];
-        if (page < 0 || page >= a.cache.n_pages) return -1;
-        return (page * a.cache.n_kv_heads + kvh) * tiles_per_page + (tile - p * tiles_per_page);
-    };
-    int where = fetch(0), where_next = fetch(32);
-    uint32_t there = 0;   // bit j: the tile issued j calls ago has a page
-    const uint8_t* src0 = a.cache.pages + lane * 16;
-    uint8_t* dst0 = ring + lane * 16;
-    auto issue = [&](int i) {   // copy tile i into its stage
-        there <<= 1;
-        if (i < count) {
-            if ((i & 31) == 0 && i) {
-                where = where_next;
-                where_next = fetch(i + 32);
-            }
-            const int at = __shfl_sync(0xffffffffu, where, i & 31);
-            if (at >= 0) {
-                there |= 1;
-                const uint8_t* src = src0 + (size_t)at * kTileB;
-                uint8_t* dst = dst0 + (i % kStages) * kTileB;
-#pragma unroll
-                for (int c = 0; c < (kChunks + 31) / 32; c++)
-                    if (kChunks % 32 == 0 || c * 32 + lane < kChunks) cp_async16(dst + c * 512, src + c * 512);
-            }
+    bool whole;
+    if (x.runs) {
+        scan_requests(x, s_before);
+        const int heads = a.cache.n_kv_heads;
+        const long total = (long)s_before[a.n_req] * heads;
+        const int per = run_tiles(total, x.runs);
+        const long start = (long)blockIdx.x * per;
+        if (blockIdx.x == 0)
+            for (int i = tid; i <= a.n_req; i += kWarps * 32) x.before[i] = s_before[i];
+        if (start >= total) return;
+        int lo = 0, hi = a.n_req;
+        while (hi - lo > 1) {      // the last request that begins at or before the run
+            const int mid = (lo + hi) >> 1;
+            if ((long)s_before[mid] * heads <= start) lo = mid;
+            else hi = mid;
         }
-        cp_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; i++) issue(i);
+        req = lo;
+        const int n = s_before[req + 1] - s_before[req];
+        const int in = (int)(start - (long)s_before[req] * heads);
+        kvh = in / n;
+        begin = in - kvh * n;
+        left = min((long)per, total - start);
+    } else {
+        // the row blocks of one split are neighbours: they read the same tiles
+        const int split = blockIdx.x / x.row_blocks;
+        rb = blockIdx.x - split * x.row_blocks, kvh = blockIdx.y, req = blockIdx.z;
+        if (!span_of(x, req, rb, sp)) return;
+        const int active = min(x.n_splits, (sp.n + x.tiles_per_split - 1) / x.tiles_per_split);
+        if (split >= active) return;
+        begin = split * x.tiles_per_split;
+        end = split == x.n_splits - 1 ? sp.n : min(sp.n, begin + x.tiles_per_split);
+        whole = active == 1;
+        slot = (((long)req * a.cache.n_kv_heads + kvh) * x.row_blocks + rb) * x.n_splits + split;
+    }
 
-    // ---- the rows' queries as operand fragments: lane (r8, q4) has channels g*32 + q4*8 .. + 7 of row r8 (+ 8) ----
-    const int rows = sp.q_len * x.group, row0 = rb * kRows;
-    uint32_t* q_sm = reinterpret_cast<uint32_t*>(smem + kWarps * kStages * kTileB);   // [NG][NT][32 lanes][4]
-    uint32_t qf[S::kQInSmem ? 1 : NG][NT][4];    // two steps of 16 channels, two registers each
-    uint32_t qs[2][NT];                          // sums of groups 2 q4, 2 q4 + 1 of row r8: [high | low half]
-    float qk[ET][2];                             // score to log2 units, for the rows of this lane's sums: 2 q4, 2 q4 + 1
-    int pos_of[ET][2];
-#pragma unroll
-    for (int e = 0; e < ET; e++) {
-        const int row = row0 + e * 8 + r8;
-        const bool has_row = row < rows;
-        const int tok = has_row ? row / x.group : 0, head = kvh * x.group + (has_row ? row % x.group : 0);
-        const T* q = (const T*)a.q + (long)(sp.q0 + tok) * a.q_tok + (long)head * a.q_head + q4 * 8;
-        float v[NG][8];
-        float top = 0.f;
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            load_row<T, 8>(q + g * kKvGroup, x.wide_q, v[g]);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (!has_row) v[g][j] = 0.f;
-                top = fmaxf(top, fabsf(v[g][j]));
-            }
+    for (;;) {
+        if (x.runs) {
+            while (!span_of(x, req, 0, sp)) req++;      // requests without queries have no tiles
+            end = (int)min((long)sp.n, begin + left);
+            left -= end - begin;
+            whole = begin == 0 && end == sp.n;
+            slot = 2 * (long)blockIdx.x + (begin == 0);
         }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the power of two above the largest magnitude; zero, subnormal and huge rows keep a finite factor
-        int ex = (int)((__float_as_uint(top) >> 23) & 255) - 126;
-        ex = min(max(ex, -120), 120);
-        const float down = __uint_as_float((uint32_t)(127 - ex) << 23), up = __uint_as_float((uint32_t)(127 + ex) << 23);
-        const float my_qk = a.scale * kLog2e * up;
+        uint8_t* ring = smem + warp * kStages * kTileB;
+        const int* table = a.table + (long)req * a.table_stride;
+
+        // this warp's tiles: idx = begin + warp + kWarps * i, i < count; where 32 of them lie (tile ordinal in the cache, or
+        // -1 for a page outside it), one per lane
+        const int mine = begin + warp;
+        const int count = mine < end ? (end - mine + kWarps - 1) / kWarps : 0;
+        auto tile_of = [&](int i) {
+            const int idx = mine + kWarps * i;
+            return idx < sp.head ? idx : sp.first + idx - sp.head;
+        };
+        auto fetch = [&](int i0) {
+            const int i = i0 + lane;
+            if (i >= count) return -1;
+            const int tile = tile_of(i), p = tile / x.page_tiles, page = table[p];
+            if (page < 0 || page >= a.cache.n_pages) return -1;
+            return (page * a.cache.n_kv_heads + kvh) * x.page_tiles.d + (tile - p * x.page_tiles.d);
+        };
+        int where = fetch(0), where_next = fetch(32);
+        const uint8_t* src0 = a.cache.pages + lane * 16;
+        uint8_t* dst0 = ring + lane * 16;
+        // copy tile i, j of the current 32, into its stage; one without a page is filled with zeros
+        auto issue = [&](int i, int j) {
+            const int at = __shfl_sync(0xffffffffu, j < 32 ? where : where_next, j & 31);
+            const uint8_t* src = src0 + (size_t)max(at, 0) * kTileB;
+            uint8_t* dst = dst0 + (i % kStages) * kTileB;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            qk[e][j] = __shfl_sync(0xffffffffu, my_qk, (2 * q4 + j) * 4);
-            pos_of[e][j] = sp.seq - sp.q_len + (row0 + e * 8 + 2 * q4 + j) / x.group;
-        }
-        qs[0][e] = qs[1][e] = 0;
-        if constexpr (SPLIT) qs[0][1] = qs[1][1] = 0;
+            for (int c = 0; c < (kChunks + 31) / 32; c++)
+                if (kChunks % 32 == 0 || c * 32 + lane < kChunks) cp_async16(dst + c * 512, src + c * 512, at >= 0 ? 16 : 0);
+            cp_commit();
+        };
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-            float t = 0.f;
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                v[g][j] *= down;
-                t += v[g][j];
-            }
-#pragma unroll
-            for (int st = 0; st < 2; st++) {
-                split2(v[g][2 * st], v[g][2 * st + 4], hi[2 * st], lo[2 * st]);
-                split2(v[g][2 * st + 1] * 0.0625f, v[g][2 * st + 5] * 0.0625f, hi[2 * st + 1], lo[2 * st + 1]);
-            }
-            if constexpr (S::kQInSmem) {
-                if (warp == 0) {
-                    reinterpret_cast<uint4*>(q_sm)[(g * NT + e) * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if constexpr (SPLIT)
-                        reinterpret_cast<uint4*>(q_sm)[(g * NT + 1) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                }
+        for (int i = 0; i < kStages - 1; i++) issue(i, i);
+
+        // ---- the rows' queries as operand fragments, made once for the block: a thread takes 8 channels of a row ----
+        const int rows = sp.q_len * x.group.d, row0 = rb * kRows;
+        uint8_t* q_at = smem + kWarps * kStages * kTileB;
+        uint4* q_sm = reinterpret_cast<uint4*>(q_at);                                       // [NG][NT][32 lanes]
+        __half* qs_sm = reinterpret_cast<__half*>(q_at + NG * NT * 512);                    // [high, low][NT][32 lanes][2]
+        float* qk_sm = reinterpret_cast<float*>(q_at + NG * NT * 512 + 2 * NT * 128);       // [kRows]
+        for (int i = tid; i < kRows * (D / 8); i += kWarps * 32) {   // whole warps, and a row within one
+            const int rr = i / (D / 8), c8 = i % (D / 8), row = row0 + rr;
+            float v[8];
+            if (row < rows) {
+                const int tok = row / x.group, head = kvh * x.group.d + row - tok * x.group.d;
+                load_row<T, 8>((const T*)a.q + (long)(sp.q0 + tok) * a.q_tok + (long)head * a.q_head + c8 * 8, x.wide_q, v);
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    qf[g][e][j] = hi[j];
-                    if constexpr (SPLIT) qf[g][1][j] = lo[j];
-                }
+                for (int j = 0; j < 8; j++) v[j] = 0.f;
+            }
+            float top = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(v[j]));
+#pragma unroll
+            for (int o = 1; o < D / 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            // the power of two above the largest magnitude; zero, subnormal and huge rows keep a finite factor
+            int ex = (int)((__float_as_uint(top) >> 23) & 255) - 126;
+            ex = min(max(ex, -120), 120);
+            const float down = __uint_as_float((uint32_t)(127 - ex) << 23), up = __uint_as_float((uint32_t)(127 + ex) << 23);
+            float t = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                v[j] *= down;
+                t += v[j];
             }
             t += __shfl_xor_sync(0xffffffffu, t, 1);
             t += __shfl_xor_sync(0xffffffffu, t, 2);
-            uint32_t th, tl;
-            split2(t, 0.f, th, tl);
-            if (q4 == g / 2) {
-                qs[0][e] |= (th & 0xffffu) << (16 * (g & 1));
-                qs[1][e] |= (tl & 0xffffu) << (16 * (g & 1));
+            uint32_t hi[4], lo[4];   // two steps of 16 channels: pairs (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                split2(v[2 * st], v[2 * st + 4], hi[2 * st], lo[2 * st]);
+                split2(v[2 * st + 1] * 0.0625f, v[2 * st + 5] * 0.0625f, hi[2 * st + 1], lo[2 * st + 1]);
             }
+            const int e = rr >> 3, g = c8 >> 2, ln = (rr & 7) * 4 + (c8 & 3);
+            q_sm[(g * NT + e) * 32 + ln] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (SPLIT) q_sm[(g * NT + 1) * 32 + ln] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            if ((c8 & 3) == 0) {     // the group's sum: columns g of the offsets' product lie in lane g / 2 of the row
+                uint32_t th, tl;
+                split2(t, 0.f, th, tl);
+                const int at = (e * 32 + (rr & 7) * 4 + (g >> 1)) * 2 + (g & 1);
+                qs_sm[at] = __ushort_as_half((uint16_t)th);
+                qs_sm[NT * 64 + at] = __ushort_as_half((uint16_t)tl);
+            }
+            if (c8 == 0) qk_sm[rr] = a.scale * kLog2e * up;
         }
-    }
-    if constexpr (S::kQInSmem) __syncthreads();
-
-    float acc[NT][NG][2][4];      // channels g*32 + r8*4 + {0, 1 | 2, 3} x rows 2 q4, 2 q4 + 1
-    float zacc[NT][4];            // group r8 x rows 2 q4, 2 q4 + 1 (the last two are not used)
-    float m[ET][2], l[ET][2];
+        __syncthreads();
+        uint32_t qf[S::kQInSmem ? 1 : NG][NT][4];
+        uint32_t qs[2][ET];          // sums of groups 2 q4, 2 q4 + 1 of row r8: high and low halves
+        float qk[ET][2];             // score to log2 units, for the rows of this lane's sums: 2 q4, 2 q4 + 1
+        int pos_of[ET][2];
+        if constexpr (!S::kQInSmem) {
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
+            for (int g = 0; g < NG; g++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) zacc[n][j] = 0.f;
+                for (int n = 0; n < NT; n++) load_words<4>(q_sm + (g * NT + n) * 32 + lane, qf[g][n]);
+        }
 #pragma unroll
-        for (int g = 0; g < NG; g++)
+        for (int e = 0; e < ET; e++) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) acc[n][g][j >> 2][j & 3] = 0.f;
-    }
+            for (int h = 0; h < 2; h++)
+                qs[h][e] = 2 * q4 < NG ? reinterpret_cast<const uint32_t*>(qs_sm)[(h * NT + e) * 32 + lane] : 0u;
 #pragma unroll
-    for (int e = 0; e < ET; e++) m[e][0] = m[e][1] = kNone, l[e][0] = l[e][1] = 0.f;
-    const int odd_shift = (r8 & 1) * 16;
-
-    for (int i = 0; i < count; i++) {
-        cp_wait<kStages - 2>();
-        __syncwarp();
-        issue(i + kStages - 1);   // into the stage that the previous step finished with (the barrier above)
-        if (!((there >> (kStages - 1)) & 1)) continue;
-        const uint8_t* t = ring + (i % kStages) * kTileB;
-        const int base = tile_of(i) * kKvTile;
-
-        // ---- scores: tokens r8, r8 + 8 x rows 2 q4, 2 q4 + 1 of each column ----
-        float sc[ET][4];
-        {
-            uint32_t w0[NG], w1[NG], k0[NG], k1[NG];
-            load_words<NG>(t + (r8 * 4 + q4) * NG * 4, w0);
-            load_words<NG>(t + ((r8 + 8) * 4 + q4) * NG * 4, w1);
-            load_words<NG>(t + kv4_off_ks(D) + (r8 >> 1) * NG * 4, k0);
-            load_words<NG>(t + kv4_off_ks(D) + ((r8 >> 1) + 4) * NG * 4, k1);
-            uint32_t m0 = 0, m1 = 0;
-            if (2 * q4 < NG) {
-                m0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_km(D) + (r8 * NG + 2 * q4) * 2);
-                m1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_km(D) + ((r8 + 8) * NG + 2 * q4) * 2);
-            }
-            float s[ET][4];
-#pragma unroll
-            for (int e = 0; e < ET; e++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) s[e][j] = 0.f;
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const uint32_t x0 = w0[g] >> 8, x1 = w1[g] >> 8;
-                uint32_t c0[4] = {w0[g] & 0x000f000fu, w1[g] & 0x000f000fu, w0[g] & 0x00f000f0u, w1[g] & 0x00f000f0u};
-                uint32_t c1[4] = {x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u};
-                if constexpr (SPLIT) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) c0[j] = mul2(c0[j], kTwo15), c1[j] = mul2(c1[j], kTwo15);
-                }
-                float c[NT][4];
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    uint32_t f[4];
-                    if constexpr (S::kQInSmem) {
-                        load_words<4>(q_sm + ((g * NT + n) * 32 + lane) * 4, f);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; j++) f[j] = qf[g][n][j];
-                    }
-                    mma16(c[n], c0, f[0], f[1], 0.f, 0.f, 0.f, 0.f);
-                    mma16(c[n], c1, f[2], f[3]);
-                }
-                const float s0 = __half2float(__ushort_as_half((uint16_t)(k0[g] >> odd_shift)));
-                const float s1 = __half2float(__ushort_as_half((uint16_t)(k1[g] >> odd_shift)));
-#pragma unroll
-                for (int e = 0; e < ET; e++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float d = SPLIT ? fmaf(c[NT - 1][j], kLoInv, c[e][j]) : c[e][j];
-                        s[e][j] = fmaf(j < 2 ? s0 : s1, d, s[e][j]);
-                    }
-            }
-#pragma unroll
-            for (int e = 0; e < ET; e++) {
-                float z[4];
-                mma8(z, m0, m1, qs[0][e]);
-                float y[4];
-                mma8(y, m0, m1, qs[1][e]);
-#pragma unroll
-                for (int j = 0; j < 4; j++) z[j] = fmaf(y[j], kLoInv, z[j]);
-#pragma unroll
-                for (int j = 0; j < 4; j++) sc[e][j] = fmaf(s[e][j], SPLIT ? 512.f : 16777216.f, z[j]);
+            for (int j = 0; j < 2; j++) {
+                qk[e][j] = qk_sm[e * 8 + 2 * q4 + j];
+                pos_of[e][j] = sp.seq - sp.q_len + (row0 + e * 8 + 2 * q4 + j) / x.group;
             }
         }
 
-        // ---- exponents relative to the running maximum; masks only where some row sees a part of the tile ----
-        const bool part = base + kKvTile - 1 > sp.p_lo ||
-                          (a.window > 0 && base <= sp.p_hi - a.window && base + kKvTile > a.sinks);
-        float ex[ET][4];
-        auto exponents = [&]() {
+        float acc[NT][NG][2][4];      // channels g*32 + r8*4 + {0, 1 | 2, 3} x rows 2 q4, 2 q4 + 1
+        float zacc[NT][4];            // group r8 x rows 2 q4, 2 q4 + 1 (the last two are not used)
+        float m[ET][2], l[ET][2];
 #pragma unroll
-            for (int e = 0; e < ET; e++)
+        for (int n = 0; n < NT; n++) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) ex[e][j] = fmaf(sc[e][j], qk[e][j & 1], -m[e][j & 1]);
-            if (part) {
+            for (int j = 0; j < 4; j++) zacc[n][j] = 0.f;
+#pragma unroll
+            for (int g = 0; g < NG; g++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) acc[n][g][j >> 2][j & 3] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < ET; e++) m[e][0] = m[e][1] = kNone, l[e][0] = l[e][1] = 0.f;
+        const int odd_shift = (r8 & 1) * 16;
+
+        // one tile, with masks where some row sees a part of it only
+        auto tile = [&](const uint8_t* t, const int base, auto masked) {
+            constexpr bool part = decltype(masked)::value;
+            // ---- scores: tokens r8, r8 + 8 x rows 2 q4, 2 q4 + 1 of each column ----
+            float sc[ET][4];
+            {
+                uint32_t w0[NG], w1[NG], k0[NG], k1[NG];
+                load_words<NG>(t + (r8 * 4 + q4) * NG * 4, w0);
+                load_words<NG>(t + ((r8 + 8) * 4 + q4) * NG * 4, w1);
+                load_words<NG>(t + kv4_off_ks(D) + (r8 >> 1) * NG * 4, k0);
+                load_words<NG>(t + kv4_off_ks(D) + ((r8 >> 1) + 4) * NG * 4, k1);
+                uint32_t m0 = 0, m1 = 0;
+                if (2 * q4 < NG) {
+                    m0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_km(D) + (r8 * NG + 2 * q4) * 2);
+                    m1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_km(D) + ((r8 + 8) * NG + 2 * q4) * 2);
+                }
+                float s[ET][4];
 #pragma unroll
                 for (int e = 0; e < ET; e++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int pos = base + r8 + (j >> 1) * 8, p = pos_of[e][j & 1];
-                        if (pos > p || (a.window > 0 && pos <= p - a.window && pos >= a.sinks)) ex[e][j] = -INFINITY;
+                    for (int j = 0; j < 4; j++) s[e][j] = 0.f;
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const uint32_t x0 = w0[g] >> 8, x1 = w1[g] >> 8;
+                    uint32_t c0[4] = {w0[g] & 0x000f000fu, w1[g] & 0x000f000fu, w0[g] & 0x00f000f0u, w1[g] & 0x00f000f0u};
+                    uint32_t c1[4] = {x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u};
+                    if constexpr (SPLIT) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) c0[j] = mul2(c0[j], kTwo15), c1[j] = mul2(c1[j], kTwo15);
                     }
-            }
-        };
-        exponents();
-        float top = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < ET; e++) top = fmaxf(top, fmaxf(fmaxf(ex[e][0], ex[e][1]), fmaxf(ex[e][2], ex[e][3])));
-        if (__any_sync(0xffffffffu, top > kSlack)) {
-#pragma unroll
-            for (int e = 0; e < ET; e++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    float now = fmaxf(ex[e][j] == -INFINITY ? -INFINITY : sc[e][j] * qk[e][j],
-                                      ex[e][j + 2] == -INFINITY ? -INFINITY : sc[e][j + 2] * qk[e][j]);
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
-                    now = fmaxf(m[e][j], now);
-                    const float f = ex2(m[e][j] - now);
-                    m[e][j] = now;
-                    l[e][j] *= f;
+                    float c[NT][4];
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
-                        if (!SPLIT && n != e) continue;
-                        zacc[n][j] *= f;
+                        uint32_t f[4];
+                        if constexpr (S::kQInSmem) {
+                            load_words<4>(q_sm + (g * NT + n) * 32 + lane, f);
+                        } else {
 #pragma unroll
-                        for (int g = 0; g < NG; g++) {
-                            acc[n][g][0][j] *= f;
-                            acc[n][g][0][j + 2] *= f;
-                            acc[n][g][1][j] *= f;
-                            acc[n][g][1][j + 2] *= f;
+                            for (int j = 0; j < 4; j++) f[j] = qf[g][n][j];
+                        }
+                        mma16(c[n], c0, f[0], f[1], 0.f, 0.f, 0.f, 0.f);
+                        mma16(c[n], c1, f[2], f[3]);
+                    }
+                    const float s0 = __half2float(__ushort_as_half((uint16_t)(k0[g] >> odd_shift)));
+                    const float s1 = __half2float(__ushort_as_half((uint16_t)(k1[g] >> odd_shift)));
+#pragma unroll
+                    for (int e = 0; e < ET; e++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const float d = SPLIT ? fmaf(c[NT - 1][j], kLoInv, c[e][j]) : c[e][j];
+                            s[e][j] = fmaf(j < 2 ? s0 : s1, d, s[e][j]);
+                        }
+                }
+#pragma unroll
+                for (int e = 0; e < ET; e++) {
+                    float z[4];
+                    mma8(z, m0, m1, qs[0][e]);
+                    float y[4];
+                    mma8(y, m0, m1, qs[1][e]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) z[j] = fmaf(y[j], kLoInv, z[j]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) sc[e][j] = fmaf(s[e][j], SPLIT ? 512.f : 16777216.f, z[j]);
+                }
+            }
+
+            // ---- exponents relative to the running maximum ----
+            float ex[ET][4];
+            auto exponents = [&]() {
+#pragma unroll
+                for (int e = 0; e < ET; e++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) ex[e][j] = fmaf(sc[e][j], qk[e][j & 1], -m[e][j & 1]);
+                if constexpr (part) {
+#pragma unroll
+                    for (int e = 0; e < ET; e++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int pos = base + r8 + (j >> 1) * 8, p = pos_of[e][j & 1];
+                            if (pos > p || (a.window > 0 && pos <= p - a.window && pos >= a.sinks)) ex[e][j] = -INFINITY;
+                        }
+                }
+            };
+            exponents();
+            float top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < ET; e++) top = fmaxf(top, fmaxf(fmaxf(ex[e][0], ex[e][1]), fmaxf(ex[e][2], ex[e][3])));
+            if (__any_sync(0xffffffffu, top > kSlack)) {
+#pragma unroll
+                for (int e = 0; e < ET; e++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        float now = fmaxf(ex[e][j] == -INFINITY ? -INFINITY : sc[e][j] * qk[e][j],
+                                          ex[e][j + 2] == -INFINITY ? -INFINITY : sc[e][j + 2] * qk[e][j]);
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+                        now = fmaxf(m[e][j], now);
+                        const float f = ex2(m[e][j] - now);
+                        m[e][j] = now;
+                        l[e][j] *= f;
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            if (!SPLIT && n != e) continue;
+                            zacc[n][j] *= f;
+#pragma unroll
+                            for (int g = 0; g < NG; g++) {
+                                acc[n][g][0][j] *= f;
+                                acc[n][g][0][j + 2] *= f;
+                                acc[n][g][1][j] *= f;
+                                acc[n][g][1][j + 2] *= f;
+                            }
                         }
                     }
-                }
-            exponents();
-        }
+                exponents();
+            }
 
-        // ---- weights, to the layout of the second product: row r8 x tokens 2 q4, + 1 (lo: of 16) and 2 q4 + 8, + 9 ----
-        uint32_t ph[ET][2], pl[ET][2];
-#pragma unroll
-        for (int e = 0; e < ET; e++) {
-            float p[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) p[j] = ex2(ex[e][j]);
-            l[e][0] += p[0] + p[2];
-            l[e][1] += p[1] + p[3];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if constexpr (SPLIT || kFp16) {
-                    split2(p[2 * h], p[2 * h + 1], ph[e][h], pl[e][h]);
-                    pl[e][h] = transpose(pl[e][h]);
-                } else {
-                    ph[e][h] = pack(p[2 * h], p[2 * h + 1]);
-                }
-                ph[e][h] = transpose(ph[e][h]);
-            }
-        }
-
-        // ---- output: scales into the weights, codes of V, offsets ----
-        uint32_t v0[NG], v1[NG], s0[NG], s1[NG];
-        load_words<NG>(t + kv4_off_vc(D) + (q4 * 8 + r8) * NG * 4, v0);
-        load_words<NG>(t + kv4_off_vc(D) + ((q4 + 4) * 8 + r8) * NG * 4, v1);
-        load_words<NG>(t + kv4_off_vs(D) + q4 * NG * 4, s0);
-        load_words<NG>(t + kv4_off_vs(D) + (q4 + 4) * NG * 4, s1);
-        {
-            uint32_t z0 = 0, z1 = 0, y0 = 0, y1 = 0;
-            if (r8 < NG) {
-                z0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vm(D) + (q4 * NG + r8) * 4);
-                z1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vm(D) + ((q4 + 4) * NG + r8) * 4);
-                y0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vs(D) + (q4 * NG + r8) * 4);
-                y1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vs(D) + ((q4 + 4) * NG + r8) * 4);
-            }
-            if (part) {
-                // a hidden token's bytes may hold anything: infinities and NaN must not meet its weight of zero.  A stored
-                // token that is not finite has a NaN scale, which still reaches the rows that do see it below.
-                z0 = finite2(z0), z1 = finite2(z1), y0 = finite2(y0), y1 = finite2(y1);
-            }
-            const uint32_t za[4] = {z0, z0, z1, z1}, ya[4] = {y0, y0, y1, y1};   // rows 8 .. 15: not used
+            // ---- weights, to the layout of the second product: row r8 x tokens 2 q4, + 1 (lo: of 16) and 2 q4 + 8, + 9 ----
+            uint32_t ph[ET][2], pl[ET][2];
 #pragma unroll
             for (int e = 0; e < ET; e++) {
-                const uint32_t minus_half = 0xb800b800u;
-                mma16(zacc[e], za, ph[e][0], ph[e][1]);
-                mma16(zacc[e], ya, mul2(ph[e][0], minus_half), mul2(ph[e][1], minus_half));
-                if constexpr (SPLIT) {
-                    mma16(zacc[1], za, pl[e][0], pl[e][1]);
-                    mma16(zacc[1], ya, mul2(pl[e][0], minus_half), mul2(pl[e][1], minus_half));
+                float p[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) p[j] = ex2(ex[e][j]);
+                l[e][0] += p[0] + p[2];
+                l[e][1] += p[1] + p[3];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if constexpr (SPLIT || kFp16) {
+                        split2(p[2 * h], p[2 * h + 1], ph[e][h], pl[e][h]);
+                        pl[e][h] = transpose(pl[e][h]);
+                    } else {
+                        ph[e][h] = pack(p[2 * h], p[2 * h + 1]);
+                    }
+                    ph[e][h] = transpose(ph[e][h]);
                 }
             }
-        }
-        uint32_t b[NT][NG][2];
+
+            // ---- output: scales into the weights, codes of V, offsets ----
+            uint32_t v0[NG], v1[NG], s0[NG], s1[NG];
+            load_words<NG>(t + kv4_off_vc(D) + (q4 * 8 + r8) * NG * 4, v0);
+            load_words<NG>(t + kv4_off_vc(D) + ((q4 + 4) * 8 + r8) * NG * 4, v1);
+            load_words<NG>(t + kv4_off_vs(D) + q4 * NG * 4, s0);
+            load_words<NG>(t + kv4_off_vs(D) + (q4 + 4) * NG * 4, s1);
+            {
+                uint32_t z0 = 0, z1 = 0, y0 = 0, y1 = 0;
+                if (r8 < NG) {
+                    z0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vm(D) + (q4 * NG + r8) * 4);
+                    z1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vm(D) + ((q4 + 4) * NG + r8) * 4);
+                    y0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vs(D) + (q4 * NG + r8) * 4);
+                    y1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vs(D) + ((q4 + 4) * NG + r8) * 4);
+                }
+                if constexpr (part) {
+                    // a hidden token's bytes may hold anything: infinities and NaN must not meet its weight of zero.  A stored
+                    // token that is not finite has a NaN scale, which still reaches the rows that do see it below.
+                    z0 = finite2(z0), z1 = finite2(z1), y0 = finite2(y0), y1 = finite2(y1);
+                }
+                const uint32_t za[4] = {z0, z0, z1, z1}, ya[4] = {y0, y0, y1, y1};   // rows 8 .. 15: not used
 #pragma unroll
-        for (int e = 0; e < ET; e++) {
-            uint32_t u0[NG], u1[NG];   // the scales, 0 where a weight is: they may not be finite
-#pragma unroll
-            for (int g = 0; g < NG; g++) u0[g] = s0[g], u1[g] = s1[g];
-            if (part) {
-                const uint32_t any0 = SPLIT || kFp16 ? ph[e][0] | pl[e][0] : ph[e][0];
-                const uint32_t any1 = SPLIT || kFp16 ? ph[e][1] | pl[e][1] : ph[e][1];
-                const uint32_t k0 = (any0 & 0x7fffu ? 0xffffu : 0u) | (any0 & 0x7fff0000u ? 0xffff0000u : 0u);
-                const uint32_t k1 = (any1 & 0x7fffu ? 0xffffu : 0u) | (any1 & 0x7fff0000u ? 0xffff0000u : 0u);
-#pragma unroll
-                for (int g = 0; g < NG; g++) u0[g] &= k0, u1[g] &= k1;
-            }
-            if constexpr (SPLIT || kFp16) {
-                const float2 h0 = halves(ph[e][0]), h1 = halves(ph[e][1]), l0 = halves(pl[e][0]), l1 = halves(pl[e][1]);
-                const float p0 = fmaf(l0.x, kLoInv, h0.x), p1 = fmaf(l0.y, kLoInv, h0.y);
-                const float p2 = fmaf(l1.x, kLoInv, h1.x), p3 = fmaf(l1.y, kLoInv, h1.y);
-#pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    const float2 a0 = halves(u0[g]), a1 = halves(u1[g]);
+                for (int e = 0; e < ET; e++) {
+                    const uint32_t minus_half = 0xb800b800u;
+                    mma16(zacc[e], za, ph[e][0], ph[e][1]);
+                    mma16(zacc[e], ya, mul2(ph[e][0], minus_half), mul2(ph[e][1], minus_half));
                     if constexpr (SPLIT) {
-                        split2(p0 * a0.x, p1 * a0.y, b[0][g][0], b[NT - 1][g][0]);
-                        split2(p2 * a1.x, p3 * a1.y, b[0][g][1], b[NT - 1][g][1]);
-                    } else {
-                        b[e][g][0] = pack(p0 * a0.x, p1 * a0.y);
-                        b[e][g][1] = pack(p2 * a1.x, p3 * a1.y);
+                        mma16(zacc[1], za, pl[e][0], pl[e][1]);
+                        mma16(zacc[1], ya, mul2(pl[e][0], minus_half), mul2(pl[e][1], minus_half));
                     }
                 }
-            } else {
+            }
+            uint32_t b[NT][NG][2];
 #pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    b[e][g][0] = mul2(ph[e][0], u0[g]);
-                    b[e][g][1] = mul2(ph[e][1], u1[g]);
+            for (int e = 0; e < ET; e++) {
+                uint32_t u0[NG], u1[NG];   // the scales, 0 where a weight is: they may not be finite
+#pragma unroll
+                for (int g = 0; g < NG; g++) u0[g] = s0[g], u1[g] = s1[g];
+                if constexpr (part) {
+                    const uint32_t any0 = SPLIT || kFp16 ? ph[e][0] | pl[e][0] : ph[e][0];
+                    const uint32_t any1 = SPLIT || kFp16 ? ph[e][1] | pl[e][1] : ph[e][1];
+                    const uint32_t k0 = (any0 & 0x7fffu ? 0xffffu : 0u) | (any0 & 0x7fff0000u ? 0xffff0000u : 0u);
+                    const uint32_t k1 = (any1 & 0x7fffu ? 0xffffu : 0u) | (any1 & 0x7fff0000u ? 0xffff0000u : 0u);
+#pragma unroll
+                    for (int g = 0; g < NG; g++) u0[g] &= k0, u1[g] &= k1;
+                }
+                if constexpr (SPLIT || kFp16) {
+                    const float2 h0 = halves(ph[e][0]), h1 = halves(ph[e][1]), l0 = halves(pl[e][0]), l1 = halves(pl[e][1]);
+                    const float p0 = fmaf(l0.x, kLoInv, h0.x), p1 = fmaf(l0.y, kLoInv, h0.y);
+                    const float p2 = fmaf(l1.x, kLoInv, h1.x), p3 = fmaf(l1.y, kLoInv, h1.y);
+#pragma unroll
+                    for (int g = 0; g < NG; g++) {
+                        const float2 a0 = halves(u0[g]), a1 = halves(u1[g]);
+                        if constexpr (SPLIT) {
+                            split2(p0 * a0.x, p1 * a0.y, b[0][g][0], b[NT - 1][g][0]);
+                            split2(p2 * a1.x, p3 * a1.y, b[0][g][1], b[NT - 1][g][1]);
+                        } else {
+                            b[e][g][0] = pack(p0 * a0.x, p1 * a0.y);
+                            b[e][g][1] = pack(p2 * a1.x, p3 * a1.y);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int g = 0; g < NG; g++) {
+                        b[e][g][0] = mul2(ph[e][0], u0[g]);
+                        b[e][g][1] = mul2(ph[e][1], u1[g]);
+                    }
                 }
             }
-        }
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            const uint32_t x0 = v0[g] >> 8, x1 = v1[g] >> 8;
-            const uint32_t c0[4] = {centred(v0[g] & 0x000f000fu, false), centred(v0[g] & 0x00f000f0u, true),
-                                    centred(v1[g] & 0x000f000fu, false), centred(v1[g] & 0x00f000f0u, true)};
-            const uint32_t c1[4] = {centred(x0 & 0x000f000fu, false), centred(x0 & 0x00f000f0u, true),
-                                    centred(x1 & 0x000f000fu, false), centred(x1 & 0x00f000f0u, true)};
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                mma16(acc[n][g][0], c0, b[n][g][0], b[n][g][1]);
-                mma16(acc[n][g][1], c1, b[n][g][0], b[n][g][1]);
-            }
-        }
-    }
-    cp_wait<0>();
-#pragma unroll
-    for (int e = 0; e < ET; e++)
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) l[e][j] += __shfl_xor_sync(0xffffffffu, l[e][j], o);
-
-    // ---- join the warps: their rows meet in shared memory (over the finished ring) ----
-    __syncthreads();
-    float* s_o = reinterpret_cast<float*>(smem);                                   // [kWarps][kRows][D]
-    float2* s_ml = reinterpret_cast<float2*>(smem + kWarps * kRows * D * 4);       // [kWarps][kRows]
-#pragma unroll
-    for (int e = 0; e < ET; e++)
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int rr = warp * kRows + e * 8 + 2 * q4 + j;
-            const float z = SPLIT ? fmaf(zacc[NT - 1][j], kLoInv, zacc[e][j]) : zacc[e][j];
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                const float zg = __shfl_sync(0xffffffffu, z, g * 4 + q4);
-                float o[4];
+                const uint32_t x0 = v0[g] >> 8, x1 = v1[g] >> 8;
+                const uint32_t c0[4] = {centred(v0[g] & 0x000f000fu, false), centred(v0[g] & 0x00f000f0u, true),
+                                        centred(v1[g] & 0x000f000fu, false), centred(v1[g] & 0x00f000f0u, true)};
+                const uint32_t c1[4] = {centred(x0 & 0x000f000fu, false), centred(x0 & 0x00f000f0u, true),
+                                        centred(x1 & 0x000f000fu, false), centred(x1 & 0x00f000f0u, true)};
 #pragma unroll
-                for (int k = 0; k < 4; k++) {   // channel g*32 + r8*4 + k
-                    const float v = SPLIT ? fmaf(acc[NT - 1][g][k >> 1][j + 2 * (k & 1)], kLoInv, acc[e][g][k >> 1][j + 2 * (k & 1)])
-                                          : acc[e][g][k >> 1][j + 2 * (k & 1)];
-                    o[k] = fmaf(v, k & 1 ? 32.f : 512.f, zg);
+                for (int n = 0; n < NT; n++) {
+                    mma16(acc[n][g][0], c0, b[n][g][0], b[n][g][1]);
+                    mma16(acc[n][g][1], c1, b[n][g][0], b[n][g][1]);
                 }
-                *reinterpret_cast<float4*>(s_o + rr * D + g * kKvGroup + r8 * 4) = make_float4(o[0], o[1], o[2], o[3]);
             }
-            if (r8 == 0) s_ml[rr] = make_float2(m[e][j], l[e][j]);
+        };
+
+        for (int i0 = 0; i0 < count; i0 += 32) {
+            const int nj = min(32, count - i0);
+            for (int j = 0; j < nj; j++) {
+                const int i = i0 + j;
+                cp_wait<kStages - 2>();
+                __syncwarp();
+                issue(i + kStages - 1, j + kStages - 1);   // into the stage that the previous step finished with (the barrier)
+                const bool there = __shfl_sync(0xffffffffu, where, j) >= 0;
+                const int base = there ? tile_of(i) * kKvTile : 1 << 30;   // without a page: behind every query
+                const bool part = base + kKvTile - 1 > sp.p_lo ||
+                                  (a.window > 0 && base <= sp.p_hi - a.window && base + kKvTile > a.sinks);
+                const uint8_t* t = ring + (i % kStages) * kTileB;
+                if (part) tile(t, base, std::true_type{});
+                else tile(t, base, std::false_type{});
+            }
+            where = where_next;
+            where_next = fetch(i0 + 64);
         }
-    __syncthreads();
-    const long unit = ((long)req * a.cache.n_kv_heads + kvh) * x.row_blocks + rb;
-    for (int i = tid; i < kRows * D / 4; i += kWarps * 32) {
-        const int rr = i / (D / 4), c4 = i % (D / 4);
-        const int rw = row0 + rr;
-        if (rw >= rows) break;
-        float mx = kNone;
+        cp_wait<0>();
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) mx = fmaxf(mx, s_ml[w * kRows + rr].x);
-        float sum = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int e = 0; e < ET; e++)
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) {
-            const float2 ml = s_ml[w * kRows + rr];
-            const float f = ex2(ml.x - mx);
-            sum = fmaf(ml.y, f, sum);
-            const float4 v = reinterpret_cast<const float4*>(s_o + (w * kRows + rr) * D)[c4];
-            o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
-        }
-        if (active == 1) {
-            const int tk = sp.q0 + rw / x.group, hd = kvh * x.group + rw % x.group;
-            const float n = sum == 0.f ? 0.f : 1.f / sum;
-            const float f[4] = {o.x * n, o.y * n, o.z * n, o.w * n};
-            T* dst = (T*)a.out + (long)tk * a.o_tok + (long)hd * a.o_head + c4 * 4;
-            if (x.wide_o) {
-                if constexpr (sizeof(T) == 4) {
-                    *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l[e][j] += __shfl_xor_sync(0xffffffffu, l[e][j], o);
+
+        // ---- join the warps: their rows meet in shared memory (over the finished ring) ----
+        __syncthreads();
+        float* s_o = reinterpret_cast<float*>(smem);                                   // [kWarps][kRows][D]
+        float2* s_ml = reinterpret_cast<float2*>(smem + kWarps * kRows * D * 4);       // [kWarps][kRows]
+#pragma unroll
+        for (int e = 0; e < ET; e++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int rr = warp * kRows + e * 8 + 2 * q4 + j;
+                const float z = SPLIT ? fmaf(zacc[NT - 1][j], kLoInv, zacc[e][j]) : zacc[e][j];
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const float zg = __shfl_sync(0xffffffffu, z, g * 4 + q4);
+                    float o[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {   // channel g*32 + r8*4 + k
+                        const float v = SPLIT ? fmaf(acc[NT - 1][g][k >> 1][j + 2 * (k & 1)], kLoInv, acc[e][g][k >> 1][j + 2 * (k & 1)])
+                                              : acc[e][g][k >> 1][j + 2 * (k & 1)];
+                        o[k] = fmaf(v, k & 1 ? 32.f : 512.f, zg);
+                    }
+                    *reinterpret_cast<float4*>(s_o + rr * D + g * kKvGroup + r8 * 4) = make_float4(o[0], o[1], o[2], o[3]);
+                }
+                if (r8 == 0) s_ml[rr] = make_float2(m[e][j], l[e][j]);
+            }
+        __syncthreads();
+        for (int i = tid; i < kRows * D / 4; i += kWarps * 32) {
+            const int rr = i / (D / 4), c4 = i % (D / 4);
+            const int rw = row0 + rr;
+            if (rw >= rows) break;
+            float mx = kNone;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) mx = fmaxf(mx, s_ml[w * kRows + rr].x);
+            float sum = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                const float2 ml = s_ml[w * kRows + rr];
+                const float f = ex2(ml.x - mx);
+                sum = fmaf(ml.y, f, sum);
+                const float4 v = reinterpret_cast<const float4*>(s_o + (w * kRows + rr) * D)[c4];
+                o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+            }
+            if (whole) {
+                const int ti = rw / x.group, tk = sp.q0 + ti, hd = kvh * x.group.d + rw - ti * x.group.d;
+                const float n = sum == 0.f ? 0.f : 1.f / sum;
+                const float f[4] = {o.x * n, o.y * n, o.z * n, o.w * n};
+                T* dst = (T*)a.out + (long)tk * a.o_tok + (long)hd * a.o_head + c4 * 4;
+                if (x.wide_o) {
+                    if constexpr (sizeof(T) == 4) {
+                        *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
+                    } else {
+                        const T e[4] = {from_f<T>(f[0]), from_f<T>(f[1]), from_f<T>(f[2]), from_f<T>(f[3])};
+                        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(e);
+                    }
                 } else {
-                    const T e[4] = {from_f<T>(f[0]), from_f<T>(f[1]), from_f<T>(f[2]), from_f<T>(f[3])};
-                    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(e);
+                    for (int j = 0; j < 4; j++) dst[j] = from_f<T>(f[j]);
                 }
+                if (a.lse && c4 == 0) a.lse[(long)tk * a.n_heads + hd] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
             } else {
-                for (int j = 0; j < 4; j++) dst[j] = from_f<T>(f[j]);
+                const long at = slot * kRows + rr;
+                reinterpret_cast<float4*>(x.part + at * D)[c4] = o;
+                if (c4 == 0) x.ml[at] = make_float2(mx, sum);
             }
-            if (a.lse && c4 == 0) a.lse[(long)tk * a.n_heads + hd] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
-        } else {
-            const long at = (unit * x.n_splits + split) * kRows + rr;
-            reinterpret_cast<float4*>(x.part + at * D)[c4] = o;
-            if (c4 == 0) x.ml[at] = make_float2(mx, sum);
         }
+        if (left <= 0) break;
+        begin = 0;
+        if (++kvh == a.cache.n_kv_heads) kvh = 0, req++;
+        __syncthreads();      // the rows in shared memory are read; the next segment's tiles go over them
     }
 }
 
@@ -650,13 +751,26 @@ __global__ void __launch_bounds__(256) join_kernel(const Args x) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     Span sp;
     if (!span_of(x, req, rb, sp)) return;
-    const int active = min(x.n_splits, max(1, (sp.n + x.tiles_per_split - 1) / x.tiles_per_split));
     const int rw = rb * kRows + rr;
-    if (active == 1 || rw >= sp.q_len * x.group) return;
-    const long unit = ((long)req * a.cache.n_kv_heads + kvh) * x.row_blocks + rb;
-    const long at = unit * x.n_splits * kRows + rr;
+    if (rw >= sp.q_len * x.group.d) return;
+    int active;
+    long at, step = kRows;      // row `rr` of the unit's first slot, and from one slot to the next
+    if (x.runs) {
+        const int heads = a.cache.n_kv_heads;
+        const int per = run_tiles((long)x.before[a.n_req] * heads, x.runs);
+        const long first = (long)x.before[req] * heads + (long)kvh * sp.n, last = first + sp.n - 1;
+        const long c0 = first / per, c1 = last / per;
+        active = (int)(c1 - c0) + 1;
+        at = (2 * c0 + 1) * kRows + rr;       // the run in which the unit begins; the others' slots are even
+        step = 2 * kRows;
+    } else {
+        active = min(x.n_splits, (sp.n + x.tiles_per_split - 1) / x.tiles_per_split);
+        at = (((long)req * a.cache.n_kv_heads + kvh) * x.row_blocks + rb) * x.n_splits * kRows + rr;
+    }
+    if (active == 1) return;
+    auto row_of = [&](int s) { return x.runs && s ? at + s * step - kRows : at + s * step; };
     float mx = kNone;
-    for (int s = lane; s < active; s += 32) mx = fmaxf(mx, x.ml[at + (long)s * kRows].x);
+    for (int s = lane; s < active; s += 32) mx = fmaxf(mx, x.ml[row_of(s)].x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     constexpr int kPer = D / 32;
@@ -665,17 +779,17 @@ __global__ void __launch_bounds__(256) join_kernel(const Args x) {
     for (int j = 0; j < kPer; j++) o[j] = 0.f;
 #pragma unroll 4
     for (int s = 0; s < active; s++) {
-        const float2 ml = x.ml[at + (long)s * kRows];
+        const float2 ml = x.ml[row_of(s)];
         const float f = ex2(ml.x - mx);
         sum = fmaf(ml.y, f, sum);
-        const float* v = x.part + (at + (long)s * kRows) * D + lane * kPer;
+        const float* v = x.part + row_of(s) * D + lane * kPer;
         float t[kPer];
 #pragma unroll
         for (int j = 0; j < kPer; j += 2) *reinterpret_cast<float2*>(t + j) = *reinterpret_cast<const float2*>(v + j);
 #pragma unroll
         for (int j = 0; j < kPer; j++) o[j] = fmaf(t[j], f, o[j]);
     }
-    const int tk = sp.q0 + rw / x.group, hd = kvh * x.group + rw % x.group;
+    const int ti = rw / x.group, tk = sp.q0 + ti, hd = kvh * x.group.d + rw - ti * x.group.d;
     const float n = sum == 0.f ? 0.f : 1.f / sum;
     T* dst = (T*)a.out + (long)tk * a.o_tok + (long)hd * a.o_head + lane * kPer;
 #pragma unroll
@@ -683,18 +797,37 @@ __global__ void __launch_bounds__(256) join_kernel(const Args x) {
     if (a.lse && lane == 0) a.lse[(long)tk * a.n_heads + hd] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
-// How the rows are blocked and the long axis is split.  Blocks of 16 rows where 16-bit queries have more than 8 (a tile's
-// codes are then unpacked for twice the rows).  Splits of at least 8 tiles (128 tokens), and about four times as many
-// blocks as the GPU holds at once: ragged lengths then even out, and the partial rows stay a few per cent of the cache bytes.
+template <int D>
+int blocks_per_sm(int nt) { return nt == 1 ? Shape<D, 1>::kBlocks : Shape<D, 2>::kBlocks; }
+
+// How the rows are blocked and the tiles are divided.  Blocks of 16 rows where 16-bit queries have more than 8: a tile's
+// codes are then unpacked for twice the rows.  Runs where each request is one block of rows, as many as fit the GPU at
+// once: a block's start (lengths, page ids, queries) costs it about as much as four tiles a warp, so fewer and longer
+// pieces win (4 x 131001 tokens, 8 kv heads: 140 us, against 145 with one block per unit and split in one wave and 160 in
+// four; 64 ragged requests up to 4096 tokens: 67 against 73 and 69; a window of 4096: 51 against 52 and 79).  Otherwise
+// splits of at least 8 tiles, about four times as many blocks as fit.
 void plan(const Kv4Attn& a, Args& x) {
-    x.group = a.n_heads / a.cache.n_kv_heads;
-    const long rows = (long)a.max_q * x.group;
+    const int group = a.n_heads / a.cache.n_kv_heads;
+    x.group = make_div(group);
+    x.page_tiles = make_div(a.cache.page_size / kKvTile);
+    const long rows = (long)a.max_q * group;
     x.block_rows = a.dtype != kF32 && rows > 8 ? 16 : 8;
     x.row_blocks = (int)((rows + x.block_rows - 1) / x.block_rows);
+    // (a block counts tiles in 32 bits)
+    const long tiles_bound = ((long)a.table_width * (a.cache.page_size / kKvTile) + 1) * a.n_req;
+    if (x.row_blocks == 1 && a.n_req <= kRunReqs && tiles_bound < 1l << 31) {
+        const int nt = a.dtype == kF32 || x.block_rows == 16 ? 2 : 1, d = a.cache.head_dim;
+        x.runs = 148 * (d == 64 ? blocks_per_sm<64>(nt) : d == 128 ? blocks_per_sm<128>(nt) : blocks_per_sm<256>(nt));
+        // no more than the longest sequences allow
+        const long most = ((long)a.max_seq / kKvTile + 1) * a.n_req * a.cache.n_kv_heads;
+        x.runs = (int)std::max<long>(1, std::min<long>(x.runs, (most + kRunMin - 1) / kRunMin));
+        x.n_splits = 1;
+        return;
+    }
     const int tiles = std::max(1, (a.max_seq + kKvTile - 1) / kKvTile);
     int span = tiles;
     if (a.window > 0)   // the widest walk of one row block
-        span = (int)std::min<long>(tiles, ((long)a.window + std::min(a.max_q, x.block_rows / x.group + 2)) / kKvTile + 2 +
+        span = (int)std::min<long>(tiles, ((long)a.window + std::min(a.max_q, x.block_rows / group + 2)) / kKvTile + 2 +
                                               ((long)a.sinks + kKvTile - 1) / kKvTile);
     const long units = (long)a.n_req * a.cache.n_kv_heads * x.row_blocks;
     const long want = std::max<long>(1, 148L * 4 * 4 / units);
@@ -702,15 +835,20 @@ void plan(const Kv4Attn& a, Args& x) {
     x.tiles_per_split = (int)per;
     x.n_splits = (int)((span + per - 1) / per);
 }
+long slots_of(const Args& x) {
+    return x.runs ? 2l * x.runs : (long)x.a.n_req * x.a.cache.n_kv_heads * x.row_blocks * x.n_splits;
+}
+bool needs_join(const Args& x) { return x.runs > 1 || x.n_splits > 1; }
 
 template <typename T, int D, int NT, bool SPLIT>
 void run_nt(const Args& x, cudaStream_t s) {
     using S = Shape<D, NT>;
     const int rows = SPLIT ? 8 : 8 * NT;
-    const int smem = std::max(kWarps * S::kStages * kv4_tile_bytes(D), kWarps * rows * (D * 4 + 8)) +
-                     (S::kQInSmem ? D / kKvGroup * NT * 32 * 16 : 0);
+    const int smem = std::max(kWarps * S::kStages * kv4_tile_bytes(D) + D / kKvGroup * NT * 512 + 2 * NT * 128 + rows * 4,
+                              kWarps * rows * (D * 4 + 8));
     cudaFuncSetAttribute(attend_kernel<T, D, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    const dim3 grid((unsigned)(x.n_splits * x.a.cache.n_kv_heads * x.row_blocks), (unsigned)x.a.n_req);
+    const dim3 grid = x.runs ? dim3((unsigned)x.runs)
+                             : dim3((unsigned)(x.n_splits * x.row_blocks), (unsigned)x.a.cache.n_kv_heads, (unsigned)x.a.n_req);
     attend_kernel<T, D, NT, SPLIT><<<grid, kWarps * 32, smem, s>>>(x);
 }
 template <typename T, int D>
@@ -718,7 +856,7 @@ void run(const Args& x, cudaStream_t s) {
     if constexpr (sizeof(T) == 4) run_nt<T, D, 2, true>(x, s);
     else if (x.block_rows == 16) run_nt<T, D, 2, false>(x, s);
     else run_nt<T, D, 1, false>(x, s);
-    if (x.n_splits == 1) return;
+    if (!needs_join(x)) return;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(x.a.cache.n_kv_heads * x.row_blocks * x.block_rows / 8), (unsigned)x.a.n_req);
     cfg.blockDim = dim3(256);
@@ -737,9 +875,10 @@ void run_d(const Args& x, cudaStream_t s) {
     else run<T, 256>(x, s);
 }
 
-size_t part_bytes(const Kv4Attn& a, const Args& x) {
-    return (size_t)a.n_req * a.cache.n_kv_heads * x.row_blocks * x.n_splits * x.block_rows * sizeof(float) * a.cache.head_dim;
+size_t part_bytes(const Args& x) {
+    return (size_t)slots_of(x) * x.block_rows * sizeof(float) * x.a.cache.head_dim;
 }
+size_t ml_bytes(const Args& x) { return (size_t)slots_of(x) * x.block_rows * sizeof(float2); }
 
 }  // namespace
 
@@ -747,8 +886,8 @@ size_t kv4_attention_workspace(const Kv4Attn& a) {
     Args x{};
     x.a = a;
     plan(a, x);
-    if (x.n_splits == 1) return 0;
-    return part_bytes(a, x) + part_bytes(a, x) / a.cache.head_dim * 2;
+    if (!x.runs && x.n_splits == 1) return 0;
+    return part_bytes(x) + ml_bytes(x) + (x.runs ? sizeof(int) * ((size_t)a.n_req + 1) : 0);
 }
 
 int launch_kv4_attention(const Kv4Attn& a, void* workspace, cudaStream_t s) {
@@ -759,11 +898,14 @@ int launch_kv4_attention(const Kv4Attn& a, void* workspace, cudaStream_t s) {
     x.wide_q = aligned16(a.q, a.q_tok, a.q_head, b);
     x.wide_o = aligned16(a.out, a.o_tok, a.o_head, b);
     x.part = (float*)workspace;
-    if (x.n_splits > 1) x.ml = (float2*)((char*)workspace + part_bytes(a, x));
+    if (x.runs || x.n_splits > 1) {
+        x.ml = (float2*)((char*)workspace + part_bytes(x));
+        x.before = (int*)((char*)x.ml + ml_bytes(x));
+    }
     if (a.dtype == kF32) run_d<float>(x, s);
     else if (a.dtype == kF16) run_d<__half>(x, s);
     else run_d<__nv_bfloat16>(x, s);
-    return x.n_splits > 1 ? 2 : 1;
+    return needs_join(x) ? 2 : 1;
 }
 
 }  // namespace draco
