@@ -4,7 +4,8 @@
 
 Objects go to <repo>/_build/ (not committed); the shared library is written next to this file
 so that it travels with the repository snapshot and is what `dracomancer_llmengine_b200`
-loads.  Rebuilds only what changed (sources or headers newer than the object).
+loads, and beside it `_decoder.so`, the Python extension of `decoder` for torch tensors.
+Rebuilds only what changed (sources or headers newer than the object).
 """
 from __future__ import annotations
 
@@ -13,12 +14,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "libdraco_moe_b200.so")
+EXT = os.path.join(PKG, "_decoder.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O2",
@@ -58,7 +61,30 @@ def build(verbose: bool = False, extra_flags=()) -> str:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
         os.replace(tmp, LIB)
+    build_decoder(verbose)
     return LIB
+
+
+def build_decoder(verbose: bool = False) -> str | None:
+    """The Python extension of `decoder` (argument checks and calls for torch tensors), where torch is installed."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    src, newest = os.path.join(CSRC, "decoder_py.cpp"), max(os.path.getmtime(h) for h in _headers())
+    if os.path.exists(EXT) and os.path.getmtime(EXT) >= max(os.path.getmtime(src), newest):
+        return EXT
+    at = os.path.dirname(torch.__file__)
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           src, "-o", EXT + ".tmp"]
+    cmd += ["-I" + d for d in (os.path.join(at, "include"), os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"),
+                               sysconfig.get_paths()["include"])]
+    cmd += ["-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(EXT + ".tmp", EXT)
+    return EXT
 
 
 if __name__ == "__main__":
