@@ -19,16 +19,28 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kPerThread = 4;   // neighbouring tokens of a thread: one search, 16-byte stores
 
-__device__ __forceinline__ int ceil_div(long a, int b) { return (int)((a + b - 1) / b); }
+struct Call {
+    BlockArgs a;
+    Div page;
+};
 
-__global__ void __launch_bounds__(kThreads) plan_blocks_kernel(const BlockArgs a) {
+__device__ __forceinline__ int pages_of(int tokens, const Div& page) {
+    const int n = tokens / page;
+    return n + (n * page.d < tokens);
+}
+
+__global__ void __launch_bounds__(kThreads) plan_blocks_kernel(const Call x) {
+    const BlockArgs& a = x.a;
     extern __shared__ int sm[];
-    int* s_cu = sm;                    // [R + 1] tokens before the request
-    int* s_pre = sm + a.n_req + 1;     // [R] pages taken before the request, -1: refused
+    const int R = a.n_req, P = a.page;
+    int* s_cu = sm;                 // [R + 1] tokens before the request
+    int* s_pre = s_cu + R + 1;      // [R] pages taken before the request, -1: refused
+    int* s_ctx = s_pre + R;         // [R] tokens cached
     __shared__ int2 s_warp[kThreads / 32];
     __shared__ int s_taken, s_refused;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int R = a.n_req, P = a.page;
+    early_launch();
+    wait_for_inputs();
     const int n_free = min(max(*a.n_free, 0), a.free_len);
     if (tid == 0) {
         s_taken = s_refused = 0;
@@ -37,40 +49,38 @@ __global__ void __launch_bounds__(kThreads) plan_blocks_kernel(const BlockArgs a
 
     // exclusive scan of (new tokens, new pages): each thread a run of requests, then warps, then the block
     const int per = (R + kThreads - 1) / kThreads, lo = min(R, tid * per), hi = min(R, lo + per);
-    auto need_of = [&](int r, int& add) {
-        const int ctx = max(a.ctx[r], 0);
-        add = max(a.add[r], 0);
-        const int pages = ceil_div((long)ctx + add, P);
-        return pages > a.width ? -1 : pages - ceil_div(ctx, P);
-    };
     int2 sum = make_int2(0, 0);
     for (int r = lo; r < hi; r++) {
-        int add;
-        const int need = need_of(r, add);
+        const int ctx = max(a.ctx[r], 0), add = max(a.add[r], 0);
+        const long all = (long)ctx + add;
+        // more than a row holds: no pages, and none counted against the requests behind it
+        const int need = all > (long)a.width * P ? -1 : pages_of((int)all, x.page) - pages_of(ctx, x.page);
+        s_ctx[r] = ctx;
+        s_pre[r] = need;
+        s_cu[r] = add;
         sum.x += add;
         sum.y += max(need, 0);
     }
     int2 inc = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, inc.x, o), y = __shfl_up_sync(0xffffffffu, inc.y, o);
-        if (lane >= o) inc.x += x, inc.y += y;
+        const int u = __shfl_up_sync(0xffffffffu, inc.x, o), v = __shfl_up_sync(0xffffffffu, inc.y, o);
+        if (lane >= o) inc.x += u, inc.y += v;
     }
     if (lane == 31) s_warp[warp] = inc;
     __syncthreads();
     int2 at = make_int2(inc.x - sum.x, inc.y - sum.y);
-    for (int w = 0; w < warp; w++) at.x += s_warp[w].x, at.y += s_warp[w].y;
+    const int warps = min(warp, (R + per * 32 - 1) / max(per * 32, 1));     // the others' sums are 0
+    for (int w = 0; w < warps; w++) at.x += s_warp[w].x, at.y += s_warp[w].y;
     const bool first = blockIdx.x == 0;
     int taken = 0, refused = 0;
     for (int r = lo; r < hi; r++) {
-        int add;
-        const int need = need_of(r, add);
+        const int ctx = s_ctx[r], need = s_pre[r], add = s_cu[r];
         const bool ok = need == 0 || (need > 0 && at.y + need <= n_free);
         s_cu[r] = at.x;
         s_pre[r] = ok ? at.y : -1;
         if (first) {
             a.cu[r] = at.x;
-            const int ctx = max(a.ctx[r], 0);
             a.seq[r] = ok ? ctx + add : ctx;
         }
         taken += ok ? need : 0;
@@ -111,17 +121,17 @@ __global__ void __launch_bounds__(kThreads) plan_blocks_kernel(const BlockArgs a
             slot[i] = pos[i] = -1;
             if (t >= total) continue;
             while (s_cu[r + 1] <= t) r++;
-            const int ctx = max(a.ctx[r], 0), p = ctx + (int)(t - s_cu[r]);
+            const int ctx = s_ctx[r], p = ctx + (int)(t - s_cu[r]);
             pos[i] = p;
             const int pre = s_pre[r];
             if (pre < 0) continue;
-            const int c = p / P, held = ceil_div(ctx, P);
+            const int c = p / x.page, held = pages_of(ctx, x.page);
             int page;
             if (c < held) {
                 page = a.table[(long)r * a.table_stride + c];
             } else {
                 page = a.free_pages[n_free - 1 - pre - (c - held)];
-                if (p - c * P == 0) a.table[(long)r * a.table_stride + c] = page;
+                if (p == c * P) a.table[(long)r * a.table_stride + c] = page;
             }
             slot[i] = page * P + (p - c * P);
         }
@@ -138,13 +148,13 @@ __global__ void __launch_bounds__(kThreads) plan_blocks_kernel(const BlockArgs a
 }  // namespace
 
 void launch_plan_blocks(const BlockArgs& a, cudaStream_t s) {
-    const size_t smem = sizeof(int) * (2 * (size_t)a.n_req + 1);
+    const size_t smem = sizeof(int) * (3 * (size_t)a.n_req + 1);
     if (smem > 40 * 1024)
         cudaFuncSetAttribute(plan_blocks_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)(sizeof(int) * (2 * (size_t)kBlockMaxReq + 1)));
+                             (int)(sizeof(int) * (3 * (size_t)kBlockMaxReq + 1)));
     const long per = (long)kThreads * kPerThread;
     const int grid = (int)std::min<long>(148, std::max<long>(1, ((long)a.cap + per - 1) / per));
-    plan_blocks_kernel<<<grid, kThreads, smem, s>>>(a);
+    launch(plan_blocks_kernel, dim3(grid), dim3(kThreads), smem, s, Call{a, make_div(a.page)});
 }
 
 }  // namespace draco

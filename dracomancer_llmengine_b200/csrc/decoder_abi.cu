@@ -36,7 +36,11 @@ int launched(const char* who, int kernels) {
     return 0;
 }
 
+// set while the package's own extension calls: it has seen that the tensors are on the GPU, and asking the driver about
+// each address again would take as long as the launch
+thread_local bool t_pointers_checked = false;
 bool on_device(std::initializer_list<const void*> ps) {
+    if (t_pointers_checked) return true;
     for (const void* p : ps)
         if (p && !abi_device_ptr(p)) return false;
     return true;
@@ -49,7 +53,7 @@ const char* cache_fault(const DracoKV4Cache* c) {
     if (c->page_size < kKvTile || c->page_size % kKvTile) return "page_size must be a multiple of 16";
     if (c->n_kv_heads < 1 || c->n_pages < 1) return "need pages and kv heads";
     if ((long)c->n_pages * c->page_size >= 1l << 31) return "n_pages * page_size must be below 2^31";
-    if (!aligned_to(c->pages, 16) || !abi_device_ptr(c->pages)) return "pages must be 16-byte aligned device memory";
+    if (!aligned_to(c->pages, 16) || !on_device({c->pages})) return "pages must be 16-byte aligned device memory";
     return nullptr;
 }
 Kv4Cache cache_of(const DracoKV4Cache* c) {
@@ -66,7 +70,7 @@ int rows_call(const char* who, bool append, const DracoKV4Cache* cache, int dtyp
     const size_t b = (size_t)dtype_bytes(dtype);
     if (!aligned_to(k, b) || !aligned_to(v, b) || !aligned_to(slots, 4))
         return refuse("%s: buffers must be aligned to their elements", who);
-    if ((long)n * cache->n_kv_heads * (cache->head_dim / 4) > 256l * 0x7fffffff)
+    if ((long)n * cache->n_kv_heads * (cache->head_dim / 8) > 0x7fffff00l)
         return refuse("%s: too many tokens for one call", who);
     const Kv4Rows r{k, v, kt, kh, vt, vh};
     if (append) launch_kv4_append(cache_of(cache), r, dtype, slots, n, (cudaStream_t)stream);
@@ -97,6 +101,9 @@ const char* attention_args(const DracoKV4Cache* cache, const DracoKV4Attention* 
 }  // namespace
 
 extern "C" {
+
+// not part of the interface: for decoder_py.cpp
+void draco_b200_pointers_checked(int on) { t_pointers_checked = on != 0; }
 
 int draco_b200_plan_blocks(const int* ctx_len, const int* new_len, int n_req, int page_size, int* block_table,
                            long table_stride, int table_width, const int* free_pages, int free_len, const int* n_free,

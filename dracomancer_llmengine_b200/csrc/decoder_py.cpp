@@ -26,6 +26,7 @@ decltype(&draco_b200_kv4_read) f_read = nullptr;
 decltype(&draco_b200_kv4_attention_workspace) f_workspace = nullptr;
 decltype(&draco_b200_kv4_attention) f_attention = nullptr;
 decltype(&draco_b200_rmsnorm_q8) f_norm = nullptr;
+void (*f_checked)(int) = nullptr;
 
 struct Refused : std::runtime_error {
     using std::runtime_error::runtime_error;
@@ -79,13 +80,15 @@ int dtype_of(const at::Tensor& t) {
     }
 }
 
-// the tensors' device made current for the call, as a launch needs it
+// the tensors' device made current for the call, as a launch needs it; made when every tensor was seen to be on it
 struct OnDevice {
     c10::DeviceIndex old, now;
     explicit OnDevice(const at::Device& d) : old(c10::cuda::current_device()), now(d.index()) {
         if (now != old) c10::cuda::set_device(now);
+        f_checked(1);
     }
     ~OnDevice() {
+        f_checked(0);
         if (now != old) c10::cuda::set_device(old);
     }
 };
@@ -133,7 +136,7 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!take("draco_b200_last_error", f_last_error) || !take("draco_b200_plan_blocks", f_plan_blocks) ||
         !take("draco_b200_kv4_append", f_append) || !take("draco_b200_kv4_read", f_read) ||
         !take("draco_b200_kv4_attention_workspace", f_workspace) || !take("draco_b200_kv4_attention", f_attention) ||
-        !take("draco_b200_rmsnorm_q8", f_norm))
+        !take("draco_b200_pointers_checked", f_checked) || !take("draco_b200_rmsnorm_q8", f_norm))
         return nullptr;
     Py_INCREF(a[0]);
     Py_XSETREF(g_error, a[0]);

@@ -116,42 +116,125 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// N consecutive values, in 16-byte pieces where `wide` (the address is then 16-byte aligned)
-template <typename T, int N>
-__device__ __forceinline__ void load_row(const T* p, bool wide, float* f) {
-    if (wide) {
-        constexpr int kPer = 16 / sizeof(T);
-        static_assert(N % kPer == 0, "whole 16-byte pieces");
+// two values of a 32-bit word of 16-bit elements, and back
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 8 consecutive values, in 16-byte pieces where `wide` (the address is then 16-byte aligned)
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool wide, float (&f)[8]) {
+    if (!wide) {
 #pragma unroll
-        for (int i = 0; i < N / kPer; i++) {
-            const uint4 u = reinterpret_cast<const uint4*>(p)[i];
-            const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-            for (int j = 0; j < kPer; j++) f[i * kPer + j] = to_f(e[j]);
-        }
+        for (int i = 0; i < 8; i++) f[i] = to_f(p[i]);
+        return;
+    }
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
     } else {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int i = 0; i < N; i++) f[i] = to_f(p[i]);
+        for (int i = 0; i < 4; i++) {
+            const float2 t = unpack2<T>(w[i]);
+            f[2 * i] = t.x, f[2 * i + 1] = t.y;
+        }
     }
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_row(T* p, bool wide, const float* f) {
-    if (wide) {
-        constexpr int kPer = 16 / sizeof(T);
-        static_assert(N % kPer == 0, "whole 16-byte pieces");
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool wide, const float (&f)[8]) {
+    if (!wide) {
 #pragma unroll
-        for (int i = 0; i < N / kPer; i++) {
-            uint4 u;
-            T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-            for (int j = 0; j < kPer; j++) e[j] = from_f<T>(f[i * kPer + j]);
-            reinterpret_cast<uint4*>(p)[i] = u;
-        }
+        for (int i = 0; i < 8; i++) p[i] = from_f<T>(f[i]);
+        return;
+    }
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
     } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) p[i] = from_f<T>(f[i]);
+        *reinterpret_cast<uint4*>(p) =
+            make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
     }
 }
+
+// asynchronous copies of 16 bytes into shared memory, in groups that complete in order
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// maximum and minimum that keep a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// bits of v + 1.5 * 2^23: for |v| < 2^22 their low byte is that of rint(v) (the addition rounds to even)
+__device__ __forceinline__ uint32_t rint_bits(float v) { return __float_as_uint(__fadd_rn(v, 12582912.f)); }
+
+// n / d for 0 <= n < 2^31 by one high product: m = floor(2^(31 + l) / d) + 1 with 2^l >= d
+struct Div {
+    uint32_t m, s;
+    int d;
+};
+inline Div make_div(int d) {
+    int l = 0;
+    while ((1l << l) < d) l++;
+    return Div{d == 1 ? 0u : (uint32_t)(((uint64_t)1 << (31 + l)) / (uint32_t)d + 1), (uint32_t)(d == 1 ? 0 : l - 1), d};
+}
+__device__ __forceinline__ int operator/(int n, const Div& v) {
+    return v.d == 1 ? n : (int)(__umulhi((uint32_t)n, v.m) >> v.s);
+}
+
+// ---- launches ----
+// Every kernel of these operators is launched so that it may start while the one before it in the stream drains, lets the
+// next one do the same (early_launch), and touches no memory before that one is complete and its writes are visible
+// (wait_for_inputs).  Back to back, small kernels then do not pay the launch latency between them.
+__device__ __forceinline__ void early_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_inputs() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename Arg>
+inline void launch(void (*kernel)(const Arg), dim3 grid, dim3 block, size_t smem, cudaStream_t s, const Arg& arg) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, arg);
+}
+
 inline bool aligned16(const void* p, long a = 0, long b = 0, int bytes = 1) {
     return ((uintptr_t)p | (uintptr_t)(a * bytes) | (uintptr_t)(b * bytes)) % 16 == 0;
 }

@@ -38,6 +38,7 @@
 #include "kv4.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace draco {
@@ -57,20 +58,6 @@ constexpr float kSlack = 3.f;       // log2 of the largest weight
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLoScale = 2048.f, kLoInv = 1.f / 2048.f;
-
-// n / d for 0 <= n < 2^31 by one high product: m = floor(2^(31 + l) / d) + 1 with 2^l >= d
-struct Div {
-    uint32_t m, s;
-    int d;
-};
-Div make_div(int d) {
-    int l = 0;
-    while ((1l << l) < d) l++;
-    return Div{d == 1 ? 0u : (uint32_t)(((uint64_t)1 << (31 + l)) / (uint32_t)d + 1), (uint32_t)(d == 1 ? 0 : l - 1), d};
-}
-__device__ __forceinline__ int operator/(int n, const Div& v) {
-    return v.d == 1 ? n : (int)(__umulhi((uint32_t)n, v.m) >> v.s);
-}
 
 struct Args {
     Kv4Attn a;
@@ -150,12 +137,6 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, int n) {
                  "r"(n)
                  : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // 4-byte words [0, N) at p (N even, p aligned to min(16, 4 N))
 template <int N>
 __device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[N]) {
@@ -252,6 +233,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_ker
     const Kv4Attn& a = x.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r8 = lane >> 2, q4 = lane & 3;
     __shared__ int s_before[kRunReqs + 1];
+    early_launch();
+    wait_for_inputs();
     // the segment: tiles [begin, end) of a unit, and where its sums go if it is not the whole unit
     int rb = 0, kvh, req, begin, end;
     long slot, left = 0;      // left: tiles of the run behind this segment
@@ -344,7 +327,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_ker
             float v[8];
             if (row < rows) {
                 const int tok = row / x.group, head = kvh * x.group.d + row - tok * x.group.d;
-                load_row<T, 8>((const T*)a.q + (long)(sp.q0 + tok) * a.q_tok + (long)head * a.q_head + c8 * 8, x.wide_q, v);
+                load8<T>((const T*)a.q + (long)(sp.q0 + tok) * a.q_tok + (long)head * a.q_head + c8 * 8, x.wide_q, v);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; j++) v[j] = 0.f;
@@ -748,7 +731,8 @@ __global__ void __launch_bounds__(256) join_kernel(const Args x) {
     const int unit_row = blockIdx.x * 8 + (threadIdx.x >> 5);       // row of (kv head, row block)
     const int rr = unit_row % kRows, ub = unit_row / kRows;
     const int rb = ub % x.row_blocks, kvh = ub / x.row_blocks, req = blockIdx.y;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    early_launch();
+    wait_for_inputs();
     Span sp;
     if (!span_of(x, req, rb, sp)) return;
     const int rw = rb * kRows + rr;
@@ -846,10 +830,16 @@ void run_nt(const Args& x, cudaStream_t s) {
     const int rows = SPLIT ? 8 : 8 * NT;
     const int smem = std::max(kWarps * S::kStages * kv4_tile_bytes(D) + D / kKvGroup * NT * 512 + 2 * NT * 128 + rows * 4,
                               kWarps * rows * (D * 4 + 8));
-    cudaFuncSetAttribute(attend_kernel<T, D, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> ready{0};      // devices on which the kernel may use its shared memory
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev > 63 || !(ready.load() >> dev & 1)) {
+        cudaFuncSetAttribute(attend_kernel<T, D, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (dev < 64) ready |= (uint64_t)1 << dev;
+    }
     const dim3 grid = x.runs ? dim3((unsigned)x.runs)
                              : dim3((unsigned)(x.n_splits * x.row_blocks), (unsigned)x.a.cache.n_kv_heads, (unsigned)x.a.n_req);
-    attend_kernel<T, D, NT, SPLIT><<<grid, kWarps * 32, smem, s>>>(x);
+    launch(attend_kernel<T, D, NT, SPLIT>, grid, dim3(kWarps * 32), smem, s, x);
 }
 template <typename T, int D>
 void run(const Args& x, cudaStream_t s) {
@@ -857,16 +847,8 @@ void run(const Args& x, cudaStream_t s) {
     else if (x.block_rows == 16) run_nt<T, D, 2, false>(x, s);
     else run_nt<T, D, 1, false>(x, s);
     if (!needs_join(x)) return;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(x.a.cache.n_kv_heads * x.row_blocks * x.block_rows / 8), (unsigned)x.a.n_req);
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, join_kernel<T, D>, x);
+    launch(join_kernel<T, D>, dim3((unsigned)(x.a.cache.n_kv_heads * x.row_blocks * x.block_rows / 8), (unsigned)x.a.n_req),
+           dim3(256), 0, s, x);
 }
 template <typename T>
 void run_d(const Args& x, cudaStream_t s) {

@@ -32,7 +32,8 @@ __all__ = ["BlockPlan", "plan_blocks", "KV4Cache", "rmsnorm_q8"]
 # the extension checks arguments and calls the entry points of the library that this package loaded
 _decoder.setup(DracoError, {name: ct.cast(getattr(lib(), name), ct.c_void_p).value for name in (
     "draco_b200_last_error", "draco_b200_plan_blocks", "draco_b200_kv4_append", "draco_b200_kv4_read",
-    "draco_b200_kv4_attention_workspace", "draco_b200_kv4_attention", "draco_b200_rmsnorm_q8")})
+    "draco_b200_kv4_attention_workspace", "draco_b200_kv4_attention", "draco_b200_rmsnorm_q8",
+    "draco_b200_pointers_checked")})
 
 
 def _need(ok, what: str):

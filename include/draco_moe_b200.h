@@ -335,8 +335,7 @@ int draco_b200_gemv_q8k(int code, const uint8_t* W, int rows, int n_in, const in
  *
  * What a decoder layer needs around the MoE FFN on the same GPU: page allocation and slot maps, a 4-bit paged KV cache,
  * attention over it, and the residual RMS norm with 8-bit output.  No counterpart in the reference.  All pointers are
- * device memory; every call is asynchronous on `stream` (null: the legacy default stream), allocates nothing, keeps
- * nothing between calls and can be captured in a CUDA graph.  Returns 0, -1 (arguments; nothing was launched) or
+ * device memory; every call is asynchronous on `stream` (null: the legacy default stream), allocates nothing and can be captured in a CUDA graph.  Returns 0, -1 (arguments; nothing was launched) or
  * -3 (CUDA error), with the text in draco_b200_last_error().  Element types (dtype): 0 fp32, 1 fp16, 2 bf16. */
 
 /* Block tables and slot maps from the requests' lengths, for n_req (<= 16384) requests, in one launch.

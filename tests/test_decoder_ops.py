@@ -562,6 +562,22 @@ def test_results_repeat():
     assert all(torch.equal(o, outs[0]) for o in outs)
 
 
+def test_attend_shared_scratch():
+    """Calls of unlike shapes in turn over one scratch buffer."""
+    rng = np.random.default_rng(21)
+    lens = [5000, 31, 700, 0, 64]
+    cache, table = make_cache(rng, lens, 16, 4, 128)
+    tab, seq = torch.from_numpy(table).cuda(), ints(lens)
+    for rows, heads, kind in ((1, 4, "f32"), (3, 32, "bf16"), (1, 64, "f16"), (20, 8, "bf16"), (1, 8, "bf16"), (9, 4, "f32")) * 2:
+        n = rows * len(lens)
+        q = torch.randn(n, heads, 128, device="cuda").to(TYPES[kind])
+        out = torch.empty_like(q)
+        cu = list(range(0, n + 1, rows))
+        cache.attend(q, out, ints(cu), seq, tab, rows, max(lens))
+        want, _ = attend_ref(cache, table, q, cu, lens, 0, 0)
+        assert rel(out, want) <= TOL[kind]
+
+
 def test_refusals():
     cache = decoder.KV4Cache.empty(4, 16, 2, 64)
     f = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
