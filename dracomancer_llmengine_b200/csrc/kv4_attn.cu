@@ -35,7 +35,7 @@
 // unit that lies in several runs is joined by a second kernel from at most two partial sums per block.  Every block finds
 // its run itself, by a scan of the lengths.  Otherwise (chunks, or more requests than that scan takes) a block takes one
 // unit, or a split of it where units are few.  Sums are joined in a fixed order: results do not depend on timing.
-#include "kv4.cuh"
+#include "kv4_attn.cuh"
 
 #include <algorithm>
 #include <atomic>
@@ -43,6 +43,8 @@
 
 namespace draco {
 namespace {
+
+using namespace attn;
 
 constexpr int kWarps = 4;
 // What a variant of the kernel takes per block: NT columns of 8 (queries, or their two halves)
@@ -53,26 +55,7 @@ struct Shape {
     static constexpr int kBlocks = D == 64 ? (NT == 1 ? 5 : 4) : D == 128 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2);
 };
 constexpr uint32_t kTwo15 = 0x78007800u;   // 2^15, 2^15 in fp16
-constexpr float kNone = -1e30f;     // maximum of a row that has seen nothing
-constexpr float kSlack = 3.f;       // log2 of the largest weight
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLoScale = 2048.f, kLoInv = 1.f / 2048.f;
-
-struct Args {
-    Kv4Attn a;
-    int row_blocks, block_rows;
-    int runs;                               // blocks of the run form (0: a block per unit and split)
-    int tiles_per_split, n_splits;          // of the other form
-    Div group;          // query heads of a kv head
-    Div page_tiles;     // tiles of a page
-    bool wide_q, wide_o;
-    // partial sums, relative to their own maximum, in slots of block_rows rows: [unit][split], or two for each run (of a
-    // unit that began in an earlier run, and of one that begins in it)
-    float* part;        // [slot][block_rows][D]
-    float2* ml;         // [slot][block_rows] maximum (log2 domain) and sum
-    int* before;        // [n_req + 1] tiles of one kv head before each request (run form; for the join)
-};
 
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
                                       float c1, float c2, float c3) {
@@ -95,11 +78,6 @@ __device__ __forceinline__ void mma8(float (&d)[4], uint32_t a0, uint32_t a1, ui
 __device__ __forceinline__ uint32_t transpose(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -155,69 +133,6 @@ __device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[N]) {
     }
 }
 
-// What a block of rows looks at: tiles [0, head) for the first tokens, then [first, first + n - head).
-struct Span {
-    int q0, q_len, seq;     // first token of the request in q, its queries, its keys
-    int p_lo, p_hi;         // positions of the block's first and last query token
-    int head, first, n;
-};
-__device__ __forceinline__ bool span_of(const Args& x, int req, int rb, Span& s) {
-    const Kv4Attn& a = x.a;
-    s.q0 = a.cu_q[req];
-    const int q1 = min(a.cu_q[req + 1], a.n_tokens);
-    s.q0 = max(s.q0, 0);
-    s.q_len = q1 - s.q0;
-    const int rows = s.q_len * x.group.d;
-    if (rb * x.block_rows >= rows) return false;
-    const long cap = min((long)a.table_width * a.cache.page_size, 1l << 30);
-    s.seq = (int)min((long)max(a.seq_len[req], 0), cap);
-    s.p_lo = s.seq - s.q_len + rb * x.block_rows / x.group;
-    s.p_hi = s.seq - s.q_len + (min((rb + 1) * x.block_rows, rows) - 1) / x.group;
-    s.head = s.first = 0;
-    s.n = 1;
-    if (s.p_hi < 0) return true;   // nothing before any query: one tile, hidden from all of them
-    const int last = s.p_hi / kKvTile;
-    if (a.window > 0 && s.p_lo - a.window + 1 > 0) {
-        s.first = (s.p_lo - a.window + 1) / kKvTile;
-        s.head = min(s.first, (min(a.sinks, s.seq) + kKvTile - 1) / kKvTile);
-    }
-    s.n = s.head + last - s.first + 1;
-    return true;
-}
-
-constexpr int kRunReqs = 1024;      // requests that a block scans
-constexpr int kRunMin = 8;          // tiles of a run: two for each warp
-
-// tiles of a run, of `total`
-__device__ __forceinline__ int run_tiles(long total, int runs) { return (int)max((long)kRunMin, (total + runs - 1) / runs); }
-
-// before[r] = tiles of one kv head in the requests before r, for the whole block
-__device__ __forceinline__ void scan_requests(const Args& x, int* before) {
-    __shared__ int s_warp[kWarps];
-    const int tid = threadIdx.x, lane = tid & 31, n = x.a.n_req;
-    const int per = (n + kWarps * 32 - 1) / (kWarps * 32), lo = min(n, tid * per), hi = min(n, lo + per);
-    int sum = 0;
-    for (int r = lo; r < hi; r++) {
-        Span sp;
-        const int t = span_of(x, r, 0, sp) ? sp.n : 0;
-        before[r + 1] = t;
-        sum += t;
-    }
-    int inc = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += y;
-    }
-    if (lane == 31) s_warp[tid >> 5] = inc;
-    if (tid == 0) before[0] = 0;
-    __syncthreads();
-    int at = inc - sum;
-    for (int w = 0; w < tid >> 5; w++) at += s_warp[w];
-    for (int r = lo; r < hi; r++) before[r + 1] = at += before[r + 1];
-    __syncthreads();
-}
-
 // NT columns of 8: 8 NT query rows, or (SPLIT) the high and low halves of 8
 template <typename T, int D, int NT, bool SPLIT>
 __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_kernel(const Args x) {
@@ -232,7 +147,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_ker
     extern __shared__ __align__(16) uint8_t smem[];
     const Kv4Attn& a = x.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r8 = lane >> 2, q4 = lane & 3;
-    __shared__ int s_before[kRunReqs + 1];
+    __shared__ int s_before[kRunUnits + 1];
     early_launch();
     wait_for_inputs();
     // the segment: tiles [begin, end) of a unit, and where its sums go if it is not the whole unit
@@ -241,26 +156,12 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_ker
     Span sp;
     bool whole;
     if (x.runs) {
-        scan_requests(x, s_before);
-        const int heads = a.cache.n_kv_heads;
-        const long total = (long)s_before[a.n_req] * heads;
-        const int per = run_tiles(total, x.runs);
-        const long start = (long)blockIdx.x * per;
+        scan_units<kWarps * 32>(x, s_before);
         if (blockIdx.x == 0)
             for (int i = tid; i <= a.n_req; i += kWarps * 32) x.before[i] = s_before[i];
-        if (start >= total) return;
-        int lo = 0, hi = a.n_req;
-        while (hi - lo > 1) {      // the last request that begins at or before the run
-            const int mid = (lo + hi) >> 1;
-            if ((long)s_before[mid] * heads <= start) lo = mid;
-            else hi = mid;
-        }
-        req = lo;
-        const int n = s_before[req + 1] - s_before[req];
-        const int in = (int)(start - (long)s_before[req] * heads);
-        kvh = in / n;
-        begin = in - kvh * n;
-        left = min((long)per, total - start);
+        const Run run = run_of(x, s_before);
+        if (!run.left) return;
+        req = run.f, kvh = run.kvh, begin = run.begin, left = run.left;     // row_blocks is 1
     } else {
         // the row blocks of one split are neighbours: they read the same tiles
         const int split = blockIdx.x / x.row_blocks;
@@ -741,8 +642,8 @@ __global__ void __launch_bounds__(256) join_kernel(const Args x) {
     long at, step = kRows;      // row `rr` of the unit's first slot, and from one slot to the next
     if (x.runs) {
         const int heads = a.cache.n_kv_heads;
-        const int per = run_tiles((long)x.before[a.n_req] * heads, x.runs);
-        const long first = (long)x.before[req] * heads + (long)kvh * sp.n, last = first + sp.n - 1;
+        const int per = run_tiles(x, (long)x.before[a.n_req * x.row_blocks] * heads);
+        const long first = (long)x.before[req * x.row_blocks + rb] * heads + (long)kvh * sp.n, last = first + sp.n - 1;
         const long c0 = first / per, c1 = last / per;
         active = (int)(c1 - c0) + 1;
         at = (2 * c0 + 1) * kRows + rr;       // the run in which the unit begins; the others' slots are even
@@ -784,8 +685,12 @@ __global__ void __launch_bounds__(256) join_kernel(const Args x) {
 template <int D>
 int blocks_per_sm(int nt) { return nt == 1 ? Shape<D, 1>::kBlocks : Shape<D, 2>::kBlocks; }
 
-// How the rows are blocked and the tiles are divided.  Blocks of 16 rows where 16-bit queries have more than 8: a tile's
-// codes are then unpacked for twice the rows.  Runs where each request is one block of rows, as many as fit the GPU at
+// How the rows are blocked and the tiles are divided.
+// Chunks: bf16 queries with more than 64 rows per request and kv head go to the tensor-core form, 128 rows a block, unless
+// lse is asked for (its keys are rounded to fp16, which bf16 output hides and an fp32 lse of few keys does not) or heads
+// are 256 wide (two blocks of that form fit an SM up to 128).
+// Otherwise blocks of 16 rows where 16-bit queries have more than 8: a tile's codes are then unpacked for twice the rows.
+// Runs where there are few enough blocks of rows to scan (one per request in this file), as many as fit the GPU at
 // once: a block's start (lengths, page ids, queries) costs it about as much as four tiles a warp, so fewer and longer
 // pieces win (4 x 131001 tokens, 8 kv heads: 140 us, against 145 with one block per unit and split in one wave and 160 in
 // four; 64 ragged requests up to 4096 tokens: 67 against 73 and 69; a window of 4096: 51 against 52 and 79).  Otherwise
@@ -795,17 +700,25 @@ void plan(const Kv4Attn& a, Args& x) {
     x.group = make_div(group);
     x.page_tiles = make_div(a.cache.page_size / kKvTile);
     const long rows = (long)a.max_q * group;
-    x.block_rows = a.dtype != kF32 && rows > 8 ? 16 : 8;
+    const bool chunk = a.dtype == kBF16 && !a.lse && a.cache.head_dim <= 128 && rows > 64;
+    x.tile = chunk ? kChunkTokens : kKvTile;
+    x.block_rows = chunk ? kChunkRows : a.dtype != kF32 && rows > 8 ? 16 : 8;
     x.row_blocks = (int)((rows + x.block_rows - 1) / x.block_rows);
+    const long units_one = (long)a.n_req * x.row_blocks;
     // (a block counts tiles in 32 bits)
-    const long tiles_bound = ((long)a.table_width * (a.cache.page_size / kKvTile) + 1) * a.n_req;
-    if (x.row_blocks == 1 && a.n_req <= kRunReqs && tiles_bound < 1l << 31) {
+    const long tiles_bound = ((long)a.table_width * (a.cache.page_size / kKvTile) + 1) * units_one;
+    x.n_splits = 1;
+    if ((chunk || x.row_blocks == 1) && units_one <= kRunUnits && tiles_bound < 1l << 31) {
         const int nt = a.dtype == kF32 || x.block_rows == 16 ? 2 : 1, d = a.cache.head_dim;
-        x.runs = 148 * (d == 64 ? blocks_per_sm<64>(nt) : d == 128 ? blocks_per_sm<128>(nt) : blocks_per_sm<256>(nt));
+        x.runs = 148 * (chunk ? 2 : d == 64 ? blocks_per_sm<64>(nt) : d == 128 ? blocks_per_sm<128>(nt) : blocks_per_sm<256>(nt));
+        x.run_min = chunk ? 4 : 8;
         // no more than the longest sequences allow
-        const long most = ((long)a.max_seq / kKvTile + 1) * a.n_req * a.cache.n_kv_heads;
-        x.runs = (int)std::max<long>(1, std::min<long>(x.runs, (most + kRunMin - 1) / kRunMin));
-        x.n_splits = 1;
+        const long most = ((long)a.max_seq / x.tile + 1) * units_one * a.cache.n_kv_heads;
+        x.runs = (int)std::max<long>(1, std::min<long>(x.runs, (most + x.run_min - 1) / x.run_min));
+        return;
+    }
+    if (chunk) {        // units enough without splits
+        x.tiles_per_split = 0x7fffffff;
         return;
     }
     const int tiles = std::max(1, (a.max_seq + kKvTile - 1) / kKvTile);
@@ -844,6 +757,7 @@ void run_nt(const Args& x, cudaStream_t s) {
 template <typename T, int D>
 void run(const Args& x, cudaStream_t s) {
     if constexpr (sizeof(T) == 4) run_nt<T, D, 2, true>(x, s);
+    else if (x.tile == kChunkTokens) launch_chunk(x, s);
     else if (x.block_rows == 16) run_nt<T, D, 2, false>(x, s);
     else run_nt<T, D, 1, false>(x, s);
     if (!needs_join(x)) return;
@@ -869,7 +783,7 @@ size_t kv4_attention_workspace(const Kv4Attn& a) {
     x.a = a;
     plan(a, x);
     if (!x.runs && x.n_splits == 1) return 0;
-    return part_bytes(x) + ml_bytes(x) + (x.runs ? sizeof(int) * ((size_t)a.n_req + 1) : 0);
+    return part_bytes(x) + ml_bytes(x) + (x.runs ? sizeof(int) * ((size_t)a.n_req * x.row_blocks + 1) : 0);
 }
 
 int launch_kv4_attention(const Kv4Attn& a, void* workspace, cudaStream_t s) {

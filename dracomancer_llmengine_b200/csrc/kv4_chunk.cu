@@ -1,0 +1,540 @@
+// Attention of chunks over the 4-bit cache on tcgen05: 128 rows (queries x heads of a kv head) a block, 64 tokens a step.
+//
+//   S = Q K^T        128 x 64, Q and K in shared memory (fp16, 128-byte swizzle), S in TMEM (fp32)
+//   P = exp(S - max) by four warps, a row a thread, back into TMEM as fp16 over S
+//   O += P V         128 x D, P from TMEM, V in shared memory with tokens contiguous, O in TMEM (fp32)
+//
+// Warps 0-3 are the softmax (thread = row = TMEM lane), warps 4-7 unpack the cache, and warp 4 issues the products (it would
+// wait for them before its next step in any case; a ninth warp costs every thread registers).  The unpacking warps read a step's codes and scales straight from global memory (L2: the blocks of rows of a request read the
+// same tiles) into registers one step ahead, and write keys (value = s c + m, one rounding to fp16) and values into two
+// buffers of shared memory.  S and P have two buffers in TMEM, so that the next step's scores are computed while this
+// step's softmax runs; two blocks share an SM, so that one's softmax runs while the other's products do.
+//
+// A channel's place inside its group of eight is the order in which a word's nibbles come apart, (0 4 1 5 2 6 3 7), in Q and
+// K alike.  Values of tokens that are not finite are stored as 0 and the token is noted: a row that sees it becomes NaN, one
+// that does not is left alone.  O is rescaled only when a row's maximum grows by more than 3 (log2), as in kv4_attn.cu.
+//
+// Every wait is bounded (2 s).  When one runs out the block raises its flag, all its roles leave their loops, the products
+// in flight are waited for, its rows become NaN, and TMEM is freed.
+#include "kv4_attn.cuh"
+#include "tc_ptx.cuh"
+
+#include <atomic>
+
+namespace draco {
+namespace attn {
+namespace {
+
+constexpr int kTok = kChunkTokens, kRows = kChunkRows;
+constexpr int kThreads = 256;
+constexpr int kTmem = 256;          // columns: O (D), and S/P buffers of 64 from column 128
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+template <int D>
+struct Layout {
+    static constexpr int kQ = kRows * D * 2;        // [D/64][128 rows][128 bytes]
+    static constexpr int kK = kTok * D * 2;         // [D/64][64 tokens][128 bytes]
+    static constexpr int kV = D * kTok * 2;         // [D channels][128 bytes]: 64 tokens
+    static constexpr int kBytes = kQ + 2 * kK + 2 * kV + 1024;
+};
+
+struct Control {
+    uint64_t kv_full[2], s_full[2], p_full[2], pv_done[2], drain;
+    uint64_t bad[2][4];         // tokens of the step with values that are not finite, as each unpacking warp saw it
+    uint32_t valid[2];          // which of the step's four tiles have a page
+    uint32_t tmem;
+    int abort;
+    float qk[kRows];
+};
+
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sync::smem_addr(bar)) : "memory");
+}
+
+// the warp's wait for a phase; false when it ran out or another role gave up
+__device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 0;; i++) {
+        if (__all_sync(0xffffffffu, sync::mbar_try(bar, parity))) return true;
+        if ((i & 63) == 63) {
+            int stop = 0;
+            if ((threadIdx.x & 31) == 0) {
+                if (*abort) stop = 1;
+                else if (t0 == 0) t0 = sync::global_ns();
+                else if (sync::global_ns() - t0 > kWaitNs) stop = 1, *abort = 1;
+            }
+            if (__shfl_sync(0xffffffffu, stop, 0)) return false;
+        }
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void load_global(const void* p, uint32_t (&w)[N]) {
+    if constexpr (N == 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+    } else if constexpr (N == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        w[0] = u.x, w[1] = u.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+__device__ __forceinline__ uint32_t as_word(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ uint32_t or_exponent(uint32_t w, uint32_t mask) {     // (w & mask) | 1024's exponent, twice
+    uint32_t t;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(t) : "r"(w), "r"(mask), "r"(0x64006400u));
+    return t;
+}
+// the four pairs of a word's codes, minus ZERO, times s plus m: halves (0 4) (1 5) (2 6) (3 7) of nibbles
+template <int ZERO>
+__device__ __forceinline__ void values4(uint32_t w, __half2 s, __half2 m, uint32_t (&out)[4]) {
+    const __half2 one = __float2half2_rn(-1024.f - ZERO);                 // 1024 + c         -> c - ZERO, exact
+    const __half2 six = __float2half2_rn(-64.f - ZERO), f = __float2half2_rn(0.0625f);   // 1024 + 16 c, likewise
+    const uint32_t x = w >> 8;
+    out[0] = as_word(__hfma2(__hadd2(as_half2(or_exponent(w, 0x000f000fu)), one), s, m));
+    out[1] = as_word(__hfma2(__hfma2(as_half2(or_exponent(w, 0x00f000f0u)), f, six), s, m));
+    out[2] = as_word(__hfma2(__hadd2(as_half2(or_exponent(x, 0x000f000fu)), one), s, m));
+    out[3] = as_word(__hfma2(__hfma2(as_half2(or_exponent(x, 0x00f000f0u)), f, six), s, m));
+}
+
+// A unit of work of the block, or the part of it that the block's run holds
+struct Segment {
+    Span sp;
+    int kvh, rb, begin, n;      // tiles [begin, begin + n)
+    bool whole;
+    long slot;
+    __device__ __forceinline__ int tile(int j) const {
+        const int idx = begin + j;
+        return idx < sp.head ? idx : sp.first + idx - sp.head;
+    }
+};
+
+// the products, issued by warp 4
+template <int D>
+struct Products {
+    uint64_t dq, dk, dv;
+    uint32_t tmem;
+    Control* c;
+    __device__ __forceinline__ Products(uint8_t* sq, uint8_t* sk, uint8_t* sv, uint32_t t, Control* ctl)
+        : dq(sdesc_sw128(sync::smem_addr(sq))), dk(sdesc_sw128(sync::smem_addr(sk))), dv(sdesc_sw128(sync::smem_addr(sv))),
+          tmem(t), c(ctl) {}
+    __device__ __forceinline__ bool scores(uint32_t step) const {
+        const uint32_t b = step & 1;
+        if (!await(&c->kv_full[b], (step >> 1) & 1, &c->abort)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+            const uint64_t k = dk + (uint64_t)(b * (Layout<D>::kK >> 4));
+#pragma unroll
+            for (int h = 0; h < D / 64; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    tc_mma_ss(tmem + 128 + 64 * b, dq + (uint64_t)(h * (kRows * 128 >> 4) + 2 * i),
+                              k + (uint64_t)(h * (kTok * 128 >> 4) + 2 * i), idesc_f16(kTok), h || i);
+            tc_commit(&c->s_full[b]);
+        }
+        __syncwarp();
+        return true;
+    }
+    __device__ __forceinline__ bool output(uint32_t step, bool first) const {
+        const uint32_t b = step & 1;
+        if (!await(&c->p_full[b], (step >> 1) & 1, &c->abort)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+            const uint64_t v = dv + (uint64_t)(b * (Layout<D>::kV >> 4));
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                tc_mma_ts(tmem, tmem + 128 + 64 * b + 8 * i, v + (uint64_t)(2 * i), idesc_f16(D), !first || i);
+            tc_commit(&c->pv_done[b]);
+        }
+        __syncwarp();
+        return true;
+    }
+};
+
+// ---- warps 4-7 ----
+template <int D>
+__device__ __forceinline__ void unpack_role(const Args& x, const Segment& g, Control* c, uint8_t* sq, uint8_t* sk, uint8_t* sv,
+                                            uint32_t step0, int req, uint32_t tmem) {
+    constexpr int NG = D / kKvGroup, GV = NG / 2, kTileB = kv4_tile_bytes(D);
+    const Kv4Attn& a = x.a;
+    const int warp = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31;
+    const int* table = a.table + (long)req * a.table_stride;
+    // where eight steps' tiles lie, one per lane (tile ordinal in the cache, -1: no page, or behind the sequence)
+    auto fetch = [&](int j0) {
+        const int j = j0 + (lane >> 2);
+        if (j >= g.n) return -1;
+        const int ct = g.tile(j) * (kTok / kKvTile) + (lane & 3);
+        if (ct * kKvTile >= g.sp.seq) return -1;
+        const int p = ct / x.page_tiles, page = table[p];
+        if (page < 0 || page >= a.cache.n_pages) return -1;
+        return (page * a.cache.n_kv_heads + g.kvh) * x.page_tiles.d + (ct - p * x.page_tiles.d);
+    };
+    int where = fetch(0), where_next = fetch(8);
+    // keys: this warp's 16 tokens, lane (q, token), twice; values: channels n*4 .. of all groups gh*GV .., 8 tokens each
+    const int kt = lane & 7, kq = lane >> 3, tq = lane & 7, vn = warp * 2 + ((lane >> 3) & 1), gh = lane >> 4;
+    uint32_t kw[2][NG], ks[2][NG], km[2][NG / 2], vw[4][GV], vs[4][GV], vm[4][GV];
+    auto load = [&](int j) {
+        const int at = (j & 7) * 4;
+        const int ok = __shfl_sync(0xffffffffu, where, at + warp), ov = __shfl_sync(0xffffffffu, where, at + (tq >> 1));
+        const uint8_t* pk = a.cache.pages + (size_t)max(ok, 0) * kTileB;
+        const uint8_t* pv = a.cache.pages + (size_t)max(ov, 0) * kTileB;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int t = kt + 8 * u;
+            load_global<NG>(pk + (t * 4 + kq) * NG * 4, kw[u]);
+            load_global<NG>(pk + kv4_off_ks(D) + (t >> 1) * NG * 4, ks[u]);
+            load_global<NG / 2>(pk + kv4_off_km(D) + t * NG * 2, km[u]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int tp = (tq & 1) * 4 + k;
+            load_global<GV>(pv + kv4_off_vc(D) + ((tp * 8 + vn) * NG + gh * GV) * 4, vw[k]);
+            load_global<GV>(pv + kv4_off_vs(D) + (tp * NG + gh * GV) * 4, vs[k]);
+            load_global<GV>(pv + kv4_off_vm(D) + (tp * NG + gh * GV) * 4, vm[k]);
+        }
+        // a tile without a page: zeros (its bytes were tile 0's)
+        if (ov < 0) {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int i = 0; i < GV; i++) vs[k][i] = vm[k][i] = 0;
+        }
+    };
+    const Products<D> products(sq, sk, sv, tmem, c);
+    load(0);
+    for (int j = 0; j < g.n; j++) {
+        const uint32_t step = step0 + j, b = step & 1;
+        if (step >= 2 && !await(&c->pv_done[b], ((step >> 1) & 1) ^ 1, &c->abort)) return;
+        const uint32_t valid = __ballot_sync(0xffffffffu, where >= 0) >> ((j & 7) * 4) & 15u;
+        uint8_t* k = sk + b * Layout<D>::kK;
+        uint8_t* v = sv + b * Layout<D>::kV;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int t = kt + 8 * u, row = warp * kKvTile + t;
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                const __half2 s2 = as_half2(ks[u][i]), m2 = as_half2(km[u][i >> 1]);
+                uint32_t o[4];
+                values4<0>(kw[u][i], t & 1 ? __high2half2(s2) : __low2half2(s2), i & 1 ? __high2half2(m2) : __low2half2(m2), o);
+                const int unit = (i & 1) * 4 + kq;      // 16 bytes of a 128-byte row: two groups
+                *reinterpret_cast<uint4*>(k + (i >> 1) * kTok * 128 + row * 128 + ((unit ^ (row & 7)) << 4)) =
+                    make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+        // tokens behind the sequence have no values; values that are not finite are noted and left out
+        const int left = g.sp.seq - g.tile(j) * kTok - tq * 8;      // of this lane's 8 tokens
+        uint32_t bad = 0;
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            const uint32_t keep = left >= 2 * p + 2 ? 0xffffffffu : left == 2 * p + 1 ? 0xffffu : 0u;
+#pragma unroll
+            for (int i = 0; i < GV; i++) {
+                uint32_t &s = vs[p][i], &m = vm[p][i];
+                s &= keep, m &= keep;
+                const __half2 z = __float2half2_rn(0.f);
+                if (as_word(__hfma2(as_half2(s), z, __hmul2(as_half2(m), z))) & 0x7fff7fffu) {
+                    const auto open = [](uint32_t w) { return (w & 0x7c00u) == 0x7c00u; };
+                    const bool b0 = open(s) || open(m), b1 = open(s >> 16) || open(m >> 16);
+                    const uint32_t fine = (b0 ? 0u : 0xffffu) | (b1 ? 0u : 0xffff0000u);
+                    s &= fine, m &= fine;
+                    bad |= (uint32_t)b0 << (2 * p) | (uint32_t)b1 << (2 * p + 1);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < GV; i++) {
+            uint32_t o[4][4];       // [token pair][channel]
+#pragma unroll
+            for (int p = 0; p < 4; p++) values4<8>(vw[p][i], as_half2(vs[p][i]), as_half2(vm[p][i]), o[p]);
+#pragma unroll
+            for (int ch = 0; ch < 4; ch++) {
+                const int row = (gh * GV + i) * kKvGroup + vn * 4 + ch;
+                *reinterpret_cast<uint4*>(v + row * 128 + ((tq ^ (row & 7)) << 4)) =
+                    make_uint4(o[0][ch], o[1][ch], o[2][ch], o[3][ch]);
+            }
+        }
+        uint64_t all = 0;
+        if (__any_sync(0xffffffffu, bad != 0)) {
+            const uint32_t lo = __reduce_or_sync(0xffffffffu, tq < 4 ? bad << (8 * tq) : 0u);
+            const uint32_t hi = __reduce_or_sync(0xffffffffu, tq < 4 ? 0u : bad << (8 * (tq - 4)));
+            all = (uint64_t)hi << 32 | lo;
+        }
+        if (lane == 0) {
+            c->bad[b][warp] = all;
+            if (warp == 0) c->valid[b] = valid;
+        }
+        sync::fence_proxy_async();      // the products read shared memory through the other proxy
+        __syncwarp();
+        if (lane == 0) arrive(&c->kv_full[b]);
+        if ((j & 7) == 7) {
+            where = where_next;
+            where_next = fetch(j + 9);
+        }
+        if (j + 1 < g.n) load(j + 1);
+        // this step's scores, then the output of the step before (its softmax ran meanwhile)
+        if (warp == 0 && (!products.scores(step) || (j && !products.output(step - 1, j == 1)))) return;
+    }
+    if (warp == 0) products.output(step0 + g.n - 1, g.n == 1);
+}
+
+// ---- warps 0-3 ----
+template <int D>
+__device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Control* c, uint32_t step0, uint32_t tmem) {
+    using T = __nv_bfloat16;
+    const Kv4Attn& a = x.a;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const uint32_t mine = tmem + ((uint32_t)(tid >> 5) << 21);       // this warp's 32 lanes
+    const int row = g.rb * kRows + tid, ti = row / x.group;
+    const int pos_q = g.sp.seq - g.sp.q_len + ti;
+    const float qk = c->qk[tid];
+    float m = kNone, l = 0.f;
+    bool ok = !c->abort;
+    for (int j = 0; j < g.n && ok; j++) {
+        const uint32_t step = step0 + j, b = step & 1, parity = (step >> 1) & 1;
+        ok = await(&c->kv_full[b], parity, &c->abort) && await(&c->s_full[b], parity, &c->abort);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t at = mine + 128 + 64 * b;
+        uint32_t v[2][32];
+        tc_ld32(at, v[0]);
+        tc_ld32(at + 32, v[1]);
+        tc_wait_ld();
+        const int base = g.tile(j) * kTok;
+        const uint32_t valid = c->valid[b];
+        const uint64_t bad = c->bad[b][0] | c->bad[b][1] | c->bad[b][2] | c->bad[b][3];
+        const bool part = base + kTok - 1 > g.sp.p_lo || valid != 15u ||
+                          (a.window > 0 && base <= g.sp.p_hi - a.window && base + kTok > a.sinks);
+        bool poison = false;
+        if (part || bad) {
+#pragma unroll
+            for (int i = 0; i < 64; i++) {
+                const int pos = base + i;
+                const bool sees = pos <= pos_q && (a.window <= 0 || pos > pos_q - a.window || pos < a.sinks) &&
+                                  (valid >> (i >> 4) & 1);
+                if (!sees) v[i >> 5][i & 31] = 0xff800000u;
+                poison |= sees && (bad >> i & 1);
+            }
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 64; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i >> 5][i & 31]));
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * qk;
+        if (__any_sync(0xffffffffu, mx - m > kSlack)) {
+            const float now = fmaxf(m, mx), f = ex2(m - now);
+            m = now;
+            l *= f;
+            if (j) {        // the sums so far, once the previous step's product is in them
+                ok = await(&c->pv_done[b ^ 1], ((step - 1) >> 1) & 1, &c->abort);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int h = 0; h < D / 16; h++) {
+                    uint32_t o[16];
+                    tc_ld16(mine + 16 * h, o);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tc_st16(mine + 16 * h, o);
+                }
+            }
+        }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t p[32];
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            const float e0 = ex2(fmaf(__uint_as_float(v[i >> 4][2 * (i & 15)]), qk, -m));
+            const float e1 = ex2(fmaf(__uint_as_float(v[i >> 4][2 * (i & 15) + 1]), qk, -m));
+            sum[i & 3] += e0 + e1;
+            p[i] = pack2<__half>(e0, e1);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (poison) l = __uint_as_float(0x7fffffffu);
+        tc_st32(at, p);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(&c->p_full[b]);
+    }
+    if (ok) {
+        const uint32_t step = step0 + g.n - 1;
+        ok = await(&c->pv_done[step & 1], (step >> 1) & 1, &c->abort);
+        tc_fence_after();
+    }
+    // ---- the rows' results ----
+    const bool has_row = row < g.sp.q_len * x.group.d;
+    const float n = !ok ? __uint_as_float(0x7fffffffu) : !g.whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    const int hd = g.kvh * x.group.d + row - ti * x.group.d;
+    T* dst = (T*)a.out + (long)(g.sp.q0 + ti) * a.o_tok + (long)hd * a.o_head;
+    float* part = x.part + (g.slot * kRows + tid) * D;
+#pragma unroll
+    for (int h = 0; h < D / 32; h++) {
+        uint32_t o[32];
+        tc_ld32(mine + 32 * h, o);
+        tc_wait_ld();
+        if (has_row && g.whole) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float f[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) f[k] = __uint_as_float(o[8 * i + k]) * n;
+                store8<T>(dst + 32 * h + 8 * i, x.wide_o, f);
+            }
+        } else if (has_row) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                reinterpret_cast<float4*>(part + 32 * h)[i] =
+                    make_float4(__uint_as_float(o[4 * i]) * n, __uint_as_float(o[4 * i + 1]) * n,
+                                __uint_as_float(o[4 * i + 2]) * n, __uint_as_float(o[4 * i + 3]) * n);
+        }
+        __syncwarp();       // together again for the next copy from TMEM
+    }
+    if (has_row && !g.whole) x.ml[g.slot * kRows + tid] = make_float2(m, l);
+    tc_fence_before();
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 2) chunk_kernel(const Args x) {
+    extern __shared__ uint8_t raw[];
+    __shared__ Control ctl;
+    __shared__ int s_before[kRunUnits + 1];
+    uint8_t* sq = raw + ((1024 - (sync::smem_addr(raw) & 1023)) & 1023);
+    uint8_t* sk = sq + Layout<D>::kQ;
+    uint8_t* sv = sk + 2 * Layout<D>::kK;
+    Control* c = &ctl;
+    const Kv4Attn& a = x.a;
+    const int tid = threadIdx.x, warp = tid >> 5;
+    early_launch();
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            sync::mbar_init(&c->kv_full[i], 4);
+            sync::mbar_init(&c->s_full[i], 1);
+            sync::mbar_init(&c->p_full[i], 4);
+            sync::mbar_init(&c->pv_done[i], 1);
+        }
+        sync::mbar_init(&c->drain, 1);
+        c->abort = 0;
+        sync::fence_init();
+    }
+    wait_for_inputs();
+    // this block's work, the same in every thread
+    Segment g;
+    int req, f = 0;
+    long left = 0;
+    if (x.runs) {
+        scan_units<kThreads>(x, s_before);
+        if (blockIdx.x == 0)
+            for (int i = tid; i <= a.n_req * x.row_blocks; i += kThreads) x.before[i] = s_before[i];
+        const Run run = run_of(x, s_before);
+        if (!run.left) return;
+        f = run.f, g.kvh = run.kvh, g.begin = run.begin, left = run.left;
+    } else {
+        g.rb = blockIdx.x, g.kvh = blockIdx.y, req = blockIdx.z;
+        if (!span_of(x, req, g.rb, g.sp)) return;
+        g.begin = 0, g.n = g.sp.n, g.whole = true, g.slot = 0;
+    }
+    if (warp == 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sync::smem_addr(&c->tmem)),
+                     "r"(kTmem)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = c->tmem;
+
+    for (uint32_t step0 = 0;;) {
+        if (x.runs) {
+#pragma unroll 1
+            for (;; f++) {      // blocks of rows without queries have no tiles
+                req = f / x.row_blocks, g.rb = f - req * x.row_blocks;
+                if (span_of(x, req, g.rb, g.sp)) break;
+            }
+            g.n = (int)min((long)g.sp.n - g.begin, left);
+            left -= g.n;
+            g.whole = g.begin == 0 && g.n == g.sp.n;
+            g.slot = 2 * (long)blockIdx.x + (g.begin == 0);
+        }
+        // ---- the rows' queries, scaled to |q| <= 1 by a power of two per row: a thread takes 8 channels ----
+        const int rows = g.sp.q_len * x.group.d;
+        for (int i = tid; i < kRows * (D / 8); i += kThreads) {      // a row lies in D / 8 lanes of one warp
+            const int rr = i / (D / 8), c8 = i % (D / 8), row = g.rb * kRows + rr;
+            float v[8];
+            if (row < rows) {
+                const int tok = row / x.group, head = g.kvh * x.group.d + row - tok * x.group.d;
+                load8<__nv_bfloat16>((const __nv_bfloat16*)a.q + (long)(g.sp.q0 + tok) * a.q_tok + (long)head * a.q_head + c8 * 8,
+                                     x.wide_q, v);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = 0.f;
+            }
+            float top = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(v[k]));
+#pragma unroll
+            for (int o = 1; o < D / 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            int ex = (int)((__float_as_uint(top) >> 23) & 255) - 126;
+            ex = min(max(ex, -120), 120);
+            const float down = __uint_as_float((uint32_t)(127 - ex) << 23), up = __uint_as_float((uint32_t)(127 + ex) << 23);
+            uint4 w;
+            w.x = pack2<__half>(v[0] * down, v[4] * down);
+            w.y = pack2<__half>(v[1] * down, v[5] * down);
+            w.z = pack2<__half>(v[2] * down, v[6] * down);
+            w.w = pack2<__half>(v[3] * down, v[7] * down);
+            *reinterpret_cast<uint4*>(sq + (c8 >> 3) * kRows * 128 + rr * 128 + (((c8 & 7) ^ (rr & 7)) << 4)) = w;
+            if (c8 == 0) c->qk[rr] = fmaxf(a.scale * kLog2e * up, 1.2e-38f);    // never 0: hidden scores are -infinity
+        }
+        sync::fence_proxy_async();
+        __syncthreads();
+        if (!c->abort || warp < 4) {
+            if (warp < 4) softmax_role<D>(x, g, c, step0, tmem);
+            else unpack_role<D>(x, g, c, sq, sk, sv, step0, req, tmem);
+        }
+        step0 += g.n;
+        if (left <= 0) break;
+        g.begin = 0;
+        if (++g.kvh == a.cache.n_kv_heads) g.kvh = 0, f++;
+        __syncthreads();        // queries and TMEM are read; the next unit's go over them
+        tc_fence_after();
+    }
+    if (warp == 4) {            // every product issued must be complete before TMEM is released
+        if (elect_one()) {
+            tc_commit(&c->drain);
+            sync::mbar_wait(&c->drain, 0);
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 4) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem) : "memory");
+    }
+}
+
+template <int D>
+void run(const Args& x, cudaStream_t s) {
+    const int smem = Layout<D>::kBytes;
+    static std::atomic<uint64_t> ready{0};      // devices on which the kernel may use its shared memory
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev > 63 || !(ready.load() >> dev & 1)) {
+        cudaFuncSetAttribute(chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (dev < 64) ready |= (uint64_t)1 << dev;
+    }
+    const dim3 grid = x.runs ? dim3((unsigned)x.runs)
+                             : dim3((unsigned)x.row_blocks, (unsigned)x.a.cache.n_kv_heads, (unsigned)x.a.n_req);
+    launch(chunk_kernel<D>, grid, dim3(kThreads), smem, s, x);
+}
+
+}  // namespace
+
+void launch_chunk(const Args& x, cudaStream_t s) {
+    if (x.a.cache.head_dim == 64) run<64>(x, s);
+    else run<128>(x, s);
+}
+
+}  // namespace attn
+}  // namespace draco

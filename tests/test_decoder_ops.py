@@ -286,7 +286,7 @@ def attend_ref(cache, table, q, cu, lens, window, sinks, scale=None):
 
 
 def attend_case(seed, kind, lens, q_lens, heads, hkv, d, page, window=0, sinks=0, max_seq=None, stride=False, scale=None,
-                holes=False):
+                holes=False, with_lse=True):
     rng = np.random.default_rng(seed)
     cache, table = make_cache(rng, lens, page, hkv, d)
     if holes:
@@ -302,7 +302,7 @@ def attend_case(seed, kind, lens, q_lens, heads, hkv, d, page, window=0, sinks=0
         out = torch.full((heads, n, d + 3), 5.0, dtype=TYPES[kind], device="cuda").transpose(0, 1)[..., 1:d + 1]
     else:
         out = torch.full((n, heads, d), 5.0, dtype=TYPES[kind], device="cuda")
-    lse = torch.full((n, heads), 5.0, device="cuda")
+    lse = torch.full((n, heads), 5.0, device="cuda") if with_lse else None
     cache.attend(q, out, ints(cu), ints(lens), torch.from_numpy(table).cuda(), max(q_lens), max_seq or max(lens),
                  scale=scale, window=window, sinks=sinks, lse=lse)
     seen_table = np.where((table >= 0) & (table < cache.pages.shape[0]), table, -1)
@@ -310,7 +310,10 @@ def attend_case(seed, kind, lens, q_lens, heads, hkv, d, page, window=0, sinks=0
     assert torch.isfinite(out).all()
     assert rel(out, want) <= TOL[kind]
     empty = torch.isinf(want_lse)
-    assert torch.equal(torch.isinf(lse).cpu(), empty) and not out.cpu()[empty].any()
+    assert not out.cpu()[empty].any()
+    if not with_lse:
+        return cache, table, q, out
+    assert torch.equal(torch.isinf(lse).cpu(), empty)
     # lse of size ~10: a few units in the last place of fp32
     assert float((lse.cpu().double() - want_lse)[~empty].abs().max() if (~empty).any() else 0) <= 2e-5
     return cache, table, q, out
@@ -340,6 +343,36 @@ def test_attend_chunks(kind, heads, hkv, d, window, sinks):
     attend_case(d + window, kind, [200, 65, 300, 9, 70, 128], [200, 1, 37, 13, 0, 128], heads, hkv, d, 16, window, sinks)
 
 
+@pytest.mark.parametrize("heads,hkv,d,page", [(8, 1, 128, 16), (4, 4, 64, 48), (6, 2, 128, 64), (16, 1, 64, 16)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (33, 5), (1, 0), (64, 200), (500, 64)])
+def test_attend_bf16_chunks_without_lse(heads, hkv, d, page, window, sinks):
+    """Blocks of 128 rows: whole sequences, chunks behind long contexts, single tokens beside them, no queries at all, more
+    queries than cached tokens, row counts around the block's."""
+    attend_case(d + window, "bf16", [200, 65, 300, 9, 70, 128, 1500, 0, 64], [200, 1, 37, 13, 0, 128, 150, 3, 16], heads, hkv, d,
+                page, window, sinks, with_lse=False)
+
+
+def test_attend_bf16_chunks_strides_holes_and_bounds():
+    attend_case(51, "bf16", [90, 400], [80, 70], 8, 2, 128, 16, stride=True, scale=0.03, with_lse=False)
+    attend_case(52, "bf16", [100, 277], [40, 100], 8, 2, 128, 16, holes=True, with_lse=False)
+    attend_case(53, "bf16", [3000, 20], [70, 20], 8, 2, 128, 32, max_seq=100, with_lse=False)   # a bound that is too low
+    attend_case(54, "bf16", [17], [17], 40, 8, 128, 16, with_lse=False)
+
+
+def test_attend_bf16_chunks_many_requests():
+    """More blocks of rows than one block scans."""
+    rng = np.random.default_rng(8)
+    q_lens = rng.integers(0, 70, 600).tolist()
+    lens = [int(q + e) for q, e in zip(q_lens, rng.integers(0, 50, 600))]
+    q_lens[5], lens[5] = 70, 90
+    attend_case(55, "bf16", lens, q_lens, 4, 1, 64, 16, with_lse=False)
+
+
+def test_attend_bf16_chunks_long_splits():
+    """A chunk behind a long context: its tiles lie in many blocks' runs."""
+    attend_case(56, "bf16", [9000, 300, 5], [33, 20, 5], 8, 2, 128, 64, with_lse=False)
+
+
 @pytest.mark.parametrize("kind", TYPES)
 def test_attend_strides_and_scale(kind):
     attend_case(5, kind, [90, 400], [2, 1], 8, 2, 128, 16, stride=True, scale=0.03)
@@ -359,15 +392,17 @@ def test_attend_pages_outside_the_cache(kind, q_lens):
 
 
 @pytest.mark.parametrize("kind", TYPES)
-@pytest.mark.parametrize("rows", [1, 21])
-def test_attend_hidden_nan(kind, rows):
+@pytest.mark.parametrize("rows", [1, 21, 80])
+@pytest.mark.parametrize("value_only", [False, True])
+def test_attend_hidden_nan(kind, rows, value_only):
     """Infinities and NaN in tokens that a row does not see leave it alone, and reach every row that sees them."""
     rng = np.random.default_rng(3)
     n, window, d, hkv = 150, 20, 128, 2
     cache, table = make_cache(rng, [n], 16, hkv, d)
     bad = torch.full((1, hkv, d), float("nan"), device="cuda")
+    fine = torch.ones(1, hkv, d, device="cuda")
     pos = 110      # hidden for a single token (position 149); inside the window of queries 129 .. 110 + 19
-    cache.append(bad, bad, ints([int(table[0, pos // 16]) * 16 + pos % 16]))
+    cache.append(fine if value_only else bad, bad, ints([int(table[0, pos // 16]) * 16 + pos % 16]))
     q = torch.from_numpy(rng.standard_normal((rows, 4, d)).astype(np.float32)).cuda().to(TYPES[kind])
     out = torch.empty_like(q)
     cache.attend(q, out, ints([0, rows]), ints([n]), torch.from_numpy(table).cuda(), rows, n, window=window, sinks=3)
