@@ -686,9 +686,9 @@ template <int D>
 int blocks_per_sm(int nt) { return nt == 1 ? Shape<D, 1>::kBlocks : Shape<D, 2>::kBlocks; }
 
 // How the rows are blocked and the tiles are divided.
-// Chunks: bf16 queries with more than 64 rows per request and kv head go to the tensor-core form, 128 rows a block, unless
+// Chunks: bf16 queries with more than 64 rows per request and kv head go to the tensor-core form, 256 rows a block, unless
 // lse is asked for (its keys are rounded to fp16, which bf16 output hides and an fp32 lse of few keys does not) or heads
-// are 256 wide (two blocks of that form fit an SM up to 128).
+// are 256 wide (the sums of two halves of the rows fill TMEM at 128).
 // Otherwise blocks of 16 rows where 16-bit queries have more than 8: a tile's codes are then unpacked for twice the rows.
 // Runs where there are few enough blocks of rows to scan (one per request in this file), as many as fit the GPU at
 // once: a block's start (lengths, page ids, queries) costs it about as much as four tiles a warp, so fewer and longer
@@ -710,7 +710,7 @@ void plan(const Kv4Attn& a, Args& x) {
     x.n_splits = 1;
     if ((chunk || x.row_blocks == 1) && units_one <= kRunUnits && tiles_bound < 1l << 31) {
         const int nt = a.dtype == kF32 || x.block_rows == 16 ? 2 : 1, d = a.cache.head_dim;
-        x.runs = 148 * (chunk ? 2 : d == 64 ? blocks_per_sm<64>(nt) : d == 128 ? blocks_per_sm<128>(nt) : blocks_per_sm<256>(nt));
+        x.runs = 148 * (chunk ? 1 : d == 64 ? blocks_per_sm<64>(nt) : d == 128 ? blocks_per_sm<128>(nt) : blocks_per_sm<256>(nt));
         x.run_min = chunk ? 4 : 8;
         // no more than the longest sequences allow
         const long most = ((long)a.max_seq / x.tile + 1) * units_one * a.cache.n_kv_heads;

@@ -120,8 +120,8 @@ __device__ __forceinline__ Run run_of(const Args& x, const int* before) {
     return Run{lo, kvh, in - kvh * n, min((long)per, total - start)};
 }
 
-// chunks of bf16 queries on the tensor cores' fifth-generation path (kv4_chunk.cu): 128 rows and 64 tokens a step
-constexpr int kChunkRows = 128, kChunkTokens = 64;
+// chunks of bf16 queries on the tensor cores' fifth-generation path (kv4_chunk.cu): 256 rows and 64 tokens a step
+constexpr int kChunkRows = 256, kChunkTokens = 64;
 void launch_chunk(const Args& x, cudaStream_t s);
 
 }  // namespace attn

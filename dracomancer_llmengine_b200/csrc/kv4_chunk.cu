@@ -1,18 +1,25 @@
-// Attention of chunks over the 4-bit cache on tcgen05: 128 rows (queries x heads of a kv head) a block, 64 tokens a step.
+// Attention of chunks over the 4-bit cache on tcgen05: 256 rows (queries x heads of a kv head) a block, 64 tokens a step.
 //
-//   S = Q K^T        128 x 64, Q and K in shared memory (fp16, 128-byte swizzle), S in TMEM (fp32)
-//   P = exp(S - max) by four warps, a row a thread, back into TMEM as fp16 over S
-//   O += P V         128 x D, P from TMEM, V in shared memory with tokens contiguous, O in TMEM (fp32)
+//   S = Q K^T        two products of 128 x 64, Q and K in shared memory (fp16, 128-byte swizzle), S in TMEM (fp32)
+//   P = exp(S - max) by two groups of four warps, a row a thread, back into TMEM as fp16 over S
+//   O += P V         128 x D each, P from TMEM, V in shared memory with tokens contiguous, O in TMEM (fp32)
 //
-// Warps 0-3 are the softmax (thread = row = TMEM lane), warps 4-7 unpack the cache, and warp 4 issues the products (it would
-// wait for them before its next step in any case; a ninth warp costs every thread registers).  The unpacking warps read a step's codes and scales straight from global memory (L2: the blocks of rows of a request read the
-// same tiles) into registers one step ahead, and write keys (value = s c + m, one rounding to fp16) and values into two
-// buffers of shared memory.  S and P have two buffers in TMEM, so that the next step's scores are computed while this
-// step's softmax runs; two blocks share an SM, so that one's softmax runs while the other's products do.
+// Warps 0-7 are the softmax (thread = row, TMEM lane = row mod 128), warps 8-11 and 12-15 unpack the cache for even and odd
+// steps, warps 16 and 17 issue the products of the two halves of the rows.  The unpacking warps read a step's codes and
+// scales straight from global memory (L2: the blocks of rows of a request read the same tiles) into registers ahead of
+// time, and write keys (value = s c + m, one rounding to fp16) and values into one of four buffers in shared memory.  S and P
+// have two buffers, so that a step's scores are computed beside the previous step's softmax.  (With two buffers of K and V a
+// step took 3600 cycles: from a product's end through unpacking, scores, softmax and product again is two steps' way.)
+//
+// Measured at 4 chunks of up to 512 queries x 32 heads over contexts up to 8192 (195 GFLOP): 283 us, 0.69 PFLOP/s, 2500
+// cycles a step: softmax 2100 (1120 for the 64 exponentials a row, of which both halves' on the exponential unit alone are
+// 1024), products 1220.  Blocks of 128 rows with four unpacking warps, one of which issued the products, two blocks an SM:
+// 392 us (unpacking 2270 cycles a step, issuing 950: each wait on a barrier costs the issuing warp about 290).
 //
 // A channel's place inside its group of eight is the order in which a word's nibbles come apart, (0 4 1 5 2 6 3 7), in Q and
 // K alike.  Values of tokens that are not finite are stored as 0 and the token is noted: a row that sees it becomes NaN, one
-// that does not is left alone.  O is rescaled only when a row's maximum grows by more than 3 (log2), as in kv4_attn.cu.
+// that does not is left alone.  O is rescaled only when a row's maximum grows by more than 8 (log2): weights then go up to
+// 256, which fp16 has room for, and the rescaling waits for the product before it, so it should be rare.
 //
 // Every wait is bounded (2 s).  When one runs out the block raises its flag, all its roles leave their loops, the products
 // in flight are waited for, its rows become NaN, and TMEM is freed.
@@ -26,22 +33,29 @@ namespace attn {
 namespace {
 
 constexpr int kTok = kChunkTokens, kRows = kChunkRows;
-constexpr int kThreads = 256;
-constexpr int kTmem = 256;          // columns: O (D), and S/P buffers of 64 from column 128
+constexpr int kThreads = 576;
+constexpr int kBufs = 4;            // of K and V
+// TMEM columns: O of the two halves at 0 and 128, their S/P buffers of 64 from 256 and 384
+constexpr int kTmem = 512;
+__device__ __forceinline__ uint32_t tmem_o(uint32_t tmem, int half) { return tmem + 128 * half; }
+__device__ __forceinline__ uint32_t tmem_s(uint32_t tmem, int half, uint32_t b) { return tmem + 256 + 128 * half + 64 * b; }
+constexpr float kRoom = 8.f;        // log2 of the largest weight
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 template <int D>
 struct Layout {
-    static constexpr int kQ = kRows * D * 2;        // [D/64][128 rows][128 bytes]
+    static constexpr int kQ = kRows * D * 2;        // [D/64][256 rows][128 bytes]
     static constexpr int kK = kTok * D * 2;         // [D/64][64 tokens][128 bytes]
     static constexpr int kV = D * kTok * 2;         // [D channels][128 bytes]: 64 tokens
-    static constexpr int kBytes = kQ + 2 * kK + 2 * kV + 1024;
+    static constexpr int kBytes = kQ + kBufs * (kK + kV) + 1024;
 };
 
-struct Control {
-    uint64_t kv_full[2], s_full[2], p_full[2], pv_done[2], drain;
-    uint64_t bad[2][4];         // tokens of the step with values that are not finite, as each unpacking warp saw it
-    uint32_t valid[2];          // which of the step's four tiles have a page
+struct alignas(16) Control {
+    uint64_t kv_full[kBufs], s_full[2][2], p_full[2][2], pv_done[2][kBufs], drain[2];      // [half][buffer]
+    // what a step's unpacking warps saw: each tile's page is there (0xf) with finite values only, or not
+    uint32_t fine[kBufs][4];
+    uint64_t bad[kBufs][4];     // tokens of the step with values that are not finite
+    uint32_t valid[kBufs];          // which of the step's four tiles have a page
     uint32_t tmem;
     int abort;
     float qk[kRows];
@@ -51,11 +65,22 @@ __device__ __forceinline__ void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sync::smem_addr(bar)) : "memory");
 }
 
+// one try, which the hardware may hold for a while but ends when the phase does (a time hint made it sleep past that:
+// 414 us for the measured chunks)
+__device__ __forceinline__ bool try_phase(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(sync::smem_addr(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // the warp's wait for a phase; false when it ran out or another role gave up
 __device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity, volatile int* abort) {
     uint64_t t0 = 0;
     for (uint32_t i = 0;; i++) {
-        if (__all_sync(0xffffffffu, sync::mbar_try(bar, parity))) return true;
+        if (__all_sync(0xffffffffu, try_phase(bar, parity))) return true;
         if ((i & 63) == 63) {
             int stop = 0;
             if ((threadIdx.x & 31) == 0) {
@@ -66,6 +91,27 @@ __device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity, volatile i
             if (__shfl_sync(0xffffffffu, stop, 0)) return false;
         }
     }
+}
+
+// two floats in one register pair: one instruction for both
+__device__ __forceinline__ uint64_t join(uint32_t a, uint32_t b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t twice(float a) { return join(__float_as_uint(a), __float_as_uint(a)); }
+__device__ __forceinline__ void split(uint64_t d, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 
 template <int N>
@@ -111,59 +157,60 @@ struct Segment {
     }
 };
 
-// the products, issued by warp 4
+// ---- warps 16 and 17: the products of one half of the rows ----
 template <int D>
-struct Products {
-    uint64_t dq, dk, dv;
-    uint32_t tmem;
-    Control* c;
-    __device__ __forceinline__ Products(uint8_t* sq, uint8_t* sk, uint8_t* sv, uint32_t t, Control* ctl)
-        : dq(sdesc_sw128(sync::smem_addr(sq))), dk(sdesc_sw128(sync::smem_addr(sk))), dv(sdesc_sw128(sync::smem_addr(sv))),
-          tmem(t), c(ctl) {}
-    __device__ __forceinline__ bool scores(uint32_t step) const {
-        const uint32_t b = step & 1;
-        if (!await(&c->kv_full[b], (step >> 1) & 1, &c->abort)) return false;
+__device__ __forceinline__ void product_role(const Segment& g, Control* c, uint8_t* sq, uint8_t* sk, uint8_t* sv, uint32_t step0,
+                                             uint32_t tmem, int half) {
+    const uint64_t dq = sdesc_sw128(sync::smem_addr(sq)) + (uint64_t)(half * (128 * 128 >> 4));
+    const uint64_t dk = sdesc_sw128(sync::smem_addr(sk)), dv = sdesc_sw128(sync::smem_addr(sv));
+    auto scores = [&](uint32_t step) {
+        const uint32_t b = step & 1, kv = step % kBufs;
+        if (!await(&c->kv_full[kv], step / kBufs & 1, &c->abort)) return false;
         tc_fence_after();
         if (elect_one()) {
-            const uint64_t k = dk + (uint64_t)(b * (Layout<D>::kK >> 4));
+            const uint64_t k = dk + (uint64_t)(kv * (Layout<D>::kK >> 4));
 #pragma unroll
             for (int h = 0; h < D / 64; h++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    tc_mma_ss(tmem + 128 + 64 * b, dq + (uint64_t)(h * (kRows * 128 >> 4) + 2 * i),
+                    tc_mma_ss(tmem_s(tmem, half, b), dq + (uint64_t)(h * (kRows * 128 >> 4) + 2 * i),
                               k + (uint64_t)(h * (kTok * 128 >> 4) + 2 * i), idesc_f16(kTok), h || i);
-            tc_commit(&c->s_full[b]);
+            tc_commit(&c->s_full[half][b]);
         }
         __syncwarp();
         return true;
-    }
-    __device__ __forceinline__ bool output(uint32_t step, bool first) const {
-        const uint32_t b = step & 1;
-        if (!await(&c->p_full[b], (step >> 1) & 1, &c->abort)) return false;
+    };
+    if (!scores(step0)) return;
+    for (int j = 0; j < g.n; j++) {
+        const uint32_t step = step0 + j, b = step & 1;
+        // the next step's scores go ahead of this step's softmax.  Their buffer held the weights of the step before this one,
+        // whose product this thread issued earlier: products complete in order
+        if (j + 1 < g.n && !scores(step + 1)) return;
+        if (!await(&c->p_full[half][b], (step >> 1) & 1, &c->abort)) return;
         tc_fence_after();
         if (elect_one()) {
-            const uint64_t v = dv + (uint64_t)(b * (Layout<D>::kV >> 4));
+            const uint64_t v = dv + (uint64_t)(step % kBufs * (Layout<D>::kV >> 4));
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                tc_mma_ts(tmem, tmem + 128 + 64 * b + 8 * i, v + (uint64_t)(2 * i), idesc_f16(D), !first || i);
-            tc_commit(&c->pv_done[b]);
+                tc_mma_ts(tmem_o(tmem, half), tmem_s(tmem, half, b) + 8 * i, v + (uint64_t)(2 * i), idesc_f16(D), j || i);
+            tc_commit(&c->pv_done[half][step % kBufs]);
         }
         __syncwarp();
-        return true;
     }
-};
+}
 
-// ---- warps 4-7 ----
+// ---- warps 8-11 and 12-15: every other step ----
 template <int D>
-__device__ __forceinline__ void unpack_role(const Args& x, const Segment& g, Control* c, uint8_t* sq, uint8_t* sk, uint8_t* sv,
-                                            uint32_t step0, int req, uint32_t tmem) {
+__device__ __forceinline__ void unpack_role(const Args& x, const Segment& g, Control* c, uint8_t* sk, uint8_t* sv, uint32_t step0,
+                                            int req) {
     constexpr int NG = D / kKvGroup, GV = NG / 2, kTileB = kv4_tile_bytes(D);
     const Kv4Attn& a = x.a;
-    const int warp = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31;
+    const int warp = (threadIdx.x >> 5) & 3, group = (threadIdx.x >> 7) & 1, lane = threadIdx.x & 31;
     const int* table = a.table + (long)req * a.table_stride;
-    // where eight steps' tiles lie, one per lane (tile ordinal in the cache, -1: no page, or behind the sequence)
-    auto fetch = [&](int j0) {
-        const int j = j0 + (lane >> 2);
+    const int j0 = (step0 ^ group) & 1;      // this group's first step of the segment
+    // where eight of this group's steps' tiles lie, one per lane (tile ordinal in the cache, -1: no page, or behind the sequence)
+    auto fetch = [&](int t0) {
+        const int j = j0 + 2 * (t0 + (lane >> 2));
         if (j >= g.n) return -1;
         const int ct = g.tile(j) * (kTok / kKvTile) + (lane & 3);
         if (ct * kKvTile >= g.sp.seq) return -1;
@@ -175,8 +222,9 @@ __device__ __forceinline__ void unpack_role(const Args& x, const Segment& g, Con
     // keys: this warp's 16 tokens, lane (q, token), twice; values: channels n*4 .. of all groups gh*GV .., 8 tokens each
     const int kt = lane & 7, kq = lane >> 3, tq = lane & 7, vn = warp * 2 + ((lane >> 3) & 1), gh = lane >> 4;
     uint32_t kw[2][NG], ks[2][NG], km[2][NG / 2], vw[4][GV], vs[4][GV], vm[4][GV];
-    auto load = [&](int j) {
-        const int at = (j & 7) * 4;
+    bool has_page = false;      // of the values
+    auto load = [&](int t) {
+        const int at = (t & 7) * 4;
         const int ok = __shfl_sync(0xffffffffu, where, at + warp), ov = __shfl_sync(0xffffffffu, where, at + (tq >> 1));
         const uint8_t* pk = a.cache.pages + (size_t)max(ok, 0) * kTileB;
         const uint8_t* pv = a.cache.pages + (size_t)max(ov, 0) * kTileB;
@@ -194,37 +242,32 @@ __device__ __forceinline__ void unpack_role(const Args& x, const Segment& g, Con
             load_global<GV>(pv + kv4_off_vs(D) + (tp * NG + gh * GV) * 4, vs[k]);
             load_global<GV>(pv + kv4_off_vm(D) + (tp * NG + gh * GV) * 4, vm[k]);
         }
-        // a tile without a page: zeros (its bytes were tile 0's)
-        if (ov < 0) {
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-#pragma unroll
-                for (int i = 0; i < GV; i++) vs[k][i] = vm[k][i] = 0;
-        }
+        has_page = ov >= 0;
     };
-    const Products<D> products(sq, sk, sv, tmem, c);
     load(0);
-    for (int j = 0; j < g.n; j++) {
-        const uint32_t step = step0 + j, b = step & 1;
-        if (step >= 2 && !await(&c->pv_done[b], ((step >> 1) & 1) ^ 1, &c->abort)) return;
-        const uint32_t valid = __ballot_sync(0xffffffffu, where >= 0) >> ((j & 7) * 4) & 15u;
+    for (int j = j0, t = 0; j < g.n; j += 2, t++) {
+        const uint32_t step = step0 + j, b = step % kBufs, before = (step / kBufs & 1) ^ 1;
+        // both halves' products have read what the buffer held
+        if (step >= kBufs && !(await(&c->pv_done[0][b], before, &c->abort) && await(&c->pv_done[1][b], before, &c->abort))) return;
+        const uint32_t valid = __ballot_sync(0xffffffffu, where >= 0) >> ((t & 7) * 4) & 15u;
         uint8_t* k = sk + b * Layout<D>::kK;
         uint8_t* v = sv + b * Layout<D>::kV;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const int t = kt + 8 * u, row = warp * kKvTile + t;
+            const int tok = kt + 8 * u, row = warp * kKvTile + tok;
 #pragma unroll
             for (int i = 0; i < NG; i++) {
                 const __half2 s2 = as_half2(ks[u][i]), m2 = as_half2(km[u][i >> 1]);
                 uint32_t o[4];
-                values4<0>(kw[u][i], t & 1 ? __high2half2(s2) : __low2half2(s2), i & 1 ? __high2half2(m2) : __low2half2(m2), o);
+                values4<0>(kw[u][i], tok & 1 ? __high2half2(s2) : __low2half2(s2), i & 1 ? __high2half2(m2) : __low2half2(m2), o);
                 const int unit = (i & 1) * 4 + kq;      // 16 bytes of a 128-byte row: two groups
                 *reinterpret_cast<uint4*>(k + (i >> 1) * kTok * 128 + row * 128 + ((unit ^ (row & 7)) << 4)) =
                     make_uint4(o[0], o[1], o[2], o[3]);
             }
         }
-        // tokens behind the sequence have no values; values that are not finite are noted and left out
-        const int left = g.sp.seq - g.tile(j) * kTok - tq * 8;      // of this lane's 8 tokens
+        // tokens behind the sequence or without a page have no values (the bytes read for the latter are tile 0's); values
+        // that are not finite are noted and left out
+        const int left = has_page ? g.sp.seq - g.tile(j) * kTok - tq * 8 : 0;      // of this lane's 8 tokens
         uint32_t bad = 0;
 #pragma unroll
         for (int p = 0; p < 4; p++) {
@@ -255,81 +298,100 @@ __device__ __forceinline__ void unpack_role(const Args& x, const Segment& g, Con
                     make_uint4(o[0][ch], o[1][ch], o[2][ch], o[3][ch]);
             }
         }
-        uint64_t all = 0;
-        if (__any_sync(0xffffffffu, bad != 0)) {
+        const bool any_bad = __any_sync(0xffffffffu, bad != 0);
+        if (any_bad) {
             const uint32_t lo = __reduce_or_sync(0xffffffffu, tq < 4 ? bad << (8 * tq) : 0u);
             const uint32_t hi = __reduce_or_sync(0xffffffffu, tq < 4 ? 0u : bad << (8 * (tq - 4)));
-            all = (uint64_t)hi << 32 | lo;
+            if (lane == 0) c->bad[b][warp] = (uint64_t)hi << 32 | lo;
+        } else if (valid != 15u && lane == 0) {
+            c->bad[b][warp] = 0;
         }
         if (lane == 0) {
-            c->bad[b][warp] = all;
+            c->fine[b][warp] = valid == 15u && !any_bad;
             if (warp == 0) c->valid[b] = valid;
         }
         sync::fence_proxy_async();      // the products read shared memory through the other proxy
         __syncwarp();
         if (lane == 0) arrive(&c->kv_full[b]);
-        if ((j & 7) == 7) {
+        if ((t & 7) == 7) {
             where = where_next;
-            where_next = fetch(j + 9);
+            where_next = fetch(t + 9);
         }
-        if (j + 1 < g.n) load(j + 1);
-        // this step's scores, then the output of the step before (its softmax ran meanwhile)
-        if (warp == 0 && (!products.scores(step) || (j && !products.output(step - 1, j == 1)))) return;
+        if (j + 2 < g.n) load(t + 1);
     }
-    if (warp == 0) products.output(step0 + g.n - 1, g.n == 1);
 }
 
-// ---- warps 0-3 ----
+// ---- warps 0-7 ----
 template <int D>
 __device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Control* c, uint32_t step0, uint32_t tmem) {
     using T = __nv_bfloat16;
     const Kv4Attn& a = x.a;
     const int tid = threadIdx.x, lane = tid & 31;
-    const uint32_t mine = tmem + ((uint32_t)(tid >> 5) << 21);       // this warp's 32 lanes
+    const int half = tid >> 7;
+    const uint32_t lanes = (uint32_t)(tid >> 5 & 3) << 21;       // this warp's 32 lanes
+    const uint32_t mine = tmem_o(tmem, half) + lanes;
     const int row = g.rb * kRows + tid, ti = row / x.group;
     const int pos_q = g.sp.seq - g.sp.q_len + ti;
     const float qk = c->qk[tid];
     float m = kNone, l = 0.f;
     bool ok = !c->abort;
     for (int j = 0; j < g.n && ok; j++) {
-        const uint32_t step = step0 + j, b = step & 1, parity = (step >> 1) & 1;
-        ok = await(&c->kv_full[b], parity, &c->abort) && await(&c->s_full[b], parity, &c->abort);
+        const uint32_t step = step0 + j, b = step & 1, parity = (step >> 1) & 1, kv = step % kBufs;
+        ok = await(&c->kv_full[kv], step / kBufs & 1, &c->abort);
+        if (!ok) break;
+        const uint4 fine = *reinterpret_cast<const uint4*>(c->fine[kv]);
+        const uint32_t at = tmem_s(tmem, half, b) + lanes;
+        const int base = g.tile(j) * kTok;
+        ok = await(&c->s_full[half][b], parity, &c->abort);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t at = mine + 128 + 64 * b;
-        uint32_t v[2][32];
-        tc_ld32(at, v[0]);
-        tc_ld32(at + 32, v[1]);
-        tc_wait_ld();
-        const int base = g.tile(j) * kTok;
-        const uint32_t valid = c->valid[b];
-        const uint64_t bad = c->bad[b][0] | c->bad[b][1] | c->bad[b][2] | c->bad[b][3];
-        const bool part = base + kTok - 1 > g.sp.p_lo || valid != 15u ||
+        uint32_t v[32];
+        tc_ld32(at, v);
+        const bool clean = fine.x & fine.y & fine.z & fine.w;
+        const bool part = base + kTok - 1 > g.sp.p_lo || !clean ||
                           (a.window > 0 && base <= g.sp.p_hi - a.window && base + kTok > a.sinks);
-        bool poison = false;
-        if (part || bad) {
+        uint32_t sees[2] = {0xffffffffu, 0xffffffffu};      // tokens of the step that the row sees
+        if (part) {
+            // up to its own position, from the window's beginning or among the first tokens
+            const auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
+            uint64_t bits = below(pos_q + 1 - base);
+            if (a.window > 0) bits &= ~below(pos_q - a.window + 1 - base) | below(a.sinks - base);
+            if (!clean) {
+                const uint32_t valid = c->valid[kv];
+                uint64_t bad = 0;
 #pragma unroll
-            for (int i = 0; i < 64; i++) {
-                const int pos = base + i;
-                const bool sees = pos <= pos_q && (a.window <= 0 || pos > pos_q - a.window || pos < a.sinks) &&
-                                  (valid >> (i >> 4) & 1);
-                if (!sees) v[i >> 5][i & 31] = 0xff800000u;
-                poison |= sees && (bad >> i & 1);
+                for (int w = 0; w < 4; w++) {
+                    if (!(valid >> w & 1)) bits &= ~(0xffffull << (16 * w));
+                    if (!c->fine[kv][w]) bad |= c->bad[kv][w];
+                }
+                if (bits & bad) l = __uint_as_float(0x7fffffffu);
             }
+            sees[0] = (uint32_t)bits, sees[1] = (uint32_t)(bits >> 32);
         }
+        // the scores are read twice, 32 at a time (the second half stays for its weights): 64 of them do not fit 96 registers
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 64; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i >> 5][i & 31]));
+        for (int h = 0; h < 2; h++) {
+            if (h) tc_ld32(at + 32, v);
+            tc_wait_ld();
+            if (part) {
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                    if (!(sees[h] >> i & 1)) v[i] = 0xff800000u;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i]));
+        }
         const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * qk;
-        if (__any_sync(0xffffffffu, mx - m > kSlack)) {
+        if (__any_sync(0xffffffffu, mx - m > kRoom)) {
             const float now = fmaxf(m, mx), f = ex2(m - now);
             m = now;
             l *= f;
             if (j) {        // the sums so far, once the previous step's product is in them
-                ok = await(&c->pv_done[b ^ 1], ((step - 1) >> 1) & 1, &c->abort);
+                ok = await(&c->pv_done[half][(step - 1) % kBufs], (step - 1) / kBufs & 1, &c->abort);
                 if (!ok) break;
                 tc_fence_after();
-#pragma unroll
+#pragma unroll 1
                 for (int h = 0; h < D / 16; h++) {
                     uint32_t o[16];
                     tc_ld16(mine + 16 * h, o);
@@ -340,26 +402,41 @@ __device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Co
                 }
             }
         }
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t p[32];
+        uint64_t sum = 0;       // two sums
+        const uint64_t qk2 = twice(qk), m2 = twice(-m);
+        uint32_t p[16];
+        auto weights = [&]() {
 #pragma unroll
-        for (int i = 0; i < 32; i++) {
-            const float e0 = ex2(fmaf(__uint_as_float(v[i >> 4][2 * (i & 15)]), qk, -m));
-            const float e1 = ex2(fmaf(__uint_as_float(v[i >> 4][2 * (i & 15) + 1]), qk, -m));
-            sum[i & 3] += e0 + e1;
-            p[i] = pack2<__half>(e0, e1);
+            for (int i = 0; i < 16; i++) {
+                float e0, e1;
+                split(fma2(join(v[2 * i], v[2 * i + 1]), qk2, m2), e0, e1);
+                e0 = ex2(e0), e1 = ex2(e1);
+                sum = add2(sum, join(__float_as_uint(e0), __float_as_uint(e1)));
+                p[i] = pack2<__half>(e0, e1);
+            }
+        };
+        weights();          // of the second half, which go over scores of the first: those are read before
+        tc_ld32(at, v);
+        tc_wait_ld();
+        tc_st16(at + 16, p);
+        if (part) {
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+                if (!(sees[0] >> i & 1)) v[i] = 0xff800000u;
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (poison) l = __uint_as_float(0x7fffffffu);
-        tc_st32(at, p);
+        weights();
+        tc_st16(at, p);
+        float sum0, sum1;
+        split(sum, sum0, sum1);
+        l += sum0 + sum1;
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive(&c->p_full[b]);
+        if (lane == 0) arrive(&c->p_full[half][b]);
     }
     if (ok) {
         const uint32_t step = step0 + g.n - 1;
-        ok = await(&c->pv_done[step & 1], (step >> 1) & 1, &c->abort);
+        ok = await(&c->pv_done[half][step % kBufs], step / kBufs & 1, &c->abort);
         tc_fence_after();
     }
     // ---- the rows' results ----
@@ -395,25 +472,27 @@ __device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Co
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, 2) chunk_kernel(const Args x) {
+__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const Args x) {
     extern __shared__ uint8_t raw[];
     __shared__ Control ctl;
     __shared__ int s_before[kRunUnits + 1];
     uint8_t* sq = raw + ((1024 - (sync::smem_addr(raw) & 1023)) & 1023);
     uint8_t* sk = sq + Layout<D>::kQ;
-    uint8_t* sv = sk + 2 * Layout<D>::kK;
+    uint8_t* sv = sk + kBufs * Layout<D>::kK;
     Control* c = &ctl;
     const Kv4Attn& a = x.a;
     const int tid = threadIdx.x, warp = tid >> 5;
     early_launch();
     if (tid == 0) {
-        for (int i = 0; i < 2; i++) {
-            sync::mbar_init(&c->kv_full[i], 4);
-            sync::mbar_init(&c->s_full[i], 1);
-            sync::mbar_init(&c->p_full[i], 4);
-            sync::mbar_init(&c->pv_done[i], 1);
+        for (int i = 0; i < kBufs; i++) sync::mbar_init(&c->kv_full[i], 4);
+        for (int h = 0; h < 2; h++) {
+            for (int i = 0; i < 2; i++) {
+                sync::mbar_init(&c->s_full[h][i], 1);
+                sync::mbar_init(&c->p_full[h][i], 4);
+            }
+            for (int i = 0; i < kBufs; i++) sync::mbar_init(&c->pv_done[h][i], 1);
+            sync::mbar_init(&c->drain[h], 1);
         }
-        sync::mbar_init(&c->drain, 1);
         c->abort = 0;
         sync::fence_init();
     }
@@ -434,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 2) chunk_kernel(const Args x) {
         if (!span_of(x, req, g.rb, g.sp)) return;
         g.begin = 0, g.n = g.sp.n, g.whole = true, g.slot = 0;
     }
-    if (warp == 4) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sync::smem_addr(&c->tmem)),
                      "r"(kTmem)
                      : "memory");
@@ -459,7 +538,8 @@ __global__ void __launch_bounds__(kThreads, 2) chunk_kernel(const Args x) {
         }
         // ---- the rows' queries, scaled to |q| <= 1 by a power of two per row: a thread takes 8 channels ----
         const int rows = g.sp.q_len * x.group.d;
-        for (int i = tid; i < kRows * (D / 8); i += kThreads) {      // a row lies in D / 8 lanes of one warp
+        // (512 threads: whole rows in a warp, the same number of turns for each)
+        for (int i = tid; i < kRows * (D / 8) && tid < 512; i += 512) {      // a row lies in D / 8 lanes of one warp
             const int rr = i / (D / 8), c8 = i % (D / 8), row = g.rb * kRows + rr;
             float v[8];
             if (row < rows) {
@@ -488,9 +568,10 @@ __global__ void __launch_bounds__(kThreads, 2) chunk_kernel(const Args x) {
         }
         sync::fence_proxy_async();
         __syncthreads();
-        if (!c->abort || warp < 4) {
-            if (warp < 4) softmax_role<D>(x, g, c, step0, tmem);
-            else unpack_role<D>(x, g, c, sq, sk, sv, step0, req, tmem);
+        if (!c->abort || warp < 8) {
+            if (warp < 8) softmax_role<D>(x, g, c, step0, tmem);
+            else if (warp < 16) unpack_role<D>(x, g, c, sk, sv, step0, req);
+            else product_role<D>(g, c, sq, sk, sv, step0, tmem, warp - 16);
         }
         step0 += g.n;
         if (left <= 0) break;
@@ -499,16 +580,16 @@ __global__ void __launch_bounds__(kThreads, 2) chunk_kernel(const Args x) {
         __syncthreads();        // queries and TMEM are read; the next unit's go over them
         tc_fence_after();
     }
-    if (warp == 4) {            // every product issued must be complete before TMEM is released
+    if (warp >= 16) {           // every product issued must be complete before TMEM is released
         if (elect_one()) {
-            tc_commit(&c->drain);
-            sync::mbar_wait(&c->drain, 0);
+            tc_commit(&c->drain[warp - 16]);
+            sync::mbar_wait(&c->drain[warp - 16], 0);
         }
         __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 4) {
+    if (warp == 16) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem) : "memory");
     }
