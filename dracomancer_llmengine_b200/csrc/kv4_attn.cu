@@ -686,9 +686,12 @@ template <int D>
 int blocks_per_sm(int nt) { return nt == 1 ? Shape<D, 1>::kBlocks : Shape<D, 2>::kBlocks; }
 
 // How the rows are blocked and the tiles are divided.
-// Chunks: bf16 queries with more than 64 rows per request and kv head go to the tensor-core form, 256 rows a block, unless
-// lse is asked for (its keys are rounded to fp16, which bf16 output hides and an fp32 lse of few keys does not) or heads
-// are 256 wide (the sums of two halves of the rows fill TMEM at 128).
+// Chunks: bf16 queries with more than 128 rows per request and kv head go to the tensor-core form, 256 rows a block (64
+// requests of 1024 tokens, 4 kv heads: 256 rows 109 us against 149, 72 rows 83 against 54); with few units over long
+// sequences, which that form's blocks of fewer, longer steps suit, from 25 rows (4 requests of 8192 tokens: 32 rows 38 us against 52,
+// 128 rows 44 against 74; but 1 of 2000 tokens, 32 rows: 20 against 15).  Not where lse is asked for (its keys are rounded to
+// fp16, which bf16 output hides and an fp32 lse of few keys does not), nor for heads 256 wide (the sums of two halves of the
+// rows fill TMEM at 128).
 // Otherwise blocks of 16 rows where 16-bit queries have more than 8: a tile's codes are then unpacked for twice the rows.
 // Runs where there are few enough blocks of rows to scan (one per request in this file), as many as fit the GPU at
 // once: a block's start (lengths, page ids, queries) costs it about as much as four tiles a warp, so fewer and longer
@@ -700,7 +703,8 @@ void plan(const Kv4Attn& a, Args& x) {
     x.group = make_div(group);
     x.page_tiles = make_div(a.cache.page_size / kKvTile);
     const long rows = (long)a.max_q * group;
-    const bool chunk = a.dtype == kBF16 && !a.lse && a.cache.head_dim <= 128 && rows > 64;
+    const bool few = (long)a.n_req * a.cache.n_kv_heads < 148 && a.max_seq >= 4096;
+    const bool chunk = a.dtype == kBF16 && !a.lse && a.cache.head_dim <= 128 && rows > (few ? 24 : 128);
     x.tile = chunk ? kChunkTokens : kKvTile;
     x.block_rows = chunk ? kChunkRows : a.dtype != kF32 && rows > 8 ? 16 : 8;
     x.row_blocks = (int)((rows + x.block_rows - 1) / x.block_rows);
