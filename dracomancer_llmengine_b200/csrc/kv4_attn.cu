@@ -156,10 +156,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_ker
     Span sp;
     bool whole;
     if (x.runs) {
-        scan_units<kWarps * 32>(x, s_before);
-        if (blockIdx.x == 0)
-            for (int i = tid; i <= a.n_req; i += kWarps * 32) x.before[i] = s_before[i];
-        const Run run = run_of(x, s_before);
+        const Run run = find_run<kWarps * 32>(x, s_before);
         if (!run.left) return;
         req = run.f, kvh = run.kvh, begin = run.begin, left = run.left;     // row_blocks is 1
     } else {
@@ -639,40 +636,45 @@ __global__ void __launch_bounds__(256) join_kernel(const Args x) {
     const int rw = rb * kRows + rr;
     if (rw >= sp.q_len * x.group.d) return;
     int active;
-    long at, step = kRows;      // row `rr` of the unit's first slot, and from one slot to the next
+    long at, step = kRows, back = 0;    // row `rr` of the unit's first slot, and how the others follow
     if (x.runs) {
-        const int heads = a.cache.n_kv_heads;
-        const int per = run_tiles(x, (long)x.before[a.n_req * x.row_blocks] * heads);
-        const long first = (long)x.before[req * x.row_blocks + rb] * heads + (long)kvh * sp.n, last = first + sp.n - 1;
-        const long c0 = first / per, c1 = last / per;
-        active = (int)(c1 - c0) + 1;
-        at = (2 * c0 + 1) * kRows + rr;       // the run in which the unit begins; the others' slots are even
-        step = 2 * kRows;
+        const int f = req * x.row_blocks + rb, per = x.before[a.n_req * x.row_blocks + 1];
+        const int first = x.before[f] * a.cache.n_kv_heads + kvh * sp.n, c0 = first / per;
+        active = (first + sp.n - 1) / per - c0 + 1;
+        at = (2l * c0 + 1) * kRows + rr;       // the run in which the unit begins; the others' slots are even
+        step = 2 * kRows, back = kRows;
     } else {
         active = min(x.n_splits, (sp.n + x.tiles_per_split - 1) / x.tiles_per_split);
         at = (((long)req * a.cache.n_kv_heads + kvh) * x.row_blocks + rb) * x.n_splits * kRows + rr;
     }
     if (active == 1) return;
-    auto row_of = [&](int s) { return x.runs && s ? at + s * step - kRows : at + s * step; };
-    float mx = kNone;
-    for (int s = lane; s < active; s += 32) mx = fmaxf(mx, x.ml[row_of(s)].x);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    auto row_of = [&](int s) { return at + s * step - (s ? back : 0); };
+    // maxima and sums a lane a part, 32 parts at a time; the running maximum as in the parts themselves
     constexpr int kPer = D / 32;
-    float sum = 0.f, o[kPer];
+    float mx = kNone, sum = 0.f, o[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; j++) o[j] = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < active; s++) {
-        const float2 ml = x.ml[row_of(s)];
-        const float f = ex2(ml.x - mx);
-        sum = fmaf(ml.y, f, sum);
-        const float* v = x.part + row_of(s) * D + lane * kPer;
-        float t[kPer];
+    for (int s0 = 0; s0 < active; s0 += 32) {
+        const int n = min(32, active - s0);
+        const float2 ml = lane < n ? x.ml[row_of(s0 + lane)] : make_float2(kNone, 0.f);
+        float top = fmaxf(mx, ml.x);
 #pragma unroll
-        for (int j = 0; j < kPer; j += 2) *reinterpret_cast<float2*>(t + j) = *reinterpret_cast<const float2*>(v + j);
+        for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        const float old = ex2(mx - top), f = lane < n ? ex2(ml.x - top) : 0.f;
+        mx = top;
+        sum = fmaf(sum, old, warp_sum(lane < n ? ml.y * f : 0.f));
 #pragma unroll
-        for (int j = 0; j < kPer; j++) o[j] = fmaf(t[j], f, o[j]);
+        for (int j = 0; j < kPer; j++) o[j] *= old;
+#pragma unroll 8
+        for (int s = 0; s < n; s++) {
+            const float* v = x.part + row_of(s0 + s) * D + lane * kPer;
+            float t[kPer];
+#pragma unroll
+            for (int j = 0; j < kPer; j += 2) *reinterpret_cast<float2*>(t + j) = *reinterpret_cast<const float2*>(v + j);
+            const float w = __shfl_sync(0xffffffffu, f, s);
+#pragma unroll
+            for (int j = 0; j < kPer; j++) o[j] = fmaf(t[j], w, o[j]);
+        }
     }
     const int ti = rw / x.group, tk = sp.q0 + ti, hd = kvh * x.group.d + rw - ti * x.group.d;
     const float n = sum == 0.f ? 0.f : 1.f / sum;
@@ -710,7 +712,7 @@ void plan(const Kv4Attn& a, Args& x) {
     x.row_blocks = (int)((rows + x.block_rows - 1) / x.block_rows);
     const long units_one = (long)a.n_req * x.row_blocks;
     // (a block counts tiles in 32 bits)
-    const long tiles_bound = ((long)a.table_width * (a.cache.page_size / kKvTile) + 1) * units_one;
+    const long tiles_bound = ((long)a.table_width * (a.cache.page_size / kKvTile) + 1) * units_one * a.cache.n_kv_heads;
     x.n_splits = 1;
     if ((chunk || x.row_blocks == 1) && units_one <= kRunUnits && tiles_bound < 1l << 31) {
         const int nt = a.dtype == kF32 || x.block_rows == 16 ? 2 : 1, d = a.cache.head_dim;
@@ -787,7 +789,7 @@ size_t kv4_attention_workspace(const Kv4Attn& a) {
     x.a = a;
     plan(a, x);
     if (!x.runs && x.n_splits == 1) return 0;
-    return part_bytes(x) + ml_bytes(x) + (x.runs ? sizeof(int) * ((size_t)a.n_req * x.row_blocks + 1) : 0);
+    return part_bytes(x) + ml_bytes(x) + (x.runs ? sizeof(int) * ((size_t)a.n_req * x.row_blocks + 2) : 0);
 }
 
 int launch_kv4_attention(const Kv4Attn& a, void* workspace, cudaStream_t s) {

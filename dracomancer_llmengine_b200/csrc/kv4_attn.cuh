@@ -24,7 +24,7 @@ struct Args {
     // unit that began in an earlier run, and of one that begins in it)
     float* part;        // [slot][block_rows][D]
     float2* ml;         // [slot][block_rows] maximum (log2 domain) and sum
-    int* before;        // [n_req * row_blocks + 1] tiles of one kv head before each block of rows (run form; for the join)
+    int* before;        // run form, for the join: see find_run()
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -65,11 +65,6 @@ __device__ __forceinline__ bool span_of(const Args& x, int req, int rb, Span& s)
 
 constexpr int kRunUnits = 1024;     // blocks of rows that a block scans
 
-// tiles of a run, of `total`
-__device__ __forceinline__ int run_tiles(const Args& x, long total) {
-    return (int)max((long)x.run_min, (total + x.runs - 1) / x.runs);
-}
-
 // before[f] = tiles of one kv head in the blocks of rows before f = request * row_blocks + block, for the whole block
 template <int THREADS>
 __device__ __forceinline__ void scan_units(const Args& x, int* before) {
@@ -102,22 +97,55 @@ __device__ __forceinline__ void scan_units(const Args& x, int* before) {
 // A block's run: where it begins, and how many tiles it has (0: none)
 struct Run {
     int f, kvh, begin;      // block of rows (with its request), kv head, first tile of that unit
-    long left;
+    int left;
 };
-__device__ __forceinline__ Run run_of(const Args& x, const int* before) {
-    const int units = x.a.n_req * x.row_blocks, heads = x.a.cache.n_kv_heads;
-    const long total = (long)before[units] * heads;
-    const int per = run_tiles(x, total);
+// The run of this block, the same in every thread; `before` is shared memory for kRunUnits + 1 values.  Block 0 leaves
+// what the join needs in x.before: the tiles before each block of rows, those of all, and a run's.  The tiles of all units
+// are below 2^31 (plan() sees to it).
+template <int THREADS>
+__device__ __forceinline__ Run find_run(const Args& x, int* before) {
+    const int units = x.a.n_req * x.row_blocks, heads = x.a.cache.n_kv_heads, tid = threadIdx.x, lane = tid & 31;
+    auto per_of = [&](int total) { return max(x.run_min, (int)(((long)total + x.runs - 1) / x.runs)); };
+    if (units <= 32) {      // each warp scans for itself
+        Span sp;
+        const int req = lane / x.row_blocks;
+        const int n = lane < units && span_of(x, req, lane - req * x.row_blocks, sp) ? sp.n : 0;
+        int inc = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        const int total = __shfl_sync(0xffffffffu, inc, 31) * heads, per = per_of(total);
+        if (blockIdx.x == 0 && tid < 32) {
+            if (lane < units) x.before[lane] = inc - n;
+            if (lane == 0) x.before[units] = total, x.before[units + 1] = per;
+        }
+        const long start = (long)blockIdx.x * per;
+        if (start >= total) return Run{0, 0, 0, 0};
+        // the last block of rows with tiles that begins at or before the run
+        const uint32_t can = __ballot_sync(0xffffffffu, n > 0 && (inc - n) * heads <= (int)start);
+        const int f = 31 - __clz(can);
+        const int n_f = __shfl_sync(0xffffffffu, n, f), in = (int)start - __shfl_sync(0xffffffffu, inc - n, f) * heads;
+        const int kvh = in / n_f;
+        return Run{f, kvh, in - kvh * n_f, min(per, total - (int)start)};
+    }
+    scan_units<THREADS>(x, before);
+    const int total = before[units] * heads, per = per_of(total);
+    if (blockIdx.x == 0) {
+        for (int i = tid; i < units; i += THREADS) x.before[i] = before[i];
+        if (tid == 0) x.before[units] = total, x.before[units + 1] = per;
+    }
     const long start = (long)blockIdx.x * per;
     if (start >= total) return Run{0, 0, 0, 0};
     int lo = 0, hi = units;
-    while (hi - lo > 1) {      // the last block of rows that begins at or before the run: it has tiles
+    while (hi - lo > 1) {      // as above: the one behind it begins after the run's start, so it has tiles
         const int mid = (lo + hi) >> 1;
-        if ((long)before[mid] * heads <= start) lo = mid;
+        if (before[mid] * heads <= (int)start) lo = mid;
         else hi = mid;
     }
-    const int n = before[lo + 1] - before[lo], in = (int)(start - (long)before[lo] * heads), kvh = in / n;
-    return Run{lo, kvh, in - kvh * n, min((long)per, total - start)};
+    const int n = before[lo + 1] - before[lo], in = (int)start - before[lo] * heads, kvh = in / n;
+    return Run{lo, kvh, in - kvh * n, min(per, total - (int)start)};
 }
 
 // chunks of bf16 queries on the tensor cores' fifth-generation path (kv4_chunk.cu): 256 rows and 64 tokens a step

@@ -502,10 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const Args x) {
     int req, f = 0;
     long left = 0;
     if (x.runs) {
-        scan_units<kThreads>(x, s_before);
-        if (blockIdx.x == 0)
-            for (int i = tid; i <= a.n_req * x.row_blocks; i += kThreads) x.before[i] = s_before[i];
-        const Run run = run_of(x, s_before);
+        const Run run = find_run<kThreads>(x, s_before);
         if (!run.left) return;
         f = run.f, g.kvh = run.kvh, g.begin = run.begin, left = run.left;
     } else {
