@@ -34,7 +34,7 @@
 // tiles of all units form one sequence, cut into as many equal runs as the GPU holds blocks; a run crosses units, and a
 // unit that lies in several runs is joined by a second kernel from at most two partial sums per block.  Every block finds
 // its run itself, by a scan of the lengths.  Otherwise (chunks, or more requests than that scan takes) a block takes one
-// unit, or a split of it where units are few.  Sums are joined in a fixed order: results do not depend on timing.
+// unit, or a split of it where units are few; short units are taken whole.  Sums are joined in a fixed order: results do not depend on timing.
 #include "kv4_attn.cuh"
 
 #include <algorithm>
@@ -46,12 +46,13 @@ namespace {
 
 using namespace attn;
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;           // of a block of the run form, or with splits
 // What a variant of the kernel takes per block: NT columns of 8 (queries, or their two halves)
 template <int D, int NT>
 struct Shape {
     static constexpr int kStages = D == 256 ? 3 : 4;                      // of a warp's ring
     static constexpr bool kQInSmem = D == 256 && NT == 2;                 // 64 registers a lane otherwise
+    static constexpr int kTeam = D == 64 ? 16 : D == 128 ? (NT == 1 ? 16 : 12) : 8;    // warps where a block takes a unit
     static constexpr int kBlocks = D == 64 ? (NT == 1 ? 5 : 4) : D == 128 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2);
 };
 constexpr uint32_t kTwo15 = 0x78007800u;   // 2^15, 2^15 in fp16
@@ -134,8 +135,8 @@ __device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[N]) {
 }
 
 // NT columns of 8: 8 NT query rows, or (SPLIT) the high and low halves of 8
-template <typename T, int D, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_kernel(const Args x) {
+template <typename T, int D, int NT, bool SPLIT, int W>
+__global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 1) attend_kernel(const Args x) {
     using S = Shape<D, NT>;
     constexpr int NG = D / kKvGroup;
     constexpr int kStages = S::kStages;
@@ -147,7 +148,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_ker
     extern __shared__ __align__(16) uint8_t smem[];
     const Kv4Attn& a = x.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r8 = lane >> 2, q4 = lane & 3;
-    __shared__ int s_before[kRunUnits + 1];
+    constexpr bool kRuns = W == kWarps;     // else a block takes a unit
+    __shared__ int s_before[kRuns ? kRunUnits + 1 : 1];
     early_launch();
     wait_for_inputs();
     // the segment: tiles [begin, end) of a unit, and where its sums go if it is not the whole unit
@@ -155,8 +157,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_ker
     long slot, left = 0;      // left: tiles of the run behind this segment
     Span sp;
     bool whole;
-    if (x.runs) {
-        const Run run = find_run<kWarps * 32>(x, s_before);
+    if (kRuns && x.runs) {
+        const Run run = find_run<W * 32>(x, s_before);
         if (!run.left) return;
         req = run.f, kvh = run.kvh, begin = run.begin, left = run.left;     // row_blocks is 1
     } else {
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_ker
     }
 
     for (;;) {
-        if (x.runs) {
+        if (kRuns && x.runs) {
             while (!span_of(x, req, 0, sp)) req++;      // requests without queries have no tiles
             end = (int)min((long)sp.n, begin + left);
             left -= end - begin;
@@ -183,12 +185,12 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_ker
         uint8_t* ring = smem + warp * kStages * kTileB;
         const int* table = a.table + (long)req * a.table_stride;
 
-        // this warp's tiles: idx = begin + warp + kWarps * i, i < count; where 32 of them lie (tile ordinal in the cache, or
+        // this warp's tiles: idx = begin + warp + W * i, i < count; where 32 of them lie (tile ordinal in the cache, or
         // -1 for a page outside it), one per lane
         const int mine = begin + warp;
-        const int count = mine < end ? (end - mine + kWarps - 1) / kWarps : 0;
+        const int count = mine < end ? (end - mine + W - 1) / W : 0;
         auto tile_of = [&](int i) {
-            const int idx = mine + kWarps * i;
+            const int idx = mine + W * i;
             return idx < sp.head ? idx : sp.first + idx - sp.head;
         };
         auto fetch = [&](int i0) {
@@ -216,11 +218,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_ker
 
         // ---- the rows' queries as operand fragments, made once for the block: a thread takes 8 channels of a row ----
         const int rows = sp.q_len * x.group.d, row0 = rb * kRows;
-        uint8_t* q_at = smem + kWarps * kStages * kTileB;
+        uint8_t* q_at = smem + W * kStages * kTileB;
         uint4* q_sm = reinterpret_cast<uint4*>(q_at);                                       // [NG][NT][32 lanes]
         __half* qs_sm = reinterpret_cast<__half*>(q_at + NG * NT * 512);                    // [high, low][NT][32 lanes][2]
         float* qk_sm = reinterpret_cast<float*>(q_at + NG * NT * 512 + 2 * NT * 128);       // [kRows]
-        for (int i = tid; i < kRows * (D / 8); i += kWarps * 32) {   // whole warps, and a row within one
+        for (int i = tid; i < kRows * (D / 8); i += W * 32) {   // whole warps, and a row within one
             const int rr = i / (D / 8), c8 = i % (D / 8), row = row0 + rr;
             float v[8];
             if (row < rows) {
@@ -552,8 +554,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_ker
 
         // ---- join the warps: their rows meet in shared memory (over the finished ring) ----
         __syncthreads();
-        float* s_o = reinterpret_cast<float*>(smem);                                   // [kWarps][kRows][D]
-        float2* s_ml = reinterpret_cast<float2*>(smem + kWarps * kRows * D * 4);       // [kWarps][kRows]
+        float* s_o = reinterpret_cast<float*>(smem);                                   // [W][kRows][D]
+        float2* s_ml = reinterpret_cast<float2*>(smem + W * kRows * D * 4);       // [W][kRows]
 #pragma unroll
         for (int e = 0; e < ET; e++)
 #pragma unroll
@@ -575,17 +577,17 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kBlocks) attend_ker
                 if (r8 == 0) s_ml[rr] = make_float2(m[e][j], l[e][j]);
             }
         __syncthreads();
-        for (int i = tid; i < kRows * D / 4; i += kWarps * 32) {
+        for (int i = tid; i < kRows * D / 4; i += W * 32) {
             const int rr = i / (D / 4), c4 = i % (D / 4);
             const int rw = row0 + rr;
             if (rw >= rows) break;
             float mx = kNone;
 #pragma unroll
-            for (int w = 0; w < kWarps; w++) mx = fmaxf(mx, s_ml[w * kRows + rr].x);
+            for (int w = 0; w < W; w++) mx = fmaxf(mx, s_ml[w * kRows + rr].x);
             float sum = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < kWarps; w++) {
+            for (int w = 0; w < W; w++) {
                 const float2 ml = s_ml[w * kRows + rr];
                 const float f = ex2(ml.x - mx);
                 sum = fmaf(ml.y, f, sum);
@@ -687,6 +689,11 @@ __global__ void __launch_bounds__(256) join_kernel(const Args x) {
 template <int D>
 int blocks_per_sm(int nt) { return nt == 1 ? Shape<D, 1>::kBlocks : Shape<D, 2>::kBlocks; }
 
+int team_of(int d, int nt) {
+    return nt == 1 ? (d == 64 ? Shape<64, 1>::kTeam : d == 128 ? Shape<128, 1>::kTeam : Shape<256, 1>::kTeam)
+                   : (d == 64 ? Shape<64, 2>::kTeam : d == 128 ? Shape<128, 2>::kTeam : Shape<256, 2>::kTeam);
+}
+
 // How the rows are blocked and the tiles are divided.
 // Chunks: bf16 queries with more than 128 rows per request and kv head go to the tensor-core form, 256 rows a block (64
 // requests of 1024 tokens, 4 kv heads: 256 rows 109 us against 149, 72 rows 83 against 54); with few units over long
@@ -695,6 +702,10 @@ int blocks_per_sm(int nt) { return nt == 1 ? Shape<D, 1>::kBlocks : Shape<D, 2>:
 // fp16, which bf16 output hides and an fp32 lse of few keys does not), nor for heads 256 wide (the sums of two halves of the
 // rows fill TMEM at 128).
 // Otherwise blocks of 16 rows where 16-bit queries have more than 8: a tile's codes are then unpacked for twice the rows.
+// A whole unit per block, with nothing to join, where units are many for their length or short: up to 148 of them with up to
+// 16 warps each (1 request of 1001 bf16 tokens, 4 kv heads: 10.7 us against 14.1 with runs, 2001 fp32 tokens 20.7 against
+// 17.1; 36 requests of 4001 tokens 23.6 against 31.8), above that with four (512 units of up to 1000 tokens: 23.6 us against
+// 37.2, 4096: 74 against 68; 192 units of 1000: 19.1 against 21.3, 2000: 28.8 against 24.9).
 // Runs where there are few enough blocks of rows to scan (one per request in this file), as many as fit the GPU at
 // once: a block's start (lengths, page ids, queries) costs it about as much as four tiles a warp, so fewer and longer
 // pieces win (4 x 131001 tokens, 8 kv heads: 140 us, against 145 with one block per unit and split in one wave and 160 in
@@ -711,9 +722,21 @@ void plan(const Kv4Attn& a, Args& x) {
     x.block_rows = chunk ? kChunkRows : a.dtype != kF32 && rows > 8 ? 16 : 8;
     x.row_blocks = (int)((rows + x.block_rows - 1) / x.block_rows);
     const long units_one = (long)a.n_req * x.row_blocks;
+    const int tiles = std::max(1, (a.max_seq + kKvTile - 1) / kKvTile);
+    int span = tiles;
+    if (a.window > 0)   // the widest walk of one row block
+        span = (int)std::min<long>(tiles, ((long)a.window + std::min(a.max_q, x.block_rows / group + 2)) / kKvTile + 2 +
+                                              ((long)a.sinks + kKvTile - 1) / kKvTile);
+    const long units = units_one * a.cache.n_kv_heads;
     // (a block counts tiles in 32 bits)
     const long tiles_bound = ((long)a.table_width * (a.cache.page_size / kKvTile) + 1) * units_one * a.cache.n_kv_heads;
     x.n_splits = 1;
+    const int warps = team_of(a.cache.head_dim, a.dtype == kF32 || x.block_rows == 16 ? 2 : 1);
+    if (!chunk && (units <= 148 ? span <= warps * (units >= 48 ? 16 : 7) : span * 3l <= units)) {
+        x.team = units <= 148;
+        x.tiles_per_split = 1 << 30;
+        return;
+    }
     if ((chunk || x.row_blocks == 1) && units_one <= kRunUnits && tiles_bound < 1l << 31) {
         const int nt = a.dtype == kF32 || x.block_rows == 16 ? 2 : 1, d = a.cache.head_dim;
         x.runs = 148 * (chunk ? 1 : d == 64 ? blocks_per_sm<64>(nt) : d == 128 ? blocks_per_sm<128>(nt) : blocks_per_sm<256>(nt));
@@ -724,15 +747,9 @@ void plan(const Kv4Attn& a, Args& x) {
         return;
     }
     if (chunk) {        // units enough without splits
-        x.tiles_per_split = 0x7fffffff;
+        x.tiles_per_split = 1 << 30;
         return;
     }
-    const int tiles = std::max(1, (a.max_seq + kKvTile - 1) / kKvTile);
-    int span = tiles;
-    if (a.window > 0)   // the widest walk of one row block
-        span = (int)std::min<long>(tiles, ((long)a.window + std::min(a.max_q, x.block_rows / group + 2)) / kKvTile + 2 +
-                                              ((long)a.sinks + kKvTile - 1) / kKvTile);
-    const long units = (long)a.n_req * a.cache.n_kv_heads * x.row_blocks;
     const long want = std::max<long>(1, 148L * 4 * 4 / units);
     const long per = std::max<long>(8, (span + want - 1) / want);
     x.tiles_per_split = (int)per;
@@ -743,22 +760,27 @@ long slots_of(const Args& x) {
 }
 bool needs_join(const Args& x) { return x.runs > 1 || x.n_splits > 1; }
 
-template <typename T, int D, int NT, bool SPLIT>
-void run_nt(const Args& x, cudaStream_t s) {
+template <typename T, int D, int NT, bool SPLIT, int W>
+void run_w(const Args& x, cudaStream_t s) {
     using S = Shape<D, NT>;
     const int rows = SPLIT ? 8 : 8 * NT;
-    const int smem = std::max(kWarps * S::kStages * kv4_tile_bytes(D) + D / kKvGroup * NT * 512 + 2 * NT * 128 + rows * 4,
-                              kWarps * rows * (D * 4 + 8));
+    const int smem = std::max(W * S::kStages * kv4_tile_bytes(D) + D / kKvGroup * NT * 512 + 2 * NT * 128 + rows * 4,
+                              W * rows * (D * 4 + 8));
     static std::atomic<uint64_t> ready{0};      // devices on which the kernel may use its shared memory
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev > 63 || !(ready.load() >> dev & 1)) {
-        cudaFuncSetAttribute(attend_kernel<T, D, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaFuncSetAttribute(attend_kernel<T, D, NT, SPLIT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (dev < 64) ready |= (uint64_t)1 << dev;
     }
     const dim3 grid = x.runs ? dim3((unsigned)x.runs)
                              : dim3((unsigned)(x.n_splits * x.row_blocks), (unsigned)x.a.cache.n_kv_heads, (unsigned)x.a.n_req);
-    launch(attend_kernel<T, D, NT, SPLIT>, grid, dim3(kWarps * 32), smem, s, x);
+    launch(attend_kernel<T, D, NT, SPLIT, W>, grid, dim3(W * 32), smem, s, x);
+}
+template <typename T, int D, int NT, bool SPLIT>
+void run_nt(const Args& x, cudaStream_t s) {
+    if (x.team) run_w<T, D, NT, SPLIT, Shape<D, NT>::kTeam>(x, s);
+    else run_w<T, D, NT, SPLIT, kWarps>(x, s);
 }
 template <typename T, int D>
 void run(const Args& x, cudaStream_t s) {

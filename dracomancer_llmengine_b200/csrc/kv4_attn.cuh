@@ -17,6 +17,7 @@ struct Args {
     int tile;                               // tokens of a step of the walk: 16 or 64
     int runs, run_min;                      // blocks of the run form (0: a block per unit and split), tiles of a run
     int tiles_per_split, n_splits;          // of the other form
+    bool team;                              // of that one, with as many warps as a block can have
     Div group;          // query heads of a kv head
     Div page_tiles;     // tiles of 16 tokens of a page
     bool wide_q, wide_o;
