@@ -34,7 +34,8 @@
 // tiles of all units form one sequence, cut into as many equal runs as the GPU holds blocks; a run crosses units, and a
 // unit that lies in several runs is joined by a second kernel from at most two partial sums per block.  Every block finds
 // its run itself, by a scan of the lengths.  Otherwise (chunks, or more requests than that scan takes) a block takes one
-// unit, or a split of it where units are few; short units are taken whole.  Sums are joined in a fixed order: results do not depend on timing.
+// unit, or a split of it where units are few; short units are taken whole.  Sums are joined in a fixed order: results do not
+// depend on timing.
 #include "kv4_attn.cuh"
 
 #include <algorithm>
@@ -711,8 +712,8 @@ int team_of(int d, int nt) {
 // How the rows are blocked and the tiles are divided.
 // Chunks: bf16 queries with more than 128 rows per request and kv head go to the tensor-core form, 256 rows a block (64
 // requests of 1024 tokens, 4 kv heads: 256 rows 109 us against 149, 72 rows 83 against 54); with few units over long
-// sequences, which that form's blocks of fewer, longer steps suit, from 25 rows (4 requests of 8192 tokens: 32 rows 38 us against 52,
-// 128 rows 44 against 74; but 1 of 2000 tokens, 32 rows: 20 against 15).  Not where lse is asked for (its keys are rounded to
+// sequences from 25 rows (4 requests of 8192 tokens: 32 rows 38 us against 52, 128 rows 44 against 74; but 1 of 2000 tokens, 32
+// rows: 20 against 15).  Not where lse is asked for (its keys are rounded to
 // fp16, which bf16 output hides and an fp32 lse of few keys does not), nor for heads 256 wide (the sums of two halves of the
 // rows fill TMEM at 128).
 // Otherwise blocks of 16 rows where 16-bit queries have more than 8: a tile's codes are then unpacked for twice the rows.
