@@ -27,8 +27,8 @@
 // The running maximum is raised only when a score exceeds it by more than 3 (log2): weights stay below 8, and most tiles
 // need neither the reduction over tokens nor the rescaling of the sums.
 //
-// Memory: a warp owns every kWarps-th tile of its block's run and copies tiles (20 D bytes, contiguous) into its own ring
-// of stages with cp.async, page ids fetched 32 tiles at a time.
+// Memory: each of a block's W warps takes every W-th tile of its run and copies tiles (20 D bytes, contiguous) into its own
+// ring of stages with cp.async, page ids fetched 32 tiles at a time.
 //
 // Work: a unit is a block of rows of one request and kv head.  Where every request is one block of rows (decode), the
 // tiles of all units form one sequence, cut into as many equal runs as the GPU holds blocks; a run crosses units, and a
@@ -712,8 +712,8 @@ int team_of(int d, int nt) {
 // How the rows are blocked and the tiles are divided.
 // Chunks: bf16 queries with more than 128 rows per request and kv head go to the tensor-core form, 256 rows a block (64
 // requests of 1024 tokens, 4 kv heads: 256 rows 109 us against 149, 72 rows 83 against 54); with few units over long
-// sequences from 25 rows (4 requests of 8192 tokens: 32 rows 38 us against 52, 128 rows 44 against 74; but 1 of 2000 tokens, 32
-// rows: 20 against 15).  Not where lse is asked for (its keys are rounded to
+// sequences, which that form's blocks of fewer, longer steps suit, from 25 rows (4 requests of 8192 tokens: 32 rows 38 us
+// against 52, 128 rows 44 against 74; but 1 of 2000 tokens, 32 rows: 20 against 15).  Not where lse is asked for (its keys are rounded to
 // fp16, which bf16 output hides and an fp32 lse of few keys does not), nor for heads 256 wide (the sums of two halves of the
 // rows fill TMEM at 128).
 // Otherwise blocks of 16 rows where 16-bit queries have more than 8: a tile's codes are then unpacked for twice the rows.

@@ -12,8 +12,9 @@
 //
 // Bound by memory: x, r, h, y and one byte a value cross once.  A block takes a row, a thread 8 neighbouring values a
 // step, kept in registers between the two uses; the values of a group of 32 to 256 lie in 4 to 32 neighbouring lanes.
-// Measured: 4096 x 4096 bf16 with residual and y 32 to 34 us, 4.6 TB/s; with 16384 rows 5.7 TB/s, where a fill alone writes
-// 3.9 TB/s and 5 of the 9 bytes a value are written.  Blocks that loop over rows and fetch the next ones ahead (registers, or a
+// Measured: 4096 x 4096 bf16 with residual and y 34 us, 4.5 TB/s (31.6 on one set of tensors); with 16384 rows
+// 5.7 TB/s, where a fill alone writes 3.9 TB/s and 5 of the 9 bytes a value are written.
+// Blocks that loop over rows and fetch the next ones ahead (registers, or a
 // ring in shared memory) took 40 us: a row per block and many blocks overlap better.
 #include "kv4.cuh"
 
