@@ -21,10 +21,16 @@
 //   fp32  queries and weights are split in two halves (x = hi + lo / 2048, 22 bits), the low halves take 8 columns more;
 //         codes of K are made normal numbers (c * 2^-9): with subnormal ones the sums of a product are aligned ten bits
 //         too high, which showed as 1e-6 of the result (2^-14 of a code; measured 1.1e-6 against 0.5e-6 without)
-//   fp16  weights are scaled in fp32 and rounded to fp16 once, as the output will be
-//   bf16  weights are rounded to fp16 and scaled there (2^-11 twice, an eighth of the output's own rounding)
+//   fp16  weights are multiplied with the scales in fp32 and rounded to fp16 once (2^-11), as the output will be
+//   bf16  weights are rounded to fp16 and multiplied with the scales there (2^-11 twice, an eighth of the output's rounding)
+// fp16 has 2^-14 as its smallest normal number, so both factors are kept well above it: the largest weight of a row is
+// 2^11 (kBias), and the scales are divided by a power of two above the largest one that the warp has met (v_exp), which
+// is raised, and the sums with it, like the running maximum.  The roundings above are those of a weight times a scale
+// down to 2^-24 of the largest weight times the largest scale; below, they are 2^-35 of that (fp32: 2^-46) in absolute
+// terms.  (With weights up to 1 and scales as they are, a first token 9 nats above 4096 others, its values near 0, cost
+// bf16 and fp16 results 2e-2 where values are 0.01.)
 //
-// The running maximum is raised only when a score exceeds it by more than 3 (log2): weights stay below 8, and most tiles
+// The running maximum is raised only when a score exceeds it by more than 3 (log2): weights stay below 2^14, and most tiles
 // need neither the reduction over tokens nor the rescaling of the sums.
 //
 // Memory: each of a block's W warps takes every W-th tile of its run and copies tiles (20 D bytes, contiguous) into its own
@@ -57,6 +63,8 @@ struct Shape {
     static constexpr int kBlocks = D == 64 ? (NT == 1 ? 5 : 4) : D == 128 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2);
 };
 constexpr uint32_t kTwo15 = 0x78007800u;   // 2^15, 2^15 in fp16
+constexpr float kSlack = 3.f;              // log2 by which weights may pass 2^kBias
+constexpr int kExpMin = -14, kExpMax = 16;  // of the values' scales: 2^(1 - exponent) is an fp16 number
 constexpr float kLoScale = 2048.f, kLoInv = 1.f / 2048.f;
 
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
@@ -118,6 +126,14 @@ __device__ __forceinline__ uint32_t centred(uint32_t codes, bool odd) {
     const __half2 d = __hfma2(*reinterpret_cast<const __half2*>(&codes), k, o);
     return *reinterpret_cast<const uint32_t*>(&d);
 }
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {      // of a NaN and a number, the number
+    const __half2 d = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+__device__ __forceinline__ bool below2(uint32_t a, uint32_t b) {        // both halves
+    return __hblt2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 // a word's halves that are infinite or NaN set to 0
 __device__ __forceinline__ uint32_t finite2(uint32_t z) {
     if ((z & 0x7c00u) == 0x7c00u) z &= 0xffff0000u;
@@ -308,6 +324,9 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
         float acc[NT][NG][2][4];      // channels g*32 + r8*4 + {0, 1 | 2, 3} x rows 2 q4, 2 q4 + 1
         float zacc[NT][4];            // group r8 x rows 2 q4, 2 q4 + 1 (the last two are not used)
         float m[ET][2], l[ET][2];
+        // values' scales are below 2^v_exp so far; they enter the operands times 2^(1 - v_exp), and the sums carry that factor
+        int v_exp = kExpMin;
+        uint32_t v_mul = pack(pow2(1 - kExpMin), pow2(1 - kExpMin));
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -321,9 +340,51 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
         for (int e = 0; e < ET; e++) m[e][0] = m[e][1] = kNone, l[e][0] = l[e][1] = 0.f;
         const int odd_shift = (r8 & 1) * 16;
 
+        // whether the scales (of tokens with a bit in `any`; none is negative) lie below 2^v_exp
+        auto fit = [&](const uint32_t (&s0)[NG], const uint32_t (&s1)[NG], uint32_t any0, uint32_t any1) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int g = 0; g < NG; g++) most = max2(most, max2(s0[g] & any0, s1[g] & any1));
+            return below2(most, (uint32_t)(v_exp + 15) * 0x04000400u);      // infinity for 2^16
+        };
+        // raise v_exp above them, and the sums with it
+        auto raise_scale = [&](const uint32_t (&s0)[NG], const uint32_t (&s1)[NG], uint32_t any0, uint32_t any1) {
+            float mx = 0.f;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const float2 a0 = halves(finite2(s0[g] & any0)), a1 = halves(finite2(s1[g] & any1));
+                mx = fmaxf(fmaxf(mx, fmaxf(a0.x, a0.y)), fmaxf(a1.x, a1.y));
+            }
+            const int top = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)) >> 23) - 126;     // mx < 2^top
+            if (top <= v_exp) return;       // infinite or NaN
+            const int now = min(top + 1, kExpMax);      // one spare: scales that grow slowly raise it seldom
+            const float f = pow2(v_exp - now);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int g = 0; g < NG; g++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) acc[n][g][j >> 2][j & 3] *= f;
+            v_exp = now;
+            v_mul = pack(pow2(1 - now), pow2(1 - now));
+        };
         // one tile, with masks where some row sees a part of it only
         auto tile = [&](const uint8_t* t, const int base, auto masked) {
             constexpr bool part = decltype(masked)::value;
+            // V's scales.  Where every row sees every token they are checked with the scores, by one vote (64 requests of 128-wide
+            // heads: 69 us against 75), else with the weights; so too for heads 256 wide, where the registers do not last for
+            // it (a window of 4096: 59 us against 65)
+            constexpr bool one_vote = !part && D < 256;
+            uint32_t v0[NG], v1[NG], s0[NG], s1[NG];
+            auto load_scales = [&]() {
+                load_words<NG>(t + kv4_off_vs(D) + q4 * NG * 4, s0);
+                load_words<NG>(t + kv4_off_vs(D) + (q4 + 4) * NG * 4, s1);
+            };
+            bool fits = true;
+            if constexpr (one_vote) {
+                load_scales();
+                fits = fit(s0, s1, 0xffffffffu, 0xffffffffu);
+            }
             // ---- scores: tokens r8, r8 + 8 x rows 2 q4, 2 q4 + 1 of each column ----
             float sc[ET][4];
             {
@@ -408,7 +469,11 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
             float top = -INFINITY;
 #pragma unroll
             for (int e = 0; e < ET; e++) top = fmaxf(top, fmaxf(fmaxf(ex[e][0], ex[e][1]), fmaxf(ex[e][2], ex[e][3])));
-            if (__any_sync(0xffffffffu, top > kSlack)) {
+            if (__any_sync(0xffffffffu, top > kBias + kSlack || !fits)) {
+                if constexpr (one_vote) {
+                    load_scales();
+                    raise_scale(s0, s1, 0xffffffffu, 0xffffffffu);
+                }
 #pragma unroll
                 for (int e = 0; e < ET; e++)
 #pragma unroll
@@ -417,7 +482,7 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
                                           ex[e][j + 2] == -INFINITY ? -INFINITY : sc[e][j + 2] * qk[e][j]);
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
-                        now = fmaxf(m[e][j], now);
+                        now = fmaxf(m[e][j], now - kBias);
                         const float f = ex2(m[e][j] - now);
                         m[e][j] = now;
                         l[e][j] *= f;
@@ -459,11 +524,9 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
             }
 
             // ---- output: scales into the weights, codes of V, offsets ----
-            uint32_t v0[NG], v1[NG], s0[NG], s1[NG];
             load_words<NG>(t + kv4_off_vc(D) + (q4 * 8 + r8) * NG * 4, v0);
             load_words<NG>(t + kv4_off_vc(D) + ((q4 + 4) * 8 + r8) * NG * 4, v1);
-            load_words<NG>(t + kv4_off_vs(D) + q4 * NG * 4, s0);
-            load_words<NG>(t + kv4_off_vs(D) + (q4 + 4) * NG * 4, s1);
+            load_scales();
             {
                 uint32_t z0 = 0, z1 = 0, y0 = 0, y1 = 0;
                 if (r8 < NG) {
@@ -489,24 +552,35 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
                     }
                 }
             }
+            // tokens with a weight: the others' scales count as 0 for the row, they may not be finite
+            uint32_t k0[ET], k1[ET], any0 = 0xffffffffu, any1 = 0xffffffffu;
+            if constexpr (part) {
+                any0 = any1 = 0;
+#pragma unroll
+                for (int e = 0; e < ET; e++) {
+                    const uint32_t p0 = SPLIT || kFp16 ? ph[e][0] | pl[e][0] : ph[e][0];
+                    const uint32_t p1 = SPLIT || kFp16 ? ph[e][1] | pl[e][1] : ph[e][1];
+                    k0[e] = (p0 & 0x7fffu ? 0xffffu : 0u) | (p0 & 0x7fff0000u ? 0xffff0000u : 0u);
+                    k1[e] = (p1 & 0x7fffu ? 0xffffu : 0u) | (p1 & 0x7fff0000u ? 0xffff0000u : 0u);
+                    any0 |= k0[e], any1 |= k1[e];
+                }
+            }
+            if constexpr (!one_vote)
+                if (!__all_sync(0xffffffffu, fit(s0, s1, any0, any1))) raise_scale(s0, s1, any0, any1);
             uint32_t b[NT][NG][2];
 #pragma unroll
             for (int e = 0; e < ET; e++) {
-                uint32_t u0[NG], u1[NG];   // the scales, 0 where a weight is: they may not be finite
+                uint32_t u0[NG], u1[NG];
 #pragma unroll
-                for (int g = 0; g < NG; g++) u0[g] = s0[g], u1[g] = s1[g];
-                if constexpr (part) {
-                    const uint32_t any0 = SPLIT || kFp16 ? ph[e][0] | pl[e][0] : ph[e][0];
-                    const uint32_t any1 = SPLIT || kFp16 ? ph[e][1] | pl[e][1] : ph[e][1];
-                    const uint32_t k0 = (any0 & 0x7fffu ? 0xffffu : 0u) | (any0 & 0x7fff0000u ? 0xffff0000u : 0u);
-                    const uint32_t k1 = (any1 & 0x7fffu ? 0xffffu : 0u) | (any1 & 0x7fff0000u ? 0xffff0000u : 0u);
-#pragma unroll
-                    for (int g = 0; g < NG; g++) u0[g] &= k0, u1[g] &= k1;
+                for (int g = 0; g < NG; g++) {
+                    u0[g] = part ? s0[g] & k0[e] : s0[g];
+                    u1[g] = part ? s1[g] & k1[e] : s1[g];
                 }
                 if constexpr (SPLIT || kFp16) {
                     const float2 h0 = halves(ph[e][0]), h1 = halves(ph[e][1]), l0 = halves(pl[e][0]), l1 = halves(pl[e][1]);
-                    const float p0 = fmaf(l0.x, kLoInv, h0.x), p1 = fmaf(l0.y, kLoInv, h0.y);
-                    const float p2 = fmaf(l1.x, kLoInv, h1.x), p3 = fmaf(l1.y, kLoInv, h1.y);
+                    const float f = pow2(1 - v_exp);
+                    const float p0 = fmaf(l0.x, kLoInv, h0.x) * f, p1 = fmaf(l0.y, kLoInv, h0.y) * f;
+                    const float p2 = fmaf(l1.x, kLoInv, h1.x) * f, p3 = fmaf(l1.y, kLoInv, h1.y) * f;
 #pragma unroll
                     for (int g = 0; g < NG; g++) {
                         const float2 a0 = halves(u0[g]), a1 = halves(u1[g]);
@@ -521,8 +595,8 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
                 } else {
 #pragma unroll
                     for (int g = 0; g < NG; g++) {
-                        b[e][g][0] = mul2(ph[e][0], u0[g]);
-                        b[e][g][1] = mul2(ph[e][1], u1[g]);
+                        b[e][g][0] = mul2(ph[e][0], mul2(u0[g], v_mul));
+                        b[e][g][1] = mul2(ph[e][1], mul2(u1[g], v_mul));
                     }
                 }
             }
@@ -571,6 +645,7 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
         __syncthreads();
         float* s_o = reinterpret_cast<float*>(smem);                                   // [W][kRows][D]
         float2* s_ml = reinterpret_cast<float2*>(smem + W * kRows * D * 4);       // [W][kRows]
+        const float unit = pow2(v_exp - 1);
 #pragma unroll
         for (int e = 0; e < ET; e++)
 #pragma unroll
@@ -585,7 +660,7 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
                     for (int k = 0; k < 4; k++) {   // channel g*32 + r8*4 + k
                         const float v = SPLIT ? fmaf(acc[NT - 1][g][k >> 1][j + 2 * (k & 1)], kLoInv, acc[e][g][k >> 1][j + 2 * (k & 1)])
                                               : acc[e][g][k >> 1][j + 2 * (k & 1)];
-                        o[k] = fmaf(v, k & 1 ? 32.f : 512.f, zg);
+                        o[k] = fmaf(v, (k & 1 ? 32.f : 512.f) * unit, zg);
                     }
                     *reinterpret_cast<float4*>(s_o + rr * D + g * kKvGroup + r8 * 4) = make_float4(o[0], o[1], o[2], o[3]);
                 }

@@ -7,7 +7,10 @@ namespace draco {
 namespace attn {
 
 constexpr float kNone = -1e30f;     // maximum of a row that has seen nothing
-constexpr float kSlack = 3.f;       // log2 of the largest weight
+// Weights are exp2(score - m), m = kBias below the row's largest score so far: the largest are 2^kBias, and fp16, in which
+// they are multiplied with values, keeps its full precision down to 2^-25 of that (17 nats below the largest score) and has
+// nothing left at 2^-36
+constexpr float kBias = 11.f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

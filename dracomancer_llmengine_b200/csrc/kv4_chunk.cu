@@ -18,8 +18,8 @@
 //
 // A channel's place inside its group of eight is the order in which a word's nibbles come apart, (0 4 1 5 2 6 3 7), in Q and
 // K alike.  Values of tokens that are not finite are stored as 0 and the token is noted: a row that sees it becomes NaN, one
-// that does not is left alone.  O is rescaled only when a row's maximum grows by more than 8 (log2): weights then go up to
-// 256, which fp16 has room for, and the rescaling waits for the product before it, so it should be rare.
+// that does not is left alone.  O is rescaled only when a row's maximum grows by more than 4 (log2): weights then go up to
+// 2^15, which fp16 has room for, and the rescaling waits for the product before it, so it should be rare.
 //
 // Every wait is bounded (2 s).  When one runs out the block raises its flag, all its roles leave their loops, the products
 // in flight are waited for, its rows become NaN, and TMEM is freed.
@@ -39,7 +39,7 @@ constexpr int kBufs = 4;            // of K and V
 constexpr int kTmem = 512;
 __device__ __forceinline__ uint32_t tmem_o(uint32_t tmem, int half) { return tmem + 128 * half; }
 __device__ __forceinline__ uint32_t tmem_s(uint32_t tmem, int half, uint32_t b) { return tmem + 256 + 128 * half + 64 * b; }
-constexpr float kRoom = 8.f;        // log2 of the largest weight
+constexpr float kRoom = 4.f;        // log2 by which weights may pass 2^kBias: below fp16's 2^16
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 template <int D>
@@ -383,8 +383,8 @@ __device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Co
             for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i]));
         }
         const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * qk;
-        if (__any_sync(0xffffffffu, mx - m > kRoom)) {
-            const float now = fmaxf(m, mx), f = ex2(m - now);
+        if (__any_sync(0xffffffffu, mx - m > kBias + kRoom)) {
+            const float now = fmaxf(m, mx - kBias), f = ex2(m - now);
             m = now;
             l *= f;
             if (j) {        // the sums so far, once the previous step's product is in them

@@ -1,0 +1,139 @@
+"""Attention over the 4-bit cache where the values' size, the scores' spread or the tokens' range are not those of unit normal
+numbers: against 64 bits, request by request."""
+import numpy as np
+import pytest
+import torch
+
+from dracomancer_llmengine_b200 import decoder
+from test_decoder_ops import TOL, TYPES, attend_ref, ints, rel
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _gpu(dlib):
+    pass
+
+
+def allowed(kind, want):
+    """TOL of the result's norm; an fp16 output has besides half its smallest step (2^-24) of absolute error a value."""
+    norm = float(torch.linalg.norm(want))
+    return TOL[kind] * norm + (2.0 ** -25 * want.numel() ** 0.5 if kind == "f16" else 0.0)
+
+
+def filled(k, v, page, spare=1, seed=0):
+    """A cache with the tokens of each request (k, v: lists of fp32 [tokens, heads, d]), its table, pages in random order."""
+    heads, d = k[0].shape[1:]
+    lens = [t.shape[0] for t in k]
+    held = [-(-n // page) for n in lens]
+    cache = decoder.KV4Cache.empty(sum(held) + spare, page, heads, d)
+    ids = np.random.default_rng(seed).permutation(sum(held) + spare)
+    table = np.full((len(lens), max(held + [1])), -1, np.int32)
+    at = 0
+    for r, n in enumerate(lens):
+        table[r, :held[r]] = ids[at:at + held[r]]
+        at += held[r]
+        pos = np.arange(n)
+        if n:
+            cache.append(k[r].cuda(), v[r].cuda(), ints((table[r, pos // page] * page + pos % page).tolist()))
+    return cache, table, lens
+
+
+def check(kind, cache, table, lens, q_lens, q, window=0, sinks=0, with_lse=False, want_cache=None):
+    cu = [sum(q_lens[:i]) for i in range(len(q_lens) + 1)]
+    out = torch.full_like(q, 5.0)
+    lse = torch.empty(q.shape[:2], device="cuda") if with_lse else None
+    cache.attend(q, out, ints(cu), ints(lens), torch.from_numpy(table).cuda(), max(q_lens), max(lens), window=window,
+                 sinks=sinks, lse=lse)
+    want, want_lse = attend_ref(cache, table, q, cu, lens, window, sinks)
+    assert torch.isfinite(out).all()
+    for r in range(len(lens)):
+        a, b = out[cu[r]:cu[r + 1]].double().cpu(), want[cu[r]:cu[r + 1]]
+        assert float(torch.linalg.norm(a - b)) <= allowed(kind, b), f"request {r}: {rel(a, b)}"
+    if with_lse:
+        assert float((lse.cpu().double() - want_lse).abs().max()) <= 2e-5
+    return out
+
+
+def dominated(n, margins, value, heads, d, seed):
+    """Requests whose first token is `margin` nats above the others and has values near 0 (a thousandth of theirs)."""
+    gen = torch.Generator().manual_seed(seed)
+    sign = torch.randn(heads, d, generator=gen).sign()
+    k, v = [], []
+    for m in margins:
+        k.append(torch.randn(n, heads, d, generator=gen))
+        v.append(value * torch.randn(n, heads, d, generator=gen))
+        k[-1][0] = sign * m / d ** 0.5      # a query of ones along the signs scores m
+        v[-1][0] *= 1e-3
+    return k, v, sign
+
+
+def queries(kind, sign, rows, per, seed):
+    """Queries near the signs of their kv head: [rows, heads, d]."""
+    gen = torch.Generator().manual_seed(seed)
+    heads, d = sign.shape
+    q = sign.repeat_interleave(per, 0) + 0.3 * torch.randn(rows, heads * per, d, generator=gen)
+    return q.cuda().to(TYPES[kind])
+
+
+MARGINS = [0.0, 6.0, 9.0, 12.0, 14.0]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("value", [1e-3, 1e-2, 0.1, 1.0, 1e3])
+@pytest.mark.parametrize("n,d,heads,per,window", [(4096, 128, 2, 4, 0), (4099, 128, 1, 16, 1500), (1001, 64, 2, 8, 0),
+                                                  (2048, 256, 1, 8, 0)])
+def test_dominating_token_single(kind, value, n, d, heads, per, window):
+    """A first token that takes most of the weight and adds nothing: the result is what the small weights of the others
+    give, in sums split over blocks and in whole units, visible as one of the first tokens beside a window."""
+    k, v, sign = dominated(n, MARGINS, value, heads, d, 1)
+    cache, table, lens = filled(k, v, 32)
+    check(kind, cache, table, lens, [1] * len(lens), queries(kind, sign, len(lens), per, 2), window, 1 if window else 0)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("value", [1e-3, 0.1, 1e3])
+@pytest.mark.parametrize("rows,window", [(40, 0), (70, 900)])
+def test_dominating_token_chunk(kind, value, rows, window):
+    """The same for chunks (bf16: the tensor-core form)."""
+    n, d, heads, per = 2048, 128, 1, 4
+    k, v, sign = dominated(n, MARGINS, value, heads, d, 3)
+    cache, table, lens = filled(k, v, 64)
+    q_lens = [rows - i for i in range(len(lens))]
+    check(kind, cache, table, lens, q_lens, queries(kind, sign, sum(q_lens), per, 4), window, 2 if window else 0)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("value", [1e-2, 1.0])
+def test_dominating_token_long(kind, value):
+    k, v, sign = dominated(100003, [12.0, 14.0], value, 1, 128, 5)
+    cache, table, lens = filled(k, v, 64)
+    check(kind, cache, table, lens, [1, 1], queries(kind, sign, 2, 8, 6))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("value", [1e-3, 1e-2, 3e4])
+def test_value_sizes(kind, value):
+    """No token dominates; values far from 1."""
+    gen = torch.Generator().manual_seed(7)
+    k = [torch.randn(n, 2, 128, generator=gen) for n in (1, 2, 40, 700, 4100)]
+    v = [(value * torch.randn(t.shape, generator=gen)).clamp(-6e4, 6e4) for t in k]
+    cache, table, lens = filled(k, v, 16)
+    q = torch.randn(len(lens), 8, 128, generator=gen).cuda().to(TYPES[kind])
+    check(kind, cache, table, lens, [1] * len(lens), q)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("order", ["up", "down", "mixed"])
+def test_value_sizes_that_change(kind, order):
+    """Values that grow, shrink or jump by factors of ten along the context, within what one sum of fp32 can hold."""
+    gen = torch.Generator().manual_seed(8)
+    n = 3000
+    size = 10.0 ** torch.linspace(-3, 3, n)
+    size = {"up": size, "down": size.flip(0), "mixed": size[torch.randperm(n, generator=gen)]}[order]
+    k = [torch.randn(n, 2, 128, generator=gen)]
+    v = [size[:, None, None] * torch.randn(n, 2, 128, generator=gen)]
+    cache, table, lens = filled(k, v, 16)
+    q = torch.randn(1, 8, 128, generator=gen).cuda().to(TYPES[kind])
+    check(kind, cache, table, lens, [1], q)
+    check(kind, cache, table, lens, [90], torch.randn(90, 4, 128, generator=gen).cuda().to(TYPES[kind]))
