@@ -227,7 +227,9 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
         auto fetch = [&](int i0) {
             const int i = i0 + lane;
             if (i >= count) return -1;
-            const int tile = tile_of(i), p = tile / x.page_tiles, page = table[p];
+            const int tile = tile_of(i);
+            if (tile * kKvTile >= sp.seq) return -1;        // the one tile of a request without keys: its row may be empty
+            const int p = tile / x.page_tiles, page = table[p];
             if (page < 0 || page >= a.cache.n_pages) return -1;
             return (page * a.cache.n_kv_heads + kvh) * x.page_tiles.d + (tile - p * x.page_tiles.d);
         };
