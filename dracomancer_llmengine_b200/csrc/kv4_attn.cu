@@ -207,7 +207,9 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
 
     for (;;) {
         if (kRuns && x.runs) {
-            while (!span_of(x, req, 0, sp)) req++;      // requests without queries have no tiles
+            // requests without queries have no tiles; the bound holds whatever the lengths are, should they change meanwhile
+            while (req < a.n_req && !span_of(x, req, 0, sp)) req++;
+            if (req >= a.n_req) return;
             end = (int)min((long)sp.n, begin + left);
             left -= end - begin;
             whole = begin == 0 && end == sp.n;
@@ -732,9 +734,12 @@ __global__ void __launch_bounds__(256) join_kernel(const Args x) {
     int active;
     long at, step = kRows, back = 0;    // row `rr` of the unit's first slot, and how the others follow
     if (x.runs) {
-        const int f = req * x.row_blocks + rb, per = x.before[a.n_req * x.row_blocks + 1];
-        const int first = x.before[f] * a.cache.n_kv_heads + kvh * sp.n, c0 = first / per;
-        active = (first + sp.n - 1) / per - c0 + 1;
+        const int f = req * x.row_blocks + rb, per = max(x.before[a.n_req * x.row_blocks + 1], 1);
+        const int first = x.before[f] * a.cache.n_kv_heads + kvh * sp.n;
+        int c0 = first / per;
+        // (the slots exist whatever was read: a workspace that another call wrote gives a wrong result, not a read out of range)
+        c0 = min(max(c0, 0), x.runs - 1);
+        active = min((first + sp.n - 1) / per - c0 + 1, x.runs - c0);
         at = (2l * c0 + 1) * kRows + rr;       // the run in which the unit begins; the others' slots are even
         step = 2 * kRows, back = kRows;
     } else {

@@ -523,11 +523,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const Args x) {
 
     for (uint32_t step0 = 0;;) {
         if (x.runs) {
+            // blocks of rows without queries have no tiles; the bound holds whatever the lengths are, should they change meanwhile
+            bool found = false;
 #pragma unroll 1
-            for (;; f++) {      // blocks of rows without queries have no tiles
+            for (; f < a.n_req * x.row_blocks && !found; f++) {
                 req = f / x.row_blocks, g.rb = f - req * x.row_blocks;
-                if (span_of(x, req, g.rb, g.sp)) break;
+                found = span_of(x, req, g.rb, g.sp);
             }
+            if (!found) break;
+            f--;
             g.n = (int)min((long)g.sp.n - g.begin, left);
             left -= g.n;
             g.whole = g.begin == 0 && g.n == g.sp.n;
