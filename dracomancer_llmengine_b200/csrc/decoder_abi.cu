@@ -104,6 +104,16 @@ extern "C" {
 
 // not part of the interface: for decoder_py.cpp
 void draco_b200_pointers_checked(int on) { t_pointers_checked = on != 0; }
+// the id of the graph capture that the stream is in, 0: none
+unsigned long long draco_b200_capture_id(void* stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &id) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusNone ? 0 : id;
+}
 
 int draco_b200_plan_blocks(const int* ctx_len, const int* new_len, int n_req, int page_size, int* block_table,
                            long table_stride, int table_width, const int* free_pages, int free_len, const int* n_free,

@@ -27,6 +27,7 @@ decltype(&draco_b200_kv4_attention_workspace) f_workspace = nullptr;
 decltype(&draco_b200_kv4_attention) f_attention = nullptr;
 decltype(&draco_b200_rmsnorm_q8) f_norm = nullptr;
 void (*f_checked)(int) = nullptr;
+unsigned long long (*f_capture_id)(void*) = nullptr;
 
 struct Refused : std::runtime_error {
     using std::runtime_error::runtime_error;
@@ -136,7 +137,7 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!take("draco_b200_last_error", f_last_error) || !take("draco_b200_plan_blocks", f_plan_blocks) ||
         !take("draco_b200_kv4_append", f_append) || !take("draco_b200_kv4_read", f_read) ||
         !take("draco_b200_kv4_attention_workspace", f_workspace) || !take("draco_b200_kv4_attention", f_attention) ||
-        !take("draco_b200_pointers_checked", f_checked) || !take("draco_b200_rmsnorm_q8", f_norm))
+        !take("draco_b200_pointers_checked", f_checked) || !take("draco_b200_capture_id", f_capture_id) || !take("draco_b200_rmsnorm_q8", f_norm))
         return nullptr;
     Py_INCREF(a[0]);
     Py_XSETREF(g_error, a[0]);
@@ -207,9 +208,10 @@ PyObject* kv4_append(PyObject*, PyObject* const* a, Py_ssize_t n) { return rows(
 PyObject* kv4_read(PyObject*, PyObject* const* a, Py_ssize_t n) { return rows(a, n, false); }
 
 // (pages, page_size, head_dim, scratch, grow, q, out, cu_q, seq_len, block_table, max_q_len, max_seq_len, scale, window,
-//  sinks, lse, stream); scratch: {stream: tensor}, grow(stream, bytes): a larger one
+//  sinks, lse, stream, workspace); where workspace is None: scratch: {stream: tensor}, for calls that no graph captures,
+//  grow(stream, bytes, capture): another buffer, of the stream or of the capture
 PyObject* kv4_attend(PyObject*, PyObject* const* a, Py_ssize_t given) {
-    return guarded(given, 17, [&] {
+    return guarded(given, 18, [&] {
         const at::Tensor &pages = tensor(a[0], "pages"), &q = tensor(a[5], "q"), &out = tensor(a[6], "out"),
                          &cu = vector_of(a[7], at::kInt, "cu_q"), &seq = vector_of(a[8], at::kInt, "seq_len"),
                          &table = tensor(a[9], "block_table");
@@ -242,22 +244,29 @@ PyObject* kv4_attend(PyObject*, PyObject* const* a, Py_ssize_t given) {
         p.max_q_len = small(a[10], "max_q_len"), p.max_seq_len = small(a[11], "max_seq_len");
         p.scale = (float)real(a[12]), p.window = small(a[13], "window"), p.sinks = small(a[14], "sinks");
         const size_t bytes = f_workspace(&c, &p);
-        if (bytes) {
-            PyObject* key = PyLong_FromVoidPtr(s);
+        if (const at::Tensor* ws = maybe(a[17], "workspace")) {
+            need(ws->device() == dev && ws->is_contiguous(), "workspace must be a contiguous tensor on the cache's device");
+            p.workspace = ws->data_ptr(), p.workspace_bytes = ws->nbytes();
+        } else if (bytes) {
+            // a captured call keeps its buffer's address, and its graph may run on any stream: captures have their own
+            const unsigned long long capture = f_capture_id(s);
+            // the per-thread default stream is another one in each thread
+            PyObject* key = s == (void*)cudaStreamPerThread ? PyLong_FromLongLong(-(long long)PyThread_get_thread_ident())
+                                                            : PyLong_FromVoidPtr(s);
             if (!key) throw PythonError{};
-            PyObject* ws = PyDict_GetItemWithError(a[3], key);    // borrowed
-            if (ws && THPVariable_Check(ws) && (size_t)THPVariable_Unpack(ws).numel() >= bytes) {
-                Py_INCREF(ws);
+            PyObject* buf = capture ? nullptr : PyDict_GetItemWithError(a[3], key);    // borrowed
+            if (buf && THPVariable_Check(buf) && THPVariable_Unpack(buf).nbytes() >= bytes) {
+                Py_INCREF(buf);
             } else {
-                ws = PyErr_Occurred() ? nullptr : PyObject_CallFunction(a[4], "On", key, (Py_ssize_t)bytes);
+                buf = PyErr_Occurred() ? nullptr : PyObject_CallFunction(a[4], "OnK", key, (Py_ssize_t)bytes, capture);
             }
             Py_DECREF(key);
-            if (!ws) throw PythonError{};
-            if (THPVariable_Check(ws)) {     // the dictionary keeps it alive
-                p.workspace = THPVariable_Unpack(ws).data_ptr();
-                p.workspace_bytes = (size_t)THPVariable_Unpack(ws).numel();
+            if (!buf) throw PythonError{};
+            if (THPVariable_Check(buf)) {     // what grow() keeps alive
+                p.workspace = THPVariable_Unpack(buf).data_ptr();
+                p.workspace_bytes = THPVariable_Unpack(buf).nbytes();
             }
-            Py_DECREF(ws);
+            Py_DECREF(buf);
         }
         return done(f_attention(&c, &p, s), "draco_b200_kv4_attention");
     });

@@ -17,10 +17,11 @@ One decode step of a layer:
 from __future__ import annotations
 
 import ctypes as ct
+import weakref
 
 import torch
 
-from . import DracoError, DracoKV4Cache, lib
+from . import DracoError, DracoKV4Attention, DracoKV4Cache, lib
 
 try:
     from . import _decoder
@@ -33,7 +34,15 @@ __all__ = ["BlockPlan", "plan_blocks", "KV4Cache", "rmsnorm_q8"]
 _decoder.setup(DracoError, {name: ct.cast(getattr(lib(), name), ct.c_void_p).value for name in (
     "draco_b200_last_error", "draco_b200_plan_blocks", "draco_b200_kv4_append", "draco_b200_kv4_read",
     "draco_b200_kv4_attention_workspace", "draco_b200_kv4_attention", "draco_b200_rmsnorm_q8",
-    "draco_b200_pointers_checked")})
+    "draco_b200_pointers_checked", "draco_b200_capture_id")})
+
+# Scratch for attention whose long axis is split over blocks.  Eager calls on a stream run one after the other and share
+# its buffer, whichever cache they read; the calls of a graph capture have a buffer of that capture and stream, which the
+# caches that it reads keep.
+_eager: dict = {}           # {device index: {stream: tensor}}
+_per_thread: list = []      # outgrown buffers of per-thread default streams: the allocator takes them all for one stream
+_captured = weakref.WeakValueDictionary()    # {(capture, stream): tensor}
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 def _need(ok, what: str):
@@ -72,7 +81,13 @@ def plan_blocks(ctx_len, new_len, block_table, free_pages, n_free, page_size: in
 class KV4Cache:
     """A paged KV cache in 4 bits over `pages`, uint8 [n_pages, n_kv_heads, page_size // 16, 20 * head_dim] (contiguous;
     1.25 bytes per key and value channel).  The pages are the caller's memory: the object adds nothing but their
-    description and a scratch buffer per stream for attention whose long axis is split over blocks."""
+    description.
+
+    Attention whose long axis is split over blocks needs scratch memory (:meth:`workspace_bytes`: 2 to 10 MB for single
+    tokens over long contexts, 40 MB for chunks).  Without `workspace=` the module keeps one buffer for each stream, for
+    all caches, and one for each graph capture, which lives as long as the caches that the capture read.  So eager calls
+    on different streams may overlap, and so may replays of different graphs, and eager calls with either.  Two replays
+    of the same graph may not, nor two calls that were given the same `workspace`."""
 
     def __init__(self, pages, page_size: int, head_dim: int):
         _need(pages.dtype is torch.uint8 and pages.is_cuda and pages.is_contiguous() and pages.dim() == 4,
@@ -84,8 +99,8 @@ class KV4Cache:
         self.pages, self.page_size, self.head_dim, self.n_kv_heads = pages, page_size, head_dim, pages.shape[1]
         self.device = pages.device
         self._desc = DracoKV4Cache(pages.data_ptr(), pages.shape[0], page_size, pages.shape[1], head_dim)
-        self._scratch: dict = {}
-        self._kept: list = []
+        self._scratch = _eager.setdefault(pages.get_device(), {})
+        self._kept: list = []       # buffers of captures
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device="cuda"):
@@ -93,15 +108,38 @@ class KV4Cache:
         return cls(torch.zeros(n_pages, n_kv_heads, page_size // 16, 20 * head_dim, dtype=torch.uint8, device=device),
                    page_size, head_dim)
 
-    def _grow(self, st: int, need: int):
-        """A scratch buffer of at least `need` bytes for stream `st`.  Outgrown ones are kept: kernels in flight or a
-        captured graph may still use them (each is at most two thirds of its successor)."""
-        on = torch.cuda.ExternalStream(st, device=self.device) if st else torch.cuda.default_stream(self.device)
-        with torch.cuda.stream(on):   # the allocator then orders the memory's earlier uses before this stream's
-            ws = torch.empty(need + need // 2, dtype=torch.uint8, device=self.device)
-        self._kept.append(ws)
-        self._scratch[st] = ws
+    def _grow(self, key: int, need: int, capture: int):
+        """A scratch buffer of at least `need` bytes for the stream `key` (below 0: this thread's default stream), or for the
+        graph `capture` that is taken of it."""
+        st = 2 if key < 0 else key
+        ws = _captured.get((capture, key)) if capture else None
+        if ws is None or ws.numel() < need:
+            on = torch.cuda.ExternalStream(st, device=self.device) if st else torch.cuda.default_stream(self.device)
+            with torch.cuda.stream(on):   # the allocator orders the memory's earlier and later uses with this stream's
+                ws = torch.empty(-(-need >> 20) << 20, dtype=torch.uint8, device=self.device)
+        if capture:     # an outgrown one stays too: the graph's earlier calls use it
+            _captured[capture, key] = ws
+            if not any(ws is t for t in self._kept):
+                self._kept.append(ws)
+        else:
+            if key < 0 and key in self._scratch:
+                _per_thread.append(self._scratch[key])
+            self._scratch[key] = ws
         return ws
+
+    def workspace_bytes(self, n_heads: int, n_req: int, max_q_len: int, max_seq_len: int, dtype=torch.bfloat16, table_width=None,
+                        window: int = 0, sinks: int = 0, lse: bool = False) -> int:
+        """Bytes of scratch that :meth:`attend` takes for such a call (0: none).  table_width: columns of the block table,
+        by default those that max_seq_len takes."""
+        width = -(-max_seq_len // self.page_size) if table_width is None else table_width
+        _need(dtype in _DTYPES, "dtype must be float32, float16 or bfloat16")
+        _need(n_heads > 0 and n_heads % self.n_kv_heads == 0 and 0 <= n_req <= 65535 and
+              min(max_q_len, max_seq_len, width, window, sinks) >= 0 and max_q_len * n_heads < 1 << 27,
+              "n_heads must be a multiple of the cache's heads, lengths, window and sinks not negative")
+        a = DracoKV4Attention(dtype=_DTYPES[dtype], n_heads=n_heads, n_req=n_req, n_tokens=max(1, n_req), table_width=width,
+                              table_stride=width, max_q_len=max_q_len, max_seq_len=max_seq_len, scale=1.0, window=window,
+                              sinks=sinks, lse=1 if lse else None)
+        return lib().draco_b200_kv4_attention_workspace(self._desc, a)
 
     def append(self, k, v, slots, stream=None):
         """Quantise k and v [tokens, n_kv_heads, head_dim] into the given slots (int32; slots outside the cache, such as
@@ -114,16 +152,17 @@ class KV4Cache:
         return k, v
 
     def attend(self, q, out, cu_q, seq_len, block_table, max_q_len: int, max_seq_len: int, scale: float | None = None,
-               window: int = 0, sinks: int = 0, lse=None, stream=None):
+               window: int = 0, sinks: int = 0, lse=None, stream=None, workspace=None):
         """Causal attention of the ragged queries q [tokens, n_heads, head_dim] into out (same shape and type).
 
         Request r's queries are tokens cu_q[r] .. cu_q[r + 1], the last ones of its seq_len[r] cached tokens; its pages are
         row r of block_table.  max_q_len and max_seq_len bound them on the host.  scale defaults to head_dim ** -0.5.
         With window > 0 a query sees the last `window` keys up to its own and the first `sinks` tokens.  lse: optional
-        fp32 [tokens, n_heads] for the log of the sum of exponentials.  Rows that see nothing are 0 (lse -inf)."""
+        fp32 [tokens, n_heads] for the log of the sum of exponentials.  Rows that see nothing are 0 (lse -inf).
+        workspace: a contiguous tensor of at least :meth:`workspace_bytes` for this call alone, instead of the module's."""
         _decoder.kv4_attend(self.pages, self.page_size, self.head_dim, self._scratch, self._grow, q, out, cu_q, seq_len,
                             block_table, max_q_len, max_seq_len, self.head_dim ** -0.5 if scale is None else scale,
-                            window, sinks, lse, _stream(stream))
+                            window, sinks, lse, _stream(stream), workspace)
         return out
 
 

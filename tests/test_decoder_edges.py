@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import dracomancer_llmengine_b200 as dm
 from dracomancer_llmengine_b200 import decoder
 from test_decoder_ops import TYPES, ints
 
@@ -29,3 +30,80 @@ def test_attend_tables_without_columns(kind, rows, heads, max_seq, with_lse):
         assert not out.any()
         if with_lse:
             assert bool((lse == -float("inf")).all())
+
+
+def split_call(seed, lens, heads=8, d=128, page=16):
+    """A cache and the arguments of a call whose long axis is split, over pages of random tokens."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    held = [-(-n // page) for n in lens]
+    cache = decoder.KV4Cache.empty(sum(held), page, 2, d)
+    slots = torch.arange(sum(held) * page, dtype=torch.int32, device="cuda")
+    kv = torch.randn(2, slots.numel(), 2, d, device="cuda", generator=gen)
+    cache.append(kv[0], kv[1], slots)
+    table = torch.full((len(lens), max(held)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for r, n in enumerate(held):
+        table[r, :n] = torch.arange(at, at + n, device="cuda")
+        at += n
+    q = torch.randn(len(lens), heads, d, device="cuda", generator=gen)
+    return cache, q, ints(list(range(len(lens) + 1))), ints(lens), table, 1, max(lens)
+
+
+def test_graphs_of_one_cache_on_two_streams():
+    """Two captured calls of one cache, with other requests and lengths, replayed at the same time, eager calls beside them:
+    none disturbs another's partial sums."""
+    cache, q, cu, seq, table, _, longest = split_call(1, [30000, 9000, 17, 24000])
+    cases = []
+    for part in (slice(0, 2), slice(1, 4)):
+        n = part.stop - part.start
+        args = (q[part].clone(), cu[:n + 1].clone(), seq[part].clone(), table[part].clone())
+        want = cache.attend(args[0], torch.empty_like(args[0]), *args[1:], 1, longest).clone()
+        out, graph = torch.empty_like(args[0]), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            cache.attend(args[0], out, *args[1:], 1, longest)
+        cases.append((graph, out, want, torch.cuda.Stream(), args))     # a graph reads its inputs where they were
+    torch.cuda.synchronize()
+    side, eager = torch.cuda.Stream(), []
+    for _ in range(50):
+        for graph, out, _, stream, _ in cases:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(side):
+            eager.append(cache.attend(q, torch.empty_like(q), cu, seq, table, 1, longest))
+    torch.cuda.synchronize()
+    for graph, out, want, _, _ in cases:
+        assert torch.equal(out, want)
+    assert all(torch.equal(e, eager[0]) for e in eager)
+    kept = {t.data_ptr() for t in cache._kept}
+    assert len(kept) == 2 and not kept & {t.data_ptr() for t in decoder._eager[cache.device.index].values()}
+
+
+def test_scratch_is_shared_by_caches_and_outgrown():
+    """Caches on one stream share its buffer; a larger call in between leaves the earlier results right."""
+    small, large = split_call(2, [5000]), split_call(3, [40000] * 6, heads=16)
+    first = [c[0].attend(c[1], torch.empty_like(c[1]), *c[2:]).clone() for c in (small, large)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        again = [c[0].attend(c[1], torch.empty_like(c[1]), *c[2:]).clone() for c in (small, large, small, large)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, first[i % 2]) for i, a in enumerate(again))
+    assert small[0]._scratch is large[0]._scratch and stream.cuda_stream in small[0]._scratch
+    assert not small[0]._kept
+
+
+def test_workspace_of_the_caller():
+    cache, q, cu, seq, table, rows, longest = split_call(4, [9000, 100])
+    want = cache.attend(q, torch.empty_like(q), cu, seq, table, rows, longest)
+    n = cache.workspace_bytes(8, 2, rows, longest, dtype=torch.float32, table_width=table.shape[1])
+    assert n > 0 and cache.workspace_bytes(8, 2, 1, 100) == 0
+    ws = torch.full((n + 64,), 255, dtype=torch.uint8, device="cuda")
+    before = dict(decoder._eager[cache.device.index])
+    got = cache.attend(q, torch.empty_like(q), cu, seq, table, rows, longest, workspace=ws[:n])
+    assert torch.equal(got, want) and bool((ws[n:] == 255).all()) and decoder._eager[cache.device.index] == before
+    for bad in (ws[:n - 1], ws[:n].cpu(), ws[::2], ws[1:n + 1], "x"):
+        with pytest.raises(dm.DracoError):
+            cache.attend(q, torch.empty_like(q), cu, seq, table, rows, longest, workspace=bad)
+    for bad in (dict(n_heads=7), dict(n_heads=0), dict(max_q_len=-1), dict(dtype=torch.float64)):
+        with pytest.raises(dm.DracoError):
+            cache.workspace_bytes(**{**dict(n_heads=8, n_req=2, max_q_len=1, max_seq_len=100), **bad})
