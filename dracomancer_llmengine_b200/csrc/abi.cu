@@ -12,6 +12,7 @@
 #include "tc_gemm.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <chrono>
 #include <cmath>
 #include <cstdarg>
@@ -55,7 +56,8 @@ int tc_min_assignments() {
     }
     return v;
 }
-long g_launches = 0;          // kernels this library launched (all devices)
+long g_launches = 0;          // kernels this library launched (all devices), those of g_others apart
+std::atomic<long> g_others{0};        // kernels of the entry points outside this file, which do not take g_mu
 
 // Optional per-phase device timing: CUDA events recorded around each phase on the launching
 // stream, resolved when read.
@@ -1426,10 +1428,7 @@ int stage_in(Ctx* c, cudaStream_t s, size_t off, const T* h, size_t n) {
 // for the entry points outside this file (abi.h)
 namespace draco {
 void abi_error(const char* text) { g_err = text; }
-void abi_count(int kernels) {
-    std::lock_guard<std::mutex> lk(g_mu);
-    g_launches += kernels;
-}
+void abi_count(int kernels) { g_others += kernels; }
 bool abi_device_ptr(const void* p) { return is_device_ptr(p); }
 }  // namespace draco
 
@@ -2243,7 +2242,7 @@ int draco_b200_ep_pull_combine(const float* const* src_partial, const int* row_o
 
 long draco_b200_launch_count(void) {
     std::lock_guard<std::mutex> lk(g_mu);
-    return g_launches;
+    return g_launches + g_others;
 }
 
 int draco_b200_set_gemm_path(int mode) {

@@ -3,6 +3,6 @@
 
 namespace draco {
 void abi_error(const char* text);           // text of draco_b200_last_error()
-void abi_count(int kernels);                // adds to draco_b200_launch_count()
+void abi_count(int kernels);                // adds to draco_b200_launch_count(); waits for no lock
 bool abi_device_ptr(const void* p);         // device or managed memory
 }  // namespace draco

@@ -1,6 +1,6 @@
 // C entry points of the decoder-layer operators (part 3 of the header): argument checks, then one launcher call.
-// They hold no state: no context, no registry, no workspace of the library's own, so they need no lock beyond the
-// launch counter's, and calls on different streams do not meet.
+// They hold no state: no context, no registry, no workspace of the library's own, so they take no lock (the launch counter
+// is atomic): calls on different streams do not meet, nor do they wait for the library's synchronous calls.
 #include "../../include/draco_moe_b200.h"
 #include "abi.h"
 #include "kv4.cuh"

@@ -1,9 +1,12 @@
 """Decoder-layer operators at the ends of what their arguments allow."""
+import threading
+import time
+
 import pytest
 import torch
 
 import dracomancer_llmengine_b200 as dm
-from dracomancer_llmengine_b200 import decoder
+from dracomancer_llmengine_b200 import decoder, synth
 from test_decoder_ops import TYPES, ints
 
 pytestmark = pytest.mark.gpu
@@ -107,3 +110,34 @@ def test_workspace_of_the_caller():
     for bad in (dict(n_heads=7), dict(n_heads=0), dict(max_q_len=-1), dict(dtype=torch.float64)):
         with pytest.raises(dm.DracoError):
             cache.workspace_bytes(**{**dict(n_heads=8, n_req=2, max_q_len=1, max_seq_len=100), **bad})
+
+
+def test_calls_do_not_wait_for_synchronous_ones():
+    """A decoder call returns while another thread is inside a synchronous call of the library, which waits for work that was
+    queued before it."""
+    layer = synth.make_layer(hidden=512, n_exp=8, n_used=2, inter=256)
+    x = torch.randn(4, layer.hidden, device="cuda")
+    out = torch.empty_like(x)
+    dm.forward(layer, x, out=out)       # weights are on the GPU from here on
+    plan, zero, one = decoder.BlockPlan(1, 4), ints([0]), ints([1])
+    table, free, count = ints([[-1, -1]]), ints([3, 4]), ints([2])
+    decoder.plan_blocks(zero, one, table, free, count, 16, plan)    # a kernel's first launch loads it, which may wait for the GPU
+    torch.cuda.synchronize()
+    side, inside, queued = torch.cuda.Stream(), threading.Event(), torch.cuda.Event()
+    torch.cuda._sleep(1_000_000_000)    # about half a second of the default stream, which the synchronous call waits for
+    queued.record()
+
+    def synchronous():
+        inside.set()
+        dm.forward(layer, x, out=out)
+
+    thread = threading.Thread(target=synchronous)
+    thread.start()
+    inside.wait()
+    time.sleep(0.1)
+    assert not queued.query()
+    decoder.plan_blocks(zero, one, table, free, count, 16, plan, stream=side)
+    assert not queued.query(), "the call waited for the synchronous one"
+    thread.join()
+    torch.cuda.synchronize()
+    assert plan.slots.tolist()[:1] == [4 * 16]
