@@ -322,4 +322,9 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_decoder", nullptr, -1, g_method
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__decoder(void) { return PyModule_Create(&g_module); }
+// torch_version: the torch whose headers this was built with
+PyMODINIT_FUNC PyInit__decoder(void) {
+    PyObject* m = PyModule_Create(&g_module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", DRACO_TORCH_VERSION)) Py_CLEAR(m);
+    return m;
+}

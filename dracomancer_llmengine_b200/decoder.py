@@ -26,7 +26,11 @@ from . import DracoError, DracoKV4Attention, DracoKV4Cache, lib
 try:
     from . import _decoder
 except ImportError as e:
-    raise DracoError("the operators' extension is missing: build it with `python -m dracomancer_llmengine_b200.build`") from e
+    raise DracoError("the operators' extension is missing or does not load: build it with "
+                     f"`python -m dracomancer_llmengine_b200.build` ({e})") from e
+if _decoder.torch_version != torch.__version__:
+    raise DracoError(f"the operators' extension was built for torch {_decoder.torch_version}, this is {torch.__version__}: "
+                     "build it again with `python -m dracomancer_llmengine_b200.build`")
 
 __all__ = ["BlockPlan", "plan_blocks", "KV4Cache", "rmsnorm_q8"]
 
