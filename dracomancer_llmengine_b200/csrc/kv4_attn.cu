@@ -458,7 +458,9 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
 #pragma unroll
                 for (int e = 0; e < ET; e++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) ex[e][j] = fmaf(sc[e][j], qk[e][j & 1], -m[e][j & 1]);
+                    // (the product is rounded by itself: m comes from such a product, and a large one's rounding, which a
+                    // fused operation leaves out, would pass for a difference of scores)
+                    for (int j = 0; j < 4; j++) ex[e][j] = __fsub_rn(__fmul_rn(sc[e][j], qk[e][j & 1]), m[e][j & 1]);
                 if constexpr (part) {
 #pragma unroll
                     for (int e = 0; e < ET; e++)
@@ -482,11 +484,11 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
                 for (int e = 0; e < ET; e++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        float now = fmaxf(ex[e][j] == -INFINITY ? -INFINITY : sc[e][j] * qk[e][j],
-                                          ex[e][j + 2] == -INFINITY ? -INFINITY : sc[e][j + 2] * qk[e][j]);
+                        float now = fmaxf(ex[e][j] == -INFINITY ? -INFINITY : __fmul_rn(sc[e][j], qk[e][j]),
+                                          ex[e][j + 2] == -INFINITY ? -INFINITY : __fmul_rn(sc[e][j + 2], qk[e][j]));
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
-                        now = fmaxf(m[e][j], now - kBias);
+                        now = fmaxf(m[e][j], below_score(now, kSlack));
                         const float f = ex2(m[e][j] - now);
                         m[e][j] = now;
                         l[e][j] *= f;

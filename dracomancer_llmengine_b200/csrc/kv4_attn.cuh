@@ -6,11 +6,16 @@
 namespace draco {
 namespace attn {
 
-constexpr float kNone = -1e30f;     // maximum of a row that has seen nothing
+constexpr float kNone = -3e38f;     // maximum of a row that has seen nothing: below every score
 // Weights are exp2(score - m), m = kBias below the row's largest score so far: the largest are 2^kBias, and fp16, in which
 // they are multiplied with values, keeps its full precision down to 2^-25 of that (17 nats below the largest score) and has
 // nothing left at 2^-36
 constexpr float kBias = 11.f;
+// m for a largest score: beyond 2^27 the numbers' steps may put m too far below it for fp16
+__device__ __forceinline__ float below_score(float score, float room) {
+    const float m = score - kBias;
+    return score - m > kBias + room ? score : m;
+}
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

@@ -27,6 +27,7 @@
 #include "tc_ptx.cuh"
 
 #include <atomic>
+#include <type_traits>
 
 namespace draco {
 namespace attn {
@@ -334,6 +335,7 @@ __device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Co
     const int pos_q = g.sp.seq - g.sp.q_len + ti;
     const float qk = c->qk[tid];
     float m = kNone, l = 0.f;
+    bool large = false;         // some row of the warp has scores of 2^22 and more
     bool ok = !c->abort;
     for (int j = 0; j < g.n && ok; j++) {
         const uint32_t step = step0 + j, b = step & 1, parity = (step >> 1) & 1, kv = step % kBufs;
@@ -382,10 +384,11 @@ __device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Co
 #pragma unroll
             for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i]));
         }
-        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * qk;
+        const float mx = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), qk);
         if (__any_sync(0xffffffffu, mx - m > kBias + kRoom)) {
-            const float now = fmaxf(m, mx - kBias), f = ex2(m - now);
+            const float now = fmaxf(m, below_score(mx, kRoom)), f = ex2(m - now);
             m = now;
+            large = __any_sync(0xffffffffu, fabsf(m) >= 4194304.f && m != kNone);
             l *= f;
             if (j) {        // the sums so far, once the previous step's product is in them
                 ok = await(&c->pv_done[half][(step - 1) % kBufs], (step - 1) / kBufs & 1, &c->abort);
@@ -405,15 +408,26 @@ __device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Co
         uint64_t sum = 0;       // two sums
         const uint64_t qk2 = twice(qk), m2 = twice(-m);
         uint32_t p[16];
-        auto weights = [&]() {
+        // (large products are rounded by themselves, as m was: what their rounding leaves would pass for a difference.  In scalar
+        // operations: the compiler fuses packed ones)
+        auto weights_of = [&](auto apart) {
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 float e0, e1;
-                split(fma2(join(v[2 * i], v[2 * i + 1]), qk2, m2), e0, e1);
+                if constexpr (decltype(apart)::value) {
+                    e0 = __fsub_rn(__fmul_rn(__uint_as_float(v[2 * i]), qk), m);
+                    e1 = __fsub_rn(__fmul_rn(__uint_as_float(v[2 * i + 1]), qk), m);
+                } else {
+                    split(fma2(join(v[2 * i], v[2 * i + 1]), qk2, m2), e0, e1);
+                }
                 e0 = ex2(e0), e1 = ex2(e1);
                 sum = add2(sum, join(__float_as_uint(e0), __float_as_uint(e1)));
                 p[i] = pack2<__half>(e0, e1);
             }
+        };
+        auto weights = [&]() {
+            if (large) weights_of(std::true_type{});
+            else weights_of(std::false_type{});
         };
         weights();          // of the second half, which go over scores of the first: those are read before
         tc_ld32(at, v);

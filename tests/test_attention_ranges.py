@@ -137,3 +137,43 @@ def test_value_sizes_that_change(kind, order):
     q = torch.randn(1, 8, 128, generator=gen).cuda().to(TYPES[kind])
     check(kind, cache, table, lens, [1], q)
     check(kind, cache, table, lens, [90], torch.randn(90, 4, 128, generator=gen).cuda().to(TYPES[kind]))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,n", [(1, 300), (1, 5000), (70, 300)])
+@pytest.mark.parametrize("negative", [False, True])
+def test_scores_of_large_magnitude(kind, rows, n, negative):
+    """Scores up to 1e32: the largest takes all the weight (they differ by far more than their rounding), whatever its size
+    and sign."""
+    d = 128
+    gen = torch.Generator().manual_seed(10)
+    sign = torch.randn(1, d, generator=gen).sign()
+    k = torch.randn(n, 1, d, generator=gen)
+    if negative:        # every score is below 0
+        k = k - sign
+    cache, table, lens = filled([k], [torch.randn(n, 1, d, generator=gen)], 32)
+    q = (sign + 0.1 * torch.randn(rows, 4, d, generator=gen) if negative else torch.randn(rows, 4, d, generator=gen))
+    q = q.cuda().to(TYPES[kind])
+    lse = torch.empty(rows, 4, device="cuda") if kind != "bf16" or rows == 1 else None
+    for scale in (1e5, 1e6, 3e7, 1e8, 1e9, 1e20, 1e30):
+        out = torch.zeros_like(q)
+        cache.attend(q, out, ints([0, rows]), ints(lens), torch.from_numpy(table).cuda(), rows, n, scale=scale, lse=lse)
+        want, want_lse = attend_ref(cache, table, q, [0, rows], lens, 0, 0, scale)
+        # rows in which the first two scores are closer than their rounding may go either way (fp16 keys: 2^-11 a channel)
+        s = torch.einsum("rhd,kd->rhk", q.double().cpu(), keys(cache, table, n)) * scale
+        mask = torch.arange(n) > torch.arange(n - rows, n)[:, None]
+        top = s.masked_fill(mask[:, None], -np.inf).topk(2, -1).values
+        clear = (top[..., 0] - top[..., 1]) > s.abs().amax() * 2.0 ** -8
+        assert int(clear.sum()) >= rows * 4 // 4
+        a, b = out.double().cpu()[clear], want[clear]
+        assert float(torch.linalg.norm(a - b)) <= allowed(kind, b), scale
+        if lse is not None:
+            assert float(((lse.cpu().double() - want_lse) / want_lse).abs().max()) <= 2.0 ** -18
+
+
+def keys(cache, table, n):
+    """fp64 keys of the one request and head of a cache."""
+    pos = np.arange(n)
+    k = torch.empty(n, 1, cache.head_dim, device="cuda")
+    cache.read(ints((table[0, pos // cache.page_size] * cache.page_size + pos % cache.page_size).tolist()), k, torch.empty_like(k))
+    return k[:, 0].double().cpu()
