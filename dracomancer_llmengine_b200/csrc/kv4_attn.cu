@@ -12,8 +12,9 @@
 //   scores: q . k = sum over groups g of s_g * (q . codes)_g + m_g * sum(q)_g.  A code's four bits are used as they are,
 //     as an fp16 subnormal (c * 2^-24, or 16 c * 2^-24 for the odd nibbles, against q / 16): one AND per two codes.
 //     Group sums come out of the products unscaled and are scaled in fp32; the offsets are one small product more.
-//     Queries are scaled to |q| <= 1 by a power of two per row first (16-bit queries then are exact in fp16); their
-//     sums have a high and a low half in every type, so the scores, and with them lse, keep fp32 precision.
+//     Queries are brought below 2^14 by a power of two per row first: 16-bit queries then are exact in fp16 down to 2^-28 (odd
+//     nibbles' 2^-24) of their row's largest, and off by 2^-39 (2^-35) of it below.  Their sums have a high and a low half
+//     in every type, so the scores, and with them lse, keep fp32 precision.
 //   output: sum_t p_t v_t = sum_t (p_t s_tg / 2) (2 c - 15) + sum_t p_t (m_tg - s_tg / 2): the weights take the scales,
 //     codes become (2 c - 15) * 2^-10 in one multiply-add.  They are centred because the sums run over the whole context:
 //     uncentred ones would grow with its length, cancel against the offsets' sum, and lose the result's low bits.
@@ -65,6 +66,7 @@ struct Shape {
 constexpr uint32_t kTwo15 = 0x78007800u;   // 2^15, 2^15 in fp16
 constexpr float kSlack = 3.f;              // log2 by which weights may pass 2^kBias
 constexpr int kExpMin = -14, kExpMax = 16;  // of the values' scales: 2^(1 - exponent) is an fp16 number
+constexpr float kSumUnit = 1.f / 32.f;     // sums of 32 queries below 2^14, and with them scores, are taken times this
 constexpr float kLoScale = 2048.f, kLoInv = 1.f / 2048.f;
 
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
@@ -272,10 +274,8 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
             for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(v[j]));
 #pragma unroll
             for (int o = 1; o < D / 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            // the power of two above the largest magnitude; zero, subnormal and huge rows keep a finite factor
-            int ex = (int)((__float_as_uint(top) >> 23) & 255) - 126;
-            ex = min(max(ex, -120), 120);
-            const float down = __uint_as_float((uint32_t)(127 - ex) << 23), up = __uint_as_float((uint32_t)(127 + ex) << 23);
+            float down, up;
+            query_unit(top, down, up);
             float t = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -295,12 +295,12 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
             if constexpr (SPLIT) q_sm[(g * NT + 1) * 32 + ln] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             if ((c8 & 3) == 0) {     // the group's sum: columns g of the offsets' product lie in lane g / 2 of the row
                 uint32_t th, tl;
-                split2(t, 0.f, th, tl);
+                split2(t * kSumUnit, 0.f, th, tl);
                 const int at = (e * 32 + (rr & 7) * 4 + (g >> 1)) * 2 + (g & 1);
                 qs_sm[at] = __ushort_as_half((uint16_t)th);
                 qs_sm[NT * 64 + at] = __ushort_as_half((uint16_t)tl);
             }
-            if (c8 == 0) qk_sm[rr] = a.scale * kLog2e * up;
+            if (c8 == 0) qk_sm[rr] = a.scale * kLog2e * up * (1.f / kSumUnit);
         }
         __syncthreads();
         uint32_t qf[S::kQInSmem ? 1 : NG][NT][4];
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
 #pragma unroll
                     for (int j = 0; j < 4; j++) z[j] = fmaf(y[j], kLoInv, z[j]);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) sc[e][j] = fmaf(s[e][j], SPLIT ? 512.f : 16777216.f, z[j]);
+                    for (int j = 0; j < 4; j++) sc[e][j] = fmaf(s[e][j], (SPLIT ? 512.f : 16777216.f) * kSumUnit, z[j]);
                 }
             }
 

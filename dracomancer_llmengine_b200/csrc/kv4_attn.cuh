@@ -42,6 +42,14 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// Queries become fp16 numbers below 2^14, by a power of two per row from its largest magnitude: those of 16-bit types keep
+// all their bits down to 2^-28 of that, and lose at most 2^-39 of it in absolute terms
+__device__ __forceinline__ void query_unit(float top, float& down, float& up) {
+    // top < 2^ex; zero and subnormal rows keep a finite factor
+    const int ex = min(max((int)((__float_as_uint(top) >> 23) & 255) - 126, -106), 128);
+    down = __uint_as_float((uint32_t)(127 + 14 - ex) << 23), up = __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
+}
+
 // What a block of rows looks at: tiles [0, head) for the first tokens, then [first, first + n - head).
 struct Span {
     int q0, q_len, seq;     // first token of the request in q, its queries, its keys

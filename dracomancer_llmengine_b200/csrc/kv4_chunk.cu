@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const Args x) {
             g.whole = g.begin == 0 && g.n == g.sp.n;
             g.slot = 2 * (long)blockIdx.x + (g.begin == 0);
         }
-        // ---- the rows' queries, scaled to |q| <= 1 by a power of two per row: a thread takes 8 channels ----
+        // ---- the rows' queries, below 2^14 by a power of two per row: a thread takes 8 channels ----
         const int rows = g.sp.q_len * x.group.d;
         // (512 threads: whole rows in a warp, the same number of turns for each)
         for (int i = tid; i < kRows * (D / 8) && tid < 512; i += 512) {      // a row lies in D / 8 lanes of one warp
@@ -570,9 +570,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const Args x) {
             for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(v[k]));
 #pragma unroll
             for (int o = 1; o < D / 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            int ex = (int)((__float_as_uint(top) >> 23) & 255) - 126;
-            ex = min(max(ex, -120), 120);
-            const float down = __uint_as_float((uint32_t)(127 - ex) << 23), up = __uint_as_float((uint32_t)(127 + ex) << 23);
+            float down, up;
+            query_unit(top, down, up);
             uint4 w;
             w.x = pack2<__half>(v[0] * down, v[4] * down);
             w.y = pack2<__half>(v[1] * down, v[5] * down);

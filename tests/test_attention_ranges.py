@@ -177,3 +177,33 @@ def keys(cache, table, n):
     k = torch.empty(n, 1, cache.head_dim, device="cuda")
     cache.read(ints((table[0, pos // cache.page_size] * cache.page_size + pos % cache.page_size).tolist()), k, torch.empty_like(k))
     return k[:, 0].double().cpu()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,n", [(1, 300), (1, 5000), (21, 300), (80, 300)])
+@pytest.mark.parametrize("large", [1e2, 1e4])
+def test_queries_of_wide_range(kind, rows, n, large):
+    """Rows whose largest channels meet keys of 0, so that channels 10^3 to 10^5 times smaller make the scores."""
+    d = 128
+    gen = torch.Generator().manual_seed(13)
+    k = 10 * torch.randn(n, 1, d, generator=gen)
+    k[..., :32] = 0.0
+    cache, table, lens = filled([k], [torch.randn(n, 1, d, generator=gen)], 16)
+    q = 0.1 * torch.randn(rows, 4, d, generator=gen)
+    q[..., :32] *= 10 * large
+    check(kind, cache, table, lens, [rows], q.cuda().to(TYPES[kind]), with_lse=rows == 1)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 21, 80])
+@pytest.mark.parametrize("size", [1e-44, 1e-38, 1e-30, 1e30, 2e38])
+def test_queries_at_the_ends_of_their_type(kind, rows, size):
+    """Rows of subnormal and of the largest numbers (keys bring the scores back to size 1 where the scale can, else to 0)."""
+    n, d = 200, 64
+    gen = torch.Generator().manual_seed(14)
+    cache, table, lens = filled([torch.randn(n, 1, d, generator=gen)], [torch.randn(n, 1, d, generator=gen)], 16)
+    q = (torch.rand(rows, 4, d, generator=gen) * 2 - 1).mul(size).to(TYPES[kind]).cuda()
+    out, scale = torch.zeros_like(q), min(0.1 / size, 1e37)
+    cache.attend(q, out, ints([0, rows]), ints(lens), torch.from_numpy(table).cuda(), rows, n, scale=scale)
+    want, _ = attend_ref(cache, table, q, [0, rows], lens, 0, 0, scale)
+    assert rel(out, want) <= TOL[kind]
