@@ -17,7 +17,8 @@
 // 392 us (unpacking 2270 cycles a step, issuing 950: each wait on a barrier costs the issuing warp about 290).
 //
 // A channel's place inside its group of eight is the order in which a word's nibbles come apart, (0 4 1 5 2 6 3 7), in Q and
-// K alike.  Values of tokens that are not finite are stored as 0 and the token is noted: a row that sees it becomes NaN, one
+// K alike.  A tile's keys, and a step's values, that fp16 cannot hold are stored times 1/16, which the scores and the weights make
+// good.  Values of tokens that are not finite are stored as 0 and the token is noted: a row that sees it becomes NaN, one
 // that does not is left alone.  O is rescaled only when a row's maximum grows by more than 4 (log2): weights then go up to
 // 2^15, which fp16 has room for, and the rescaling waits for the product before it, so it should be rare.
 //
@@ -53,10 +54,11 @@ struct Layout {
 
 struct alignas(16) Control {
     uint64_t kv_full[kBufs], s_full[2][2], p_full[2][2], pv_done[2][kBufs], drain[2];      // [half][buffer]
-    // what a step's unpacking warps saw: each tile's page is there (0xf) with finite values only, or not
+    // what a step's unpacking warps saw: pages everywhere, values finite, and none beyond fp16, or not
     uint32_t fine[kBufs][4];
     uint64_t bad[kBufs][4];     // tokens of the step with values that are not finite
-    uint32_t valid[kBufs];          // which of the step's four tiles have a page
+    uint32_t valid[kBufs];          // which of the step's four tiles have a page; bit 4: values are stored times 1/16
+    uint32_t keys_small[kBufs][4];  // whether a tile's keys are
     uint32_t tmem;
     int abort;
     float qk[kRows];
@@ -134,6 +136,15 @@ __device__ __forceinline__ uint32_t or_exponent(uint32_t w, uint32_t mask) {    
     asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(t) : "r"(w), "r"(mask), "r"(0x64006400u));
     return t;
 }
+// 0, or NaN where a group's values are not finite or cannot be held in fp16 (scale times the lowest or highest code, less ZERO,
+// plus the offset: infinity times 0 is NaN), added to the same of other groups
+template <int ZERO>
+__device__ __forceinline__ __half2 open2(__half2 s, __half2 m, __half2 sum) {
+    const __half2 z = __float2half2_rn(0.f);
+    if (ZERO) sum = __hfma2(__hfma2(s, __float2half2_rn((float)-ZERO), m), z, sum);
+    return __hfma2(__hfma2(s, __float2half2_rn(15.f - ZERO), m), z, sum);
+}
+__device__ __forceinline__ bool is_open(__half2 sum) { return as_word(sum) & 0x7fff7fffu; }
 // the four pairs of a word's codes, minus ZERO, times s plus m: halves (0 4) (1 5) (2 6) (3 7) of nibbles
 template <int ZERO>
 __device__ __forceinline__ void values4(uint32_t w, __half2 s, __half2 m, uint32_t (&out)[4]) {
@@ -253,38 +264,84 @@ __device__ __forceinline__ void unpack_role(const Args& x, const Segment& g, Con
         const uint32_t valid = __ballot_sync(0xffffffffu, where >= 0) >> ((t & 7) * 4) & 15u;
         uint8_t* k = sk + b * Layout<D>::kK;
         uint8_t* v = sv + b * Layout<D>::kV;
+        const __half2 sixteenth = __float2half2_rn(0.0625f);
+        // the scales and offsets of this lane's tokens, twice each
+        auto key_scale = [&](int u, int i) {
+            const __half2 s2 = as_half2(ks[u][i]);
+            return (kt + 8 * u) & 1 ? __high2half2(s2) : __low2half2(s2);
+        };
+        auto key_offset = [&](int u, int i) {
+            const __half2 m2 = as_half2(km[u][i >> 1]);
+            return i & 1 ? __high2half2(m2) : __low2half2(m2);
+        };
+        const __half2 zero = __float2half2_rn(0.f);
+        __half2 open = zero;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < NG; i++) open = open2<0>(key_scale(u, i), key_offset(u, i), open);
+        const bool keys_small = __any_sync(0xffffffffu, is_open(open));
+        if (keys_small) {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < NG; i++) {
+                    ks[u][i] = as_word(__hmul2(as_half2(ks[u][i]), sixteenth));
+                    if (i & 1) km[u][i >> 1] = as_word(__hmul2(as_half2(km[u][i >> 1]), sixteenth));
+                }
+        }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const int tok = kt + 8 * u, row = warp * kKvTile + tok;
 #pragma unroll
             for (int i = 0; i < NG; i++) {
-                const __half2 s2 = as_half2(ks[u][i]), m2 = as_half2(km[u][i >> 1]);
                 uint32_t o[4];
-                values4<0>(kw[u][i], tok & 1 ? __high2half2(s2) : __low2half2(s2), i & 1 ? __high2half2(m2) : __low2half2(m2), o);
+                values4<0>(kw[u][i], key_scale(u, i), key_offset(u, i), o);
                 const int unit = (i & 1) * 4 + kq;      // 16 bytes of a 128-byte row: two groups
                 *reinterpret_cast<uint4*>(k + (i >> 1) * kTok * 128 + row * 128 + ((unit ^ (row & 7)) << 4)) =
                     make_uint4(o[0], o[1], o[2], o[3]);
             }
         }
         // tokens behind the sequence or without a page have no values (the bytes read for the latter are tile 0's); values
-        // that are not finite are noted and left out
+        // that are not finite are noted and left out; where fp16 cannot hold one, those of the step are taken times 1/16 (the
+        // largest that scale and offset give is 9 times fp16's) and their weights times 16.  Every warp of the group has the
+        // scales of all tokens and channel groups, and comes to the same.
         const int left = has_page ? g.sp.seq - g.tile(j) * kTok - tq * 8 : 0;      // of this lane's 8 tokens
         uint32_t bad = 0;
+        bool values_small = false;
+        open = zero;
 #pragma unroll
         for (int p = 0; p < 4; p++) {
             const uint32_t keep = left >= 2 * p + 2 ? 0xffffffffu : left == 2 * p + 1 ? 0xffffu : 0u;
 #pragma unroll
             for (int i = 0; i < GV; i++) {
-                uint32_t &s = vs[p][i], &m = vm[p][i];
-                s &= keep, m &= keep;
-                const __half2 z = __float2half2_rn(0.f);
-                if (as_word(__hfma2(as_half2(s), z, __hmul2(as_half2(m), z))) & 0x7fff7fffu) {
-                    const auto open = [](uint32_t w) { return (w & 0x7c00u) == 0x7c00u; };
-                    const bool b0 = open(s) || open(m), b1 = open(s >> 16) || open(m >> 16);
+                vs[p][i] &= keep, vm[p][i] &= keep;
+                open = open2<8>(as_half2(vs[p][i]), as_half2(vm[p][i]), open);
+            }
+        }
+        if (__any_sync(0xffffffffu, is_open(open))) {
+            open = zero;
+#pragma unroll
+            for (int p = 0; p < 4; p++)
+#pragma unroll
+                for (int i = 0; i < GV; i++) {
+                    uint32_t &s = vs[p][i], &m = vm[p][i];
+                    const auto infinite = [](uint32_t w) { return (w & 0x7c00u) == 0x7c00u; };
+                    const bool b0 = infinite(s) || infinite(m), b1 = infinite(s >> 16) || infinite(m >> 16);
                     const uint32_t fine = (b0 ? 0u : 0xffffu) | (b1 ? 0u : 0xffff0000u);
                     s &= fine, m &= fine;
                     bad |= (uint32_t)b0 << (2 * p) | (uint32_t)b1 << (2 * p + 1);
+                    open = open2<8>(as_half2(s), as_half2(m), open);
                 }
+            values_small = __any_sync(0xffffffffu, is_open(open));
+            if (values_small) {
+#pragma unroll
+                for (int p = 0; p < 4; p++)
+#pragma unroll
+                    for (int i = 0; i < GV; i++) {
+                        vs[p][i] = as_word(__hmul2(as_half2(vs[p][i]), sixteenth));
+                        vm[p][i] = as_word(__hmul2(as_half2(vm[p][i]), sixteenth));
+                    }
             }
         }
 #pragma unroll
@@ -304,12 +361,13 @@ __device__ __forceinline__ void unpack_role(const Args& x, const Segment& g, Con
             const uint32_t lo = __reduce_or_sync(0xffffffffu, tq < 4 ? bad << (8 * tq) : 0u);
             const uint32_t hi = __reduce_or_sync(0xffffffffu, tq < 4 ? 0u : bad << (8 * (tq - 4)));
             if (lane == 0) c->bad[b][warp] = (uint64_t)hi << 32 | lo;
-        } else if (valid != 15u && lane == 0) {
+        } else if (lane == 0) {
             c->bad[b][warp] = 0;
         }
         if (lane == 0) {
-            c->fine[b][warp] = valid == 15u && !any_bad;
-            if (warp == 0) c->valid[b] = valid;
+            c->fine[b][warp] = valid == 15u && !any_bad && !keys_small && !values_small;
+            c->keys_small[b][warp] = keys_small;
+            if (warp == 0) c->valid[b] = valid | (uint32_t)values_small << 4;
         }
         sync::fence_proxy_async();      // the products read shared memory through the other proxy
         __syncwarp();
@@ -353,6 +411,8 @@ __device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Co
         const bool part = base + kTok - 1 > g.sp.p_lo || !clean ||
                           (a.window > 0 && base <= g.sp.p_hi - a.window && base + kTok > a.sinks);
         uint32_t sees[2] = {0xffffffffu, 0xffffffffu};      // tokens of the step that the row sees
+        uint32_t keys16 = 0;        // tiles whose keys are stored times 1/16
+        float up = 1.f, room = kRoom;       // of the weights: 16 where the values are
         if (part) {
             // up to its own position, from the window's beginning or among the first tokens
             const auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
@@ -365,28 +425,36 @@ __device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Co
                 for (int w = 0; w < 4; w++) {
                     if (!(valid >> w & 1)) bits &= ~(0xffffull << (16 * w));
                     if (!c->fine[kv][w]) bad |= c->bad[kv][w];
+                    keys16 |= c->keys_small[kv][w] << w;
                 }
+                if (valid >> 4) up = 16.f, room = 0.f;
                 if (bits & bad) l = __uint_as_float(0x7fffffffu);
             }
             sees[0] = (uint32_t)bits, sees[1] = (uint32_t)(bits >> 32);
         }
+        auto masked = [&](int h) {
+            if (keys16) {
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                    if (keys16 >> (2 * h + (i >> 4)) & 1) v[i] = __float_as_uint(__uint_as_float(v[i]) * 16.f);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+                if (!(sees[h] >> i & 1)) v[i] = 0xff800000u;
+        };
         // the scores are read twice, 32 at a time (the second half stays for its weights): 64 of them do not fit 96 registers
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             if (h) tc_ld32(at + 32, v);
             tc_wait_ld();
-            if (part) {
-#pragma unroll
-                for (int i = 0; i < 32; i++)
-                    if (!(sees[h] >> i & 1)) v[i] = 0xff800000u;
-            }
+            if (part) masked(h);
 #pragma unroll
             for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i]));
         }
         const float mx = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), qk);
-        if (__any_sync(0xffffffffu, mx - m > kBias + kRoom)) {
-            const float now = fmaxf(m, below_score(mx, kRoom)), f = ex2(m - now);
+        if (__any_sync(0xffffffffu, mx - m > kBias + room)) {
+            const float now = fmaxf(m, below_score(mx, room)), f = ex2(m - now);
             m = now;
             large = __any_sync(0xffffffffu, fabsf(m) >= 4194304.f && m != kNone);
             l *= f;
@@ -422,22 +490,18 @@ __device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Co
                 }
                 e0 = ex2(e0), e1 = ex2(e1);
                 sum = add2(sum, join(__float_as_uint(e0), __float_as_uint(e1)));
-                p[i] = pack2<__half>(e0, e1);
+                p[i] = decltype(apart)::value ? pack2<__half>(e0 * up, e1 * up) : pack2<__half>(e0, e1);
             }
         };
         auto weights = [&]() {
-            if (large) weights_of(std::true_type{});
+            if (large || up != 1.f) weights_of(std::true_type{});
             else weights_of(std::false_type{});
         };
         weights();          // of the second half, which go over scores of the first: those are read before
         tc_ld32(at, v);
         tc_wait_ld();
         tc_st16(at + 16, p);
-        if (part) {
-#pragma unroll
-            for (int i = 0; i < 32; i++)
-                if (!(sees[0] >> i & 1)) v[i] = 0xff800000u;
-        }
+        if (part) masked(0);
         weights();
         tc_st16(at, p);
         float sum0, sum1;

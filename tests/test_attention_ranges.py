@@ -207,3 +207,40 @@ def test_queries_at_the_ends_of_their_type(kind, rows, size):
     cache.attend(q, out, ints([0, rows]), ints(lens), torch.from_numpy(table).cuda(), rows, n, scale=scale)
     want, _ = attend_ref(cache, table, q, [0, rows], lens, 0, 0, scale)
     assert rel(out, want) <= TOL[kind]
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 21, 80])
+@pytest.mark.parametrize("size", [7e4, 4e5, 1e30])
+def test_values_beyond_fp16(kind, rows, size):
+    """Values that fp16 cannot hold (the cache can, up to its scale's range): rows that see the token have its part, rows that
+    do not are left alone."""
+    n, d, window, pos = 150, 128, 20, 110
+    gen = torch.Generator().manual_seed(11)
+    k, v = torch.randn(n, 1, d, generator=gen), torch.randn(n, 1, d, generator=gen)
+    v[pos] = size * torch.rand(1, d, generator=gen) * torch.randn(1, d, generator=gen).sign()
+    cache, table, lens = filled([k], [v], 16)
+    q = torch.randn(rows, 4, d, generator=gen).cuda().to(TYPES[kind])
+    out = torch.zeros_like(q)
+    cache.attend(q, out, ints([0, rows]), ints(lens), torch.from_numpy(table).cuda(), rows, n, window=window)
+    want, _ = attend_ref(cache, table, q, [0, rows], lens, window, 0)
+    assert torch.isfinite(out).all()
+    for i in range(rows):
+        a, b = out[i].double().cpu(), want[i]
+        assert float(torch.linalg.norm(a - b)) <= TOL[kind] * float(torch.linalg.norm(b)), (i, n - rows + i)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows", [1, 21, 80])
+@pytest.mark.parametrize("size", [7e4, 4e5])
+def test_keys_beyond_fp16(kind, rows, size):
+    """Keys that fp16 cannot hold, in one token of each of three tiles, against queries that keep the scores ordinary."""
+    n, d = 150, 128
+    gen = torch.Generator().manual_seed(12)
+    k, v = torch.randn(n, 1, d, generator=gen), torch.randn(n, 1, d, generator=gen)
+    for pos in (3, 70, 110):
+        k[pos, 0, 32:64] = size * torch.randn(32, generator=gen).clamp(-1.5, 1.5)
+    cache, table, lens = filled([k], [v], 16)
+    q = torch.randn(rows, 4, d, generator=gen)
+    q[..., 32:64] *= 1e-6       # those channels' part of a score is of size 1
+    check(kind, cache, table, lens, [rows], q.cuda().to(TYPES[kind]))
