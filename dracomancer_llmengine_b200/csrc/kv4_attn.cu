@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
     constexpr int ET = SPLIT ? 1 : NT;          // columns of 8 query rows
     constexpr int kRows = 8 * ET;
     constexpr bool kFp16 = sizeof(T) == 2 && !SPLIT && std::is_same<T, __half>::value;
+    constexpr float kLeast = SPLIT || kFp16 ? 1.f / 34359738368.f : 1.f / 16777216.f;   // 2^-35 or 2^-24: weights above 0
     extern __shared__ __align__(16) uint8_t smem[];
     const Kv4Attn& a = x.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r8 = lane >> 2, q4 = lane & 3;
@@ -514,7 +515,12 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
             for (int e = 0; e < ET; e++) {
                 float p[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) p[j] = ex2(ex[e][j]);
+                for (int j = 0; j < 4; j++) {
+                    p[j] = ex2(ex[e][j]);
+                    // a seen token's weight is not 0 (the smallest that the halves hold instead, 2^-46 or 2^-35 of the largest), so that
+                    // what is not finite in it reaches the row: below, a weight of 0 stands for a hidden token
+                    if (part && p[j] < kLeast && ex[e][j] != -INFINITY) p[j] = kLeast;
+                }
                 l[e][0] += p[0] + p[2];
                 l[e][1] += p[1] + p[3];
 #pragma unroll
@@ -558,7 +564,7 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
                     }
                 }
             }
-            // tokens with a weight: the others' scales count as 0 for the row, they may not be finite
+            // tokens with a weight: the others are hidden, their scales count as 0 for the row, they may not be finite
             uint32_t k0[ET], k1[ET], any0 = 0xffffffffu, any1 = 0xffffffffu;
             if constexpr (part) {
                 any0 = any1 = 0;

@@ -244,3 +244,26 @@ def test_keys_beyond_fp16(kind, rows, size):
     q = torch.randn(rows, 4, d, generator=gen)
     q[..., 32:64] *= 1e-6       # those channels' part of a score is of size 1
     check(kind, cache, table, lens, [rows], q.cuda().to(TYPES[kind]))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows", [1, 21, 80])
+@pytest.mark.parametrize("pos", [70, 146])
+def test_nan_values_with_vanishing_weight(kind, rows, pos):
+    """A token whose values are NaN and whose weight is e^-60 of the row's: 0 in any number, and yet NaN times it is NaN, in
+    tiles that every row sees and in those that some see a part of.  Rows that do not see it are left alone."""
+    n, d = 150, 128
+    gen = torch.Generator().manual_seed(9)
+    sign = torch.randn(1, d, generator=gen).sign()
+    k = 0.05 * torch.randn(n, 1, d, generator=gen)
+    k[pos // 16 * 16] = sign * 60 / d ** 0.5       # of the same tile: one warp takes both
+    v = torch.randn(n, 1, d, generator=gen)
+    v[pos] = float("nan")
+    cache, table, lens = filled([k], [v], 16)
+    q = sign.repeat_interleave(4, 0) + 0.01 * torch.randn(rows, 4, d, generator=gen)
+    q = q.cuda().to(TYPES[kind])
+    out = torch.zeros_like(q)
+    cache.attend(q, out, ints([0, rows]), ints(lens), torch.from_numpy(table).cuda(), rows, n)
+    sees = torch.arange(n - rows, n) >= pos
+    assert torch.equal(torch.isnan(out).all(-1).all(-1).cpu(), sees)
+    assert torch.equal(torch.isnan(out).any(-1).any(-1).cpu(), sees)
