@@ -159,7 +159,9 @@ _SIGS = {
     "draco_b200_kv4_read": ([ct.POINTER(DracoKV4Cache), ct.c_int, _vp, ct.c_long, ct.c_long, _vp, ct.c_long,
                              ct.c_long, _vp, ct.c_int, _vp], ct.c_int),
     "draco_b200_capture_id": ([_vp], ct.c_ulonglong),
+    "draco_b200_test_kv4_barrier_extra": ([ct.c_int], ct.c_int),
     "draco_b200_kv4_attention_workspace": ([ct.POINTER(DracoKV4Cache), ct.POINTER(DracoKV4Attention)], ct.c_size_t),
+    "draco_b200_kv4_attention_checked": ([ct.POINTER(DracoKV4Cache), ct.POINTER(DracoKV4Attention), _vp, ct.c_int, _vp], ct.c_int),
     "draco_b200_kv4_attention": ([ct.POINTER(DracoKV4Cache), ct.POINTER(DracoKV4Attention), _vp], ct.c_int),
     "draco_b200_rmsnorm_q8": ([ct.POINTER(DracoNormQ8), _vp], ct.c_int),
 }

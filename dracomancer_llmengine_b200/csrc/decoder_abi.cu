@@ -39,6 +39,7 @@ int launched(const char* who, int kernels) {
 // set while the package's own extension calls: it has seen that the tensors are on the GPU, and asking the driver about
 // each address again would take as long as the launch
 thread_local bool t_pointers_checked = false;
+thread_local int t_test_extra = 0;
 bool on_device(std::initializer_list<const void*> ps) {
     if (t_pointers_checked) return true;
     for (const void* p : ps)
@@ -94,7 +95,7 @@ const char* attention_args(const DracoKV4Cache* cache, const DracoKV4Attention* 
     a = Kv4Attn{cache_of(cache), p->q, p->out, p->lse, p->q_token_stride, p->q_head_stride, p->out_token_stride,
                 p->out_head_stride, p->n_heads, p->n_req, p->n_tokens, p->cu_q, p->seq_len, p->block_table,
                 p->table_stride, p->table_width, p->max_q_len, std::min(p->max_seq_len, most), p->scale, p->window > most ? 0 : p->window,
-                std::min(p->sinks, most), p->dtype};
+                std::min(p->sinks, most), p->dtype, nullptr, 0, 0};
     return nullptr;
 }
 
@@ -104,6 +105,13 @@ extern "C" {
 
 // not part of the interface: for decoder_py.cpp
 void draco_b200_pointers_checked(int on) { t_pointers_checked = on != 0; }
+// for tests, of this thread's next attention calls: one arrival more than ever comes is expected at some barriers of the
+// tensor-core form (1: a step's keys, 2: its weights, 3: its products; 0: none), so that waits run out; returns the old value
+int draco_b200_test_kv4_barrier_extra(int which) {
+    const int old = t_test_extra;
+    if (which >= 0 && which <= 3) t_test_extra = which;
+    return old;
+}
 // the id of the graph capture that the stream is in, 0: none
 unsigned long long draco_b200_capture_id(void* stream) {
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
@@ -172,17 +180,26 @@ size_t draco_b200_kv4_attention_workspace(const DracoKV4Cache* cache, const Drac
 }
 
 int draco_b200_kv4_attention(const DracoKV4Cache* cache, const DracoKV4Attention* args, void* stream) {
+    return draco_b200_kv4_attention_checked(cache, args, nullptr, 0, stream);
+}
+
+int draco_b200_kv4_attention_checked(const DracoKV4Cache* cache, const DracoKV4Attention* args, int* status,
+                                     int wait_limit_us, void* stream) {
     const char* who = "draco_b200_kv4_attention";
     Kv4Attn a;
     if (const char* f = attention_args(cache, args, a)) return refuse("%s: %s", who, f);
+    if (wait_limit_us < 0 || wait_limit_us > 2000000) return refuse("%s: need 0 <= wait_limit_us <= 2000000", who);
+    a.status = status;
+    a.test_extra = t_test_extra;
+    a.wait_ns = wait_limit_us ? wait_limit_us * 1000l : 2000000000l;
     if (!a.n_req || !a.n_tokens || !a.max_q) return 0;
     if (!a.q || !a.out || !a.cu_q || !a.seq_len || (!a.table && a.table_width))
         return refuse("%s: null pointer", who);
-    if (!on_device({a.q, a.out, a.lse, a.cu_q, a.seq_len, a.table, args->workspace}))
+    if (!on_device({a.q, a.out, a.lse, a.cu_q, a.seq_len, a.table, args->workspace, status}))
         return refuse("%s: buffers must be device memory", who);
     const size_t b = (size_t)dtype_bytes(a.dtype);
-    if (!aligned_to(a.q, b) || !aligned_to(a.out, b) || !aligned_to(args->workspace, 16))
-        return refuse("%s: q and out must be aligned to their elements, the workspace to 16 bytes", who);
+    if (!aligned_to(a.q, b) || !aligned_to(a.out, b) || !aligned_to(args->workspace, 16) || !aligned_to(status, 4))
+        return refuse("%s: q, out and status must be aligned to their elements, the workspace to 16 bytes", who);
     const size_t need = kv4_attention_workspace(a);
     if (need && (!args->workspace || args->workspace_bytes < need))
         return refuse("%s: the workspace must have %zu bytes", who, need);

@@ -24,7 +24,7 @@ decltype(&draco_b200_plan_blocks) f_plan_blocks = nullptr;
 decltype(&draco_b200_kv4_append) f_append = nullptr;
 decltype(&draco_b200_kv4_read) f_read = nullptr;
 decltype(&draco_b200_kv4_attention_workspace) f_workspace = nullptr;
-decltype(&draco_b200_kv4_attention) f_attention = nullptr;
+decltype(&draco_b200_kv4_attention_checked) f_attention = nullptr;
 decltype(&draco_b200_rmsnorm_q8) f_norm = nullptr;
 void (*f_checked)(int) = nullptr;
 unsigned long long (*f_capture_id)(void*) = nullptr;
@@ -136,7 +136,7 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
     };
     if (!take("draco_b200_last_error", f_last_error) || !take("draco_b200_plan_blocks", f_plan_blocks) ||
         !take("draco_b200_kv4_append", f_append) || !take("draco_b200_kv4_read", f_read) ||
-        !take("draco_b200_kv4_attention_workspace", f_workspace) || !take("draco_b200_kv4_attention", f_attention) ||
+        !take("draco_b200_kv4_attention_workspace", f_workspace) || !take("draco_b200_kv4_attention_checked", f_attention) ||
         !take("draco_b200_pointers_checked", f_checked) || !take("draco_b200_capture_id", f_capture_id) || !take("draco_b200_rmsnorm_q8", f_norm))
         return nullptr;
     Py_INCREF(a[0]);
@@ -208,10 +208,10 @@ PyObject* kv4_append(PyObject*, PyObject* const* a, Py_ssize_t n) { return rows(
 PyObject* kv4_read(PyObject*, PyObject* const* a, Py_ssize_t n) { return rows(a, n, false); }
 
 // (pages, page_size, head_dim, scratch, grow, q, out, cu_q, seq_len, block_table, max_q_len, max_seq_len, scale, window,
-//  sinks, lse, stream, workspace); where workspace is None: scratch: {stream: tensor}, for calls that no graph captures,
+//  sinks, lse, stream, workspace, status); where workspace is None: scratch: {stream: tensor}, for calls that no graph captures,
 //  grow(stream, bytes, capture): another buffer, of the stream or of the capture
 PyObject* kv4_attend(PyObject*, PyObject* const* a, Py_ssize_t given) {
-    return guarded(given, 18, [&] {
+    return guarded(given, 19, [&] {
         const at::Tensor &pages = tensor(a[0], "pages"), &q = tensor(a[5], "q"), &out = tensor(a[6], "out"),
                          &cu = vector_of(a[7], at::kInt, "cu_q"), &seq = vector_of(a[8], at::kInt, "seq_len"),
                          &table = tensor(a[9], "block_table");
@@ -268,7 +268,9 @@ PyObject* kv4_attend(PyObject*, PyObject* const* a, Py_ssize_t given) {
             }
             Py_DECREF(buf);
         }
-        return done(f_attention(&c, &p, s), "draco_b200_kv4_attention");
+        const at::Tensor& status = vector_of(a[18], at::kInt, "status");
+        need(status.device() == dev && status.numel() > 0, "status must be on the cache's device");
+        return done(f_attention(&c, &p, status.data_ptr<int>(), 0, s), "draco_b200_kv4_attention");
     });
 }
 

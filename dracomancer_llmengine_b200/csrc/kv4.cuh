@@ -71,6 +71,9 @@ struct Kv4Attn {
     float scale;
     int window, sinks;
     int dtype;
+    int* status;            // or null: waits that ran out are noted there
+    long wait_ns;           // their limit
+    int test_extra;         // 1, 2, 3: arrivals that never come are expected for a step's keys, weights or products (tests)
 };
 size_t kv4_attention_workspace(const Kv4Attn& a);
 // returns the number of kernels launched

@@ -22,8 +22,9 @@
 // that does not is left alone.  O is rescaled only when a row's maximum grows by more than 4 (log2): weights then go up to
 // 2^15, which fp16 has room for, and the rescaling waits for the product before it, so it should be rare.
 //
-// Every wait is bounded (2 s).  When one runs out the block raises its flag, all its roles leave their loops, the products
-// in flight are waited for, its rows become NaN, and TMEM is freed.
+// Every wait is bounded (2 s, or the call's limit).  When one runs out the block raises its flag and notes which it was in the
+// call's status word, all its roles leave their loops, the products in flight are waited for, its rows become NaN, and TMEM
+// is freed.
 #include "kv4_attn.cuh"
 #include "tc_ptx.cuh"
 
@@ -42,7 +43,8 @@ constexpr int kTmem = 512;
 __device__ __forceinline__ uint32_t tmem_o(uint32_t tmem, int half) { return tmem + 128 * half; }
 __device__ __forceinline__ uint32_t tmem_s(uint32_t tmem, int half, uint32_t b) { return tmem + 256 + 128 * half + 64 * b; }
 constexpr float kRoom = 4.f;        // log2 by which weights may pass 2^kBias: below fp16's 2^16
-constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr int kGaveUp = 0x100;      // in the status word, with the wait's bit below it
+enum Wait { kWaitKeys, kWaitWeights, kWaitBuffer, kWaitStep, kWaitScores, kWaitSums, kWaitLast, kWaitDrain };
 
 template <int D>
 struct Layout {
@@ -80,7 +82,7 @@ __device__ __forceinline__ bool try_phase(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 // the warp's wait for a phase; false when it ran out or another role gave up
-__device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity, volatile int* abort) {
+__device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity, volatile int* abort, const Kv4Attn& a, int which) {
     uint64_t t0 = 0;
     for (uint32_t i = 0;; i++) {
         if (__all_sync(0xffffffffu, try_phase(bar, parity))) return true;
@@ -89,7 +91,10 @@ __device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity, volatile i
             if ((threadIdx.x & 31) == 0) {
                 if (*abort) stop = 1;
                 else if (t0 == 0) t0 = sync::global_ns();
-                else if (sync::global_ns() - t0 > kWaitNs) stop = 1, *abort = 1;
+                else if (sync::global_ns() - t0 > (uint64_t)a.wait_ns) {
+                    stop = 1, *abort = 1;
+                    if (a.status) atomicOr(a.status, kGaveUp | 1 << which);
+                }
             }
             if (__shfl_sync(0xffffffffu, stop, 0)) return false;
         }
@@ -171,13 +176,13 @@ struct Segment {
 
 // ---- warps 16 and 17: the products of one half of the rows ----
 template <int D>
-__device__ __forceinline__ void product_role(const Segment& g, Control* c, uint8_t* sq, uint8_t* sk, uint8_t* sv, uint32_t step0,
-                                             uint32_t tmem, int half) {
+__device__ __forceinline__ void product_role(const Args& x, const Segment& g, Control* c, uint8_t* sq, uint8_t* sk, uint8_t* sv,
+                                             uint32_t step0, uint32_t tmem, int half) {
     const uint64_t dq = sdesc_sw128(sync::smem_addr(sq)) + (uint64_t)(half * (128 * 128 >> 4));
     const uint64_t dk = sdesc_sw128(sync::smem_addr(sk)), dv = sdesc_sw128(sync::smem_addr(sv));
     auto scores = [&](uint32_t step) {
         const uint32_t b = step & 1, kv = step % kBufs;
-        if (!await(&c->kv_full[kv], step / kBufs & 1, &c->abort)) return false;
+        if (!await(&c->kv_full[kv], step / kBufs & 1, &c->abort, x.a, kWaitKeys)) return false;
         tc_fence_after();
         if (elect_one()) {
             const uint64_t k = dk + (uint64_t)(kv * (Layout<D>::kK >> 4));
@@ -198,7 +203,7 @@ __device__ __forceinline__ void product_role(const Segment& g, Control* c, uint8
         // the next step's scores go ahead of this step's softmax.  Their buffer held the weights of the step before this one,
         // whose product this thread issued earlier: products complete in order
         if (j + 1 < g.n && !scores(step + 1)) return;
-        if (!await(&c->p_full[half][b], (step >> 1) & 1, &c->abort)) return;
+        if (!await(&c->p_full[half][b], (step >> 1) & 1, &c->abort, x.a, kWaitWeights)) return;
         tc_fence_after();
         if (elect_one()) {
             const uint64_t v = dv + (uint64_t)(step % kBufs * (Layout<D>::kV >> 4));
@@ -260,7 +265,9 @@ __device__ __forceinline__ void unpack_role(const Args& x, const Segment& g, Con
     for (int j = j0, t = 0; j < g.n; j += 2, t++) {
         const uint32_t step = step0 + j, b = step % kBufs, before = (step / kBufs & 1) ^ 1;
         // both halves' products have read what the buffer held
-        if (step >= kBufs && !(await(&c->pv_done[0][b], before, &c->abort) && await(&c->pv_done[1][b], before, &c->abort))) return;
+        if (step >= kBufs && !(await(&c->pv_done[0][b], before, &c->abort, a, kWaitBuffer) &&
+                               await(&c->pv_done[1][b], before, &c->abort, a, kWaitBuffer)))
+            return;
         const uint32_t valid = __ballot_sync(0xffffffffu, where >= 0) >> ((t & 7) * 4) & 15u;
         uint8_t* k = sk + b * Layout<D>::kK;
         uint8_t* v = sv + b * Layout<D>::kV;
@@ -397,12 +404,12 @@ __device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Co
     bool ok = !c->abort;
     for (int j = 0; j < g.n && ok; j++) {
         const uint32_t step = step0 + j, b = step & 1, parity = (step >> 1) & 1, kv = step % kBufs;
-        ok = await(&c->kv_full[kv], step / kBufs & 1, &c->abort);
+        ok = await(&c->kv_full[kv], step / kBufs & 1, &c->abort, a, kWaitStep);
         if (!ok) break;
         const uint4 fine = *reinterpret_cast<const uint4*>(c->fine[kv]);
         const uint32_t at = tmem_s(tmem, half, b) + lanes;
         const int base = g.tile(j) * kTok;
-        ok = await(&c->s_full[half][b], parity, &c->abort);
+        ok = await(&c->s_full[half][b], parity, &c->abort, a, kWaitScores);
         if (!ok) break;
         tc_fence_after();
         uint32_t v[32];
@@ -459,7 +466,7 @@ __device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Co
             large = __any_sync(0xffffffffu, fabsf(m) >= 4194304.f && m != kNone);
             l *= f;
             if (j) {        // the sums so far, once the previous step's product is in them
-                ok = await(&c->pv_done[half][(step - 1) % kBufs], (step - 1) / kBufs & 1, &c->abort);
+                ok = await(&c->pv_done[half][(step - 1) % kBufs], (step - 1) / kBufs & 1, &c->abort, a, kWaitSums);
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll 1
@@ -514,7 +521,7 @@ __device__ __forceinline__ void softmax_role(const Args& x, const Segment& g, Co
     }
     if (ok) {
         const uint32_t step = step0 + g.n - 1;
-        ok = await(&c->pv_done[half][step % kBufs], step / kBufs & 1, &c->abort);
+        ok = await(&c->pv_done[half][step % kBufs], step / kBufs & 1, &c->abort, a, kWaitLast);
         tc_fence_after();
     }
     // ---- the rows' results ----
@@ -562,13 +569,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const Args x) {
     const int tid = threadIdx.x, warp = tid >> 5;
     early_launch();
     if (tid == 0) {
-        for (int i = 0; i < kBufs; i++) sync::mbar_init(&c->kv_full[i], 4);
+        for (int i = 0; i < kBufs; i++) sync::mbar_init(&c->kv_full[i], 4 + (a.test_extra == 1));
         for (int h = 0; h < 2; h++) {
             for (int i = 0; i < 2; i++) {
                 sync::mbar_init(&c->s_full[h][i], 1);
-                sync::mbar_init(&c->p_full[h][i], 4);
+                sync::mbar_init(&c->p_full[h][i], 4 + (a.test_extra == 2));
             }
-            for (int i = 0; i < kBufs; i++) sync::mbar_init(&c->pv_done[h][i], 1);
+            for (int i = 0; i < kBufs; i++) sync::mbar_init(&c->pv_done[h][i], 1 + (a.test_extra == 3));
             sync::mbar_init(&c->drain[h], 1);
         }
         c->abort = 0;
@@ -649,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const Args x) {
         if (!c->abort || warp < 8) {
             if (warp < 8) softmax_role<D>(x, g, c, step0, tmem);
             else if (warp < 16) unpack_role<D>(x, g, c, sk, sv, step0, req);
-            else product_role<D>(g, c, sq, sk, sv, step0, tmem, warp - 16);
+            else product_role<D>(x, g, c, sq, sk, sv, step0, tmem, warp - 16);
         }
         step0 += g.n;
         if (left <= 0) break;
@@ -661,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const Args x) {
     if (warp >= 16) {           // every product issued must be complete before TMEM is released
         if (elect_one()) {
             tc_commit(&c->drain[warp - 16]);
-            sync::mbar_wait(&c->drain[warp - 16], 0);
+            if (!sync::mbar_wait(&c->drain[warp - 16], 0) && a.status) atomicOr(a.status, kGaveUp | 1 << kWaitDrain);
         }
         __syncwarp();
     }

@@ -37,7 +37,7 @@ __all__ = ["BlockPlan", "plan_blocks", "KV4Cache", "rmsnorm_q8"]
 # the extension checks arguments and calls the entry points of the library that this package loaded
 _decoder.setup(DracoError, {name: ct.cast(getattr(lib(), name), ct.c_void_p).value for name in (
     "draco_b200_last_error", "draco_b200_plan_blocks", "draco_b200_kv4_append", "draco_b200_kv4_read",
-    "draco_b200_kv4_attention_workspace", "draco_b200_kv4_attention", "draco_b200_rmsnorm_q8",
+    "draco_b200_kv4_attention_workspace", "draco_b200_kv4_attention_checked", "draco_b200_rmsnorm_q8",
     "draco_b200_pointers_checked", "draco_b200_capture_id")})
 
 # Scratch for attention whose long axis is split over blocks.  Eager calls on a stream run one after the other and share
@@ -85,7 +85,8 @@ def plan_blocks(ctx_len, new_len, block_table, free_pages, n_free, page_size: in
 class KV4Cache:
     """A paged KV cache in 4 bits over `pages`, uint8 [n_pages, n_kv_heads, page_size // 16, 20 * head_dim] (contiguous;
     1.25 bytes per key and value channel).  The pages are the caller's memory: the object adds nothing but their
-    description.
+    description and `status`, one int32 on the GPU.  It is 0 unless a wait inside the kernel of a call ran out (2 s), whose rows
+    are then NaN; calls only ever set bits in it, and a server that reads its results reads it with them.
 
     Attention whose long axis is split over blocks needs scratch memory (:meth:`workspace_bytes`: 2 to 10 MB for single
     tokens over long contexts, 40 MB for chunks).  Without `workspace=` the module keeps one buffer for each stream, for
@@ -105,6 +106,7 @@ class KV4Cache:
         self._desc = DracoKV4Cache(pages.data_ptr(), pages.shape[0], page_size, pages.shape[1], head_dim)
         self._scratch = _eager.setdefault(pages.get_device(), {})
         self._kept: list = []       # buffers of captures
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device="cuda"):
@@ -166,7 +168,7 @@ class KV4Cache:
         workspace: a contiguous tensor of at least :meth:`workspace_bytes` for this call alone, instead of the module's."""
         _decoder.kv4_attend(self.pages, self.page_size, self.head_dim, self._scratch, self._grow, q, out, cu_q, seq_len,
                             block_table, max_q_len, max_seq_len, self.head_dim ** -0.5 if scale is None else scale,
-                            window, sinks, lse, _stream(stream), workspace)
+                            window, sinks, lse, _stream(stream), workspace, self.status)
         return out
 
 

@@ -404,6 +404,11 @@ typedef struct DracoKV4Attention {
 } DracoKV4Attention;
 size_t draco_b200_kv4_attention_workspace(const DracoKV4Cache* cache, const DracoKV4Attention* args);
 int draco_b200_kv4_attention(const DracoKV4Cache* cache, const DracoKV4Attention* args, void* stream);
+/* The same with a status word on the device (or null), which the call only ever sets bits in: a block of the tensor-core form
+ * (chunks of bf16) whose waits run out after wait_limit_us (1 .. 2000000; 0: 2 s) gives up, writes NaN to its rows, and sets 0x100
+ * and the bit of the wait.  0 after the call is complete: no wait ran out in it or in any earlier call with that word. */
+int draco_b200_kv4_attention_checked(const DracoKV4Cache* cache, const DracoKV4Attention* args, int* status,
+                                     int wait_limit_us, void* stream);
 
 /* Residual addition, RMS norm and 8-bit output, row by row (hidden values each, row strides in elements):
  *   h = x + residual rounded to dtype (h and residual given together; h may be residual or x), h = x without one

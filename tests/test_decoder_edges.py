@@ -141,3 +141,41 @@ def test_calls_do_not_wait_for_synchronous_ones():
     thread.join()
     torch.cuda.synchronize()
     assert plan.slots.tolist()[:1] == [4 * 16]
+
+
+@pytest.mark.parametrize("which", [1, 2, 3])
+def test_a_wait_that_runs_out_is_reported(which):
+    """Barriers that expect an arrival which never comes (a step's keys, weights or products), and waits of up to a
+    millisecond: the kernel ends, says so, and gives NaN, not wrong numbers; the next call is right."""
+    d, rows, n = 128, 300, 6000
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    cache = decoder.KV4Cache.empty(n // 64 + 1, 64, 2, d)
+    kv = torch.randn(2, n, 2, d, device="cuda", generator=gen)
+    cache.append(kv[0], kv[1], torch.arange(n, dtype=torch.int32, device="cuda"))
+    table = torch.arange(n // 64 + 1, dtype=torch.int32, device="cuda")[None]
+    q = torch.randn(rows, 8, d, device="cuda", generator=gen).bfloat16()
+    cu, seq = ints([0, rows]), ints([n])
+    want = cache.attend(q, torch.empty_like(q), cu, seq, table, rows, n)
+    assert torch.isfinite(want).all() and cache.status.tolist() == [0]
+    out, status = torch.zeros_like(q), ints([0])
+    a = dm.DracoKV4Attention(q.data_ptr(), out.data_ptr(), None, 8 * d, d, 8 * d, d, 2, 8, 1, rows, cu.data_ptr(), seq.data_ptr(),
+                             table.data_ptr(), table.shape[1], table.shape[1], rows, n, d ** -0.5, 0, 0, None, 0)
+    ws = torch.empty(dm.lib().draco_b200_kv4_attention_workspace(cache._desc, a), dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    call = lambda limit, word=status: dm.lib().draco_b200_kv4_attention_checked(  # noqa: E731
+        cache._desc, a, word.data_ptr(), limit, torch.cuda.current_stream().cuda_stream)
+    assert dm.lib().draco_b200_test_kv4_barrier_extra(which) == 0
+    try:
+        assert call(1000) == 0, dm.last_error()
+    finally:
+        assert dm.lib().draco_b200_test_kv4_barrier_extra(0) == which
+    torch.cuda.synchronize()
+    # 0x100 and the bits of waits; 0x80 would be products that were still in flight at the end
+    assert status.item() & 0x100 and status.item() & 0x7f and not status.item() & ~0x17f
+    assert torch.isnan(out).all()
+    status.zero_()
+    for limit in (0, 2000000):
+        assert call(limit) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and status.item() == 0
+    assert call(-1) == -1 and call(2000001) == -1 and call(0, torch.zeros(1, dtype=torch.int32)) == -1
