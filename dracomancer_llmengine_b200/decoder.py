@@ -76,7 +76,8 @@ def plan_blocks(ctx_len, new_len, block_table, free_pages, n_free, page_size: in
     ctx_len, new_len: int32 [n_req]; block_table: int32 [n_req, width], new entries are written in place; free_pages:
     int32, of which the first n_free[0] are free, taken from the end; page_size: tokens of a page.  Results go to `plan`
     (its n_free is the next call's n_free: n_free itself is not changed).  Requests that the list or their row of the
-    table has no room for are counted in plan.refused and get slots -1."""
+    table has no room for are counted in plan.refused and get slots -1; their rows of this step's attention mean nothing
+    and are to be dropped (plan.refused is read with the step's results, a request's seq_len that did not grow says which)."""
     _decoder.plan_blocks(ctx_len, new_len, block_table, free_pages, n_free, page_size, plan.cu_new, plan.seq_len,
                          plan.slots, plan.positions, plan.n_free, plan.refused, _stream(stream))
     return plan

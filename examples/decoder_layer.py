@@ -70,8 +70,11 @@ class Server:
         return ffn.to(x.dtype)
 
     def check(self):
-        """Relative error of the last step's attention against 64 bits, over the cache's own values."""
+        """Relative error of the last step's attention against 64 bits, over the cache's own values.  Raises where the step
+        had no pages for a request."""
         q, got, plan = self.last
+        if int(plan.refused):       # read with the results: rows of requests without pages mean nothing
+            raise RuntimeError(f"{int(plan.refused)} requests found no free page in this step")
         want = torch.zeros(got.shape, dtype=torch.float64, device="cuda")
         cu, seq = plan.cu_new.tolist(), plan.seq_len.tolist()
         for r, n in enumerate(seq):

@@ -343,7 +343,9 @@ int draco_b200_gemv_q8k(int code, const uint8_t* W, int rows, int n_in, const in
  * ceil(ctx/page_size) pages, in the first entries of its row of block_table ([n_req] rows, table_stride entries apart,
  * table_width usable), and takes the pages that it lacks from the end of free_pages[0 .. *n_free) in request order;
  * their ids are written to its row, the rest of the table is left as it is.  A request whose pages the list no longer
- * has, counting those of every request before it, or which a row cannot hold, is refused: no page, slots -1.
+ * has, counting those of every request before it, or which a row cannot hold, is refused: no page, slots -1.  Its tokens
+ * stay in cu_new, so attention over cu_new and seq_len gives their rows numbers without a meaning (its queries then pass for
+ * the last ctx tokens, of which the new ones are none): drop them, and give the request its turn when pages are free.
  *   cu_new[n_req+1]   tokens before each request;    seq_len[r]   ctx + new, or ctx where refused
  *   slots, positions [max_tokens]   for token i of request r (at cu_new[r] + i): position ctx + i, and slot
  *                     page * page_size + position % page_size; -1 for tokens of refused requests (slots) and past the

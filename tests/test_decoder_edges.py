@@ -1,4 +1,6 @@
 """Decoder-layer operators at the ends of what their arguments allow."""
+import importlib.util
+import os
 import threading
 import time
 
@@ -179,3 +181,23 @@ def test_a_wait_that_runs_out_is_reported(which):
         torch.cuda.synchronize()
         assert torch.equal(out, want) and status.item() == 0
     assert call(-1) == -1 and call(2000001) == -1 and call(0, torch.zeros(1, dtype=torch.int32)) == -1
+
+
+def test_example_does_not_use_rows_of_refused_requests():
+    """A step that finds no page for a request: its rows are not taken for results."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "decoder_layer.py")
+    spec = importlib.util.spec_from_file_location("decoder_layer", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    layer = example.Layer(torch.bfloat16)
+    server = example.Server(layer, 2, 64)
+    step = lambda n: server.step(*torch.randn(2, sum(n), layer.hidden, device="cuda").bfloat16(), ints(n), max(n))  # noqa: E731
+    step([30, 5])
+    assert server.check() < 5e-3
+    server.n_free.zero_()
+    step([1, 1])        # both have room in their pages
+    assert server.check() < 5e-3
+    step([10, 1])
+    with pytest.raises(RuntimeError, match="1 requests found no free page"):
+        server.check()
+    assert server.ctx.tolist() == [31, 7]
