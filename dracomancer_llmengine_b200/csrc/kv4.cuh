@@ -178,11 +178,7 @@ __device__ __forceinline__ void store8(T* p, bool wide, const float (&f)[8]) {
     }
 }
 
-// asynchronous copies of 16 bytes into shared memory, in groups that complete in order
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
-                 : "memory");
-}
+// asynchronous copies into shared memory, in groups that complete in order
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {
