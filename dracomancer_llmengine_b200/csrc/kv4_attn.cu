@@ -377,9 +377,9 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
         auto tile = [&](const uint8_t* t, const int base, auto masked) {
             constexpr bool part = decltype(masked)::value;
             // V's scales.  Where every row sees every token they are checked with the scores, by one vote (64 requests of 128-wide
-            // heads: 69 us against 75), else with the weights; so too for heads 256 wide, where the registers do not last for
-            // it (a window of 4096: 59 us against 65)
-            constexpr bool one_vote = !part && D < 256;
+            // heads: 69 us against 75), else with the weights; so too where the registers do not last for it: heads 256 wide
+            // (a window of 4096: 59 us against 65) and two columns (4 fp16 chunks of 512: 1340 us against 1414)
+            constexpr bool one_vote = !part && D < 256 && NT == 1;
             uint32_t v0[NG], v1[NG], s0[NG], s1[NG];
             auto load_scales = [&]() {
                 load_words<NG>(t + kv4_off_vs(D) + q4 * NG * 4, s0);
