@@ -11,9 +11,10 @@
 // have two buffers, so that a step's scores are computed beside the previous step's softmax.  (With two buffers of K and V a
 // step took 3600 cycles: from a product's end through unpacking, scores, softmax and product again is two steps' way.)
 //
-// Measured at 4 chunks of up to 512 queries x 32 heads over contexts up to 8192 (195 GFLOP): 283 us, 0.69 PFLOP/s, 2500
-// cycles a step: softmax 2100 (1120 for the 64 exponentials a row, of which both halves' on the exponential unit alone are
-// 1024), products 1220.  Blocks of 128 rows with four unpacking warps, one of which issued the products, two blocks an SM:
+// Measured at 4 chunks of up to 512 queries x 32 heads over contexts up to 8192 (194 GFLOP): 302 us, 0.64 PFLOP/s, 2660
+// cycles a step, softmax bound.  (283 us and 2500 cycles before keys' and values' range was checked and weights were raised: of
+// these softmax 2100, with 1120 for the 64 exponentials a row, of which both halves' on the exponential unit alone are
+// 1024; products 1220.)  Blocks of 128 rows with four unpacking warps, one of which issued the products, two blocks an SM:
 // 392 us (unpacking 2270 cycles a step, issuing 950: each wait on a barrier costs the issuing warp about 290).
 //
 // A channel's place inside its group of eight is the order in which a word's nibbles come apart, (0 4 1 5 2 6 3 7), in Q and

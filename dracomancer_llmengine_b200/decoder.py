@@ -163,7 +163,8 @@ class KV4Cache:
         """Causal attention of the ragged queries q [tokens, n_heads, head_dim] into out (same shape and type).
 
         Request r's queries are tokens cu_q[r] .. cu_q[r + 1], the last ones of its seq_len[r] cached tokens; its pages are
-        row r of block_table.  max_q_len and max_seq_len bound them on the host.  scale defaults to head_dim ** -0.5.
+        row r of block_table.  max_q_len and max_seq_len bound them on the host and choose the kernel's form: loose
+        bounds cost time, max_q_len above all.  scale defaults to head_dim ** -0.5.
         With window > 0 a query sees the last `window` keys up to its own and the first `sinks` tokens.  lse: optional
         fp32 [tokens, n_heads] for the log of the sum of exponentials.  Rows that see nothing are 0 (lse -inf).
         workspace: a contiguous tensor of at least :meth:`workspace_bytes` for this call alone, instead of the module's."""

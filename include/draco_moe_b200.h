@@ -388,7 +388,8 @@ int draco_b200_kv4_read(const DracoKV4Cache* cache, int dtype, void* k, long k_t
  *   of the sum of exponentials, -infinity where nothing is seen.
  * block_table: n_req rows of table_width entries, table_stride entries apart; lengths beyond a row (or 2^30) are cut to it, entries
  * outside the cache count as not seen.  max_q_len and max_seq_len (host values) bound the requests' lengths: queries past max_q_len get
- * no output, a longer sequence only runs slower.  workspace: draco_b200_kv4_attention_workspace() bytes, 16-byte
+ * no output, a longer sequence only runs slower.  The kernel's form goes by them, so loose bounds cost time (single tokens under
+ * max_q_len 16: 1.4 to 3 times as much).  workspace: draco_b200_kv4_attention_workspace() bytes, 16-byte
  * aligned, any content; calls that may overlap on the GPU need workspaces of their own. */
 typedef struct DracoKV4Attention {
     const void* q;
