@@ -14,28 +14,22 @@
 //     Group sums come out of the products unscaled and are scaled in fp32; the offsets are one small product more.
 //     Queries are brought below 2^14 by a power of two per row first: 16-bit queries then are exact in fp16 down to 2^-28 (odd
 //     nibbles' 2^-24) of their row's largest, and off by 2^-39 (2^-35) of it below.  Their sums have a high and a low half
-//     in every type.  Scores of size 4, and with them lse, are off by 1e-6 on average in fp32 and by 1.5e-6 in 16-bit types (6e-6
-//     and 9e-6 at most of 1600; plain fp32 sums 0.4e-6 and 2.7e-6).
-//   output, 16-bit queries: sum_t p_t v_t with v_t = s_tg (c - 8) + m_tg in fp16.  A code's four bits become a number by the
-//     exponent of 1024 and are centred, scaled and moved in two more instructions a pair.
-//   output, fp32: sum_t p_t v_t = sum_t (p_t s_tg / 2) (2 c - 15) + sum_t p_t (m_tg - s_tg / 2): the weights take the scales,
+//     in every type, so the scores, and with them lse, keep fp32 precision.
+//   output: sum_t p_t v_t = sum_t (p_t s_tg / 2) (2 c - 15) + sum_t p_t (m_tg - s_tg / 2): the weights take the scales,
 //     codes become (2 c - 15) * 2^-10 in one multiply-add.  They are centred because the sums run over the whole context:
 //     uncentred ones would grow with its length, cancel against the offsets' sum, and lose the result's low bits.
 // Precision of the operands, by the type of queries and output:
 //   fp32  queries and weights are split in two halves (x = hi + lo / 2048, 22 bits), the low halves take 8 columns more;
 //         codes of K are made normal numbers (c * 2^-9): with subnormal ones the sums of a product are aligned ten bits
 //         too high, which showed as 1e-6 of the result (2^-14 of a code; measured 1.1e-6 against 0.5e-6 without)
-//   fp16  values are rounded to fp16 (2^-11 of each, as the output will be), weights have a high and a low half (22 bits,
-//         two products): a weight's rounding is the same in all channels, and a row that one small weight makes had it whole
-//   bf16  values are rounded to fp16 and weights too (2^-11 each, an eighth of the output's own rounding)
-// (16-bit types had the fp32 form, with a weight times a scale rounded once: where a group has one large channel, what the rest
-// owe to rounding was 8e-4 of the result.)
-// fp16 has 2^-14 as its smallest normal number, so weights are kept well above it: the largest of a row is 2^11 (kBias), and
-// roundings are as above down to 2^-25 of that, 2^-36 of it in absolute terms below.  In fp32 the scales are divided by a
-// power of two above the largest one that the warp has met (v_exp), which is raised, and the sums with it, like the running
-// maximum; a weight times a scale is then off by 2^-46 of the largest weight times the largest scale at most.  (With weights up
-// to 1 and scales as they were, a first token 9 nats above 4096 others, its values near 0, cost bf16 and fp16 results 2e-2 where
-// values are 0.01.)
+//   fp16  weights are multiplied with the scales in fp32 and rounded to fp16 once (2^-11), as the output will be
+//   bf16  weights are rounded to fp16 and multiplied with the scales there (2^-11 twice, an eighth of the output's rounding)
+// fp16 has 2^-14 as its smallest normal number, so both factors are kept well above it: the largest weight of a row is
+// 2^11 (kBias), and the scales are divided by a power of two above the largest one that the warp has met (v_exp), which
+// is raised, and the sums with it, like the running maximum.  The roundings above are those of a weight times a scale
+// down to 2^-24 of the largest weight times the largest scale; below, they are 2^-35 of that (fp32: 2^-46) in absolute
+// terms.  (With weights up to 1 and scales as they are, a first token 9 nats above 4096 others, its values near 0, cost
+// bf16 and fp16 results 2e-2 where values are 0.01.)
 //
 // The running maximum is raised only when a score exceeds it by more than 3 (log2): weights stay below 2^14, and most tiles
 // need neither the reduction over tokens nor the rescaling of the sums.
@@ -85,14 +79,19 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     mma16(d, a, b0, b1, d[0], d[1], d[2], d[3]);
 }
-// d += a b, the product by itself, added in the fp32 adder.  The tensor core's own addition to a running sum cuts
+// d += a b.  APART: the product by itself, added in the fp32 adder.  The tensor core's own addition to a running sum cuts
 // what does not fit instead of rounding it, always towards zero, which over thousands of tokens showed in fp32 results
 // (60001 tokens: 1.0e-6 of the result, 0.5e-6 apart)
+template <bool APART>
 __device__ __forceinline__ void add16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    float c[4];
-    mma16(c, a, b0, b1, 0.f, 0.f, 0.f, 0.f);
+    if constexpr (APART) {
+        float c[4];
+        mma16(c, a, b0, b1, 0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < 4; j++) d[j] += c[j];
+        for (int j = 0; j < 4; j++) d[j] += c[j];
+    } else {
+        mma16(d, a, b0, b1);
+    }
 }
 // d = a b with k = 8
 __device__ __forceinline__ void mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
@@ -168,43 +167,6 @@ __device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[N]) {
     }
 }
 
-// V's scales and offsets of a tile, in its stage of the ring: tokens that no row sees (behind p_hi) and those that are not finite
-// get values of 0; where fp16 cannot hold a value, the tile's are taken times 1/16 (the largest that a scale and an offset give
-// is 9 times fp16's).  Returns the tokens that are not finite in bits 0 .. 15, and bit 16: times 1/16.
-template <int D>
-__device__ __forceinline__ uint32_t look_over(uint8_t* t, int base, int p_hi) {
-    constexpr int NG = D / kKvGroup, kWords = 8 * NG, N = (kWords + 31) / 32;      // words of pairs of tokens
-    const int lane = threadIdx.x & 31;
-    uint32_t* s = reinterpret_cast<uint32_t*>(t + kv4_off_vs(D));
-    uint32_t* o = reinterpret_cast<uint32_t*>(t + kv4_off_vm(D));
-    uint32_t sw[N], ow[N], bits = 0;
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-        const int at = lane + 32 * k, pair = at / NG, pos = base + 2 * pair;
-        const uint32_t seen = (pos <= p_hi ? 0xffffu : 0u) | (pos < p_hi ? 0xffff0000u : 0u);
-        sw[k] = at < kWords ? s[at] & seen : 0u, ow[k] = at < kWords ? o[at] & seen : 0u;
-        const auto infinite = [](uint32_t w) { return (w & 0x7c00u) == 0x7c00u; };
-        const uint32_t b0 = infinite(sw[k]) || infinite(ow[k]), b1 = infinite(sw[k] >> 16) || infinite(ow[k] >> 16);
-        bits |= (b0 | b1 << 1) << (2 * pair & 31);
-    }
-    const uint32_t bad = __reduce_or_sync(0xffffffffu, bits);
-    __half2 open = __float2half2_rn(0.f);
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-        const uint32_t b = bad >> (2 * ((lane + 32 * k) / NG) & 31), fine = (b & 1 ? 0u : 0xffffu) | (b & 2 ? 0u : 0xffff0000u);
-        sw[k] &= fine, ow[k] &= fine;
-        open = open2<8>(as_half2(sw[k]), as_half2(ow[k]), open);
-    }
-    const bool small = __any_sync(0xffffffffu, is_open(open));
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-        const uint32_t unit = small ? 0x2c002c00u : 0x3c003c00u;       // 1/16 or 1
-        if (lane + 32 * k < kWords) s[lane + 32 * k] = mul2(sw[k], unit), o[lane + 32 * k] = mul2(ow[k], unit);
-    }
-    __syncwarp();
-    return bad | (uint32_t)small << 16;
-}
-
 // NT columns of 8: 8 NT query rows, or (SPLIT) the high and low halves of 8
 template <typename T, int D, int NT, bool SPLIT, int W>
 __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 1) attend_kernel(const Args x) {
@@ -216,7 +178,7 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
     constexpr int ET = SPLIT ? 1 : NT;          // columns of 8 query rows
     constexpr int kRows = 8 * ET;
     constexpr bool kFp16 = sizeof(T) == 2 && !SPLIT && std::is_same<T, __half>::value;
-    constexpr float kLeast = SPLIT ? 1.f / 34359738368.f : 1.f / 16777216.f;    // 2^-35 or 2^-24: weights above 0
+    constexpr float kLeast = SPLIT || kFp16 ? 1.f / 34359738368.f : 1.f / 16777216.f;   // 2^-35 or 2^-24: weights above 0
     extern __shared__ __align__(16) uint8_t smem[];
     const Kv4Attn& a = x.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r8 = lane >> 2, q4 = lane & 3;
@@ -365,37 +327,37 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
         }
 
         float acc[NT][NG][2][4];      // channels g*32 + r8*4 + {0, 1 | 2, 3} x rows 2 q4, 2 q4 + 1
-        [[maybe_unused]] float zacc[NT][4];     // SPLIT: group r8 x rows 2 q4, 2 q4 + 1 (the last two are not used)
+        float zacc[NT][4];            // group r8 x rows 2 q4, 2 q4 + 1 (the last two are not used)
         float m[ET][2], l[ET][2];
-        // SPLIT: values' scales are below 2^v_exp so far; they enter the operands times 2^(1 - v_exp), and acc carries that factor
-        [[maybe_unused]] int v_exp = kExpMin;
-        auto clear = [&]() {
+        // values' scales are below 2^v_exp so far; they enter the operands times 2^(1 - v_exp), and the sums carry that factor
+        int v_exp = kExpMin;
+        uint32_t v_mul = pack(pow2(1 - kExpMin), pow2(1 - kExpMin));
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
+        for (int n = 0; n < NT; n++) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) zacc[n][j] = 0.f;
+            for (int j = 0; j < 4; j++) zacc[n][j] = 0.f;
 #pragma unroll
-                for (int g = 0; g < NG; g++)
+            for (int g = 0; g < NG; g++)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) acc[n][g][j >> 2][j & 3] = 0.f;
-            }
+                for (int j = 0; j < 8; j++) acc[n][g][j >> 2][j & 3] = 0.f;
+        }
 #pragma unroll
-            for (int e = 0; e < ET; e++) m[e][0] = m[e][1] = kNone, l[e][0] = l[e][1] = 0.f;
-        };
-        clear();
+        for (int e = 0; e < ET; e++) m[e][0] = m[e][1] = kNone, l[e][0] = l[e][1] = 0.f;
         const int odd_shift = (r8 & 1) * 16;
 
-        // SPLIT: raise v_exp above a tile's scales (none is negative), and acc with it
-        [[maybe_unused]] auto raise_scale = [&](const uint32_t (&s0)[NG], const uint32_t (&s1)[NG]) {
+        // whether the scales (of tokens with a bit in `any`; none is negative) lie below 2^v_exp
+        auto fit = [&](const uint32_t (&s0)[NG], const uint32_t (&s1)[NG], uint32_t any0, uint32_t any1) {
             uint32_t most = 0;
 #pragma unroll
-            for (int g = 0; g < NG; g++) most = max2(most, max2(s0[g], s1[g]));
-            // (2^v_exp is infinity for 2^16)
-            if (__all_sync(0xffffffffu, below2(most, (uint32_t)(v_exp + 15) * 0x04000400u))) return;
+            for (int g = 0; g < NG; g++) most = max2(most, max2(s0[g] & any0, s1[g] & any1));
+            return below2(most, (uint32_t)(v_exp + 15) * 0x04000400u);      // infinity for 2^16
+        };
+        // raise v_exp above them, and the sums with it
+        auto raise_scale = [&](const uint32_t (&s0)[NG], const uint32_t (&s1)[NG], uint32_t any0, uint32_t any1) {
             float mx = 0.f;
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                const float2 a0 = halves(finite2(s0[g])), a1 = halves(finite2(s1[g]));
+                const float2 a0 = halves(finite2(s0[g] & any0)), a1 = halves(finite2(s1[g] & any1));
                 mx = fmaxf(fmaxf(mx, fmaxf(a0.x, a0.y)), fmaxf(a1.x, a1.y));
             }
             const int top = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)) >> 23) - 126;     // mx < 2^top
@@ -409,15 +371,24 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
 #pragma unroll
                     for (int j = 0; j < 8; j++) acc[n][g][j >> 2][j & 3] *= f;
             v_exp = now;
+            v_mul = pack(pow2(1 - now), pow2(1 - now));
         };
         // one tile, with masks where some row sees a part of it only
-        auto tile = [&](uint8_t* t, const int base, auto masked, auto looked) {
-            constexpr bool part = decltype(masked)::value, careful = decltype(looked)::value;
-            [[maybe_unused]] uint32_t bad = 0;      // tokens with values that are not finite
-            [[maybe_unused]] bool small = false;    // values are taken times 1/16, weights times 16
-            if constexpr (careful) {
-                const uint32_t found = look_over<D>(t, base, sp.p_hi);
-                bad = found & 0xffffu, small = found >> 16;
+        auto tile = [&](const uint8_t* t, const int base, auto masked) {
+            constexpr bool part = decltype(masked)::value;
+            // V's scales.  Where every row sees every token they are checked with the scores, by one vote (64 requests of 128-wide
+            // heads: 69 us against 75), else with the weights; so too where the registers do not last for it: heads 256 wide
+            // (a window of 4096: 59 us against 65) and two columns (4 fp16 chunks of 512: 1340 us against 1414)
+            constexpr bool one_vote = !part && D < 256 && NT == 1;
+            uint32_t v0[NG], v1[NG], s0[NG], s1[NG];
+            auto load_scales = [&]() {
+                load_words<NG>(t + kv4_off_vs(D) + q4 * NG * 4, s0);
+                load_words<NG>(t + kv4_off_vs(D) + (q4 + 4) * NG * 4, s1);
+            };
+            bool fits = true;
+            if constexpr (one_vote) {
+                load_scales();
+                fits = fit(s0, s1, 0xffffffffu, 0xffffffffu);
             }
             // ---- scores: tokens r8, r8 + 8 x rows 2 q4, 2 q4 + 1 of each column ----
             float sc[ET][4];
@@ -505,8 +476,11 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
             float top = -INFINITY;
 #pragma unroll
             for (int e = 0; e < ET; e++) top = fmaxf(top, fmaxf(fmaxf(ex[e][0], ex[e][1]), fmaxf(ex[e][2], ex[e][3])));
-            const float slack = careful && small ? 0.f : kSlack;
-            if (__any_sync(0xffffffffu, top > kBias + slack)) {
+            if (__any_sync(0xffffffffu, top > kBias + kSlack || !fits)) {
+                if constexpr (one_vote) {
+                    load_scales();
+                    raise_scale(s0, s1, 0xffffffffu, 0xffffffffu);
+                }
 #pragma unroll
                 for (int e = 0; e < ET; e++)
 #pragma unroll
@@ -515,14 +489,14 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
                                           ex[e][j + 2] == -INFINITY ? -INFINITY : __fmul_rn(sc[e][j + 2], qk[e][j]));
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
-                        now = fmaxf(m[e][j], below_score(now, slack));
+                        now = fmaxf(m[e][j], below_score(now, kSlack));
                         const float f = ex2(m[e][j] - now);
                         m[e][j] = now;
                         l[e][j] *= f;
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
                             if (!SPLIT && n != e) continue;
-                            if (SPLIT) zacc[n][j] *= f;
+                            zacc[n][j] *= f;
 #pragma unroll
                             for (int g = 0; g < NG; g++) {
                                 acc[n][g][0][j] *= f;
@@ -536,8 +510,7 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
             }
 
             // ---- weights, to the layout of the second product: row r8 x tokens 2 q4, + 1 (lo: of 16) and 2 q4 + 8, + 9 ----
-            uint32_t ph[ET][2];
-            [[maybe_unused]] uint32_t pl[ET][2];
+            uint32_t ph[ET][2], pl[ET][2];
 #pragma unroll
             for (int e = 0; e < ET; e++) {
                 float p[4];
@@ -546,178 +519,133 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
                     p[j] = ex2(ex[e][j]);
                     // a seen token's weight is not 0 (the smallest that the halves hold instead, 2^-46 or 2^-35 of the largest), so that
                     // what is not finite in it reaches the row: below, a weight of 0 stands for a hidden token
-                    if ((SPLIT ? part : careful) && p[j] < kLeast && ex[e][j] != -INFINITY) p[j] = kLeast;
+                    if (part && p[j] < kLeast && ex[e][j] != -INFINITY) p[j] = kLeast;
                 }
                 l[e][0] += p[0] + p[2];
                 l[e][1] += p[1] + p[3];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    if constexpr (SPLIT) {
+                    if constexpr (SPLIT || kFp16) {
                         split2(p[2 * h], p[2 * h + 1], ph[e][h], pl[e][h]);
+                        pl[e][h] = transpose(pl[e][h]);
                     } else {
-                        if (careful && small) p[2 * h] *= 16.f, p[2 * h + 1] *= 16.f;
                         ph[e][h] = pack(p[2 * h], p[2 * h + 1]);
-                        if constexpr (kFp16) {      // what the rounding left
-                            const float2 f = halves(ph[e][h]);
-                            pl[e][h] = pack(p[2 * h] - f.x, p[2 * h + 1] - f.y);
-                        }
                     }
                     ph[e][h] = transpose(ph[e][h]);
-                    if constexpr (SPLIT || kFp16) pl[e][h] = transpose(pl[e][h]);
                 }
             }
 
-            // tokens with a weight: the others are hidden
-            [[maybe_unused]] const auto weighted = [](uint32_t w) {
-                return (w & 0x7fffu ? 0xffffu : 0u) | (w & 0x7fff0000u ? 0xffff0000u : 0u);
-            };
-            if constexpr (SPLIT) {
-                // ---- output: scales into the weights, codes of V, offsets ----
-                uint32_t v0[NG], v1[NG], s0[NG], s1[NG];
-                load_words<NG>(t + kv4_off_vc(D) + (q4 * 8 + r8) * NG * 4, v0);
-                load_words<NG>(t + kv4_off_vc(D) + ((q4 + 4) * 8 + r8) * NG * 4, v1);
-                load_words<NG>(t + kv4_off_vs(D) + q4 * NG * 4, s0);
-                load_words<NG>(t + kv4_off_vs(D) + (q4 + 4) * NG * 4, s1);
-                {
-                    uint32_t z0 = 0, z1 = 0, y0 = 0, y1 = 0;
-                    if (r8 < NG) {
-                        z0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vm(D) + (q4 * NG + r8) * 4);
-                        z1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vm(D) + ((q4 + 4) * NG + r8) * 4);
-                        y0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vs(D) + (q4 * NG + r8) * 4);
-                        y1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vs(D) + ((q4 + 4) * NG + r8) * 4);
-                    }
-                    if constexpr (part) {
-                        // a hidden token's bytes may hold anything: infinities and NaN must not meet its weight of zero.  A stored
-                        // token that is not finite has a NaN scale, which still reaches the rows that do see it below.
-                        z0 = finite2(z0), z1 = finite2(z1), y0 = finite2(y0), y1 = finite2(y1);
-                    }
-                    const uint32_t za[4] = {z0, z0, z1, z1}, ya[4] = {y0, y0, y1, y1};   // rows 8 .. 15: not used
-                    const uint32_t minus_half = 0xb800b800u;
-                    add16(zacc[0], za, ph[0][0], ph[0][1]);
-                    add16(zacc[0], ya, mul2(ph[0][0], minus_half), mul2(ph[0][1], minus_half));
-                    add16(zacc[1], za, pl[0][0], pl[0][1]);
-                    add16(zacc[1], ya, mul2(pl[0][0], minus_half), mul2(pl[0][1], minus_half));
+            // ---- output: scales into the weights, codes of V, offsets ----
+            load_words<NG>(t + kv4_off_vc(D) + (q4 * 8 + r8) * NG * 4, v0);
+            load_words<NG>(t + kv4_off_vc(D) + ((q4 + 4) * 8 + r8) * NG * 4, v1);
+            load_scales();
+            {
+                uint32_t z0 = 0, z1 = 0, y0 = 0, y1 = 0;
+                if (r8 < NG) {
+                    z0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vm(D) + (q4 * NG + r8) * 4);
+                    z1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vm(D) + ((q4 + 4) * NG + r8) * 4);
+                    y0 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vs(D) + (q4 * NG + r8) * 4);
+                    y1 = *reinterpret_cast<const uint32_t*>(t + kv4_off_vs(D) + ((q4 + 4) * NG + r8) * 4);
                 }
-                // the scales of hidden tokens count as 0, they may not be finite
                 if constexpr (part) {
-                    const uint32_t k0 = weighted(ph[0][0] | pl[0][0]), k1 = weighted(ph[0][1] | pl[0][1]);
-#pragma unroll
-                    for (int g = 0; g < NG; g++) s0[g] &= k0, s1[g] &= k1;
+                    // a hidden token's bytes may hold anything: infinities and NaN must not meet its weight of zero.  A stored
+                    // token that is not finite has a NaN scale, which still reaches the rows that do see it below.
+                    z0 = finite2(z0), z1 = finite2(z1), y0 = finite2(y0), y1 = finite2(y1);
                 }
-                raise_scale(s0, s1);
-                uint32_t b[NT][NG][2];
-                {
-                    const float2 h0 = halves(ph[0][0]), h1 = halves(ph[0][1]), l0 = halves(pl[0][0]), l1 = halves(pl[0][1]);
+                const uint32_t za[4] = {z0, z0, z1, z1}, ya[4] = {y0, y0, y1, y1};   // rows 8 .. 15: not used
+#pragma unroll
+                for (int e = 0; e < ET; e++) {
+                    const uint32_t minus_half = 0xb800b800u;
+                    add16<SPLIT>(zacc[e], za, ph[e][0], ph[e][1]);
+                    add16<SPLIT>(zacc[e], ya, mul2(ph[e][0], minus_half), mul2(ph[e][1], minus_half));
+                    if constexpr (SPLIT) {
+                        add16<SPLIT>(zacc[1], za, pl[e][0], pl[e][1]);
+                        add16<SPLIT>(zacc[1], ya, mul2(pl[e][0], minus_half), mul2(pl[e][1], minus_half));
+                    }
+                }
+            }
+            // tokens with a weight: the others are hidden, their scales count as 0 for the row, they may not be finite
+            uint32_t k0[ET], k1[ET], any0 = 0xffffffffu, any1 = 0xffffffffu;
+            if constexpr (part) {
+                any0 = any1 = 0;
+#pragma unroll
+                for (int e = 0; e < ET; e++) {
+                    const uint32_t p0 = SPLIT || kFp16 ? ph[e][0] | pl[e][0] : ph[e][0];
+                    const uint32_t p1 = SPLIT || kFp16 ? ph[e][1] | pl[e][1] : ph[e][1];
+                    k0[e] = (p0 & 0x7fffu ? 0xffffu : 0u) | (p0 & 0x7fff0000u ? 0xffff0000u : 0u);
+                    k1[e] = (p1 & 0x7fffu ? 0xffffu : 0u) | (p1 & 0x7fff0000u ? 0xffff0000u : 0u);
+                    any0 |= k0[e], any1 |= k1[e];
+                }
+            }
+            if constexpr (!one_vote)
+                if (!__all_sync(0xffffffffu, fit(s0, s1, any0, any1))) raise_scale(s0, s1, any0, any1);
+            uint32_t b[NT][NG][2];
+#pragma unroll
+            for (int e = 0; e < ET; e++) {
+                uint32_t u0[NG], u1[NG];
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    u0[g] = part ? s0[g] & k0[e] : s0[g];
+                    u1[g] = part ? s1[g] & k1[e] : s1[g];
+                }
+                if constexpr (SPLIT || kFp16) {
+                    const float2 h0 = halves(ph[e][0]), h1 = halves(ph[e][1]), l0 = halves(pl[e][0]), l1 = halves(pl[e][1]);
                     const float f = pow2(1 - v_exp);
                     const float p0 = fmaf(l0.x, kLoInv, h0.x) * f, p1 = fmaf(l0.y, kLoInv, h0.y) * f;
                     const float p2 = fmaf(l1.x, kLoInv, h1.x) * f, p3 = fmaf(l1.y, kLoInv, h1.y) * f;
 #pragma unroll
                     for (int g = 0; g < NG; g++) {
-                        const float2 a0 = halves(s0[g]), a1 = halves(s1[g]);
-                        split2(p0 * a0.x, p1 * a0.y, b[0][g][0], b[1][g][0]);
-                        split2(p2 * a1.x, p3 * a1.y, b[0][g][1], b[1][g][1]);
-                    }
-                }
-#pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    const uint32_t x0 = v0[g] >> 8, x1 = v1[g] >> 8;
-                    const uint32_t c0[4] = {centred(v0[g] & 0x000f000fu, false), centred(v0[g] & 0x00f000f0u, true),
-                                            centred(v1[g] & 0x000f000fu, false), centred(v1[g] & 0x00f000f0u, true)};
-                    const uint32_t c1[4] = {centred(x0 & 0x000f000fu, false), centred(x0 & 0x00f000f0u, true),
-                                            centred(x1 & 0x000f000fu, false), centred(x1 & 0x00f000f0u, true)};
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        add16(acc[n][g][0], c0, b[n][g][0], b[n][g][1]);
-                        add16(acc[n][g][1], c1, b[n][g][0], b[n][g][1]);
-                    }
-                }
-            } else {
-                // ---- output: values, times the weights ----
-                if (careful && bad) {
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint32_t b = bad >> (2 * q4 + 8 * h), nan = (b & 1 ? 0x7fffu : 0u) | (b & 2 ? 0x7fff0000u : 0u);
-#pragma unroll
-                        for (int e = 0; e < ET; e++) ph[e][h] |= weighted(ph[e][h]) & nan;
-                    }
-                }
-                constexpr int GC = NG < 4 ? NG : 4;     // groups at a time
-                const auto known = [&](int pos) { return (pos <= sp.p_hi ? 0xffffu : 0u) | (pos < sp.p_hi ? 0xffff0000u : 0u); };
-                [[maybe_unused]] const uint32_t keep0 = known(base + 2 * q4), keep1 = known(base + 2 * q4 + 8);
-#pragma unroll
-                for (int gc = 0; gc < NG; gc += GC) {
-                    uint32_t v0[GC], v1[GC], s0[GC], s1[GC], o0[GC], o1[GC];
-                    load_words<GC>(t + kv4_off_vc(D) + ((q4 * 8 + r8) * NG + gc) * 4, v0);
-                    load_words<GC>(t + kv4_off_vc(D) + (((q4 + 4) * 8 + r8) * NG + gc) * 4, v1);
-                    load_words<GC>(t + kv4_off_vs(D) + (q4 * NG + gc) * 4, s0);
-                    load_words<GC>(t + kv4_off_vs(D) + ((q4 + 4) * NG + gc) * 4, s1);
-                    load_words<GC>(t + kv4_off_vm(D) + (q4 * NG + gc) * 4, o0);
-                    load_words<GC>(t + kv4_off_vm(D) + ((q4 + 4) * NG + gc) * 4, o1);
-                    if constexpr (part && !careful) {       // no row sees tokens behind the last one's position
-#pragma unroll
-                        for (int i = 0; i < GC; i++) s0[i] &= keep0, s1[i] &= keep1, o0[i] &= keep0, o1[i] &= keep1;
-                    }
-#pragma unroll
-                    for (int i = 0; i < GC; i++) {
-                        uint32_t a0[4], a1[4];
-                        values4<8>(v0[i], as_half2(s0[i]), as_half2(o0[i]), a0);
-                        values4<8>(v1[i], as_half2(s1[i]), as_half2(o1[i]), a1);
-                        const uint32_t c0[4] = {a0[0], a0[1], a1[0], a1[1]}, c1[4] = {a0[2], a0[3], a1[2], a1[3]};
-#pragma unroll
-                        for (int e = 0; e < ET; e++) {
-                            mma16(acc[e][gc + i][0], c0, ph[e][0], ph[e][1]);
-                            mma16(acc[e][gc + i][1], c1, ph[e][0], ph[e][1]);
-                            if constexpr (kFp16) {
-                                mma16(acc[e][gc + i][0], c0, pl[e][0], pl[e][1]);
-                                mma16(acc[e][gc + i][1], c1, pl[e][0], pl[e][1]);
-                            }
+                        const float2 a0 = halves(u0[g]), a1 = halves(u1[g]);
+                        if constexpr (SPLIT) {
+                            split2(p0 * a0.x, p1 * a0.y, b[0][g][0], b[NT - 1][g][0]);
+                            split2(p2 * a1.x, p3 * a1.y, b[0][g][1], b[NT - 1][g][1]);
+                        } else {
+                            b[e][g][0] = pack(p0 * a0.x, p1 * a0.y);
+                            b[e][g][1] = pack(p2 * a1.x, p3 * a1.y);
                         }
                     }
+                } else {
+#pragma unroll
+                    for (int g = 0; g < NG; g++) {
+                        b[e][g][0] = mul2(ph[e][0], mul2(u0[g], v_mul));
+                        b[e][g][1] = mul2(ph[e][1], mul2(u1[g], v_mul));
+                    }
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const uint32_t x0 = v0[g] >> 8, x1 = v1[g] >> 8;
+                const uint32_t c0[4] = {centred(v0[g] & 0x000f000fu, false), centred(v0[g] & 0x00f000f0u, true),
+                                        centred(v1[g] & 0x000f000fu, false), centred(v1[g] & 0x00f000f0u, true)};
+                const uint32_t c1[4] = {centred(x0 & 0x000f000fu, false), centred(x0 & 0x00f000f0u, true),
+                                        centred(x1 & 0x000f000fu, false), centred(x1 & 0x00f000f0u, true)};
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    add16<SPLIT>(acc[n][g][0], c0, b[n][g][0], b[n][g][1]);
+                    add16<SPLIT>(acc[n][g][1], c1, b[n][g][0], b[n][g][1]);
                 }
             }
         };
 
-        auto walk = [&](auto looked) {
-            for (int i0 = 0; i0 < count; i0 += 32) {
-                const int nj = min(32, count - i0);
-                for (int j = 0; j < nj; j++) {
-                    const int i = i0 + j;
-                    cp_wait<kStages - 2>();
-                    __syncwarp();
-                    issue(i + kStages - 1, j + kStages - 1);   // into the stage that the previous step finished with (the barrier)
-                    const bool there = __shfl_sync(0xffffffffu, where, j) >= 0;
-                    const int base = there ? tile_of(i) * kKvTile : 1 << 30;   // without a page: behind every query
-                    const bool part = base + kKvTile - 1 > sp.p_lo ||
-                                      (a.window > 0 && base <= sp.p_hi - a.window && base + kKvTile > a.sinks);
-                    uint8_t* t = ring + (i % kStages) * kTileB;
-                    if constexpr (decltype(looked)::value) tile(t, base, std::true_type{}, looked);
-                    else if (part) tile(t, base, std::true_type{}, looked);
-                    else tile(t, base, std::false_type{}, looked);
-                }
-                where = where_next;
-                where_next = fetch(i0 + 64);
+        for (int i0 = 0; i0 < count; i0 += 32) {
+            const int nj = min(32, count - i0);
+            for (int j = 0; j < nj; j++) {
+                const int i = i0 + j;
+                cp_wait<kStages - 2>();
+                __syncwarp();
+                issue(i + kStages - 1, j + kStages - 1);   // into the stage that the previous step finished with (the barrier)
+                const bool there = __shfl_sync(0xffffffffu, where, j) >= 0;
+                const int base = there ? tile_of(i) * kKvTile : 1 << 30;   // without a page: behind every query
+                const bool part = base + kKvTile - 1 > sp.p_lo ||
+                                  (a.window > 0 && base <= sp.p_hi - a.window && base + kKvTile > a.sinks);
+                const uint8_t* t = ring + (i % kStages) * kTileB;
+                if (part) tile(t, base, std::true_type{});
+                else tile(t, base, std::false_type{});
             }
-            cp_wait<0>();
-        };
-        walk(std::false_type{});
-        if constexpr (!SPLIT) {
-            // Values that are not finite in hidden tokens, or beyond fp16, leave sums that are not finite.  The walk is then taken
-            // again, and each tile looked over first
-            float open = 0.f;       // NaN where a sum is infinite or NaN
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int g = 0; g < NG; g++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) open = fmaf(acc[n][g][j >> 2][j & 3], 0.f, open);
-            if (__any_sync(0xffffffffu, open != 0.f)) {
-                clear();
-                where = fetch(0), where_next = fetch(32);
-#pragma unroll
-                for (int i = 0; i < kStages - 1; i++) issue(i, i);
-                walk(std::true_type{});
-            }
+            where = where_next;
+            where_next = fetch(i0 + 64);
         }
+        cp_wait<0>();
 #pragma unroll
         for (int e = 0; e < ET; e++)
 #pragma unroll
@@ -729,21 +657,22 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
         __syncthreads();
         float* s_o = reinterpret_cast<float*>(smem);                                   // [W][kRows][D]
         float2* s_ml = reinterpret_cast<float2*>(smem + W * kRows * D * 4);       // [W][kRows]
-        [[maybe_unused]] const float unit = SPLIT ? pow2(v_exp - 1) : 1.f;
+        const float unit = pow2(v_exp - 1);
 #pragma unroll
         for (int e = 0; e < ET; e++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int rr = warp * kRows + e * 8 + 2 * q4 + j;
-                [[maybe_unused]] const float z = SPLIT ? fmaf(zacc[NT - 1][j], kLoInv, zacc[e][j]) : 0.f;
+                const float z = SPLIT ? fmaf(zacc[NT - 1][j], kLoInv, zacc[e][j]) : zacc[e][j];
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
-                    [[maybe_unused]] const float zg = SPLIT ? __shfl_sync(0xffffffffu, z, g * 4 + q4) : 0.f;
+                    const float zg = __shfl_sync(0xffffffffu, z, g * 4 + q4);
                     float o[4];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {   // channel g*32 + r8*4 + k
-                        const float v = acc[e][g][k >> 1][j + 2 * (k & 1)];
-                        o[k] = SPLIT ? fmaf(fmaf(acc[NT - 1][g][k >> 1][j + 2 * (k & 1)], kLoInv, v), (k & 1 ? 32.f : 512.f) * unit, zg) : v;
+                        const float v = SPLIT ? fmaf(acc[NT - 1][g][k >> 1][j + 2 * (k & 1)], kLoInv, acc[e][g][k >> 1][j + 2 * (k & 1)])
+                                              : acc[e][g][k >> 1][j + 2 * (k & 1)];
+                        o[k] = fmaf(v, (k & 1 ? 32.f : 512.f) * unit, zg);
                     }
                     *reinterpret_cast<float4*>(s_o + rr * D + g * kKvGroup + r8 * 4) = make_float4(o[0], o[1], o[2], o[3]);
                 }

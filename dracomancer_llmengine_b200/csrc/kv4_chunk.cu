@@ -135,6 +135,33 @@ __device__ __forceinline__ void load_global(const void* p, uint32_t (&w)[N]) {
         w[0] = *reinterpret_cast<const uint32_t*>(p);
     }
 }
+__device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+__device__ __forceinline__ uint32_t as_word(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ uint32_t or_exponent(uint32_t w, uint32_t mask) {     // (w & mask) | 1024's exponent, twice
+    uint32_t t;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(t) : "r"(w), "r"(mask), "r"(0x64006400u));
+    return t;
+}
+// 0, or NaN where a group's values are not finite or cannot be held in fp16 (scale times the lowest or highest code, less ZERO,
+// plus the offset: infinity times 0 is NaN), added to the same of other groups
+template <int ZERO>
+__device__ __forceinline__ __half2 open2(__half2 s, __half2 m, __half2 sum) {
+    const __half2 z = __float2half2_rn(0.f);
+    if (ZERO) sum = __hfma2(__hfma2(s, __float2half2_rn((float)-ZERO), m), z, sum);
+    return __hfma2(__hfma2(s, __float2half2_rn(15.f - ZERO), m), z, sum);
+}
+__device__ __forceinline__ bool is_open(__half2 sum) { return as_word(sum) & 0x7fff7fffu; }
+// the four pairs of a word's codes, minus ZERO, times s plus m: halves (0 4) (1 5) (2 6) (3 7) of nibbles
+template <int ZERO>
+__device__ __forceinline__ void values4(uint32_t w, __half2 s, __half2 m, uint32_t (&out)[4]) {
+    const __half2 one = __float2half2_rn(-1024.f - ZERO);                 // 1024 + c         -> c - ZERO, exact
+    const __half2 six = __float2half2_rn(-64.f - ZERO), f = __float2half2_rn(0.0625f);   // 1024 + 16 c, likewise
+    const uint32_t x = w >> 8;
+    out[0] = as_word(__hfma2(__hadd2(as_half2(or_exponent(w, 0x000f000fu)), one), s, m));
+    out[1] = as_word(__hfma2(__hfma2(as_half2(or_exponent(w, 0x00f000f0u)), f, six), s, m));
+    out[2] = as_word(__hfma2(__hadd2(as_half2(or_exponent(x, 0x000f000fu)), one), s, m));
+    out[3] = as_word(__hfma2(__hfma2(as_half2(or_exponent(x, 0x00f000f0u)), f, six), s, m));
+}
 
 // A unit of work of the block, or the part of it that the block's run holds
 struct Segment {
