@@ -14,7 +14,8 @@
 //     Group sums come out of the products unscaled and are scaled in fp32; the offsets are one small product more.
 //     Queries are brought below 2^14 by a power of two per row first: 16-bit queries then are exact in fp16 down to 2^-28 (odd
 //     nibbles' 2^-24) of their row's largest, and off by 2^-39 (2^-35) of it below.  Their sums have a high and a low half
-//     in every type, so the scores, and with them lse, keep fp32 precision.
+//     in every type.  Scores of size 4, and with them lse, are off by 1e-6 on average in fp32 and by 1.5e-6 in 16-bit types (6e-6
+//     and 9e-6 at most of 1600; plain fp32 sums 0.4e-6 and 2.7e-6).
 //   output: sum_t p_t v_t = sum_t (p_t s_tg / 2) (2 c - 15) + sum_t p_t (m_tg - s_tg / 2): the weights take the scales,
 //     codes become (2 c - 15) * 2^-10 in one multiply-add.  They are centred because the sums run over the whole context:
 //     uncentred ones would grow with its length, cancel against the offsets' sum, and lose the result's low bits.
@@ -22,8 +23,11 @@
 //   fp32  queries and weights are split in two halves (x = hi + lo / 2048, 22 bits), the low halves take 8 columns more;
 //         codes of K are made normal numbers (c * 2^-9): with subnormal ones the sums of a product are aligned ten bits
 //         too high, which showed as 1e-6 of the result (2^-14 of a code; measured 1.1e-6 against 0.5e-6 without)
-//   fp16  weights are multiplied with the scales in fp32 and rounded to fp16 once (2^-11), as the output will be
-//   bf16  weights are rounded to fp16 and multiplied with the scales there (2^-11 twice, an eighth of the output's rounding)
+//   fp16  weights, and their products with the scales, have a high and a low half (22 bits, two products into the same sums):
+//         with a rounded one, what the channels beside a large one of their group owe to rounding was 8e-4 of the result (codes
+//         and offsets cancel there), and a row that one small weight makes had that weight's rounding in all channels
+//   bf16  weights are rounded to fp16 and multiplied with the scales there (2^-11 twice, an eighth of the output's rounding; beside
+//         a large channel 1e-3 of the result, below the output's 1.7e-3)
 // fp16 has 2^-14 as its smallest normal number, so both factors are kept well above it: the largest weight of a row is
 // 2^11 (kBias), and the scales are divided by a power of two above the largest one that the warp has met (v_exp), which
 // is raised, and the sums with it, like the running maximum.  The roundings above are those of a weight times a scale
@@ -61,7 +65,9 @@ struct Shape {
     static constexpr int kStages = D == 256 ? 3 : 4;                      // of a warp's ring
     static constexpr bool kQInSmem = D == 256 && NT == 2;                 // 64 registers a lane otherwise
     static constexpr int kTeam = D == 64 ? 16 : D == 128 ? (NT == 1 ? 16 : 12) : 8;    // warps where a block takes a unit
-    static constexpr int kBlocks = D == 64 ? (NT == 1 ? 5 : 4) : D == 128 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2);
+    // of an SM.  Heads 256 wide: three leave 168 registers, of which the sums take most (a window of 4096: fp16 52 us against 70,
+    // bf16 48 against 67)
+    static constexpr int kBlocks = D == 64 ? (NT == 1 ? 5 : 4) : D == 128 ? (NT == 1 ? 4 : 3) : 2;
 };
 constexpr uint32_t kTwo15 = 0x78007800u;   // 2^15, 2^15 in fp16
 constexpr float kSlack = 3.f;              // log2 by which weights may pass 2^kBias
@@ -132,6 +138,12 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {      // of a 
     const __half2 d = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&d);
 }
+// a b + c
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+    const __half2 d = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                              *reinterpret_cast<const __half2*>(&c));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
 __device__ __forceinline__ bool below2(uint32_t a, uint32_t b) {        // both halves
     return __hblt2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
 }
@@ -178,7 +190,7 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
     constexpr int ET = SPLIT ? 1 : NT;          // columns of 8 query rows
     constexpr int kRows = 8 * ET;
     constexpr bool kFp16 = sizeof(T) == 2 && !SPLIT && std::is_same<T, __half>::value;
-    constexpr float kLeast = SPLIT || kFp16 ? 1.f / 34359738368.f : 1.f / 16777216.f;   // 2^-35 or 2^-24: weights above 0
+    constexpr float kLeast = SPLIT ? 1.f / 34359738368.f : 1.f / 16777216.f;    // 2^-35 or 2^-24: weights above 0
     extern __shared__ __align__(16) uint8_t smem[];
     const Kv4Attn& a = x.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r8 = lane >> 2, q4 = lane & 3;
@@ -377,9 +389,9 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
         auto tile = [&](const uint8_t* t, const int base, auto masked) {
             constexpr bool part = decltype(masked)::value;
             // V's scales.  Where every row sees every token they are checked with the scores, by one vote (64 requests of 128-wide
-            // heads: 69 us against 75), else with the weights; so too where the registers do not last for it: heads 256 wide
-            // (a window of 4096: 59 us against 65) and two columns (4 fp16 chunks of 512: 1340 us against 1414)
-            constexpr bool one_vote = !part && D < 256 && NT == 1;
+            // heads: 69 us against 75), else with the weights; so too with two columns, where the registers do not last for it (4
+            // fp16 chunks of 512: 1340 us against 1414)
+            constexpr bool one_vote = !part && NT == 1;
             uint32_t v0[NG], v1[NG], s0[NG], s1[NG];
             auto load_scales = [&]() {
                 load_words<NG>(t + kv4_off_vs(D) + q4 * NG * 4, s0);
@@ -510,7 +522,8 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
             }
 
             // ---- weights, to the layout of the second product: row r8 x tokens 2 q4, + 1 (lo: of 16) and 2 q4 + 8, + 9 ----
-            uint32_t ph[ET][2], pl[ET][2];
+            uint32_t ph[ET][2];
+            [[maybe_unused]] uint32_t pl[ET][2];
 #pragma unroll
             for (int e = 0; e < ET; e++) {
                 float p[4];
@@ -525,13 +538,17 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
                 l[e][1] += p[1] + p[3];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    if constexpr (SPLIT || kFp16) {
+                    if constexpr (SPLIT) {
                         split2(p[2 * h], p[2 * h + 1], ph[e][h], pl[e][h]);
-                        pl[e][h] = transpose(pl[e][h]);
                     } else {
                         ph[e][h] = pack(p[2 * h], p[2 * h + 1]);
+                        if constexpr (kFp16) {      // what the rounding left
+                            const float2 f = halves(ph[e][h]);
+                            pl[e][h] = pack(p[2 * h] - f.x, p[2 * h + 1] - f.y);
+                        }
                     }
                     ph[e][h] = transpose(ph[e][h]);
+                    if constexpr (SPLIT || kFp16) pl[e][h] = transpose(pl[e][h]);
                 }
             }
 
@@ -558,9 +575,16 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
                     const uint32_t minus_half = 0xb800b800u;
                     add16<SPLIT>(zacc[e], za, ph[e][0], ph[e][1]);
                     add16<SPLIT>(zacc[e], ya, mul2(ph[e][0], minus_half), mul2(ph[e][1], minus_half));
-                    if constexpr (SPLIT) {
-                        add16<SPLIT>(zacc[1], za, pl[e][0], pl[e][1]);
-                        add16<SPLIT>(zacc[1], ya, mul2(pl[e][0], minus_half), mul2(pl[e][1], minus_half));
+                    if constexpr (SPLIT || kFp16) {
+                        float(&z)[4] = zacc[SPLIT ? 1 : e];
+                        if constexpr (SPLIT) {
+                            add16<SPLIT>(z, za, pl[e][0], pl[e][1]);
+                            add16<SPLIT>(z, ya, mul2(pl[e][0], minus_half), mul2(pl[e][1], minus_half));
+                        } else {        // of the low half, an offset that is rounded is enough
+                            const uint32_t w0 = fma2(y0, minus_half, z0), w1 = fma2(y1, minus_half, z1);
+                            const uint32_t wa[4] = {w0, w0, w1, w1};
+                            add16<SPLIT>(z, wa, pl[e][0], pl[e][1]);
+                        }
                     }
                 }
             }
@@ -579,41 +603,33 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
             }
             if constexpr (!one_vote)
                 if (!__all_sync(0xffffffffu, fit(s0, s1, any0, any1))) raise_scale(s0, s1, any0, any1);
-            uint32_t b[NT][NG][2];
-#pragma unroll
-            for (int e = 0; e < ET; e++) {
-                uint32_t u0[NG], u1[NG];
-#pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    u0[g] = part ? s0[g] & k0[e] : s0[g];
-                    u1[g] = part ? s1[g] & k1[e] : s1[g];
-                }
-                if constexpr (SPLIT || kFp16) {
-                    const float2 h0 = halves(ph[e][0]), h1 = halves(ph[e][1]), l0 = halves(pl[e][0]), l1 = halves(pl[e][1]);
-                    const float f = pow2(1 - v_exp);
-                    const float p0 = fmaf(l0.x, kLoInv, h0.x) * f, p1 = fmaf(l0.y, kLoInv, h0.y) * f;
-                    const float p2 = fmaf(l1.x, kLoInv, h1.x) * f, p3 = fmaf(l1.y, kLoInv, h1.y) * f;
-#pragma unroll
-                    for (int g = 0; g < NG; g++) {
-                        const float2 a0 = halves(u0[g]), a1 = halves(u1[g]);
-                        if constexpr (SPLIT) {
-                            split2(p0 * a0.x, p1 * a0.y, b[0][g][0], b[NT - 1][g][0]);
-                            split2(p2 * a1.x, p3 * a1.y, b[0][g][1], b[NT - 1][g][1]);
-                        } else {
-                            b[e][g][0] = pack(p0 * a0.x, p1 * a0.y);
-                            b[e][g][1] = pack(p2 * a1.x, p3 * a1.y);
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int g = 0; g < NG; g++) {
-                        b[e][g][0] = mul2(ph[e][0], mul2(u0[g], v_mul));
-                        b[e][g][1] = mul2(ph[e][1], mul2(u1[g], v_mul));
-                    }
-                }
+            [[maybe_unused]] float p0, p1, p2, p3;
+            if constexpr (SPLIT) {
+                const float2 h0 = halves(ph[0][0]), h1 = halves(ph[0][1]), l0 = halves(pl[0][0]), l1 = halves(pl[0][1]);
+                const float f = pow2(1 - v_exp);
+                p0 = fmaf(l0.x, kLoInv, h0.x) * f, p1 = fmaf(l0.y, kLoInv, h0.y) * f;
+                p2 = fmaf(l1.x, kLoInv, h1.x) * f, p3 = fmaf(l1.y, kLoInv, h1.y) * f;
             }
 #pragma unroll
             for (int g = 0; g < NG; g++) {
+                uint32_t b[NT][2];                          // weights times scales
+                [[maybe_unused]] uint32_t r[NT][2];         // fp16: what their rounding left
+                if constexpr (SPLIT) {
+                    const float2 a0 = halves(part ? s0[g] & k0[0] : s0[g]), a1 = halves(part ? s1[g] & k1[0] : s1[g]);
+                    split2(p0 * a0.x, p1 * a0.y, b[0][0], b[NT - 1][0]);
+                    split2(p2 * a1.x, p3 * a1.y, b[0][1], b[NT - 1][1]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < ET; e++) {
+                        const uint32_t u[2] = {mul2(part ? s0[g] & k0[e] : s0[g], v_mul), mul2(part ? s1[g] & k1[e] : s1[g], v_mul)};
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            b[e][h] = mul2(ph[e][h], u[h]);
+                            // (a fused product less its own rounding is exact)
+                            if constexpr (kFp16) r[e][h] = fma2(pl[e][h], u[h], fma2(ph[e][h], u[h], b[e][h] ^ 0x80008000u));
+                        }
+                    }
+                }
                 const uint32_t x0 = v0[g] >> 8, x1 = v1[g] >> 8;
                 const uint32_t c0[4] = {centred(v0[g] & 0x000f000fu, false), centred(v0[g] & 0x00f000f0u, true),
                                         centred(v1[g] & 0x000f000fu, false), centred(v1[g] & 0x00f000f0u, true)};
@@ -621,8 +637,12 @@ __global__ void __launch_bounds__(W * 32, W == kWarps ? Shape<D, NT>::kBlocks : 
                                         centred(x1 & 0x000f000fu, false), centred(x1 & 0x00f000f0u, true)};
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    add16<SPLIT>(acc[n][g][0], c0, b[n][g][0], b[n][g][1]);
-                    add16<SPLIT>(acc[n][g][1], c1, b[n][g][0], b[n][g][1]);
+                    add16<SPLIT>(acc[n][g][0], c0, b[n][0], b[n][1]);
+                    add16<SPLIT>(acc[n][g][1], c1, b[n][0], b[n][1]);
+                    if constexpr (kFp16) {
+                        add16<SPLIT>(acc[n][g][0], c0, r[n][0], r[n][1]);
+                        add16<SPLIT>(acc[n][g][1], c1, r[n][0], r[n][1]);
+                    }
                 }
             }
         };

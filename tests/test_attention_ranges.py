@@ -267,3 +267,28 @@ def test_nan_values_with_vanishing_weight(kind, rows, pos):
     sees = torch.arange(n - rows, n) >= pos
     assert torch.equal(torch.isnan(out).all(-1).all(-1).cpu(), sees)
     assert torch.equal(torch.isnan(out).any(-1).any(-1).cpu(), sees)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n", [2, 3, 40])
+def test_short_rows_behind_a_dominating_token(kind, n):
+    """Rows that one or a few small weights make: a weight's rounding then is the result's, in all channels alike."""
+    k, v, sign = dominated(n, [5.0 + 0.01 * i for i in range(300)], 1.0, 1, 64, 15)
+    cache, table, lens = filled(k, v, 16)
+    check(kind, cache, table, lens, [1] * len(lens), queries(kind, sign, len(lens), 1, 16))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows", [1, 21, 80])
+@pytest.mark.parametrize("n", [2, 5, 300])
+def test_values_with_outlier_channels(kind, rows, n):
+    """Groups of values with one large channel and the rest near 0: the rest's part of the result is near 0 too."""
+    gen = torch.Generator().manual_seed(17)
+    k, v = [], []
+    for _ in range(8):
+        k.append(torch.randn(n, 1, 128, generator=gen))
+        v.append(1e-3 * torch.randn(n, 1, 128, generator=gen))
+        v[-1][..., 5::32] = 10 * torch.randn(n, 1, 4, generator=gen)
+    cache, table, lens = filled(k, v, 16)
+    q_lens = [min(rows, n)] * len(lens)
+    check(kind, cache, table, lens, q_lens, torch.randn(sum(q_lens), 8, 128, generator=gen).cuda().to(TYPES[kind]))
