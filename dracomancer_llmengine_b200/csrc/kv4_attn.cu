@@ -820,7 +820,8 @@ int team_of(int d, int nt) {
 }
 
 // How the rows are blocked and the tiles are divided, by the call's bounds max_q and max_seq, which the host knows.  (The times
-// below were taken before the kernels checked scales and ranges, which costs 4 to 9 % on either side of each comparison.)
+// below were taken before the kernels checked scales and ranges and had low halves in fp16, which cost 4 to 17 % on either side of
+// each comparison.)
 // Chunks: bf16 queries with more than 128 rows per request and kv head go to the tensor-core form, 256 rows a block (64
 // requests of 1024 tokens, 4 kv heads: 256 rows 109 us against 149, 72 rows 83 against 54); with few units over long
 // sequences, which that form's blocks of fewer, longer steps suit, from 25 rows (4 requests of 8192 tokens: 32 rows 38 us

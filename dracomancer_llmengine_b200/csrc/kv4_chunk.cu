@@ -11,7 +11,7 @@
 // have two buffers, so that a step's scores are computed beside the previous step's softmax.  (With two buffers of K and V a
 // step took 3600 cycles: from a product's end through unpacking, scores, softmax and product again is two steps' way.)
 //
-// Measured at 4 chunks of up to 512 queries x 32 heads over contexts up to 8192 (194 GFLOP): 302 us, 0.64 PFLOP/s, 2660
+// Measured at 4 chunks of up to 512 queries x 32 heads over contexts up to 8192 (194 GFLOP): 299 us, 0.65 PFLOP/s, 2650
 // cycles a step, softmax bound.  (283 us and 2500 cycles before keys' and values' range was checked and weights were raised: of
 // these softmax 2100, with 1120 for the 64 exponentials a row, of which both halves' on the exponential unit alone are
 // 1024; products 1220.)  Blocks of 128 rows with four unpacking warps, one of which issued the products, two blocks an SM:
