@@ -89,8 +89,8 @@ class KV4Cache:
     description and `status`, one int32 on the GPU.  It is 0 unless a wait inside the kernel of a call ran out (2 s), whose rows
     are then NaN; calls only ever set bits in it, and a server that reads its results reads it with them.
 
-    Attention whose long axis is split over blocks needs scratch memory (:meth:`workspace_bytes`: 2 to 10 MB for single
-    tokens over long contexts, 40 MB for chunks).  Without `workspace=` the module keeps one buffer for each stream, for
+    Attention whose long axis is split over blocks needs scratch memory (:meth:`workspace_bytes`: some MB for single
+    tokens over long contexts, up to 40 MB for chunks).  Without `workspace=` the module keeps one buffer for each stream, for
     all caches, and one for each graph capture, which lives as long as the caches that the capture read.  So eager calls
     on different streams may overlap, and so may replays of different graphs, and eager calls with either.  Two replays
     of the same graph may not, nor two calls that were given the same `workspace`."""

@@ -419,7 +419,8 @@ int draco_b200_kv4_attention_checked(const DracoKV4Cache* cache, const DracoKV4A
  *   codes, per group of u = h * weight with a = max |u|:  fmt 0: int8 rint(u * (127 / a)), fmt 1: e4m3(u * (448 / a))
  *   scales[row][group] = a / 127 (or 448) * rstd, so that code * scale is the normalised value
  * group: 32, 64, 128, 256 or 0 (one scale a row), dividing hidden.  A group with a < 2^-100 has code and scale 0, one
- * with an infinity or NaN a NaN scale. */
+ * with an infinity or NaN a NaN scale.  The sum of squares is fp32: rows with values of 1e19 and more overflow it, and their
+ * y and scales are 0. */
 typedef struct DracoNormQ8 {
     const void *x, *residual;
     const float* weight;
