@@ -8,7 +8,8 @@ bind it in place of the CPU libraries, plus `draco_b200_*` extensions (whole-lay
 a token batch, routing only, activation mode, weight registry).
 
 `decoder` has the operators of a decoder layer around the MoE FFN for torch CUDA tensors: block planning, the 4-bit
-paged KV cache, attention over it, and the residual RMS norm with 8-bit output.
+paged KV cache, attention over it, the residual RMS norm with 8-bit output, and the products of such rows with 8-bit
+weights: projections, experts' gate/up and down products, the plan that sorts a batch by expert and the sum of its rows.
 
 This module is the Python face of that library, mirroring how the reference's drivers call
 it (`src/qwen35_engine.py:92-131`, `src/qwen35_prefill.py:65-83`, `src/k2_engine.py:97-106`):
@@ -89,6 +90,22 @@ class DracoNormQ8(ct.Structure):
                 ("group", ct.c_int), ("eps", ct.c_float)]
 
 
+class DracoLinearQ8(ct.Structure):
+    """Layout of `DracoLinearQ8` in include/draco_moe_b200.h."""
+    _fields_ = [("x", _vp), ("x_scales", _vp), ("w", _vp), ("w_scales", _vp), ("offsets", _vp), ("rows", _vp), ("out", _vp),
+                ("out_scales", _vp), ("x_stride", ct.c_long), ("x_scales_stride", ct.c_long), ("out_stride", ct.c_long),
+                ("out_scales_stride", ct.c_long), ("n_x", ct.c_int), ("n_rows", ct.c_int), ("n", ct.c_int), ("k", ct.c_int),
+                ("n_groups", ct.c_int), ("dtype", ct.c_int), ("swiglu", ct.c_int), ("status", _vp),
+                ("wait_limit_us", ct.c_int)]
+
+
+class DracoCombineExperts(ct.Structure):
+    """Layout of `DracoCombineExperts` in include/draco_moe_b200.h."""
+    _fields_ = [("y", _vp), ("pos", _vp), ("weights", _vp), ("add", _vp), ("out", _vp), ("y_stride", ct.c_long),
+                ("pos_stride", ct.c_long), ("weights_stride", ct.c_long), ("add_stride", ct.c_long), ("out_stride", ct.c_long),
+                ("n_y", ct.c_int), ("n_tokens", ct.c_int), ("n_used", ct.c_int), ("hidden", ct.c_int), ("dtype", ct.c_int)]
+
+
 # name: (argtypes, restype) -- the reference drivers' own ctypes signatures where they exist
 _SIGS = {
     "m6_granite_moe": ([_f, _u64, _i, _f] + [ct.c_int] * 5 + [_f, _f], None),
@@ -164,6 +181,10 @@ _SIGS = {
     "draco_b200_kv4_attention_checked": ([ct.POINTER(DracoKV4Cache), ct.POINTER(DracoKV4Attention), _vp, ct.c_int, _vp], ct.c_int),
     "draco_b200_kv4_attention": ([ct.POINTER(DracoKV4Cache), ct.POINTER(DracoKV4Attention), _vp], ct.c_int),
     "draco_b200_rmsnorm_q8": ([ct.POINTER(DracoNormQ8), _vp], ct.c_int),
+    "draco_b200_linear_q8": ([ct.POINTER(DracoLinearQ8), _vp], ct.c_int),
+    "draco_b200_test_q8_barrier_extra": ([ct.c_int], ct.c_int),
+    "draco_b200_plan_experts": ([_vp] + [ct.c_int] * 4 + [_vp] * 4, ct.c_int),
+    "draco_b200_combine_experts": ([ct.POINTER(DracoCombineExperts), _vp], ct.c_int),
 }
 
 _LIB = None

@@ -4,6 +4,7 @@
 #include "../../include/draco_moe_b200.h"
 #include "abi.h"
 #include "kv4.cuh"
+#include "q8.cuh"
 
 #include <algorithm>
 #include <cstdarg>
@@ -40,6 +41,7 @@ int launched(const char* who, int kernels) {
 // each address again would take as long as the launch
 thread_local bool t_pointers_checked = false;
 thread_local int t_test_extra = 0;
+thread_local int t_test_q8_extra = 0;
 bool on_device(std::initializer_list<const void*> ps) {
     if (t_pointers_checked) return true;
     for (const void* p : ps)
@@ -110,6 +112,12 @@ void draco_b200_pointers_checked(int on) { t_pointers_checked = on != 0; }
 int draco_b200_test_kv4_barrier_extra(int which) {
     const int old = t_test_extra;
     if (which >= 0 && which <= 3) t_test_extra = which;
+    return old;
+}
+// the same for the 8-bit products' tensor-core form (1: a step's operands, 2: its product, 3: a join of a block's column maxima)
+int draco_b200_test_q8_barrier_extra(int which) {
+    const int old = t_test_q8_extra;
+    if (which >= 0 && which <= 3) t_test_q8_extra = which;
     return old;
 }
 // the id of the graph capture that the stream is in, 0: none
@@ -229,6 +237,86 @@ int draco_b200_rmsnorm_q8(const DracoNormQ8* p, void* stream) {
                      p->h_stride, p->y_stride, p->codes_stride, p->scales_stride, p->n_rows, p->hidden, g, p->dtype,
                      p->fmt, p->eps};
     launch_rmsnorm_q8(a, (cudaStream_t)stream);
+    return launched(who, 1);
+}
+
+int draco_b200_linear_q8(const DracoLinearQ8* p, void* stream) {
+    const char* who = p && p->swiglu ? "draco_b200_swiglu_q8" : "draco_b200_linear_q8";
+    if (!p) return refuse("%s: null arguments", who);
+    if (p->n_x < 0 || p->n_rows < 0 || p->n < 1 || p->k < 1 || p->n_groups < 1 || p->n_groups > kQ8MaxGroups ||
+        (!p->swiglu && (p->dtype < 0 || p->dtype > 2)))
+        return refuse("%s: need n_x, n_rows >= 0, n, k >= 1, 1 <= n_groups <= %d, dtype 0..2", who, kQ8MaxGroups);
+    if (p->n > (1 << 24) || p->k > (1 << 24) || p->n_rows > (1 << 24) || p->n_x > (1 << 24))
+        return refuse("%s: n, k, n_rows and n_x must be at most 2^24", who);
+    if (!p->offsets && p->n_groups != 1) return refuse("%s: more than one group takes offsets", who);
+    if (p->n_rows && !p->rows && p->n_x != p->n_rows) return refuse("%s: without rows n_x must be n_rows", who);
+    if (p->wait_limit_us < 0 || p->wait_limit_us > 2000000) return refuse("%s: need 0 <= wait_limit_us <= 2000000", who);
+    const long nb = (p->n + kQ8Block - 1) / kQ8Block;
+    if (p->x_stride < 0 || p->x_scales_stride < 0 || (p->n_rows > 1 && p->out_stride < p->n) ||
+        (p->swiglu && p->n_rows > 1 && p->out_scales_stride < nb))
+        return refuse("%s: strides must not be negative, nor those of outputs below a row", who);
+    if (((long)p->n_rows / 16 + p->n_groups + 1) * nb > 0x7fffffffl) return refuse("%s: too large for one call", who);
+    if (p->n_rows == 0) return 0;
+    if (!p->w || !p->w_scales || !p->out || (p->n_x && (!p->x || !p->x_scales)) || (p->swiglu && !p->out_scales))
+        return refuse("%s: null pointer", who);
+    if (!on_device({p->x, p->x_scales, p->w, p->w_scales, p->offsets, p->rows, p->out, p->out_scales, p->status}))
+        return refuse("%s: buffers must be device memory", who);
+    const size_t b = p->swiglu ? 1 : (size_t)dtype_bytes(p->dtype);
+    if (!aligned_to(p->out, b) || !aligned_to(p->x_scales, 4) || !aligned_to(p->w_scales, 4) || !aligned_to(p->offsets, 4) ||
+        !aligned_to(p->rows, 4) || !aligned_to(p->out_scales, 4) || !aligned_to(p->status, 4))
+        return refuse("%s: buffers must be aligned to their elements", who);
+    const Q8Args a{(const uint8_t*)p->x, p->x_scales, (const uint8_t*)p->w, p->w_scales, p->offsets, p->rows, p->out,
+                   p->out_scales, p->x_stride, p->x_scales_stride, p->out_stride, p->out_scales_stride, p->n_x, p->n_rows,
+                   p->n, p->k, p->n_groups, p->dtype, p->swiglu != 0, p->status,
+                   p->wait_limit_us ? p->wait_limit_us * 1000l : 2000000000l, t_test_q8_extra};
+    if (!launch_q8(a, (cudaStream_t)stream)) {
+        cudaGetLastError();
+        refuse("%s: the launch could not be set up", who);
+        return -3;
+    }
+    return launched(who, 1);
+}
+
+int draco_b200_plan_experts(const int* order, int n_tokens, int n_used, int first, int n_experts, int* offsets, int* rows,
+                            int* pos, void* stream) {
+    const char* who = "draco_b200_plan_experts";
+    if (n_tokens < 0 || n_used < 1 || n_experts < 1 || n_experts > kPlanMaxExperts || (long)n_tokens * n_used > 1l << 24)
+        return refuse("%s: need n_tokens >= 0, n_used >= 1, 1 <= n_experts <= %d, n_tokens * n_used <= 2^24", who,
+                      kPlanMaxExperts);
+    const int n = n_tokens * n_used;
+    if (!offsets || (n && (!order || !rows || !pos))) return refuse("%s: null pointer", who);
+    if (!on_device({order, offsets, rows, pos})) return refuse("%s: buffers must be device memory", who);
+    if (!aligned_to(order, 4) || !aligned_to(offsets, 4) || !aligned_to(rows, 4) || !aligned_to(pos, 4))
+        return refuse("%s: buffers must be aligned to their elements", who);
+    if (n && (order == pos || order == rows || rows == pos)) return refuse("%s: outputs must not overlap inputs", who);
+    if (!launch_plan_experts(PlanExpertsArgs{order, offsets, rows, pos, n, n_used, n_experts, first}, (cudaStream_t)stream)) {
+        const cudaError_t e = cudaGetLastError();
+        refuse("%s: launch failed: %s", who, cudaGetErrorString(e));
+        return -3;
+    }
+    return launched(who, 1);
+}
+
+int draco_b200_combine_experts(const DracoCombineExperts* p, void* stream) {
+    const char* who = "draco_b200_combine_experts";
+    if (!p) return refuse("%s: null arguments", who);
+    if (p->dtype < 0 || p->dtype > 2 || p->n_y < 0 || p->n_tokens < 0 || p->n_used < 0 || p->hidden < 1)
+        return refuse("%s: need dtype 0..2, n_y, n_tokens, n_used >= 0, hidden >= 1", who);
+    if (p->y_stride < 0 || p->add_stride < 0 || p->pos_stride < 0 || p->weights_stride < 0 ||
+        (p->n_tokens > 1 && p->out_stride < p->hidden))
+        return refuse("%s: strides must not be negative, nor out's below a row", who);
+    if ((long)p->n_tokens * p->hidden >= 1l << 39) return refuse("%s: too large for one call", who);
+    if (p->n_tokens == 0) return 0;
+    if (!p->out || (p->n_used && (!p->pos || !p->weights)) || (p->n_used && p->n_y && !p->y))
+        return refuse("%s: null pointer", who);
+    if (!on_device({p->y, p->pos, p->weights, p->add, p->out})) return refuse("%s: buffers must be device memory", who);
+    const size_t b = (size_t)dtype_bytes(p->dtype);
+    if (!aligned_to(p->y, b) || !aligned_to(p->add, b) || !aligned_to(p->out, b) || !aligned_to(p->pos, 4) ||
+        !aligned_to(p->weights, 4))
+        return refuse("%s: buffers must be aligned to their elements", who);
+    const CombineArgs a{p->y, p->pos, p->weights, p->add, p->out, p->y_stride, p->add_stride, p->out_stride, p->pos_stride,
+                        p->weights_stride, p->n_y, p->n_tokens, p->n_used, p->hidden, p->dtype};
+    launch_combine_experts(a, (cudaStream_t)stream);
     return launched(who, 1);
 }
 

@@ -26,6 +26,9 @@ decltype(&draco_b200_kv4_read) f_read = nullptr;
 decltype(&draco_b200_kv4_attention_workspace) f_workspace = nullptr;
 decltype(&draco_b200_kv4_attention_checked) f_attention = nullptr;
 decltype(&draco_b200_rmsnorm_q8) f_norm = nullptr;
+decltype(&draco_b200_linear_q8) f_linear = nullptr;
+decltype(&draco_b200_plan_experts) f_plan_experts = nullptr;
+decltype(&draco_b200_combine_experts) f_combine = nullptr;
 void (*f_checked)(int) = nullptr;
 unsigned long long (*f_capture_id)(void*) = nullptr;
 
@@ -59,7 +62,7 @@ long number(PyObject* o) {
 }
 int small(PyObject* o, const char* what) {
     const long v = number(o);
-    if (v < -2147483647l || v > 2147483647l) throw Refused(std::string(what) + " does not fit 32 bits");
+    if (v < -2147483648l || v > 2147483647l) throw Refused(std::string(what) + " does not fit 32 bits");
     return (int)v;
 }
 double real(PyObject* o) {
@@ -137,7 +140,9 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!take("draco_b200_last_error", f_last_error) || !take("draco_b200_plan_blocks", f_plan_blocks) ||
         !take("draco_b200_kv4_append", f_append) || !take("draco_b200_kv4_read", f_read) ||
         !take("draco_b200_kv4_attention_workspace", f_workspace) || !take("draco_b200_kv4_attention_checked", f_attention) ||
-        !take("draco_b200_pointers_checked", f_checked) || !take("draco_b200_capture_id", f_capture_id) || !take("draco_b200_rmsnorm_q8", f_norm))
+        !take("draco_b200_pointers_checked", f_checked) || !take("draco_b200_capture_id", f_capture_id) || !take("draco_b200_rmsnorm_q8", f_norm) ||
+        !take("draco_b200_linear_q8", f_linear) || !take("draco_b200_plan_experts", f_plan_experts) ||
+        !take("draco_b200_combine_experts", f_combine))
         return nullptr;
     Py_INCREF(a[0]);
     Py_XSETREF(g_error, a[0]);
@@ -311,6 +316,140 @@ PyObject* rmsnorm_q8(PyObject*, PyObject* const* a, Py_ssize_t given) {
     });
 }
 
+// the rows and weights of both 8-bit products; n: a weight's rows (its last dimensions are [n, k])
+void q8_operands(DracoLinearQ8& p, const at::Tensor& x, const at::Tensor& xs, const at::Tensor& w, const at::Tensor& ws,
+                 const at::Tensor* offsets, const at::Tensor* rows, const at::Tensor* status, int64_t mats, int64_t n_rows) {
+    const int64_t lead = mats > 1 ? 1 : 0;     // the dimension of gate and up
+    need(x.dim() == 2 && x.scalar_type() == at::kFloat8_e4m3fn && (x.stride(1) == 1 || x.size(1) <= 1),
+         "x must be a float8_e4m3fn tensor [rows, k] with contiguous rows");
+    const int64_t k = x.size(1), kb = (k + 127) / 128;
+    need(xs.dim() == 2 && xs.scalar_type() == at::kFloat && xs.size(0) == x.size(0) && xs.size(1) == kb &&
+             (xs.stride(1) == 1 || kb <= 1),
+         "x_scales must be an fp32 tensor [rows, ceil(k / 128)] with contiguous rows");
+    const int64_t dims = (offsets ? 3 : 2) + lead;
+    need(w.scalar_type() == at::kFloat8_e4m3fn && w.dim() == dims && w.is_contiguous() && w.size(dims - 1) == k &&
+             (!lead || w.size(dims - 3) == 2),
+         lead ? "w must be a contiguous float8_e4m3fn tensor [2, n, k], or [groups, 2, n, k] with offsets"
+              : "w must be a contiguous float8_e4m3fn tensor [n, k], or [groups, n, k] with offsets");
+    const int64_t n = w.size(dims - 2), nb = (n + 127) / 128, groups = offsets ? w.size(0) : 1;
+    need(ws.scalar_type() == at::kFloat && ws.dim() == dims && ws.is_contiguous() && ws.size(dims - 1) == kb &&
+             ws.size(dims - 2) == nb && (!lead || ws.size(dims - 3) == 2) && (!offsets || ws.size(0) == groups),
+         "w_scales must be a contiguous fp32 tensor of w's shape with a value for each 128 x 128 block");
+    need(!offsets || offsets->numel() == groups + 1, "offsets must have one value more than w has groups");
+    need(rows ? rows->numel() == n_rows : x.size(0) == n_rows, "there must be one row of x, or of rows, for each output row");
+    p.x = x.data_ptr(), p.x_scales = xs.data_ptr<float>(), p.w = w.data_ptr(), p.w_scales = ws.data_ptr<float>();
+    p.offsets = offsets ? offsets->data_ptr<int>() : nullptr, p.rows = rows ? rows->data_ptr<int>() : nullptr;
+    p.x_stride = x.stride(0), p.x_scales_stride = xs.stride(0);
+    p.n_x = fits(x.size(0), "the number of rows"), p.n_rows = fits(n_rows, "the number of rows"), p.n = fits(n, "n");
+    p.k = fits(k, "k"), p.n_groups = fits(groups, "the number of groups");
+    p.status = status ? status->data_ptr<int>() : nullptr;
+}
+const at::Tensor* maybe_ints(PyObject* o, const char* what) { return o == Py_None ? nullptr : &vector_of(o, at::kInt, what); }
+
+// (x, x_scales, w, w_scales, out, offsets, rows, status, stream)
+PyObject* linear_q8(PyObject*, PyObject* const* a, Py_ssize_t given) {
+    return guarded(given, 9, [&] {
+        const at::Tensor &x = tensor(a[0], "x"), &xs = tensor(a[1], "x_scales"), &w = tensor(a[2], "w"),
+                         &ws = tensor(a[3], "w_scales"), &out = tensor(a[4], "out");
+        const at::Tensor *offsets = maybe_ints(a[5], "offsets"), *rows = maybe_ints(a[6], "rows"),
+                         *status = maybe_ints(a[7], "status");
+        DracoLinearQ8 p{};
+        need(out.dim() == 2 && dtype_of(out) >= 0 && (out.stride(1) == 1 || out.size(1) <= 1),
+             "out must be a floating tensor [rows, n] with contiguous rows");
+        q8_operands(p, x, xs, w, ws, offsets, rows, status, 1, out.size(0));
+        need(out.size(1) == p.n, "out must have a column for each of w's rows");
+        const at::Device dev = x.device();
+        need(x.is_cuda(), "tensors must be on the GPU");
+        for (const at::Tensor* t : {&xs, &w, &ws, &out, offsets, rows, status})
+            need(!t || t->device() == dev, "tensors must be on one device");
+        need(!status || status->numel() > 0, "status must have a value");
+        const OnDevice on(dev);
+        p.out = out.data_ptr(), p.out_stride = out.stride(0), p.dtype = dtype_of(out);
+        return done(f_linear(&p, stream_of(a[8], dev)), "draco_b200_linear_q8");
+    });
+}
+
+// (x, x_scales, w, w_scales, codes, scales, offsets, rows, status, stream)
+PyObject* swiglu_q8(PyObject*, PyObject* const* a, Py_ssize_t given) {
+    return guarded(given, 10, [&] {
+        const at::Tensor &x = tensor(a[0], "x"), &xs = tensor(a[1], "x_scales"), &w = tensor(a[2], "w"),
+                         &ws = tensor(a[3], "w_scales"), &codes = tensor(a[4], "codes"), &scales = tensor(a[5], "scales");
+        const at::Tensor *offsets = maybe_ints(a[6], "offsets"), *rows = maybe_ints(a[7], "rows"),
+                         *status = maybe_ints(a[8], "status");
+        DracoLinearQ8 p{};
+        need(codes.dim() == 2 && codes.scalar_type() == at::kFloat8_e4m3fn && (codes.stride(1) == 1 || codes.size(1) <= 1),
+             "codes must be a float8_e4m3fn tensor [rows, n] with contiguous rows");
+        q8_operands(p, x, xs, w, ws, offsets, rows, status, 2, codes.size(0));
+        const int64_t nb = (p.n + 127) / 128;
+        need(codes.size(1) == p.n, "codes must have a column for each of w's rows");
+        need(scales.dim() == 2 && scales.scalar_type() == at::kFloat && scales.size(0) == codes.size(0) &&
+                 scales.size(1) == nb && (scales.stride(1) == 1 || nb <= 1),
+             "scales must be an fp32 tensor [rows, ceil(n / 128)] with contiguous rows");
+        const at::Device dev = x.device();
+        need(x.is_cuda(), "tensors must be on the GPU");
+        for (const at::Tensor* t : {&xs, &w, &ws, &codes, &scales, offsets, rows, status})
+            need(!t || t->device() == dev, "tensors must be on one device");
+        need(!status || status->numel() > 0, "status must have a value");
+        const OnDevice on(dev);
+        p.out = codes.data_ptr(), p.out_stride = codes.stride(0), p.swiglu = 1;
+        p.out_scales = scales.data_ptr<float>(), p.out_scales_stride = scales.stride(0);
+        return done(f_linear(&p, stream_of(a[9], dev)), "draco_b200_swiglu_q8");
+    });
+}
+
+// (order, first, offsets, rows, pos, stream)
+PyObject* plan_experts(PyObject*, PyObject* const* a, Py_ssize_t given) {
+    return guarded(given, 6, [&] {
+        const at::Tensor &order = tensor(a[0], "order"), &offsets = vector_of(a[2], at::kInt, "offsets"),
+                         &rows = vector_of(a[3], at::kInt, "rows"), &pos = tensor(a[4], "pos");
+        need(order.dim() == 2 && order.scalar_type() == at::kInt && order.is_cuda() && order.is_contiguous(),
+             "order must be a contiguous int32 tensor [tokens, used] on the GPU");
+        need(pos.dim() == 2 && pos.scalar_type() == at::kInt && pos.is_contiguous() && pos.size(1) == order.size(1) &&
+                 pos.size(0) >= order.size(0) && rows.numel() >= order.numel() && offsets.numel() >= 2,
+             "the plan must be for as many tokens, and for as many experts a token");
+        const at::Device dev = order.device();
+        for (const at::Tensor* t : {&offsets, &rows, &pos}) need(t->device() == dev, "tensors must be on one device");
+        const OnDevice on(dev);
+        return done(f_plan_experts(order.data_ptr<int>(), fits(order.size(0), "the number of tokens"),
+                                   fits(order.size(1), "used"), small(a[1], "first"),
+                                   fits(offsets.numel() - 1, "the number of experts"), offsets.data_ptr<int>(),
+                                   rows.data_ptr<int>(), pos.data_ptr<int>(), stream_of(a[5], dev)),
+                    "draco_b200_plan_experts");
+    });
+}
+
+// (y, pos, weights, out, add, stream)
+PyObject* combine_experts(PyObject*, PyObject* const* a, Py_ssize_t given) {
+    return guarded(given, 6, [&] {
+        const at::Tensor &y = tensor(a[0], "y"), &pos = tensor(a[1], "pos"), &w = tensor(a[2], "weights"),
+                         &out = tensor(a[3], "out");
+        const at::Tensor* add = maybe(a[4], "add");
+        const int dtype = dtype_of(out);
+        need(dtype >= 0 && out.is_cuda() && out.dim() == 2, "out must be a floating tensor [tokens, hidden] on the GPU");
+        const int64_t n = out.size(0), hidden = out.size(1);
+        for (const at::Tensor* t : {&y, &out, add})
+            need(!t || (t->dim() == 2 && t->scalar_type() == out.scalar_type() && t->size(1) == hidden &&
+                        (t->stride(1) == 1 || hidden <= 1)),
+                 "y, out and add must be of one type and width, with contiguous rows");
+        need(!add || add->size(0) == n, "add must have out's shape");
+        need(pos.dim() == 2 && pos.scalar_type() == at::kInt && pos.size(0) == n && (pos.stride(1) == 1 || pos.size(1) <= 1) &&
+                 w.dim() == 2 && w.scalar_type() == at::kFloat && w.sizes() == pos.sizes() &&
+                 (w.stride(1) == 1 || w.size(1) <= 1),
+             "pos (int32) and weights (fp32) must be [tokens, used] with contiguous rows");
+        const at::Device dev = out.device();
+        for (const at::Tensor* t : {&y, &pos, &w, add}) need(!t || t->device() == dev, "tensors must be on one device");
+        const OnDevice on(dev);
+        DracoCombineExperts p{};
+        p.y = y.data_ptr(), p.pos = pos.data_ptr<int>(), p.weights = w.data_ptr<float>();
+        p.add = add ? add->data_ptr() : nullptr, p.out = out.data_ptr();
+        p.y_stride = y.stride(0), p.pos_stride = pos.stride(0), p.weights_stride = w.stride(0);
+        p.add_stride = add ? add->stride(0) : 0, p.out_stride = out.stride(0);
+        p.n_y = fits(y.size(0), "the number of rows"), p.n_tokens = fits(n, "the number of tokens");
+        p.n_used = fits(pos.size(1), "used"), p.hidden = fits(hidden, "hidden"), p.dtype = dtype;
+        return done(f_combine(&p, stream_of(a[5], dev)), "draco_b200_combine_experts");
+    });
+}
+
 using Fast = PyObject* (*)(PyObject*, PyObject* const*, Py_ssize_t);
 PyCFunction as_method(Fast f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)); }
 PyMethodDef g_methods[] = {{"setup", as_method(setup), METH_FASTCALL, nullptr},
@@ -319,6 +458,10 @@ PyMethodDef g_methods[] = {{"setup", as_method(setup), METH_FASTCALL, nullptr},
                            {"kv4_read", as_method(kv4_read), METH_FASTCALL, nullptr},
                            {"kv4_attend", as_method(kv4_attend), METH_FASTCALL, nullptr},
                            {"rmsnorm_q8", as_method(rmsnorm_q8), METH_FASTCALL, nullptr},
+                           {"linear_q8", as_method(linear_q8), METH_FASTCALL, nullptr},
+                           {"swiglu_q8", as_method(swiglu_q8), METH_FASTCALL, nullptr},
+                           {"plan_experts", as_method(plan_experts), METH_FASTCALL, nullptr},
+                           {"combine_experts", as_method(combine_experts), METH_FASTCALL, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_decoder", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

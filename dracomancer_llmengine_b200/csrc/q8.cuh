@@ -1,0 +1,65 @@
+// Arguments and launchers of the 8-bit products (e4m3 rows and weights with block scales) and of the operators that sort a
+// batch by expert and add the experts' rows up again.
+#pragma once
+#include "kv4.cuh"
+
+namespace draco {
+
+constexpr int kQ8Block = 128;       // inner values, and rows of a weight, that share a scale
+constexpr int kQ8MaxGroups = 1024;
+
+// Row m of group g: out[m] = x[rows ? rows[m] : m] . w[g]^T, block by block of the inner size with both scales.
+// swiglu: w[g] holds two matrices, gate and up; out are e4m3 codes and out_scales theirs.
+struct Q8Args {
+    const uint8_t* x;           // [n_x][k], rows x_row bytes apart
+    const float* xs;            // [n_x][k_blocks], rows xs_row floats apart
+    const uint8_t* w;           // [groups][1 or 2][n][k]
+    const float* ws;            // [groups][1 or 2][n_blocks][k_blocks]
+    const int* offsets;         // [groups + 1], or null: one group of all rows
+    const int* rows;            // [n_rows], or null
+    void* out;                  // [n_rows][n], rows out_row elements apart
+    float* out_scales;          // [n_rows][n_blocks], rows os_row apart (swiglu)
+    long x_row, xs_row, out_row, os_row;
+    int n_x, n_rows, n, k, groups;
+    int dtype;                  // of out (products)
+    bool swiglu;
+    int* status;                // or null: waits that ran out are noted there
+    long wait_ns;               // their limit
+    int test_extra;             // 1, 2, 3: an arrival that never comes is expected at a barrier (tests)
+};
+// false: a CUDA call before the launch failed
+bool launch_q8(const Q8Args& a, cudaStream_t s);
+bool q8_tc_fits(const Q8Args& a);
+bool launch_q8_tc(const Q8Args& a, cudaStream_t s);
+
+// a group's rows; offsets that are out of order or out of range give fewer rows, never one outside the output
+struct Q8Span {
+    int first, count;
+};
+__device__ __forceinline__ Q8Span q8_span(const int* offsets, int g, int n_rows) {
+    if (!offsets) return Q8Span{0, n_rows};
+    const int a = min(max(offsets[g], 0), n_rows), b = min(max(offsets[g + 1], a), n_rows);
+    return Q8Span{a, b - a};
+}
+
+struct PlanExpertsArgs {
+    const int* order;           // [n]
+    int* offsets;               // [experts + 1]
+    int *rows, *pos;            // [n]
+    int n, used, experts, first;
+};
+constexpr int kPlanMaxExperts = 1024;
+bool launch_plan_experts(const PlanExpertsArgs& a, cudaStream_t s);
+
+struct CombineArgs {
+    const void* y;              // [n_y][hidden]
+    const int* pos;             // [tokens][used]
+    const float* weights;       // [tokens][used]
+    const void* add;            // [tokens][hidden] or null
+    void* out;                  // [tokens][hidden]
+    long y_row, add_row, out_row, pos_row, w_row;
+    int n_y, tokens, used, hidden, dtype;
+};
+void launch_combine_experts(const CombineArgs& a, cudaStream_t s);
+
+}  // namespace draco

@@ -1,6 +1,8 @@
 """Operators of a decoder layer around the MoE FFN, on torch CUDA tensors: page allocation and slot maps
-(:func:`plan_blocks`), a 4-bit paged KV cache (:class:`KV4Cache`: append, read, attend) and the residual RMS norm with
-8-bit output (:func:`rmsnorm_q8`).
+(:func:`plan_blocks`), a 4-bit paged KV cache (:class:`KV4Cache`: append, read, attend), the residual RMS norm with
+8-bit output (:func:`rmsnorm_q8`), and products of such rows with e4m3 weights: projections and experts' products
+(:func:`linear_q8`), gate/up products with SwiGLU and 8-bit output (:func:`swiglu_q8`), the plan that sorts a batch by expert
+(:func:`plan_experts`) and the weighted sum of the experts' rows (:func:`combine_experts`).
 
 Every call is asynchronous on `stream` (default: torch's current stream of the tensors' device), writes into tensors that
 the caller owns and can be captured in a CUDA graph.  Wrong arguments raise :class:`DracoError` before anything is
@@ -13,6 +15,14 @@ One decode step of a layer:
     cache.append(k, v, plan.slots)
     cache.attend(q, out, plan.cu_new, plan.seq_len, table, max_q_len, max_seq_len)
     rmsnorm_q8(proj, w_ffn, eps, codes, scales, residual=res, h=res, y=y)   # then forward(layer, y, ...)
+
+With e4m3 weights the projections are linear_q8 of the norm's codes (float8_e4m3fn, group 128), and the experts, with
+order and weights [tokens, used] from the router:
+
+    plan_experts(order, plan)
+    swiglu_q8(codes, scales, w_gate_up, w_gate_up_scales, act, act_scales, offsets=plan.offsets, rows=plan.rows)
+    linear_q8(act, act_scales, w_down, w_down_scales, rows_out, offsets=plan.offsets)
+    combine_experts(rows_out, plan.pos, weights, out, add=shared)
 """
 from __future__ import annotations
 
@@ -32,13 +42,15 @@ if _decoder.torch_version != torch.__version__:
     raise DracoError(f"the operators' extension was built for torch {_decoder.torch_version}, this is {torch.__version__}: "
                      "build it again with `python -m dracomancer_llmengine_b200.build`")
 
-__all__ = ["BlockPlan", "plan_blocks", "KV4Cache", "rmsnorm_q8"]
+__all__ = ["BlockPlan", "plan_blocks", "KV4Cache", "rmsnorm_q8", "linear_q8", "swiglu_q8", "ExpertPlan", "plan_experts",
+           "combine_experts"]
 
 # the extension checks arguments and calls the entry points of the library that this package loaded
 _decoder.setup(DracoError, {name: ct.cast(getattr(lib(), name), ct.c_void_p).value for name in (
     "draco_b200_last_error", "draco_b200_plan_blocks", "draco_b200_kv4_append", "draco_b200_kv4_read",
     "draco_b200_kv4_attention_workspace", "draco_b200_kv4_attention_checked", "draco_b200_rmsnorm_q8",
-    "draco_b200_pointers_checked", "draco_b200_capture_id")})
+    "draco_b200_pointers_checked", "draco_b200_capture_id", "draco_b200_linear_q8", "draco_b200_plan_experts",
+    "draco_b200_combine_experts")})
 
 # Scratch for attention whose long axis is split over blocks.  Eager calls on a stream run one after the other and share
 # its buffer, whichever cache they read; the calls of a graph capture have a buffer of that capture and stream, which the
@@ -181,3 +193,56 @@ def rmsnorm_q8(x, weight, eps: float, codes, scales, residual=None, h=None, y=No
     With `residual` the norm is that of h = x + residual, stored in `h` (which may be x or residual itself).  `y`
     (optional, x's type) gets the normalised row unquantised, for the router and whatever else takes full precision."""
     _decoder.rmsnorm_q8(x, weight, eps, codes, scales, residual, h, y, group, _stream(stream))
+
+
+def linear_q8(x, x_scales, w, w_scales, out, offsets=None, rows=None, stream=None, status=None):
+    """Products of e4m3 rows and weights with block scales, as :func:`rmsnorm_q8` writes the rows (float8_e4m3fn, group 128):
+    out[m, n] = sum over blocks b of 128 of x_scales[m, b] * w_scales[n // 128, b] * (x[m, b] . w[n, b]).
+
+    x [rows, k] float8_e4m3fn, x_scales fp32 [rows, ceil(k / 128)]; w [n, k] and w_scales [ceil(n / 128), ceil(k / 128)],
+    contiguous; out [rows, n] fp32, fp16 or bf16 (sums are fp32, rounded once).
+    With `offsets` (int32 [groups + 1], on the GPU, not falling) w is [groups, n, k]: group g's weight is for rows
+    offsets[g] .. offsets[g + 1], and rows from offsets[groups] on are left as they were.  With `rows` (int32, one for each
+    row of out) row m takes row rows[m] of x; it is zero where rows[m] is none of x's.
+    Rows of x and weights that start on 16 bytes (k % 16 == 0) take the tensor cores, others a slow form.
+    status (int32 [1], optional): bits are set in it if a wait inside the kernel ran out (2 s); the rows concerned are NaN."""
+    _decoder.linear_q8(x, x_scales, w, w_scales, out, offsets, rows, status, _stream(stream))
+    return out
+
+
+def swiglu_q8(x, x_scales, w, w_scales, codes, scales, offsets=None, rows=None, stream=None, status=None):
+    """Gate and up products, silu(gate) * up, and its 8-bit form, in one call: the rows of the next :func:`linear_q8`.
+
+    As :func:`linear_q8`, with the two weights in w [2, n, k] (or [groups, 2, n, k]: gate, then up) and w_scales
+    [.., 2, ceil(n / 128), ceil(k / 128)]; codes float8_e4m3fn [rows, n] and scales fp32 [rows, ceil(n / 128)]: with a the
+    largest magnitude of a row's 128 values, the codes are e4m3(value * (448 / a)) and the scale is a / 448."""
+    _decoder.swiglu_q8(x, x_scales, w, w_scales, codes, scales, offsets, rows, status, _stream(stream))
+    return codes, scales
+
+
+class ExpertPlan:
+    """What :func:`plan_experts` writes for up to `max_tokens` tokens of `n_used` experts each, of `n_experts` that the caller
+    has: `offsets` [n_experts + 1], `rows` [max_tokens * n_used], `pos` [max_tokens, n_used]; all int32."""
+
+    def __init__(self, max_tokens: int, n_used: int, n_experts: int, device="cuda"):
+        make = lambda *n: torch.zeros(*n, dtype=torch.int32, device=device)  # noqa: E731
+        self.offsets, self.rows, self.pos = make(n_experts + 1), make(max_tokens * n_used), make(max_tokens, n_used)
+
+
+def plan_experts(order, plan: ExpertPlan, first: int = 0, stream=None):
+    """Sort the assignments order (int32 [tokens, used], expert ids) by expert, tokens in order within each.
+
+    plan.offsets[e] .. plan.offsets[e + 1] are the places of expert first + e; plan.rows has the token of each place (from
+    the last expert's end on it is left as it was), plan.pos the place of each assignment, -1 for experts outside
+    first .. first + n_experts."""
+    _decoder.plan_experts(order, first, plan.offsets, plan.rows, plan.pos, _stream(stream))
+    return plan
+
+
+def combine_experts(y, pos, weights, out, add=None, stream=None):
+    """out[t] = add[t] + sum over k of weights[t, k] * y[pos[t, k]]: fp32 sums in the order of k, one rounding.
+
+    y [rows, hidden], out and add (optional, may be out) [tokens, hidden] of one type; pos int32 and weights fp32
+    [tokens, used].  Places outside y, such as -1, count as nothing."""
+    _decoder.combine_experts(y, pos, weights, out, add, _stream(stream))
+    return out

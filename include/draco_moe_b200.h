@@ -334,7 +334,8 @@ int draco_b200_gemv_q8k(int code, const uint8_t* W, int rows, int n_in, const in
 /* ============================ Part 3: decoder-layer operators ============================
  *
  * What a decoder layer needs around the MoE FFN on the same GPU: page allocation and slot maps, a 4-bit paged KV cache,
- * attention over it, and the residual RMS norm with 8-bit output.  No counterpart in the reference.  All pointers are
+ * attention over it, the residual RMS norm with 8-bit output, and products of such 8-bit rows with 8-bit weights, by expert
+ * too.  No counterpart in the reference.  All pointers are
  * device memory; every call is asynchronous on `stream` (null: the legacy default stream), allocates nothing and can be captured in a CUDA graph.  Returns 0, -1 (arguments; nothing was launched) or
  * -3 (CUDA error), with the text in draco_b200_last_error().  Element types (dtype): 0 fp32, 1 fp16, 2 bf16. */
 
@@ -431,6 +432,58 @@ typedef struct DracoNormQ8 {
     float eps;
 } DracoNormQ8;
 int draco_b200_rmsnorm_q8(const DracoNormQ8* args, void* stream);
+
+/* Products of rows and weights in 8-bit floating point (e4m3) with block scales, of which rmsnorm_q8 writes the rows
+ * (fmt 1, group 128).  With blocks of 128,
+ *   out[m][n] = sum over b of x_scales[r][b] * w_scales[g][n / 128][b] * (sum over k of block b of x[r][k] * w[g][n][k])
+ * x: [n_x][k] codes, w: [n_groups][n][k], w_scales: [n_groups][ceil(n / 128)][ceil(k / 128)], both contiguous; x_scales:
+ * [n_x][ceil(k / 128)]; strides of rows in elements.  Sums are fp32, rounded once to dtype.
+ * offsets (n_groups + 1 values, not falling; null: one group of all n_rows rows): group g's rows are offsets[g] ..
+ * offsets[g + 1] of the output, and no row from offsets[n_groups] on is written.  rows (or null: r = m): row m of the output
+ * takes row r = rows[m] of x; it is zero where rows[m] is none of x's.
+ * swiglu: w[g] holds two matrices, gate and up ([n_groups][2][n][k]; scales [n_groups][2][ceil(n / 128)][ceil(k / 128)]);
+ * with h = gate / (1 + exp(-gate)) * up and a the largest |h| of a row's 128 columns, out is e4m3(h * (448 / a)) and
+ * out_scales [n_rows][ceil(n / 128)] a / 448: rows for the next product.  a < 2^-100: code and scale 0; an infinity or NaN
+ * in the block: the scale is NaN.
+ * At most 1024 groups, n, k, n_rows and n_x at most 2^24.  x, its rows' stride and w in whole 16 bytes (k % 16 == 0) take the tensor cores,
+ * anything else a slow form.  status, wait_limit_us: as in draco_b200_kv4_attention_checked (rows of a block whose waits
+ * ran out are NaN). */
+typedef struct DracoLinearQ8 {
+    const void* x;
+    const float* x_scales;
+    const void* w;
+    const float* w_scales;
+    const int *offsets, *rows;
+    void* out;
+    float* out_scales;
+    long x_stride, x_scales_stride, out_stride, out_scales_stride;
+    int n_x, n_rows, n, k, n_groups, dtype, swiglu;
+    int* status;
+    int wait_limit_us;
+} DracoLinearQ8;
+int draco_b200_linear_q8(const DracoLinearQ8* args, void* stream);
+
+/* Sorts the assignments order[n_tokens][n_used] (expert ids as the router gives them) by expert: those of experts first ..
+ * first + n_experts, the slice that the caller has, in token order within each.
+ *   offsets[n_experts + 1]   where each expert's rows start
+ *   rows[n_tokens * n_used]  the token of each sorted assignment; entries from offsets[n_experts] on are left as they were
+ *   pos[n_tokens * n_used]   where each assignment went, -1 for experts outside the slice
+ * At most 1024 experts and 2^24 assignments.  One launch, no workspace. */
+int draco_b200_plan_experts(const int* order, int n_tokens, int n_used, int first, int n_experts, int* offsets, int* rows,
+                            int* pos, void* stream);
+
+/* out[t] = add[t] + sum over k ascending of weights[t][k] * y[pos[t][k]] (hidden values each, fp32 sums, one rounding to
+ * dtype; add may be null and may be out; pos entries outside 0 .. n_y count as nothing). */
+typedef struct DracoCombineExperts {
+    const void* y;
+    const int* pos;
+    const float* weights;
+    const void* add;
+    void* out;
+    long y_stride, pos_stride, weights_stride, add_stride, out_stride;
+    int n_y, n_tokens, n_used, hidden, dtype;
+} DracoCombineExperts;
+int draco_b200_combine_experts(const DracoCombineExperts* args, void* stream);
 
 #ifdef __cplusplus
 }
