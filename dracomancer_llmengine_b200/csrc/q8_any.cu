@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(kN) q8_any_kernel(const Call c) {
 }  // namespace
 
 bool launch_q8(const Q8Args& a, cudaStream_t s) {
+    if (q8_tc_fits(a)) return launch_q8_tc(a, s);
     Call c{a, 0};
     c.n_tiles = a.swiglu ? (a.n + kQ8Block - 1) / kQ8Block : (a.n + kN - 1) / kN;
     const long slots = (a.n_rows + kM - 1) / kM + (a.offsets ? std::min(a.groups, a.n_rows) : 0);   // a group adds one short tile at most

@@ -470,3 +470,34 @@ def test_stream_argument():
         decoder.linear_q8(x, xs, w, ws, out, stream=stream)
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("which,bits", [(1, 0x101), (2, 0x102), (3, 0x104)])
+@pytest.mark.parametrize("rows,n", [(5, 256), (300, 512)])
+def test_waits_that_run_out(rows, n, which, bits, swiglu):
+    """Barriers of the tensor-core form that expect an arrival which never comes: the call ends, its rows are NaN, the status
+    says which wait it was (others may have run out with it), and the next call is right."""
+    if which == 3 and not swiglu:
+        pytest.skip("the product has no join")
+    x, xs, w, ws = operands(rows, 256, n, gen_of(which), (2,) if swiglu else ())
+    status = ints(0)
+    a = dm.DracoLinearQ8(x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), n_x=rows, n_rows=rows, n=n, k=256, n_groups=1,
+                         x_stride=256, x_scales_stride=2, out_stride=n, swiglu=int(swiglu), status=status.data_ptr(), wait_limit_us=2000)
+    out, scales = torch.zeros(rows, n, dtype=torch.uint8 if swiglu else torch.float32, device=DEV), torch.zeros(rows, cdiv(n, 128), device=DEV)
+    a.out, a.out_scales, a.out_scales_stride = out.data_ptr(), scales.data_ptr(), scales.shape[1]
+    L = dm.lib()
+    torch.cuda.synchronize()
+    assert L.draco_b200_test_q8_barrier_extra(which) == 0
+    try:
+        assert L.draco_b200_linear_q8(a, None) == 0
+    finally:
+        assert L.draco_b200_test_q8_barrier_extra(0) == which
+    torch.cuda.synchronize()
+    assert int(status) & bits == bits
+    assert (scales if swiglu else out).isnan().all()
+    assert L.draco_b200_linear_q8(a, None) == 0
+    torch.cuda.synchronize()
+    assert not (scales if swiglu else out).isnan().any()
+    if not swiglu:
+        same(out, *plain(x, xs, w, ws), "f32")
