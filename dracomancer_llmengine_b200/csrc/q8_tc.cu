@@ -35,16 +35,17 @@ namespace {
 
 using sync::smem_addr;
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 384, kStagingWarp = 1024;
 constexpr int kStatusOperands = 1, kStatusProduct = 2, kStatusJoin = 4, kStatusBuffer = 8, kStatusStage = 16;
 constexpr float kTiny = 7.888609e-31f;   // 2^-100
 constexpr int kSmemMost = 227 * 1024;
 
 struct Call {
-    CUtensorMap x, w;
+    CUtensorMap x, xt, w;       // x in boxes of 32 rows (of one, where rows are given by index) and of 128
     Q8Args a;
     int n_tiles;        // column tiles (with SwiGLU: of 128 columns)
     int vec;            // rows of the output start on 16 bytes
+    int vec_xs;         // and those of x's scales
 };
 
 template <int MT, int NT, bool SW>
@@ -53,9 +54,10 @@ struct Cfg {
     static constexpr int kA = MT * 128, kB = NT * 128, kStage = kA + kB;
     static constexpr int kBuffers = NT == 256 ? 2 : NT == 128 ? 4 : 8;
     static constexpr int kColumns = NT * kBuffers;                      // a power of two, 128 to 512
-    static constexpr int kActive = MT == 128 ? 8 : 2;                   // consumer warps that have rows
-    static constexpr int kStaging = kActive * 32 * 64;
-    static constexpr int kTops = SW ? 2 * kCluster * 2 * MT * 4 : 0;    // two tiles' maxima, of each half of each block
+    static constexpr int kParts = 2;                                    // warps that share a row's columns
+    static constexpr int kActive = MT / 32 * kParts;                    // consumer warps that have rows
+    static constexpr int kStaging = kActive * kStagingWarp;
+    static constexpr int kTops = SW ? 2 * kCluster * kParts * MT * 4 : 0;   // two tiles' maxima, of each part of each block
     static constexpr int kMisc = 2048 + 2 * 4 * (kQ8MaxGroups + 1);
     // the product reads 128 rows from a stage of MT: what lies behind the ring has to be there
     static constexpr int kPad = kStaging + kTops + kMisc >= 16384 ? 0 : 16384;
@@ -87,8 +89,8 @@ struct Groups {
 };
 
 // bounded wait; false: the limit ran out here (noted in *fail) or somewhere else in the block before
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* fail, long limit, int code) {
-    if (sync::mbar_try(bar, parity)) return true;
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* fail, long limit, int code, bool ready = false) {
+    if (ready || sync::mbar_try(bar, parity)) return true;
     const uint64_t t0 = sync::global_ns();
     for (uint32_t i = 1;; i++) {
         if (sync::mbar_try(bar, parity)) return true;
@@ -100,6 +102,15 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
             }
         }
     }
+}
+// whether the phase is over, without waiting
+__device__ __forceinline__ bool test_bar(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(smem_addr(bar)), "r"(parity)
+                 : "memory");
+    return ok != 0;
 }
 __device__ __forceinline__ bool try_cluster(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
@@ -118,11 +129,11 @@ __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x,
         "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
         : "memory");
 }
-__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int u, uint64_t* bar) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
             smem_addr(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(smem_addr(bar))
         : "memory");
 }
 __device__ __forceinline__ void tma_gather(void* dst, const CUtensorMap* map, int x, int4 rows, uint64_t* bar) {
@@ -143,10 +154,12 @@ __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint3
 
 template <int N>
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&v)[N]) {
-    if constexpr (N == 16) {
+    if constexpr (N == 32) {
+        tc_ld32(addr, v);
+    } else if constexpr (N == 16) {
         tc_ld16(addr, v);
     } else {
-        static_assert(N == 8, "8 or 16 columns");
+        static_assert(N == 8, "8, 16 or 32 columns");
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                      : "r"(addr)
@@ -154,39 +167,45 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&v)[N]) {
     }
 }
 
-// two fp32 values of a register pair
-__device__ __forceinline__ uint64_t pair(uint32_t a, uint32_t b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ float2 split(uint64_t v) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-    return f;
-}
-__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t a, uint64_t b) {
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
-}
-
-// acc += scale * the block's product, for COLS columns from `addr`; the next piece is on its way while one is added
-template <int COLS>
-__device__ __forceinline__ void add_block(uint64_t (&acc)[COLS / 2], uint32_t addr, float scale) {
-    constexpr int C = COLS < 16 ? COLS : 16, N = COLS / C;
-    const uint64_t s = pair(__float_as_uint(scale), __float_as_uint(scale));
+// acc += scale * the block's product, for COLS columns from `addr`; the next piece is on its way while one is added.  `read`
+// is called when the last one has arrived.
+#ifndef Q8_PIECE
+#define Q8_PIECE 32
+#endif
+template <int COLS, typename F>
+__device__ __forceinline__ void add_block(float2 (&acc)[COLS / 2], uint32_t addr, float scale, F&& read) {
+    constexpr int C = COLS < Q8_PIECE ? COLS : Q8_PIECE, N = COLS / C;
+    const float2 s = make_float2(scale, scale);
     uint32_t v[2][C];
     tmem_load<C>(addr, v[0]);
 #pragma unroll
     for (int i = 0; i < N; i++) {
         tc_wait_ld();
         if (i + 1 < N) tmem_load<C>(addr + (i + 1) * C, v[(i + 1) & 1]);
+        else read();
 #pragma unroll
-        for (int j = 0; j < C / 2; j++) fma2(acc[i * (C / 2) + j], pair(v[i & 1][2 * j], v[i & 1][2 * j + 1]), s);
+        for (int j = 0; j < C / 2; j++)
+            acc[i * (C / 2) + j] = __ffma2_rn(make_float2(__uint_as_float(v[i & 1][2 * j]), __uint_as_float(v[i & 1][2 * j + 1])), s,
+                                              acc[i * (C / 2) + j]);
     }
 }
 
-// 32 rows of BYTES bytes, one a lane, to memory in pieces of 16 bytes side by side (through the warp's staging buffer: 64 bytes
-// a row, the piece's place turned by the row so that eight rows' pieces lie in different banks)
+// up to 16 bytes of a row, `left` of which are inside it
+__device__ __forceinline__ void store_piece(uint8_t* p, const uint8_t* src, long left, bool vec, int elem) {
+    if (vec && left >= 16) {
+        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(src);
+        return;
+    }
+    for (int e = 0; e < 16; e += elem) {
+        if (e >= left) break;
+        if (elem == 4) *reinterpret_cast<uint32_t*>(p + e) = *reinterpret_cast<const uint32_t*>(src + e);
+        else if (elem == 2) *reinterpret_cast<uint16_t*>(p + e) = *reinterpret_cast<const uint16_t*>(src + e);
+        else p[e] = src[e];
+    }
+}
+
+// 32 rows of BYTES bytes, one a lane, to memory in pieces of 16 bytes side by side, through the warp's staging buffer (1 KB; a
+// piece's place is turned by its row, so that eight rows' pieces lie in different banks)
 template <int BYTES>
 __device__ __forceinline__ void store_rows(uint8_t* staging, int lane, const uint32_t (&v)[BYTES / 4], uint8_t* out, long row_bytes,
                                            int rows, long left, bool vec, int elem) {
@@ -194,43 +213,39 @@ __device__ __forceinline__ void store_rows(uint8_t* staging, int lane, const uin
         if (lane >= rows) return;
         uint8_t* p = out + lane * row_bytes;
         if (vec && left >= BYTES) {
-            *reinterpret_cast<uint2*>(p) = make_uint2(v[0], v[1]);
-        } else {
+#pragma unroll
+            for (int i = 0; i < BYTES / 4; i++) reinterpret_cast<uint32_t*>(p)[i] = v[i];
+        } else if (elem == 1) {
 #pragma unroll
             for (int i = 0; i < BYTES; i++)
                 if (i < left) p[i] = (uint8_t)(v[i / 4] >> (8 * (i & 3)));
+        } else {
+#pragma unroll
+            for (int i = 0; i < BYTES / 2; i++)
+                if (2 * i < left) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
         }
     } else {
-        constexpr int P = BYTES / 16;       // pieces of a row
-        __syncwarp();
+        constexpr int P = BYTES / 16, ROWS = P == 4 ? 16 : 32;      // pieces of a row, rows at a time
+        auto place = [](int r, int i) { return (r % ROWS) * BYTES + (P == 4 ? i ^ ((r >> 1) & 3) : P == 2 ? i ^ ((r >> 2) & 1) : i) * 16; };
 #pragma unroll
-        for (int i = 0; i < P; i++)
-            *reinterpret_cast<uint4*>(staging + lane * 64 + ((i ^ ((lane >> 1) & 3)) * 16)) =
-                make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        __syncwarp();
+        for (int r0 = 0; r0 < 32; r0 += ROWS) {
+            __syncwarp();
+            if (lane >= r0 && lane < r0 + ROWS)
 #pragma unroll
-        for (int i = 0; i < P; i++) {
-            const int r = i * (32 / P) + lane / P, c = lane % P;
-            if (r >= rows) continue;
-            const uint8_t* src = staging + r * 64 + ((c ^ ((r >> 1) & 3)) * 16);
-            uint8_t* p = out + r * row_bytes + c * 16;
-            const long here = left - c * 16;
-            if (vec && here >= 16) {
-                *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(src);
-            } else {
-                for (int e = 0; e < 16; e += elem) {
-                    if (e >= here) break;
-                    if (elem == 4) *reinterpret_cast<uint32_t*>(p + e) = *reinterpret_cast<const uint32_t*>(src + e);
-                    else if (elem == 2) *reinterpret_cast<uint16_t*>(p + e) = *reinterpret_cast<const uint16_t*>(src + e);
-                    else p[e] = src[e];
-                }
+                for (int i = 0; i < P; i++)
+                    *reinterpret_cast<uint4*>(staging + place(lane, i)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < ROWS * P / 32; i++) {
+                const int r = r0 + (i * 32 + lane) / P, c = lane % P;
+                if (r < rows) store_piece(out + r * row_bytes + c * 16, staging + place(r, c), left - c * 16, vec, elem);
             }
         }
     }
 }
 
 template <typename T, int COLS>
-__device__ __forceinline__ void store_product(uint8_t* staging, int lane, const uint64_t (&acc)[COLS / 2], bool zero, uint8_t* out,
+__device__ __forceinline__ void store_product(uint8_t* staging, int lane, const float2 (&acc)[COLS / 2], bool zero, uint8_t* out,
                                               long row_bytes, int rows, long left, bool vec) {
     constexpr int S = sizeof(T), C = COLS * S < 64 ? COLS : 64 / S;     // columns of a piece
 #pragma unroll
@@ -238,7 +253,7 @@ __device__ __forceinline__ void store_product(uint8_t* staging, int lane, const 
         uint32_t v[C * S / 4];
 #pragma unroll
         for (int j = 0; j < C / 2; j++) {
-            float2 f = split(acc[i * (C / 2) + j]);
+            float2 f = acc[i * (C / 2) + j];
             if (zero) f = make_float2(0.f, 0.f);
             if constexpr (S == 4) v[2 * j] = __float_as_uint(f.x), v[2 * j + 1] = __float_as_uint(f.y);
             else v[j] = pack2<T>(f.x, f.y);
@@ -257,15 +272,15 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
     float* const tops = (float*)(staging + C::kStaging);
     uint64_t* const full = (uint64_t*)((uint8_t*)tops + C::kTops);
     uint64_t* const empty = full + S;
-    uint64_t* const tfull = empty + S;
-    uint64_t* const tempty = tfull + B;
-    uint64_t* const join = tempty + B;          // [2]
+    uint64_t* const tfull = empty + S;          // [2][B], of the halves of the columns
+    uint64_t* const tempty = tfull + 2 * B;
+    uint64_t* const join = tempty + 2 * B;      // [2]
     uint64_t* const drain = join + 2;
     uint32_t* const s_tmem = (uint32_t*)(drain + 1);
     int* const s_fail = (int*)(s_tmem + 1);
     int* const s_pre = (int*)((uint8_t*)full + 2048);
     int* const s_off = s_pre + kQ8MaxGroups + 1;
-    static_assert((2 * 32 + 2 * 8 + 3) * 8 + 8 <= 2048, "the barriers have their place");
+    static_assert((2 * 32 + 4 * 8 + 3) * 8 + 8 <= 2048, "the barriers have their place");
 
     const Q8Args& a = c.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -273,18 +288,19 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
     early_launch();
     if (warp == 0 && lane == 0) {
         for (int i = 0; i < S; i++) {
-            sync::mbar_init(full + i, 1 + (a.test_extra == 1));
-            sync::mbar_init(empty + i, 1);
+            sync::mbar_init(full + i, 2 + (a.test_extra == 1));
+            sync::mbar_init(empty + i, 2);
         }
-        for (int i = 0; i < B; i++) {
+        for (int i = 0; i < 2 * B; i++) {
             sync::mbar_init(tfull + i, 1 + (a.test_extra == 2));
-            sync::mbar_init(tempty + i, C::kActive);
+            sync::mbar_init(tempty + i, C::kActive / 2);
         }
-        for (int i = 0; i < 2; i++) sync::mbar_init(join + i, CL * 2 * MT + (a.test_extra == 3));
-        sync::mbar_init(drain, 1);
+        for (int i = 0; i < 2; i++) sync::mbar_init(join + i, CL * C::kParts * MT + (a.test_extra == 3));
+        sync::mbar_init(drain, 2);
         *s_fail = 0;
         sync::fence_init();
         asm volatile("prefetch.tensormap [%0];" ::"l"(&c.x) : "memory");
+        if (MT == 128) asm volatile("prefetch.tensormap [%0];" ::"l"(&c.xt) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&c.w) : "memory");
     }
     if (warp == 1) {
@@ -293,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     wait_for_inputs();
-    if (warp == 2) {        // row tiles before each group
+    if (warp == 3) {        // row tiles before each group
         int before = 0;
         for (int g0 = 0; g0 < a.groups; g0 += 32) {
             const int g = g0 + lane;
@@ -326,18 +342,18 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
     volatile int* const fail = s_fail;
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 0) {
-            int stage = 0, g = 0;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 0 || warp == 2) {       // copies of the weight, of x
+            const bool of_x = warp == 2;
+            int stage = 0, g = 0, filled = 0;
             uint32_t parity = 1;
             bool go = true;
-            int filled = 0;
             for (int t = first; go && t < total; t += step) {
                 const Tile tile = groups.at(t, g);
                 const int n0 = SW ? tile.col * kQ8Block + rank * (NT / 2) : tile.col * NT;
                 int4 rows = make_int4(0, 0, 0, 0);
-                int boxes;
-                if (a.rows) {           // a lane fetches four rows
+                int boxes = (tile.rows + 31) / 32;
+                if (of_x && a.rows) {           // a lane fetches four rows
                     int r[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
@@ -346,30 +362,28 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
                     }
                     rows = make_int4(r[0], r[1], r[2], r[3]);
                     boxes = (tile.rows + 3) / 4;
-                } else {
-                    boxes = (tile.rows + 31) / 32;
                 }
-                const uint32_t bytes = (uint32_t)boxes * (a.rows ? 512 : 4096) + C::kB;
+                const uint32_t bytes = of_x ? (uint32_t)boxes * (a.rows ? 512 : 4096) : C::kB;
                 for (int b = 0; b < kb; b++) {
-                    go = wait_bar(empty + stage, parity, fail, a.wait_ns, kStatusStage);
-                    go = __all_sync(0xffffffffu, go);
+                    go = __all_sync(0xffffffffu, wait_bar(empty + stage, parity, fail, a.wait_ns, kStatusStage));
                     if (!go) break;
                     uint8_t* const pa = ring + stage * C::kStage;
-                    uint8_t* const pb = pa + C::kA;
-                    if (lane == 0) {
+                    if (elect_one()) {
                         sync::mbar_expect_tx(full + stage, bytes);
-                        if constexpr (SW) {
-                            tma_3d(pb, &c.w, b * kQ8Block, n0, tile.group * 2, full + stage);
-                            tma_3d(pb + C::kB / 2, &c.w, b * kQ8Block, n0, tile.group * 2 + 1, full + stage);
-                        } else {
-                            tma_3d(pb, &c.w, b * kQ8Block, n0, tile.group, full + stage);
+                        if (!of_x) {
+                            tma_4d(pa + C::kA, &c.w, b * kQ8Block, n0, 0, tile.group, full + stage);
+                            if constexpr (SW)
+                                tma_4d(pa + C::kA + C::kB / 2, &c.w, b * kQ8Block, n0 + NT / 4, 0, tile.group, full + stage);
+                        } else if (!a.rows) {
+                            if (MT == 128 && boxes == 4)
+                                tma_2d(pa, &c.xt, b * kQ8Block, tile.first, full + stage);
+                            else
+                                for (int i = 0; i < boxes; i++)
+                                    tma_2d(pa + i * 4096, &c.x, b * kQ8Block, tile.first + i * 32, full + stage);
                         }
-                        if (!a.rows)
-                            for (int i = 0; i < boxes; i++)
-                                tma_2d(pa + i * 4096, &c.x, b * kQ8Block, tile.first + i * 32, full + stage);
                     }
                     __syncwarp();
-                    if (a.rows && lane < boxes) tma_gather(pa + lane * 512, &c.x, b * kQ8Block, rows, full + stage);
+                    if (of_x && a.rows && lane < boxes) tma_gather(pa + lane * 512, &c.x, b * kQ8Block, rows, full + stage);
                     filled = min(filled + 1, S);
                     if (++stage == S) stage = 0, parity ^= 1;
                 }
@@ -379,25 +393,27 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
                 const uint64_t t0 = sync::global_ns();
                 while (!sync::mbar_try(full + stage, parity ^ 1) && sync::global_ns() - t0 < 10000000ull) {}
             }
-        } else if (warp == 1) {
-            constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        } else {        // products of one half of the weight's rows
+            constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(NT / 2 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+            const int half = warp >> 1;
             int stage = 0, buf = 0;
             uint32_t parity = 0, bparity = 1;
             bool go = true;
             for (int t = first; go && t < total; t += step) {
                 for (int b = 0; b < kb; b++) {
-                    go = wait_bar(tempty + buf, bparity, fail, a.wait_ns, kStatusBuffer) &&
+                    go = wait_bar(tempty + half * B + buf, bparity, fail, a.wait_ns, kStatusBuffer) &&
                          wait_bar(full + stage, parity, fail, a.wait_ns, kStatusOperands);
                     go = __all_sync(0xffffffffu, go);
                     if (!go) break;
                     tc_fence_after();
                     if (elect_one()) {
                         const uint64_t da = sdesc_sw128(smem_addr(ring + stage * C::kStage));
-                        const uint64_t db = sdesc_sw128(smem_addr(ring + stage * C::kStage + C::kA));
+                        const uint64_t db = sdesc_sw128(smem_addr(ring + stage * C::kStage + C::kA + half * (C::kB / 2)));
 #pragma unroll
-                        for (int i = 0; i < 4; i++) mma_f8(tmem + buf * NT, da + 2 * i, db + 2 * i, idesc, i > 0);
+                        for (int j = 0; j < 4; j++)
+                            mma_f8(tmem + buf * NT + half * (NT / 2), da + 2 * j, db + 2 * j, idesc, j > 0);
                         tc_commit(empty + stage);
-                        tc_commit(tfull + buf);
+                        tc_commit(tfull + half * B + buf);
                     }
                     __syncwarp();
                     if (++stage == S) stage = 0, parity ^= 1;
@@ -411,106 +427,111 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
             while (!sync::mbar_try(drain, 0) && sync::global_ns() - t0 < sync::kWaitLimitNs) {}
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-        const int quarter = warp & 3, half = (warp - 4) >> 2;
-        if (quarter * 32 < MT) {
-            constexpr int COLS = NT / 2;                    // of this warp; with SwiGLU half of them gate, half up
-            constexpr int CH = NT >= 128 ? 4 : 8;           // blocks whose scales are fetched together
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        const int quarter = warp & 3, part = (warp - 4) >> 2;
+        if (quarter * 32 < MT && part < C::kParts) {
+            constexpr int COLS = NT / C::kParts;            // of this warp; with SwiGLU half of them gate, half up
+            constexpr int CH = 4;                           // blocks whose scales are fetched together, as many ahead
             const int nb = (a.n + kQ8Block - 1) / kQ8Block;
             const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-            uint8_t* const mine = staging + (MT == 128 ? warp - 4 : half) * 2048;
+            uint8_t* const mine = staging + (part * (MT / 32) + quarter) * kStagingWarp;
+            const int half = part;
+            uint64_t* const hfull = tfull + half * B;
             int buf = 0, g = 0, turn = 0;
             uint32_t parity = 0;
 
-            // scales of the next CH blocks, fetched while the ones before are in use (those of a tile's first blocks during
-            // the end of the tile before)
+            // scales, fetched ahead through the ends of tiles: those of block `at_b` of tile `at_t` come next
             const float *px = nullptr, *pw = nullptr, *pu = nullptr;
-            bool there = false;
-            float nx[CH], nw[CH], nu[CH];
-            auto begin = [&](const Tile& tile) {
-                const int r = quarter * 32 + lane;
-                int src = -1;
-                if (r < tile.rows) src = a.rows ? a.rows[tile.first + r] : tile.first + r;
-                there = src >= 0 && src < a.n_x;
-                px = a.xs + (long)(there ? src : 0) * a.xs_row;
-                if constexpr (SW) {
-                    pw = a.ws + ((long)tile.group * 2 * nb + tile.col) * kb;
-                    pu = pw + (long)nb * kb;
+            int at_t = first, at_b = 0, at_g = 0;
+            float nx[CH], nw = 0.f, nu = 0.f;               // lane i has the weight's scale of block i
+#pragma unroll
+            for (int i = 0; i < CH; i++) nx[i] = 0.f;
+            auto row_of = [&](const Tile& tile) {       // this lane's row of x; outside x: not there
+                const int r = min(quarter * 32 + lane, tile.rows - 1);
+                return a.rows ? a.rows[tile.first + r] : tile.first + r;
+            };
+            auto fetch = [&] {
+                if (at_t >= total) return;
+                if (at_b == 0) {
+                    const Tile tile = groups.at(at_t, at_g);
+                    const int src = row_of(tile);
+                    px = a.xs + (long)(src >= 0 && src < a.n_x ? src : 0) * a.xs_row;
+                    if constexpr (SW) {
+                        pw = a.ws + ((long)tile.group * 2 * nb + tile.col) * kb;
+                        pu = pw + (long)nb * kb;
+                    } else {
+                        pw = a.ws + ((long)tile.group * nb + min(tile.col * NT + part * COLS, a.n - 1) / kQ8Block) * kb;
+                    }
+                }
+                const int mine_b = min(at_b + (lane & (CH - 1)), kb - 1);
+                nw = pw[mine_b];
+                if constexpr (SW) nu = pu[mine_b];
+                if (c.vec_xs && at_b + CH <= kb) {
+                    const float4 v = *reinterpret_cast<const float4*>(px + at_b);
+                    nx[0] = v.x, nx[1] = v.y, nx[2] = v.z, nx[3] = v.w;
                 } else {
-                    const int n = min(tile.col * NT + half * COLS, a.n - 1);
-                    pw = a.ws + ((long)tile.group * nb + n / kQ8Block) * kb;
-                }
-            };
-            auto fetch = [&](int b) {
 #pragma unroll
-                for (int i = 0; i < CH; i++) {
-                    const bool in = b + i < kb;
-                    nx[i] = in && there ? px[b + i] : 0.f;
-                    nw[i] = in ? pw[b + i] : 0.f;
-                    if constexpr (SW) nu[i] = in ? pu[b + i] : 0.f;
+                    for (int i = 0; i < CH; i++)
+                        if (at_b + i < kb) nx[i] = px[at_b + i];
                 }
+                at_b += CH;
+                if (at_b >= kb) at_b = 0, at_t += step;
             };
-            Tile tile{};
-            if (first < total) {
-                tile = groups.at(first, g);
-                begin(tile);
-                fetch(0);
-            }
-            bool go = true;
-            for (int t = first; t < total; t += step) {
-                const Tile now = tile;
-                const bool zero = !there;
-                uint64_t acc[SW ? COLS / 4 : COLS / 2] = {}, acc_u[SW ? COLS / 4 : 1] = {};
+            fetch();
+
+            bool go = true, ready = false;
+            int t = first;
+            for (; t < total; t += step) {
+                const Tile now = groups.at(t, g);
+                float2 acc[SW ? COLS / 4 : COLS / 2] = {}, acc_u[SW ? COLS / 4 : 1] = {};
                 const bool idle = quarter * 32 >= now.rows;
-                for (int b0 = 0; b0 < kb; b0 += CH) {
-                    float s[CH], u[CH];
+                const int src = row_of(now);
+                const bool zero = src < 0 || src >= a.n_x;
+                for (int b0 = 0; go && b0 < kb; b0 += CH) {
+                    float cx[CH];
+                    const float cw = nw, cu = nu;
+#pragma unroll
+                    for (int i = 0; i < CH; i++) cx[i] = nx[i];
+                    fetch();
 #pragma unroll
                     for (int i = 0; i < CH; i++) {
-                        s[i] = nx[i] * nw[i];
-                        if constexpr (SW) u[i] = nx[i] * nu[i];
-                    }
-                    if (b0 + CH < kb) {
-                        fetch(b0 + CH);
-                    } else if (t + step < total) {
-                        tile = groups.at(t + step, g);
-                        begin(tile);
-                        fetch(0);
-                    }
-#pragma unroll
-                    for (int i = 0; i < CH; i++) {
-                        if (b0 + i >= kb || !go) continue;
-                        go = __all_sync(0xffffffffu, wait_bar(tfull + buf, parity, fail, a.wait_ns, kStatusProduct));
-                        if (!go) continue;
-                        tc_fence_after();
-                        if (!idle) {
-                            const uint32_t at = lanes + buf * NT;
-                            if constexpr (SW) {
-                                add_block<COLS / 2>(acc, at + half * (COLS / 2), s[i]);
-                                add_block<COLS / 2>(acc_u, at + COLS + half * (COLS / 2), u[i]);
-                            } else {
-                                add_block<COLS>(acc, at + half * COLS, s[i]);
-                            }
+                        if (b0 + i >= kb) break;
+                        if (!ready && !__all_sync(0xffffffffu, wait_bar(hfull + buf, parity, fail, a.wait_ns, kStatusProduct))) {
+                            go = false;
+                            break;
                         }
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(tempty + buf)) : "memory");
+                        tc_fence_after();
+                        uint64_t* const done = tempty + half * B + buf;
+                        const uint32_t at = lanes + buf * NT + half * (NT / 2);
+                        const float s = cx[i] * __shfl_sync(0xffffffffu, cw, i);
                         if (++buf == B) buf = 0, parity ^= 1;
+                        auto read = [&] {       // the buffer is free, and whether the next one is full is known by the time it matters
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(done)) : "memory");
+                            ready = __all_sync(0xffffffffu, test_bar(hfull + buf, parity));
+                        };
+                        if (idle) {
+                            read();
+                        } else if constexpr (SW) {
+                            add_block<COLS / 2>(acc, at, s, [] {});
+                            add_block<COLS / 2>(acc_u, at + NT / 4, cx[i] * __shfl_sync(0xffffffffu, cu, i), read);
+                        } else {
+                            add_block<COLS>(acc, at, s, read);
+                        }
                     }
                 }
-                const uint64_t nan2 = 0x7fc000007fc00000ull;
-                if (!go)
-#pragma unroll
-                    for (uint64_t& v : acc) v = nan2;
+                if (!go) break;
                 const int rows = min(now.rows - quarter * 32, 32);
                 const long row = now.first + quarter * 32;
                 if constexpr (!SW) {
                     if (!idle) {
-                        const int n0 = now.col * NT + half * COLS;
+                        const int n0 = now.col * NT + part * COLS;
                         auto put = [&](auto kind) {
                             using T = decltype(kind);
                             const long rb = a.out_row * (long)sizeof(T);
                             if (n0 < a.n)
-                                store_product<T, COLS>(mine, lane, acc, zero && go, (uint8_t*)a.out + row * rb + (long)n0 * sizeof(T), rb,
+                                store_product<T, COLS>(mine, lane, acc, zero, (uint8_t*)a.out + row * rb + (long)n0 * sizeof(T), rb,
                                                        rows, (long)(a.n - n0) * sizeof(T), c.vec);
                         };
                         if (a.dtype == kF32) put(0.f);
@@ -520,48 +541,45 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
                 } else {
                     constexpr int H = COLS / 2;             // columns of the result
                     float h[H], top = 0.f;
-                    const int n0 = now.col * kQ8Block + rank * (NT / 2) + half * H;
+                    const int n0 = now.col * kQ8Block + rank * (NT / 2) + part * H;
 #pragma unroll
                     for (int j = 0; j < H / 2; j++) {
-                        const float2 gate = split(acc[j]), up = split(acc_u[j]);
+                        const float2 gate = acc[j], up = acc_u[j];
                         h[2 * j] = __fdividef(gate.x, 1.f + expf(-gate.x)) * up.x;
                         h[2 * j + 1] = __fdividef(gate.y, 1.f + expf(-gate.y)) * up.y;
                     }
 #pragma unroll
                     for (int j = 0; j < H; j++) {
-                        if (zero && go) h[j] = 0.f;
+                        if (zero) h[j] = 0.f;
                         top = max_nan(top, fabsf(h[j]));
                     }
                     // the row's maximum over all 128 columns
-                    float* const slots = tops + turn * (CL * 2 * MT);
-                    const uint32_t slot = smem_addr(slots + (rank * 2 + half) * MT + quarter * 32 + lane), bar = smem_addr(join + (turn & 1));
-                    if (go) {
+                    float* const slots = tops + turn * (CL * C::kParts * MT);
+                    const uint32_t slot = smem_addr(slots + (rank * C::kParts + part) * MT + quarter * 32 + lane), bar = smem_addr(join + (turn & 1));
 #pragma unroll
-                        for (int p = 0; p < CL; p++) {
-                            uint32_t to, at;
-                            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(slot), "r"(p));
-                            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(bar), "r"(p));
-                            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(top) : "memory");
-                            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory");
-                        }
-                        const uint32_t jp = (uint32_t)((t - first) / step >> 1) & 1;
-                        bool ok = try_cluster(join + turn, jp);
-                        const uint64_t t0 = sync::global_ns();
-                        for (uint32_t i = 1; !ok; i++) {
-                            ok = try_cluster(join + turn, jp);
-                            if (ok || (i & 31)) continue;
-                            if (*fail) break;
-                            if (sync::global_ns() - t0 > (uint64_t)a.wait_ns) {
-                                atomicOr((int*)fail, kStatusJoin);
-                                break;
-                            }
-                        }
-                        go = __all_sync(0xffffffffu, ok);
-                        if (go)
-#pragma unroll
-                            for (int p = 0; p < CL * 2; p++) top = max_nan(top, slots[p * MT + quarter * 32 + lane]);
+                    for (int p = 0; p < CL; p++) {
+                        uint32_t to, at;
+                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(slot), "r"(p));
+                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(bar), "r"(p));
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(top) : "memory");
+                        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory");
                     }
-                    if (!go) top = __int_as_float(0x7fc00000);
+                    const uint32_t jp = (uint32_t)((t - first) / step >> 1) & 1;
+                    bool ok = try_cluster(join + turn, jp);
+                    const uint64_t t0 = sync::global_ns();
+                    for (uint32_t i = 1; !ok; i++) {
+                        ok = try_cluster(join + turn, jp);
+                        if (ok || (i & 31)) continue;
+                        if (*fail) break;
+                        if (sync::global_ns() - t0 > (uint64_t)a.wait_ns) {
+                            atomicOr((int*)fail, kStatusJoin);
+                            break;
+                        }
+                    }
+                    go = __all_sync(0xffffffffu, ok);
+                    if (!go) break;
+#pragma unroll
+                    for (int p = 0; p < CL * C::kParts; p++) top = max_nan(top, slots[p * MT + quarter * 32 + lane]);
                     turn ^= 1;
                     if (!idle) {
                         const float inv = top < kTiny ? 0.f : __fdiv_rn(448.f, top);
@@ -574,9 +592,28 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
                         }
                         if (n0 < a.n)
                             store_rows<H>(mine, lane, v, (uint8_t*)a.out + row * a.out_row + n0, a.out_row, rows, a.n - n0, c.vec, 1);
-                        if (rank == 0 && half == 0 && lane < rows)
+                        if (rank == 0 && part == 0 && lane < rows)
                             a.out_scales[(row + lane) * a.os_row + now.col] =
                                 top < kTiny ? 0.f : top <= 3.402823466e38f ? __fdiv_rn(top, 448.f) : __int_as_float(0x7fc00000);
+                    }
+                }
+            }
+            // a wait ran out: what this block had not finished becomes NaN
+            for (; t < total; t += step) {
+                const Tile tile = groups.at(t, g);
+                const int r = quarter * 32 + lane;
+                if (r >= tile.rows) continue;
+                const long row = tile.first + r;
+                if constexpr (SW) {
+                    constexpr int H = COLS / 2;
+                    const int n0 = tile.col * kQ8Block + rank * (NT / 2) + part * H;
+                    for (int n = n0; n < min(n0 + H, a.n); n++) ((uint8_t*)a.out)[row * a.out_row + n] = 0x7f;
+                    a.out_scales[row * a.os_row + tile.col] = __int_as_float(0x7fc00000);
+                } else {
+                    const int n0 = tile.col * NT + part * COLS;
+                    for (int n = n0; n < min(n0 + COLS, a.n); n++) {
+                        if (a.dtype == kF32) ((uint32_t*)a.out)[row * a.out_row + n] = 0x7fc00000;
+                        else ((uint16_t*)a.out)[row * a.out_row + n] = a.dtype == kF16 ? 0x7e00 : 0x7fc0;
                     }
                 }
             }
@@ -611,7 +648,7 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
 }
 
 bool map_bytes(CUtensorMap* m, int dims, const void* base, const cuuint64_t* size, const cuuint64_t* stride, const cuuint32_t* box) {
-    const cuuint32_t ones[3] = {1, 1, 1};
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
     const auto f = encoder();
     return f && f(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, dims, const_cast<void*>(base), size, stride, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -644,14 +681,17 @@ bool launch_k(const Q8Args& a, cudaStream_t s) {
     c.n_tiles = SW ? (a.n + kQ8Block - 1) / kQ8Block : (a.n + NT - 1) / NT;
     const int elem = SW ? 1 : dtype_bytes(a.dtype);
     c.vec = aligned16(a.out, a.out_row, 0, elem) || (a.n_rows == 1 && aligned16(a.out));
+    c.vec_xs = aligned16(a.xs, a.xs_row, 0, 4);
     const cuuint64_t xd[2] = {(cuuint64_t)a.k, (cuuint64_t)a.n_x};
     const cuuint64_t xst[1] = {(cuuint64_t)(a.n_x == 1 ? (a.k + 15) / 16 * 16 : a.x_row)};
     const cuuint32_t xbox[2] = {128, a.rows ? 1u : 32u};
     const int mats = SW ? 2 : 1;
-    const cuuint64_t wd[3] = {(cuuint64_t)a.k, (cuuint64_t)a.n, (cuuint64_t)a.groups * mats};
-    const cuuint64_t wst[2] = {(cuuint64_t)a.k, (cuuint64_t)a.n * a.k};
-    const cuuint32_t wbox[3] = {128, (cuuint32_t)(SW ? NT / 2 : NT), 1};
-    if (!map_bytes(&c.x, 2, a.x, xd, xst, xbox) || !map_bytes(&c.w, 3, a.w, wd, wst, wbox)) return false;
+    const cuuint64_t wd[4] = {(cuuint64_t)a.k, (cuuint64_t)a.n, (cuuint64_t)mats, (cuuint64_t)a.groups};
+    const cuuint64_t wst[3] = {(cuuint64_t)a.k, (cuuint64_t)a.n * a.k, (cuuint64_t)a.n * a.k * mats};
+    const cuuint32_t wbox[4] = {128, (cuuint32_t)(SW ? NT / 4 : NT), (cuuint32_t)mats, 1};
+    if (!map_bytes(&c.x, 2, a.x, xd, xst, xbox) || !map_bytes(&c.w, 4, a.w, wd, wst, wbox)) return false;
+    const cuuint32_t tbox[2] = {128, 128};
+    if (MT == 128 && !a.rows && !map_bytes(&c.xt, 2, a.x, xd, xst, tbox)) return false;
 
     auto kernel = q8_tc_kernel<MT, NT, SW>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return false;
@@ -676,8 +716,6 @@ bool launch_k(const Q8Args& a, cudaStream_t s) {
 
 template <int MT, bool SW>
 bool launch_n(const Q8Args& a, int nt, cudaStream_t s) {
-    if constexpr (!SW)
-        if (nt == 16) return launch_k<MT, 16, SW>(a, s);
     return nt == 256 ? launch_k<MT, 256, SW>(a, s) : nt == 128 ? launch_k<MT, 128, SW>(a, s)
            : nt == 64 ? launch_k<MT, 64, SW>(a, s) : launch_k<MT, 32, SW>(a, s);
 }
@@ -695,7 +733,7 @@ bool launch_q8_tc(const Q8Args& a, cudaStream_t s) {
     // the widest tile that gives every SM one
     const long cols = a.swiglu ? 2l * a.n : a.n;
     int nt = 256;
-    while (nt > (a.swiglu ? 32 : 16) && row_tiles * ((cols + nt - 1) / nt) < 148) nt >>= 1;
+    while (nt > 32 && row_tiles * ((cols + nt - 1) / nt) < 148) nt >>= 1;
     if (a.swiglu) return few ? launch_n<32, true>(a, nt, s) : launch_n<128, true>(a, nt, s);
     return few ? launch_n<32, false>(a, nt, s) : launch_n<128, false>(a, nt, s);
 }
