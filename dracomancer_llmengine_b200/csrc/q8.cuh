@@ -31,6 +31,8 @@ struct Q8Args {
 bool launch_q8(const Q8Args& a, cudaStream_t s);
 bool q8_tc_fits(const Q8Args& a);
 bool launch_q8_tc(const Q8Args& a, cudaStream_t s);
+bool launch_q8_few(const Q8Args& a, cudaStream_t s);
+bool launch_q8_any(const Q8Args& a, cudaStream_t s);
 
 // a group's rows; offsets that are out of order or out of range give fewer rows, never one outside the output
 struct Q8Span {
@@ -41,6 +43,42 @@ __device__ __forceinline__ Q8Span q8_span(const int* offsets, int g, int n_rows)
     const int a = min(max(offsets[g], 0), n_rows), b = min(max(offsets[g + 1], a), n_rows);
     return Q8Span{a, b - a};
 }
+
+// the group and rows of the row tile `slot` of tiles of M rows; count 0: there is no such tile.  By a whole warp.
+struct Q8Where {
+    int group, first, count;
+};
+template <int M>
+__device__ __forceinline__ Q8Where q8_locate(const Q8Args& a, int slot) {
+    const int lane = threadIdx.x & 31;
+    if (!a.offsets) {
+        const int left = a.n_rows - slot * M;
+        return Q8Where{0, slot * M, left > 0 ? min(left, M) : 0};
+    }
+    int before = 0;
+    for (int g0 = 0; g0 < a.groups; g0 += 32) {
+        const int g = g0 + lane;
+        const Q8Span sp = g < a.groups ? q8_span(a.offsets, g, a.n_rows) : Q8Span{0, 0};
+        const int tiles = (sp.count + M - 1) / M;
+        int sum = tiles;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        const int lo = before + sum - tiles;
+        const uint32_t hit = __ballot_sync(0xffffffffu, slot >= lo && slot < lo + tiles);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            const int first = __shfl_sync(0xffffffffu, sp.first + (slot - lo) * M, src);
+            const int left = __shfl_sync(0xffffffffu, sp.count - (slot - lo) * M, src);
+            return Q8Where{g0 + src, first, min(left, M)};
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return Q8Where{0, 0, 0};
+}
+// row tiles of M rows that there are at most: a group adds one short tile
+inline long q8_slots(const Q8Args& a, int m) { return ((long)a.n_rows + m - 1) / m + (a.offsets ? (a.groups < a.n_rows ? a.groups : a.n_rows) : 0); }
 
 struct PlanExpertsArgs {
     const int* order;           // [n]

@@ -26,40 +26,11 @@ __device__ __forceinline__ float code_value(uint8_t c) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
 }
 
-// the group and rows of row tile `slot`; count 0: there is no such tile.  By one warp.
-struct Where {
-    int group, first, count;
-};
-__device__ Where locate(const Q8Args& a, int slot) {
-    const int lane = threadIdx.x & 31;
-    int before = 0;
-    for (int g0 = 0; g0 < a.groups; g0 += 32) {
-        const int g = g0 + lane;
-        const Q8Span sp = g < a.groups ? q8_span(a.offsets, g, a.n_rows) : Q8Span{0, 0};
-        const int tiles = (sp.count + kM - 1) / kM;
-        int sum = tiles;
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
-        }
-        const int lo = before + sum - tiles;
-        const uint32_t hit = __ballot_sync(0xffffffffu, slot >= lo && slot < lo + tiles);
-        if (hit) {
-            const int src = __ffs(hit) - 1;
-            const int first = __shfl_sync(0xffffffffu, sp.first + (slot - lo) * kM, src);
-            const int left = __shfl_sync(0xffffffffu, sp.count - (slot - lo) * kM, src);
-            return Where{g0 + src, first, min(left, kM)};
-        }
-        before += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    return Where{0, 0, 0};
-}
-
 template <typename T, bool SWIGLU>
 __global__ void __launch_bounds__(kN) q8_any_kernel(const Call c) {
     early_launch();
     wait_for_inputs();
-    __shared__ Where s_at;
+    __shared__ Q8Where s_at;
     __shared__ int s_row[kM];
     __shared__ float s_x[kM][kStep];
     __shared__ uint8_t s_w[kN][kStep + 1];
@@ -67,7 +38,7 @@ __global__ void __launch_bounds__(kN) q8_any_kernel(const Call c) {
     const Q8Args& a = c.a;
     const int tid = threadIdx.x, slot = blockIdx.x / c.n_tiles, tile = blockIdx.x % c.n_tiles;
     if (tid < 32) {
-        const Where w = locate(a, slot);
+        const Q8Where w = q8_locate<kM>(a, slot);
         if (tid == 0) s_at = w;
         if (tid < kM) {
             int r = -1;
@@ -79,7 +50,7 @@ __global__ void __launch_bounds__(kN) q8_any_kernel(const Call c) {
         }
     }
     __syncthreads();
-    const Where at = s_at;
+    const Q8Where at = s_at;
     if (!at.count) return;
 
     const int kb = (a.k + kQ8Block - 1) / kQ8Block, nb = (a.n + kQ8Block - 1) / kQ8Block;
@@ -151,12 +122,10 @@ __global__ void __launch_bounds__(kN) q8_any_kernel(const Call c) {
 
 }  // namespace
 
-bool launch_q8(const Q8Args& a, cudaStream_t s) {
-    if (q8_tc_fits(a)) return launch_q8_tc(a, s);
+bool launch_q8_any(const Q8Args& a, cudaStream_t s) {
     Call c{a, 0};
     c.n_tiles = a.swiglu ? (a.n + kQ8Block - 1) / kQ8Block : (a.n + kN - 1) / kN;
-    const long slots = (a.n_rows + kM - 1) / kM + (a.offsets ? std::min(a.groups, a.n_rows) : 0);   // a group adds one short tile at most
-    const dim3 grid((unsigned)(slots * c.n_tiles)), block(kN);
+    const dim3 grid((unsigned)(q8_slots(a, kM) * c.n_tiles)), block(kN);
     if (a.swiglu) launch(q8_any_kernel<float, true>, grid, block, 0, s, c);
     else if (a.dtype == kF32) launch(q8_any_kernel<float, false>, grid, block, 0, s, c);
     else if (a.dtype == kF16) launch(q8_any_kernel<__half, false>, grid, block, 0, s, c);

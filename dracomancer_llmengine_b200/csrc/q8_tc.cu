@@ -29,13 +29,17 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstdlib>
 
 namespace draco {
 namespace {
 
 using sync::smem_addr;
 
-constexpr int kThreads = 384, kStagingWarp = 1024;
+constexpr int kStagingWarp = 2048;
+#ifndef Q8_WIDE
+#define Q8_WIDE 512
+#endif
 constexpr int kStatusOperands = 1, kStatusProduct = 2, kStatusJoin = 4, kStatusBuffer = 8, kStatusStage = 16;
 constexpr float kTiny = 7.888609e-31f;   // 2^-100
 constexpr int kSmemMost = 227 * 1024;
@@ -51,18 +55,21 @@ struct Call {
 template <int MT, int NT, bool SW>
 struct Cfg {
     static constexpr int kCluster = SW ? 256 / NT : 1;
-    static constexpr int kA = MT * 128, kB = NT * 128, kStage = kA + kB;
-    static constexpr int kBuffers = NT == 256 ? 2 : NT == 128 ? 4 : 8;
-    static constexpr int kColumns = NT * kBuffers;                      // a power of two, 128 to 512
-    static constexpr int kParts = 2;                                    // warps that share a row's columns
+    static constexpr int kPer = NT <= 64 ? 2 : 1;                       // blocks of 128 inner values of a stage
+    static constexpr int kA = MT * 128, kB = NT * 128, kStage = kPer * (kA + kB);
+    static constexpr int kSets = kPer == 1 ? 2 : 1;                     // parts of a stage's products that are handed on alone
+    static constexpr int kBuffers = NT == 256 ? 2 : NT == 32 ? 8 : 4;   // a stage's products each
+    static constexpr int kColumns = kPer * NT * kBuffers;               // 512
+    static constexpr int kParts = NT >= Q8_WIDE ? 4 : 2;                // warps that share a row's columns
+    static constexpr int kThreads = 128 + 128 * kParts;
     static constexpr int kActive = MT / 32 * kParts;                    // consumer warps that have rows
-    static constexpr int kStaging = kActive * kStagingWarp;
+    static constexpr int kStaging = kActive * kStagingWarp / (kParts / 2);
     static constexpr int kTops = SW ? 2 * kCluster * kParts * MT * 4 : 0;   // two tiles' maxima, of each part of each block
-    static constexpr int kMisc = 2048 + 2 * 4 * (kQ8MaxGroups + 1);
+    static constexpr int kMisc = 1024 + 2 * 4 * (kQ8MaxGroups + 1) + 8 * 128;
     // the product reads 128 rows from a stage of MT: what lies behind the ring has to be there
     static constexpr int kPad = kStaging + kTops + kMisc >= 16384 ? 0 : 16384;
     static constexpr int kFit = (kSmemMost - 1024 - kStaging - kTops - kMisc - kPad) / kStage;
-    static constexpr int kStages = kFit > 32 ? 32 : kFit;
+    static constexpr int kStages = kFit > 16 ? 16 : kFit;
     static constexpr int kSmem = 1024 + kStages * kStage + kStaging + kTops + kMisc + kPad;
 };
 
@@ -70,22 +77,35 @@ struct Tile {
     int group, first, rows, col;
 };
 
-// the group's first row tile is its predecessors' number (pre); off: where its rows start
+// The tiles, group by group, in a group its row tiles first.
 struct Groups {
-    const int *pre, *off;
-    int groups, n_tiles, mt;
-    __device__ __forceinline__ int total() const {
-        return (int)min((long)pre[groups] * n_tiles, 0x7ff00000l);
+    const int *pre, *off;       // row tiles before each group, where its rows start
+    int groups, n_tiles, mt, total, at_once, me;
+
+    __device__ __forceinline__ Groups(const int* pre_, const int* off_, int groups_, int n_tiles_, int mt_, int at_once_, int me_)
+        : pre(pre_), off(off_), groups(groups_), n_tiles(n_tiles_), mt(mt_), at_once(at_once_), me(me_) {
+        total = (int)min((long)pre[groups] * n_tiles, 0x7ff00000l);
     }
-    // the tile t, whose group is g or a later one
-    __device__ __forceinline__ Tile at(int t, int& g) const {
-        while ((long)pre[g + 1] * n_tiles <= t) g++;
+    __device__ __forceinline__ Tile at(int t) const {
+        int g = 0;
+        for (int n = groups; n > 1;) {          // the last group that starts at or before t and is not empty
+            const int half = n >> 1;
+            if ((long)pre[g + half] * n_tiles <= t) g += half, n -= half;
+            else n = half;
+        }
         const int lo = pre[g], tiles = pre[g + 1] - lo;
         const unsigned in = (unsigned)(t - (long)lo * n_tiles);
         const int col = (int)(in / (unsigned)tiles), m = (int)(in - (unsigned)col * tiles);
         const int first = off[g], count = max(off[g + 1] - first, 0);
         return Tile{g, first + m * mt, min(count - m * mt, mt), col};
     }
+};
+// this block's (or cluster's) tiles
+struct Walk {
+    const Groups& groups;
+    int t;
+    __device__ __forceinline__ explicit Walk(const Groups& g) : groups(g), t(g.me - g.at_once) {}
+    __device__ __forceinline__ bool next() { return (t += groups.at_once) < groups.total; }
 };
 
 // bounded wait; false: the limit ran out here (noted in *fail) or somewhere else in the block before
@@ -136,14 +156,10 @@ __device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x,
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(smem_addr(bar))
         : "memory");
 }
-__device__ __forceinline__ void tma_gather(void* dst, const CUtensorMap* map, int x, int4 rows, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
-        "%6}], [%7];" ::"r"(smem_addr(dst)),
-        "l"(map), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(smem_addr(bar))
-        : "memory");
+// 16 bytes, or 16 zeros (bytes 0)
+__device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
-
 __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -204,9 +220,10 @@ __device__ __forceinline__ void store_piece(uint8_t* p, const uint8_t* src, long
     }
 }
 
-// 32 rows of BYTES bytes, one a lane, to memory in pieces of 16 bytes side by side, through the warp's staging buffer (1 KB; a
-// piece's place is turned by its row, so that eight rows' pieces lie in different banks)
-template <int BYTES>
+// 32 rows of BYTES bytes, one a lane, to memory in pieces of 16 bytes side by side, through the warp's staging buffer (2 KB; a
+// piece's place is turned by its row, so that eight rows' pieces lie in different banks).  A few rows go directly: the lanes
+// that have one need no other's.
+template <int BYTES, int STAGING>
 __device__ __forceinline__ void store_rows(uint8_t* staging, int lane, const uint32_t (&v)[BYTES / 4], uint8_t* out, long row_bytes,
                                            int rows, long left, bool vec, int elem) {
     if constexpr (BYTES < 16) {
@@ -225,12 +242,23 @@ __device__ __forceinline__ void store_rows(uint8_t* staging, int lane, const uin
                 if (2 * i < left) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
         }
     } else {
-        constexpr int P = BYTES / 16, ROWS = P == 4 ? 16 : 32;      // pieces of a row, rows at a time
-        auto place = [](int r, int i) { return (r % ROWS) * BYTES + (P == 4 ? i ^ ((r >> 1) & 3) : P == 2 ? i ^ ((r >> 2) & 1) : i) * 16; };
+        constexpr int P = BYTES / 16;       // pieces of a row
+        if (rows <= 4) {
+            if (lane >= rows) return;
+#pragma unroll
+            for (int i = 0; i < P; i++) {
+                const uint4 u = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                if (vec && left >= 16 * i + 16) *reinterpret_cast<uint4*>(out + lane * row_bytes + i * 16) = u;
+                else store_piece(out + lane * row_bytes + i * 16, reinterpret_cast<const uint8_t*>(&u), left - i * 16, false, elem);
+            }
+            return;
+        }
+        constexpr int ROWS = STAGING / BYTES < 32 ? STAGING / BYTES : 32;       // at a time
+        auto place = [](int r, int i) { return r % ROWS * BYTES + (P == 4 ? i ^ ((r >> 1) & 3) : P == 2 ? i ^ ((r >> 2) & 1) : i) * 16; };
 #pragma unroll
         for (int r0 = 0; r0 < 32; r0 += ROWS) {
             __syncwarp();
-            if (lane >= r0 && lane < r0 + ROWS)
+            if (ROWS == 32 || (lane >= r0 && lane < r0 + ROWS))
 #pragma unroll
                 for (int i = 0; i < P; i++)
                     *reinterpret_cast<uint4*>(staging + place(lane, i)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
@@ -244,7 +272,7 @@ __device__ __forceinline__ void store_rows(uint8_t* staging, int lane, const uin
     }
 }
 
-template <typename T, int COLS>
+template <typename T, int COLS, int STAGING>
 __device__ __forceinline__ void store_product(uint8_t* staging, int lane, const float2 (&acc)[COLS / 2], bool zero, uint8_t* out,
                                               long row_bytes, int rows, long left, bool vec) {
     constexpr int S = sizeof(T), C = COLS * S < 64 ? COLS : 64 / S;     // columns of a piece
@@ -258,12 +286,12 @@ __device__ __forceinline__ void store_product(uint8_t* staging, int lane, const 
             if constexpr (S == 4) v[2 * j] = __float_as_uint(f.x), v[2 * j + 1] = __float_as_uint(f.y);
             else v[j] = pack2<T>(f.x, f.y);
         }
-        store_rows<C * S>(staging, lane, v, out + i * C * S, row_bytes, rows, left - (long)i * C * S, vec, S);
+        store_rows<C * S, STAGING>(staging, lane, v, out + i * C * S, row_bytes, rows, left - (long)i * C * S, vec, S);
     }
 }
 
 template <int MT, int NT, bool SW>
-__global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constant__ Call c) {
+__global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(const __grid_constant__ Call c) {
     using C = Cfg<MT, NT, SW>;
     constexpr int S = C::kStages, B = C::kBuffers, CL = C::kCluster;
     extern __shared__ uint8_t s_raw[];
@@ -272,15 +300,16 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
     float* const tops = (float*)(staging + C::kStaging);
     uint64_t* const full = (uint64_t*)((uint8_t*)tops + C::kTops);
     uint64_t* const empty = full + S;
-    uint64_t* const tfull = empty + S;          // [2][B], of the halves of the columns
+    uint64_t* const tfull = empty + S;          // [sets][B]
     uint64_t* const tempty = tfull + 2 * B;
     uint64_t* const join = tempty + 2 * B;      // [2]
     uint64_t* const drain = join + 2;
     uint32_t* const s_tmem = (uint32_t*)(drain + 1);
     int* const s_fail = (int*)(s_tmem + 1);
-    int* const s_pre = (int*)((uint8_t*)full + 2048);
+    int* const s_pre = (int*)((uint8_t*)full + 1024);
     int* const s_off = s_pre + kQ8MaxGroups + 1;
-    static_assert((2 * 32 + 4 * 8 + 3) * 8 + 8 <= 2048, "the barriers have their place");
+    const uint8_t** const s_src = (const uint8_t**)(s_off + kQ8MaxGroups + 1);     // [128] rows of x of the tile that is being fetched
+    static_assert((2 * 16 + 4 * 8 + 3) * 8 + 8 <= 1024, "the barriers have their place");
 
     const Q8Args& a = c.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -288,19 +317,19 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
     early_launch();
     if (warp == 0 && lane == 0) {
         for (int i = 0; i < S; i++) {
-            sync::mbar_init(full + i, 2 + (a.test_extra == 1));
+            sync::mbar_init(full + i, 1 + (a.rows ? 32 : 1) + (a.test_extra == 1));
             sync::mbar_init(empty + i, 2);
         }
         for (int i = 0; i < 2 * B; i++) {
-            sync::mbar_init(tfull + i, 1 + (a.test_extra == 2));
-            sync::mbar_init(tempty + i, C::kActive / 2);
+            sync::mbar_init(tfull + i, C::kPer + (a.test_extra == 2));
+            sync::mbar_init(tempty + i, C::kActive / C::kSets);
         }
         for (int i = 0; i < 2; i++) sync::mbar_init(join + i, CL * C::kParts * MT + (a.test_extra == 3));
         sync::mbar_init(drain, 2);
         *s_fail = 0;
         sync::fence_init();
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&c.x) : "memory");
-        if (MT == 128) asm volatile("prefetch.tensormap [%0];" ::"l"(&c.xt) : "memory");
+        if (!a.rows) asm volatile("prefetch.tensormap [%0];" ::"l"(&c.x) : "memory");
+        if (!a.rows && MT == 128) asm volatile("prefetch.tensormap [%0];" ::"l"(&c.xt) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&c.w) : "memory");
     }
     if (warp == 1) {
@@ -336,84 +365,108 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
     }
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
-    const Groups groups{s_pre, s_off, a.groups, c.n_tiles, MT};
-    const int total = groups.total(), first = (int)blockIdx.x / CL, step = (int)gridDim.x / CL;
+    const Groups groups(s_pre, s_off, a.groups, c.n_tiles, MT, (int)gridDim.x / CL, (int)blockIdx.x / CL);
     const int kb = (a.k + kQ8Block - 1) / kQ8Block;
     volatile int* const fail = s_fail;
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kParts == 2 ? 40 : 32));
+        int stage = 0;
+        bool go = true;
+        Walk walk(groups);
         if (warp == 0 || warp == 2) {       // copies of the weight, of x
             const bool of_x = warp == 2;
-            int stage = 0, g = 0, filled = 0;
+            int filled = 0;
             uint32_t parity = 1;
-            bool go = true;
-            for (int t = first; go && t < total; t += step) {
-                const Tile tile = groups.at(t, g);
+            while (go && walk.next()) {
+                const Tile tile = groups.at(walk.t);
                 const int n0 = SW ? tile.col * kQ8Block + rank * (NT / 2) : tile.col * NT;
-                int4 rows = make_int4(0, 0, 0, 0);
-                int boxes = (tile.rows + 31) / 32;
-                if (of_x && a.rows) {           // a lane fetches four rows
-                    int r[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        r[i] = a.rows[tile.first + min(lane * 4 + i, tile.rows - 1)];
-                        if (r[i] < 0 || r[i] >= a.n_x) r[i] = 0;        // not used: the row becomes zero
+                const bool tall = MT == 128 && tile.rows > 32;      // one box of 128 rows, else of 32
+                if (of_x && a.rows) {
+                    __syncwarp();
+                    for (int r = lane; r < tile.rows; r += 32) {
+                        const int src = a.rows[tile.first + r];
+                        s_src[r] = a.x + (src >= 0 && src < a.n_x ? src : 0) * a.x_row;     // not used where it is none: the row becomes zero
                     }
-                    rows = make_int4(r[0], r[1], r[2], r[3]);
-                    boxes = (tile.rows + 3) / 4;
+                    __syncwarp();
                 }
-                const uint32_t bytes = of_x ? (uint32_t)boxes * (a.rows ? 512 : 4096) : C::kB;
-                for (int b = 0; b < kb; b++) {
+                for (int b = 0; b < kb; b += C::kPer) {
                     go = __all_sync(0xffffffffu, wait_bar(empty + stage, parity, fail, a.wait_ns, kStatusStage));
                     if (!go) break;
                     uint8_t* const pa = ring + stage * C::kStage;
-                    if (elect_one()) {
-                        sync::mbar_expect_tx(full + stage, bytes);
-                        if (!of_x) {
-                            tma_4d(pa + C::kA, &c.w, b * kQ8Block, n0, 0, tile.group, full + stage);
-                            if constexpr (SW)
-                                tma_4d(pa + C::kA + C::kB / 2, &c.w, b * kQ8Block, n0 + NT / 4, 0, tile.group, full + stage);
-                        } else if (!a.rows) {
-                            if (MT == 128 && boxes == 4)
-                                tma_2d(pa, &c.xt, b * kQ8Block, tile.first, full + stage);
-                            else
-                                for (int i = 0; i < boxes; i++)
-                                    tma_2d(pa + i * 4096, &c.x, b * kQ8Block, tile.first + i * 32, full + stage);
+                    uint8_t* const pb = pa + C::kPer * C::kA;
+                    const int here = C::kPer == 1 ? 1 : min(C::kPer, kb - b);
+                    if (of_x && a.rows) {
+                        // a row's 128 bytes by eight lanes; the 16-byte pieces lie where the 128-byte swizzle of the operand has them
+                        const int sub = lane >> 3, piece = lane & 7;
+                        for (int j = 0; j < here; j++) {
+                            const int k0 = (b + j) * kQ8Block + piece * 16;
+                            const int bytes = k0 < a.k ? 16 : 0;                // behind the row: zeros
+                            const int from = bytes ? k0 : 0;
+                            const uint32_t even = smem_addr(pa + j * C::kA) + sub * 128 + ((piece ^ sub) << 4), odd = even ^ 64;
+                            int r = sub;
+                            for (; r + 28 < tile.rows; r += 32) {
+                                const uint8_t* src[8];
+#pragma unroll
+                                for (int i = 0; i < 8; i++) src[i] = s_src[r + 4 * i];
+#pragma unroll
+                                for (int i = 0; i < 8; i++) copy16((i & 1 ? odd : even) + (r - sub + 4 * i) * 128, src[i] + from, bytes);
+                            }
+                            for (; r < tile.rows; r += 4) copy16(((r - sub) & 4 ? odd : even) + (r - sub) * 128, s_src[r] + from, bytes);
+                        }
+                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(full + stage)) : "memory");
+                    } else if (elect_one()) {
+                        sync::mbar_expect_tx(full + stage, (uint32_t)here * (!of_x ? C::kB : tall ? 16384 : 4096));
+#pragma unroll
+                        for (int j = 0; j < C::kPer; j++) {
+                            if (j >= here) break;
+                            const int k0 = (b + j) * kQ8Block;
+                            if (!of_x) {
+                                tma_4d(pb + j * C::kB, &c.w, k0, n0, 0, tile.group, full + stage);
+                                if constexpr (SW && C::kPer == 1)
+                                    tma_4d(pb + C::kB / 2, &c.w, k0, n0 + NT / 4, 0, tile.group, full + stage);
+                            } else {
+                                tma_2d(pa + j * C::kA, tall ? &c.xt : &c.x, k0, tile.first, full + stage);
+                            }
                         }
                     }
                     __syncwarp();
-                    if (of_x && a.rows && lane < boxes) tma_gather(pa + lane * 512, &c.x, b * kQ8Block, rows, full + stage);
                     filled = min(filled + 1, S);
                     if (++stage == S) stage = 0, parity ^= 1;
                 }
             }
-            for (int i = 0; i < filled; i++) {      // whatever happened, copies in flight land before the memory is another's
+            // whatever happened, copies in flight land before the memory is another's
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            for (int i = 0; i < filled; i++) {
                 if (--stage < 0) stage = S - 1, parity ^= 1;
                 const uint64_t t0 = sync::global_ns();
                 while (!sync::mbar_try(full + stage, parity ^ 1) && sync::global_ns() - t0 < 10000000ull) {}
             }
-        } else {        // products of one half of the weight's rows
-            constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(NT / 2 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-            const int half = warp >> 1;
-            int stage = 0, buf = 0;
+        } else {        // products: of one half of the weight's rows, or of every second block
+            constexpr int N = NT / C::kSets;
+            constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+            const int which = warp >> 1, set = C::kSets == 2 ? which : 0;
+            const uint32_t off_a = C::kSets == 2 ? 0 : which * C::kA, off_b = C::kPer * C::kA + which * (C::kSets == 2 ? C::kB / 2 : C::kB);
+            int buf = 0;
             uint32_t parity = 0, bparity = 1;
-            bool go = true;
-            for (int t = first; go && t < total; t += step) {
-                for (int b = 0; b < kb; b++) {
-                    go = wait_bar(tempty + half * B + buf, bparity, fail, a.wait_ns, kStatusBuffer) &&
+            while (go && walk.next()) {
+                for (int b = 0; b < kb; b += C::kPer) {
+                    go = wait_bar(tempty + set * B + buf, bparity, fail, a.wait_ns, kStatusBuffer) &&
                          wait_bar(full + stage, parity, fail, a.wait_ns, kStatusOperands);
                     go = __all_sync(0xffffffffu, go);
                     if (!go) break;
+                    if (a.rows) sync::fence_proxy_async();      // rows came by copies of the generic proxy
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint64_t da = sdesc_sw128(smem_addr(ring + stage * C::kStage));
-                        const uint64_t db = sdesc_sw128(smem_addr(ring + stage * C::kStage + C::kA + half * (C::kB / 2)));
+                        if (C::kSets == 2 || b + which < kb) {
+                            const uint64_t da = sdesc_sw128(smem_addr(ring + stage * C::kStage + off_a));
+                            const uint64_t db = sdesc_sw128(smem_addr(ring + stage * C::kStage + off_b));
+                            const uint32_t d = tmem + buf * (C::kPer * NT) + which * N;
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            mma_f8(tmem + buf * NT + half * (NT / 2), da + 2 * j, db + 2 * j, idesc, j > 0);
+                            for (int j = 0; j < 4; j++) mma_f8(d, da + 2 * j, db + 2 * j, idesc, j > 0);
+                        }
                         tc_commit(empty + stage);
-                        tc_commit(tfull + half * B + buf);
+                        tc_commit(tfull + set * B + buf);
                     }
                     __syncwarp();
                     if (++stage == S) stage = 0, parity ^= 1;
@@ -427,22 +480,30 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
             while (!sync::mbar_try(drain, 0) && sync::global_ns() - t0 < sync::kWaitLimitNs) {}
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kParts == 2 ? 232 : 112));
         const int quarter = warp & 3, part = (warp - 4) >> 2;
-        if (quarter * 32 < MT && part < C::kParts) {
+        if (quarter * 32 < MT) {
             constexpr int COLS = NT / C::kParts;            // of this warp; with SwiGLU half of them gate, half up
             constexpr int CH = 4;                           // blocks whose scales are fetched together, as many ahead
             const int nb = (a.n + kQ8Block - 1) / kQ8Block;
-            const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-            uint8_t* const mine = staging + (part * (MT / 32) + quarter) * kStagingWarp;
-            const int half = part;
-            uint64_t* const hfull = tfull + half * B;
-            int buf = 0, g = 0, turn = 0;
+            // this warp's columns of a buffer (with SwiGLU those of gate, and those of up behind)
+            const int set = C::kSets == 2 ? part / (C::kParts / 2) : 0;
+            const uint32_t columns = tmem + ((uint32_t)(quarter * 32) << 16) + set * (NT / 2) +
+                                     (C::kSets == 2 ? part % (C::kParts / 2) : part) * (SW ? COLS / 2 : COLS);
+            constexpr uint32_t to_up = C::kSets == 1 ? NT / 2 : NT / 4;
+            uint8_t* const mine = staging + (part * (MT / 32) + quarter) * (kStagingWarp / (C::kParts / 2));
+            uint64_t* const my_full = tfull + set * B;
+            uint64_t* const my_empty = tempty + set * B;
+            int buf = 0, turn = 0, joins = 0;
             uint32_t parity = 0;
 
             // scales, fetched ahead through the ends of tiles: those of block `at_b` of tile `at_t` come next
             const float *px = nullptr, *pw = nullptr, *pu = nullptr;
-            int at_t = first, at_b = 0, at_g = 0;
+            Walk ahead(groups);
+            bool more = ahead.next();
+            Tile coming{};                                  // the tile of the blocks that were fetched last
+            bool coming_zero = false;
+            int at_b = 0;
             float nx[CH], nw = 0.f, nu = 0.f;               // lane i has the weight's scale of block i
 #pragma unroll
             for (int i = 0; i < CH; i++) nx[i] = 0.f;
@@ -451,10 +512,11 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
                 return a.rows ? a.rows[tile.first + r] : tile.first + r;
             };
             auto fetch = [&] {
-                if (at_t >= total) return;
+                if (!more) return;
                 if (at_b == 0) {
-                    const Tile tile = groups.at(at_t, at_g);
+                    const Tile tile = coming = groups.at(ahead.t);
                     const int src = row_of(tile);
+                    coming_zero = src < 0 || src >= a.n_x;
                     px = a.xs + (long)(src >= 0 && src < a.n_x ? src : 0) * a.xs_row;
                     if constexpr (SW) {
                         pw = a.ws + ((long)tile.group * 2 * nb + tile.col) * kb;
@@ -475,49 +537,56 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
                         if (at_b + i < kb) nx[i] = px[at_b + i];
                 }
                 at_b += CH;
-                if (at_b >= kb) at_b = 0, at_t += step;
+                if (at_b >= kb) at_b = 0, more = ahead.next();
             };
             fetch();
 
             bool go = true, ready = false;
-            int t = first;
-            for (; t < total; t += step) {
-                const Tile now = groups.at(t, g);
+            Walk walk(groups);
+            bool left = walk.next();
+            for (; left; left = walk.next()) {
+                const Tile now = coming;
+                const bool zero = coming_zero;
                 float2 acc[SW ? COLS / 4 : COLS / 2] = {}, acc_u[SW ? COLS / 4 : 1] = {};
                 const bool idle = quarter * 32 >= now.rows;
-                const int src = row_of(now);
-                const bool zero = src < 0 || src >= a.n_x;
+                uint64_t* done = nullptr;
+                uint32_t at = 0;
                 for (int b0 = 0; go && b0 < kb; b0 += CH) {
                     float cx[CH];
                     const float cw = nw, cu = nu;
 #pragma unroll
                     for (int i = 0; i < CH; i++) cx[i] = nx[i];
                     fetch();
-#pragma unroll
-                    for (int i = 0; i < CH; i++) {
-                        if (b0 + i >= kb) break;
-                        if (!ready && !__all_sync(0xffffffffu, wait_bar(hfull + buf, parity, fail, a.wait_ns, kStatusProduct))) {
-                            go = false;
-                            break;
+                    // one copy of the code: the instruction cache is too small for four
+#pragma unroll 1
+                    for (int i = 0; i < CH && b0 + i < kb; i++) {
+                        const int j = C::kPer == 1 ? 0 : i % C::kPer;
+                        if (j == 0) {
+                            if (!ready && !__all_sync(0xffffffffu, wait_bar(my_full + buf, parity, fail, a.wait_ns, kStatusProduct))) {
+                                go = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            done = my_empty + buf;
+                            at = columns + buf * (C::kPer * NT);
+                            if (++buf == B) buf = 0, parity ^= 1;
                         }
-                        tc_fence_after();
-                        uint64_t* const done = tempty + half * B + buf;
-                        const uint32_t at = lanes + buf * NT + half * (NT / 2);
-                        const float s = cx[i] * __shfl_sync(0xffffffffu, cw, i);
-                        if (++buf == B) buf = 0, parity ^= 1;
                         auto read = [&] {       // the buffer is free, and whether the next one is full is known by the time it matters
+                            if (C::kPer > 1 && j != C::kPer - 1 && b0 + i + 1 < kb) return;
                             tc_fence_before();
                             __syncwarp();
                             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(done)) : "memory");
-                            ready = __all_sync(0xffffffffu, test_bar(hfull + buf, parity));
+                            ready = __all_sync(0xffffffffu, test_bar(my_full + buf, parity));
                         };
+                        const float s = cx[0] * __shfl_sync(0xffffffffu, cw, i), u = SW ? cx[0] * __shfl_sync(0xffffffffu, cu, i) : 0.f;
+                        cx[0] = cx[1], cx[1] = cx[2], cx[2] = cx[3];
                         if (idle) {
                             read();
                         } else if constexpr (SW) {
-                            add_block<COLS / 2>(acc, at, s, [] {});
-                            add_block<COLS / 2>(acc_u, at + NT / 4, cx[i] * __shfl_sync(0xffffffffu, cu, i), read);
+                            add_block<COLS / 2>(acc, at + j * NT, s, [] {});
+                            add_block<COLS / 2>(acc_u, at + j * NT + to_up, u, read);
                         } else {
-                            add_block<COLS>(acc, at, s, read);
+                            add_block<COLS>(acc, at + j * NT, s, read);
                         }
                     }
                 }
@@ -531,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
                             using T = decltype(kind);
                             const long rb = a.out_row * (long)sizeof(T);
                             if (n0 < a.n)
-                                store_product<T, COLS>(mine, lane, acc, zero, (uint8_t*)a.out + row * rb + (long)n0 * sizeof(T), rb,
+                                store_product<T, COLS, kStagingWarp / (C::kParts / 2)>(mine, lane, acc, zero, (uint8_t*)a.out + row * rb + (long)n0 * sizeof(T), rb,
                                                        rows, (long)(a.n - n0) * sizeof(T), c.vec);
                         };
                         if (a.dtype == kF32) put(0.f);
@@ -555,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
                     }
                     // the row's maximum over all 128 columns
                     float* const slots = tops + turn * (CL * C::kParts * MT);
-                    const uint32_t slot = smem_addr(slots + (rank * C::kParts + part) * MT + quarter * 32 + lane), bar = smem_addr(join + (turn & 1));
+                    const uint32_t slot = smem_addr(slots + (rank * C::kParts + part) * MT + quarter * 32 + lane), bar = smem_addr(join + turn);
 #pragma unroll
                     for (int p = 0; p < CL; p++) {
                         uint32_t to, at;
@@ -564,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
                         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(top) : "memory");
                         asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory");
                     }
-                    const uint32_t jp = (uint32_t)((t - first) / step >> 1) & 1;
+                    const uint32_t jp = (uint32_t)(joins++ >> 1) & 1;
                     bool ok = try_cluster(join + turn, jp);
                     const uint64_t t0 = sync::global_ns();
                     for (uint32_t i = 1; !ok; i++) {
@@ -591,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
                             v[j] = (uint32_t)lo | (uint32_t)hi << 16;
                         }
                         if (n0 < a.n)
-                            store_rows<H>(mine, lane, v, (uint8_t*)a.out + row * a.out_row + n0, a.out_row, rows, a.n - n0, c.vec, 1);
+                            store_rows<H, kStagingWarp / (C::kParts / 2)>(mine, lane, v, (uint8_t*)a.out + row * a.out_row + n0, a.out_row, rows, a.n - n0, c.vec, 1);
                         if (rank == 0 && part == 0 && lane < rows)
                             a.out_scales[(row + lane) * a.os_row + now.col] =
                                 top < kTiny ? 0.f : top <= 3.402823466e38f ? __fdiv_rn(top, 448.f) : __int_as_float(0x7fc00000);
@@ -599,8 +668,8 @@ __global__ void __launch_bounds__(kThreads, 1) q8_tc_kernel(const __grid_constan
                 }
             }
             // a wait ran out: what this block had not finished becomes NaN
-            for (; t < total; t += step) {
-                const Tile tile = groups.at(t, g);
+            for (; left; left = walk.next()) {
+                const Tile tile = groups.at(walk.t);
                 const int r = quarter * 32 + lane;
                 if (r >= tile.rows) continue;
                 const long row = tile.first + r;
@@ -684,19 +753,19 @@ bool launch_k(const Q8Args& a, cudaStream_t s) {
     c.vec_xs = aligned16(a.xs, a.xs_row, 0, 4);
     const cuuint64_t xd[2] = {(cuuint64_t)a.k, (cuuint64_t)a.n_x};
     const cuuint64_t xst[1] = {(cuuint64_t)(a.n_x == 1 ? (a.k + 15) / 16 * 16 : a.x_row)};
-    const cuuint32_t xbox[2] = {128, a.rows ? 1u : 32u};
+    const cuuint32_t xbox[2] = {128, 32};
     const int mats = SW ? 2 : 1;
     const cuuint64_t wd[4] = {(cuuint64_t)a.k, (cuuint64_t)a.n, (cuuint64_t)mats, (cuuint64_t)a.groups};
     const cuuint64_t wst[3] = {(cuuint64_t)a.k, (cuuint64_t)a.n * a.k, (cuuint64_t)a.n * a.k * mats};
-    const cuuint32_t wbox[4] = {128, (cuuint32_t)(SW ? NT / 4 : NT), (cuuint32_t)mats, 1};
-    if (!map_bytes(&c.x, 2, a.x, xd, xst, xbox) || !map_bytes(&c.w, 4, a.w, wd, wst, wbox)) return false;
+    const cuuint32_t wbox[4] = {128, (cuuint32_t)(!SW ? NT : C::kPer == 1 ? NT / 4 : NT / 2), (cuuint32_t)mats, 1};
+    if ((!a.rows && !map_bytes(&c.x, 2, a.x, xd, xst, xbox)) || !map_bytes(&c.w, 4, a.w, wd, wst, wbox)) return false;
     const cuuint32_t tbox[2] = {128, 128};
     if (MT == 128 && !a.rows && !map_bytes(&c.xt, 2, a.x, xd, xst, tbox)) return false;
 
     auto kernel = q8_tc_kernel<MT, NT, SW>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return false;
     cudaLaunchConfig_t cfg{};
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(C::kThreads);
     cfg.dynamicSmemBytes = C::kSmem;
     cfg.stream = s;
     cudaLaunchAttribute at[2] = {};
@@ -733,9 +802,17 @@ bool launch_q8_tc(const Q8Args& a, cudaStream_t s) {
     // the widest tile that gives every SM one
     const long cols = a.swiglu ? 2l * a.n : a.n;
     int nt = 256;
-    while (nt > 32 && row_tiles * ((cols + nt - 1) / nt) < 148) nt >>= 1;
+    if (const char* f = getenv("Q8_NT")) nt = atoi(f);
+    else while (nt > 32 && row_tiles * ((cols + nt - 1) / nt) < 148) nt >>= 1;
     if (a.swiglu) return few ? launch_n<32, true>(a, nt, s) : launch_n<128, true>(a, nt, s);
     return few ? launch_n<32, false>(a, nt, s) : launch_n<128, false>(a, nt, s);
+}
+
+bool launch_q8(const Q8Args& a, cudaStream_t s) {
+    if (!q8_tc_fits(a)) return launch_q8_any(a, s);
+    const char* few = getenv("Q8_FEW");
+    if (few ? atoi(few) >= a.n_rows : a.n_rows <= 16) return launch_q8_few(a, s);
+    return launch_q8_tc(a, s);
 }
 
 }  // namespace draco

@@ -474,7 +474,7 @@ def test_stream_argument():
 
 @pytest.mark.parametrize("swiglu", [False, True])
 @pytest.mark.parametrize("which,bits", [(1, 0x101), (2, 0x102), (3, 0x104)])
-@pytest.mark.parametrize("rows,n", [(5, 256), (300, 512)])
+@pytest.mark.parametrize("rows,n", [(20, 256), (300, 512)])
 def test_waits_that_run_out(rows, n, which, bits, swiglu):
     """Barriers of the tensor-core form that expect an arrival which never comes: the call ends, its rows are NaN, the status
     says which wait it was (others may have run out with it), and the next call is right."""
