@@ -49,7 +49,6 @@ struct Call {
     Q8Args a;
     int n_tiles;        // column tiles (with SwiGLU: of 128 columns)
     int vec;            // rows of the output start on 16 bytes
-    int vec_xs;         // and those of x's scales
 };
 
 template <int MT, int NT, bool SW>
@@ -65,12 +64,19 @@ struct Cfg {
     static constexpr int kActive = MT / 32 * kParts;                    // consumer warps that have rows
     static constexpr int kStaging = kActive * kStagingWarp / (kParts / 2);
     static constexpr int kTops = SW ? 2 * kCluster * kParts * MT * 4 : 0;   // two tiles' maxima, of each part of each block
-    static constexpr int kMisc = 1024 + 2 * 4 * (kQ8MaxGroups + 1) + 8 * 128;
+    // a block's scales: of MT rows of x, and two of the weight (of the halves of the columns, or of gate and up).  They stay until
+    // the block's product has been added: the copies of a stage wait for the product S stages before, which waited for its
+    // buffer, so that S + B stages' scales are in use at most.
+    static constexpr int kScale = MT + 4;
+    static constexpr int kMiscBut = 640 + 2 * 4 * (kQ8MaxGroups + 1) + 8 * 128;
     // the product reads 128 rows from a stage of MT: what lies behind the ring has to be there
-    static constexpr int kPad = kStaging + kTops + kMisc >= 16384 ? 0 : 16384;
-    static constexpr int kFit = (kSmemMost - 1024 - kStaging - kTops - kMisc - kPad) / kStage;
-    static constexpr int kStages = kFit > 16 ? 16 : kFit;
-    static constexpr int kSmem = 1024 + kStages * kStage + kStaging + kTops + kMisc + kPad;
+    static constexpr int kPad = kStaging + kTops + kMiscBut >= 16384 ? 0 : 16384;
+    static constexpr int kFixed = 1024 + kStaging + kTops + kMiscBut + kPad;
+    static constexpr int turns(int stages) { return stages + kBuffers <= 8 ? 8 : stages + kBuffers <= 16 ? 16 : 32; }
+    static constexpr int bytes(int stages) { return kFixed + stages * kStage + turns(stages) * kPer * kScale * 4; }
+    static constexpr int most(int stages) { return stages <= 2 || bytes(stages) <= kSmemMost ? stages : most(stages - 1); }
+    static constexpr int kStages = most(16), kTurns = turns(kStages);   // kTurns: stages whose scales are kept
+    static constexpr int kSmem = bytes(kStages);
 };
 
 struct Tile {
@@ -155,6 +161,9 @@ __device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x,
             smem_addr(dst)),
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(smem_addr(bar))
         : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const float* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 // 16 bytes, or 16 zeros (bytes 0)
 __device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from, int bytes) {
@@ -306,10 +315,11 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
     uint64_t* const drain = join + 2;
     uint32_t* const s_tmem = (uint32_t*)(drain + 1);
     int* const s_fail = (int*)(s_tmem + 1);
-    int* const s_pre = (int*)((uint8_t*)full + 1024);
+    float* const s_scales = (float*)((uint8_t*)full + 640);                 // [kTurns][blocks of a stage][kScale]
+    int* const s_pre = (int*)(s_scales + C::kTurns * C::kPer * C::kScale);
     int* const s_off = s_pre + kQ8MaxGroups + 1;
     const uint8_t** const s_src = (const uint8_t**)(s_off + kQ8MaxGroups + 1);     // [128] rows of x of the tile that is being fetched
-    static_assert((2 * 16 + 4 * 8 + 3) * 8 + 8 <= 1024, "the barriers have their place");
+    static_assert((2 * 16 + 4 * 8 + 3) * 8 + 8 <= 640, "the barriers have their place");
 
     const Q8Args& a = c.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -317,11 +327,11 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
     early_launch();
     if (warp == 0 && lane == 0) {
         for (int i = 0; i < S; i++) {
-            sync::mbar_init(full + i, 1 + (a.rows ? 32 : 1) + (a.test_extra == 1));
-            sync::mbar_init(empty + i, 2);
+            sync::mbar_init(full + i, 1 + (a.rows ? 0 : 1) + 32 + (a.test_extra == 1));
+            sync::mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 2 * B; i++) {
-            sync::mbar_init(tfull + i, C::kPer + (a.test_extra == 2));
+            sync::mbar_init(tfull + i, 1 + (a.test_extra == 2));
             sync::mbar_init(tempty + i, C::kActive / C::kSets);
         }
         for (int i = 0; i < 2; i++) sync::mbar_init(join + i, CL * C::kParts * MT + (a.test_extra == 3));
@@ -370,18 +380,30 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
     volatile int* const fail = s_fail;
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kParts == 2 ? 40 : 32));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kParts == 2 ? 72 : 32));
         int stage = 0;
         bool go = true;
         Walk walk(groups);
         if (warp == 0 || warp == 2) {       // copies of the weight, of x
             const bool of_x = warp == 2;
-            int filled = 0;
+            int filled = 0, turn = 0;
             uint32_t parity = 1;
             while (go && walk.next()) {
                 const Tile tile = groups.at(walk.t);
                 const int n0 = SW ? tile.col * kQ8Block + rank * (NT / 2) : tile.col * NT;
                 const bool tall = MT == 128 && tile.rows > 32;      // one box of 128 rows, else of 32
+                const float* scales[MT / 32];                       // of x's rows lane, lane + 32, ..
+                const float* wscale = nullptr;                      // lanes 0 and 1
+                if (of_x) {
+#pragma unroll
+                    for (int i = 0; i < MT / 32; i++) {
+                        const int r = tile.first + min(lane + 32 * i, tile.rows - 1), src = a.rows ? a.rows[r] : r;
+                        scales[i] = a.xs + (long)(src >= 0 && src < a.n_x ? src : 0) * a.xs_row;
+                    }
+                    const int nb = (a.n + kQ8Block - 1) / kQ8Block, second = lane & 1;
+                    const int block = SW ? tile.col : min(tile.col * NT + second * (NT / 2), a.n - 1) / kQ8Block;
+                    wscale = a.ws + ((long)tile.group * (SW ? 2 * nb : nb) + block + (SW ? second * nb : 0)) * kb;
+                }
                 if (of_x && a.rows) {
                     __syncwarp();
                     for (int r = lane; r < tile.rows; r += 32) {
@@ -414,7 +436,6 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                             }
                             for (; r < tile.rows; r += 4) copy16(((r - sub) & 4 ? odd : even) + (r - sub) * 128, s_src[r] + from, bytes);
                         }
-                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(full + stage)) : "memory");
                     } else if (elect_one()) {
                         sync::mbar_expect_tx(full + stage, (uint32_t)here * (!of_x ? C::kB : tall ? 16384 : 4096));
 #pragma unroll
@@ -430,6 +451,16 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                             }
                         }
                     }
+                    if (of_x) {
+                        for (int j = 0; j < here; j++) {
+                            const uint32_t to = smem_addr(s_scales + (turn * C::kPer + j) * C::kScale);
+#pragma unroll
+                            for (int i = 0; i < MT / 32; i++) copy4(to + (lane + 32 * i) * 4, scales[i] + b + j);
+                            if (lane < 2) copy4(to + (MT + lane) * 4, wscale + b + j);
+                        }
+                        if (++turn == C::kTurns) turn = 0;
+                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(full + stage)) : "memory");
+                    }
                     __syncwarp();
                     filled = min(filled + 1, S);
                     if (++stage == S) stage = 0, parity ^= 1;
@@ -442,36 +473,45 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                 const uint64_t t0 = sync::global_ns();
                 while (!sync::mbar_try(full + stage, parity ^ 1) && sync::global_ns() - t0 < 10000000ull) {}
             }
-        } else {        // products: of one half of the weight's rows, or of every second block
+        } else {        // products of every second stage, in two parts: halves of the weight's rows, or the stage's two blocks
             constexpr int N = NT / C::kSets;
             constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-            const int which = warp >> 1, set = C::kSets == 2 ? which : 0;
-            const uint32_t off_a = C::kSets == 2 ? 0 : which * C::kA, off_b = C::kPer * C::kA + which * (C::kSets == 2 ? C::kB / 2 : C::kB);
-            int buf = 0;
+            constexpr uint32_t step_a = C::kSets == 2 ? 0 : C::kA, step_b = C::kSets == 2 ? C::kB / 2 : C::kB;
+            const int which = warp >> 1, per_tile = (kb + C::kPer - 1) / C::kPer;
+            const long tiles = groups.total > groups.me ? (groups.total - groups.me + groups.at_once - 1) / groups.at_once : 0;
+            int buf = which % B, at = which % per_tile;
+            stage = which;
             uint32_t parity = 0, bparity = 1;
-            while (go && walk.next()) {
-                for (int b = 0; b < kb; b += C::kPer) {
-                    go = wait_bar(tempty + set * B + buf, bparity, fail, a.wait_ns, kStatusBuffer) &&
-                         wait_bar(full + stage, parity, fail, a.wait_ns, kStatusOperands);
-                    go = __all_sync(0xffffffffu, go);
-                    if (!go) break;
-                    if (a.rows) sync::fence_proxy_async();      // rows came by copies of the generic proxy
-                    tc_fence_after();
-                    if (elect_one()) {
-                        if (C::kSets == 2 || b + which < kb) {
-                            const uint64_t da = sdesc_sw128(smem_addr(ring + stage * C::kStage + off_a));
-                            const uint64_t db = sdesc_sw128(smem_addr(ring + stage * C::kStage + off_b));
-                            const uint32_t d = tmem + buf * (C::kPer * NT) + which * N;
+            const uint64_t desc_a = sdesc_sw128(smem_addr(ring)), desc_b = sdesc_sw128(smem_addr(ring + C::kPer * C::kA));
+            for (long i = which; i < tiles * per_tile; i += 2) {
+                go = __all_sync(0xffffffffu, wait_bar(full + stage, parity, fail, a.wait_ns, kStatusOperands));
+                if (!go) break;
+                if (a.rows) sync::fence_proxy_async();      // rows came by copies of the generic proxy
+                const uint64_t da = desc_a + (uint32_t)(stage * (C::kStage >> 4)), db = desc_b + (uint32_t)(stage * (C::kStage >> 4));
 #pragma unroll
-                            for (int j = 0; j < 4; j++) mma_f8(d, da + 2 * j, db + 2 * j, idesc, j > 0);
+                for (int h = 0; h < 2; h++) {
+                    if (h < C::kSets) {     // the buffer after the operands: it is what comes late
+                        go = __all_sync(0xffffffffu, wait_bar(tempty + h * B + buf, bparity, fail, a.wait_ns, kStatusBuffer));
+                        if (!go) break;
+                        tc_fence_after();
+                    }
+                    if (elect_one()) {
+                        if (C::kSets == 2 || h == 0 || at * C::kPer + h < kb) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                mma_f8(tmem + buf * (C::kPer * NT) + h * N, da + ((h * step_a) >> 4) + 2 * j, db + ((h * step_b) >> 4) + 2 * j,
+                                       idesc, j > 0);
                         }
-                        tc_commit(empty + stage);
-                        tc_commit(tfull + set * B + buf);
+                        if (C::kSets == 2 || h == 1) tc_commit(tfull + (C::kSets == 2 ? h * B : 0) + buf);
+                        if (h == 1) tc_commit(empty + stage);
                     }
                     __syncwarp();
-                    if (++stage == S) stage = 0, parity ^= 1;
-                    if (++buf == B) buf = 0, bparity ^= 1;
                 }
+                if (!go) break;
+                stage += 2, buf += 2, at += 2;
+                if (stage >= S) stage -= S, parity ^= 1;
+                if (buf >= B) buf -= B, bparity ^= 1;
+                while (at >= per_tile) at -= per_tile;
             }
             // whatever happened, products in flight end before their TMEM is freed
             if (elect_one()) tc_commit(drain);
@@ -480,12 +520,10 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             while (!sync::mbar_try(drain, 0) && sync::global_ns() - t0 < sync::kWaitLimitNs) {}
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kParts == 2 ? 232 : 112));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kParts == 2 ? 216 : 112));
         const int quarter = warp & 3, part = (warp - 4) >> 2;
         if (quarter * 32 < MT) {
             constexpr int COLS = NT / C::kParts;            // of this warp; with SwiGLU half of them gate, half up
-            constexpr int CH = 4;                           // blocks whose scales are fetched together, as many ahead
-            const int nb = (a.n + kQ8Block - 1) / kQ8Block;
             // this warp's columns of a buffer (with SwiGLU those of gate, and those of up behind)
             const int set = C::kSets == 2 ? part / (C::kParts / 2) : 0;
             const uint32_t columns = tmem + ((uint32_t)(quarter * 32) << 16) + set * (NT / 2) +
@@ -494,101 +532,57 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             uint8_t* const mine = staging + (part * (MT / 32) + quarter) * (kStagingWarp / (C::kParts / 2));
             uint64_t* const my_full = tfull + set * B;
             uint64_t* const my_empty = tempty + set * B;
-            int buf = 0, turn = 0, joins = 0;
+            int buf = 0, turn = 0, joins = 0, slot = 0;
             uint32_t parity = 0;
-
-            // scales, fetched ahead through the ends of tiles: those of block `at_b` of tile `at_t` come next
-            const float *px = nullptr, *pw = nullptr, *pu = nullptr;
-            Walk ahead(groups);
-            bool more = ahead.next();
-            Tile coming{};                                  // the tile of the blocks that were fetched last
-            bool coming_zero = false;
-            int at_b = 0;
-            float nx[CH], nw = 0.f, nu = 0.f;               // lane i has the weight's scale of block i
-#pragma unroll
-            for (int i = 0; i < CH; i++) nx[i] = 0.f;
-            auto row_of = [&](const Tile& tile) {       // this lane's row of x; outside x: not there
-                const int r = min(quarter * 32 + lane, tile.rows - 1);
-                return a.rows ? a.rows[tile.first + r] : tile.first + r;
-            };
-            auto fetch = [&] {
-                if (!more) return;
-                if (at_b == 0) {
-                    const Tile tile = coming = groups.at(ahead.t);
-                    const int src = row_of(tile);
-                    coming_zero = src < 0 || src >= a.n_x;
-                    px = a.xs + (long)(src >= 0 && src < a.n_x ? src : 0) * a.xs_row;
-                    if constexpr (SW) {
-                        pw = a.ws + ((long)tile.group * 2 * nb + tile.col) * kb;
-                        pu = pw + (long)nb * kb;
-                    } else {
-                        pw = a.ws + ((long)tile.group * nb + min(tile.col * NT + part * COLS, a.n - 1) / kQ8Block) * kb;
-                    }
-                }
-                const int mine_b = min(at_b + (lane & (CH - 1)), kb - 1);
-                nw = pw[mine_b];
-                if constexpr (SW) nu = pu[mine_b];
-                if (c.vec_xs && at_b + CH <= kb) {
-                    const float4 v = *reinterpret_cast<const float4*>(px + at_b);
-                    nx[0] = v.x, nx[1] = v.y, nx[2] = v.z, nx[3] = v.w;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < CH; i++)
-                        if (at_b + i < kb) nx[i] = px[at_b + i];
-                }
-                at_b += CH;
-                if (at_b >= kb) at_b = 0, more = ahead.next();
-            };
-            fetch();
 
             bool go = true, ready = false;
             Walk walk(groups);
             bool left = walk.next();
             for (; left; left = walk.next()) {
-                const Tile now = coming;
-                const bool zero = coming_zero;
+                const Tile now = groups.at(walk.t);
                 float2 acc[SW ? COLS / 4 : COLS / 2] = {}, acc_u[SW ? COLS / 4 : 1] = {};
                 const bool idle = quarter * 32 >= now.rows;
                 uint64_t* done = nullptr;
                 uint32_t at = 0;
-                for (int b0 = 0; go && b0 < kb; b0 += CH) {
-                    float cx[CH];
-                    const float cw = nw, cu = nu;
-#pragma unroll
-                    for (int i = 0; i < CH; i++) cx[i] = nx[i];
-                    fetch();
-                    // one copy of the code: the instruction cache is too small for four
+                // one copy of the code: the instruction cache is too small for several
 #pragma unroll 1
-                    for (int i = 0; i < CH && b0 + i < kb; i++) {
-                        const int j = C::kPer == 1 ? 0 : i % C::kPer;
-                        if (j == 0) {
-                            if (!ready && !__all_sync(0xffffffffu, wait_bar(my_full + buf, parity, fail, a.wait_ns, kStatusProduct))) {
-                                go = false;
-                                break;
-                            }
-                            tc_fence_after();
-                            done = my_empty + buf;
-                            at = columns + buf * (C::kPer * NT);
-                            if (++buf == B) buf = 0, parity ^= 1;
+                for (int b = 0; b < kb; b++) {
+                    const int j = C::kPer == 1 ? 0 : b % C::kPer;
+                    if (j == 0) {
+                        if (!ready && !__all_sync(0xffffffffu, wait_bar(my_full + buf, parity, fail, a.wait_ns, kStatusProduct))) {
+                            go = false;
+                            break;
                         }
-                        auto read = [&] {       // the buffer is free, and whether the next one is full is known by the time it matters
-                            if (C::kPer > 1 && j != C::kPer - 1 && b0 + i + 1 < kb) return;
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(done)) : "memory");
-                            ready = __all_sync(0xffffffffu, test_bar(my_full + buf, parity));
-                        };
-                        const float s = cx[0] * __shfl_sync(0xffffffffu, cw, i), u = SW ? cx[0] * __shfl_sync(0xffffffffu, cu, i) : 0.f;
-                        cx[0] = cx[1], cx[1] = cx[2], cx[2] = cx[3];
-                        if (idle) {
-                            read();
-                        } else if constexpr (SW) {
-                            add_block<COLS / 2>(acc, at + j * NT, s, [] {});
-                            add_block<COLS / 2>(acc_u, at + j * NT + to_up, u, read);
-                        } else {
-                            add_block<COLS>(acc, at + j * NT, s, read);
-                        }
+                        tc_fence_after();
+                        done = my_empty + buf;
+                        at = columns + buf * (C::kPer * NT);
+                        if (++buf == B) buf = 0, parity ^= 1;
                     }
+                    const float* const sc = s_scales + (slot * C::kPer + j) * C::kScale;
+                    const float sx = sc[quarter * 32 + lane];
+                    const float2 sw = *reinterpret_cast<const float2*>(sc + MT);
+                    const bool last = C::kPer == 1 || j == C::kPer - 1 || b + 1 == kb;
+                    if (last && ++slot == C::kTurns) slot = 0;
+                    auto read = [&] {       // the buffer is free, and whether the next one is full is known by the time it matters
+                        if (!last) return;
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(done)) : "memory");
+                        ready = __all_sync(0xffffffffu, test_bar(my_full + buf, parity));
+                    };
+                    if (idle) {
+                        read();
+                    } else if constexpr (SW) {
+                        add_block<COLS / 2>(acc, at + j * NT, sx * sw.x, [] {});
+                        add_block<COLS / 2>(acc_u, at + j * NT + to_up, sx * sw.y, read);
+                    } else {
+                        add_block<COLS>(acc, at + j * NT, sx * (part * COLS < NT / 2 ? sw.x : sw.y), read);
+                    }
+                }
+                bool zero = false;      // a row that takes none of x's
+                if (a.rows && quarter * 32 + lane < now.rows) {
+                    const int src = a.rows[now.first + quarter * 32 + lane];
+                    zero = src < 0 || src >= a.n_x;
                 }
                 if (!go) break;
                 const int rows = min(now.rows - quarter * 32, 32);
@@ -750,7 +744,6 @@ bool launch_k(const Q8Args& a, cudaStream_t s) {
     c.n_tiles = SW ? (a.n + kQ8Block - 1) / kQ8Block : (a.n + NT - 1) / NT;
     const int elem = SW ? 1 : dtype_bytes(a.dtype);
     c.vec = aligned16(a.out, a.out_row, 0, elem) || (a.n_rows == 1 && aligned16(a.out));
-    c.vec_xs = aligned16(a.xs, a.xs_row, 0, 4);
     const cuuint64_t xd[2] = {(cuuint64_t)a.k, (cuuint64_t)a.n_x};
     const cuuint64_t xst[1] = {(cuuint64_t)(a.n_x == 1 ? (a.k + 15) / 16 * 16 : a.x_row)};
     const cuuint32_t xbox[2] = {128, 32};
