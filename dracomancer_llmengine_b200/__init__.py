@@ -183,6 +183,7 @@ _SIGS = {
     "draco_b200_rmsnorm_q8": ([ct.POINTER(DracoNormQ8), _vp], ct.c_int),
     "draco_b200_linear_q8": ([ct.POINTER(DracoLinearQ8), _vp], ct.c_int),
     "draco_b200_test_q8_barrier_extra": ([ct.c_int], ct.c_int),
+    "draco_b200_test_q8_form": ([ct.c_int], ct.c_int),
     "draco_b200_plan_experts": ([_vp] + [ct.c_int] * 4 + [_vp] * 4, ct.c_int),
     "draco_b200_combine_experts": ([ct.POINTER(DracoCombineExperts), _vp], ct.c_int),
 }

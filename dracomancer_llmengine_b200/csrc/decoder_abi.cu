@@ -41,7 +41,7 @@ int launched(const char* who, int kernels) {
 // each address again would take as long as the launch
 thread_local bool t_pointers_checked = false;
 thread_local int t_test_extra = 0;
-thread_local int t_test_q8_extra = 0;
+thread_local int t_test_q8_extra = 0, t_test_q8_form = 0;
 bool on_device(std::initializer_list<const void*> ps) {
     if (t_pointers_checked) return true;
     for (const void* p : ps)
@@ -118,6 +118,14 @@ int draco_b200_test_kv4_barrier_extra(int which) {
 int draco_b200_test_q8_barrier_extra(int which) {
     const int old = t_test_q8_extra;
     if (which >= 0 && which <= 3) t_test_q8_extra = which;
+    return old;
+}
+// for tests, of this thread's next calls of the 8-bit products: 1 the form for few rows, 2 the one for any address, 32 to 256 the
+// tensor cores with so many columns a tile, 0 (the default) the one that is chosen; returns the old value
+int draco_b200_test_q8_form(int form) {
+    const int old = t_test_q8_form;
+    if (form >= 0 && form <= 2) t_test_q8_form = form;
+    if (form == 32 || form == 64 || form == 128 || form == 256) t_test_q8_form = form;
     return old;
 }
 // the id of the graph capture that the stream is in, 0: none
@@ -268,7 +276,7 @@ int draco_b200_linear_q8(const DracoLinearQ8* p, void* stream) {
     const Q8Args a{(const uint8_t*)p->x, p->x_scales, (const uint8_t*)p->w, p->w_scales, p->offsets, p->rows, p->out,
                    p->out_scales, p->x_stride, p->x_scales_stride, p->out_stride, p->out_scales_stride, p->n_x, p->n_rows,
                    p->n, p->k, p->n_groups, p->dtype, p->swiglu != 0, p->status,
-                   p->wait_limit_us ? p->wait_limit_us * 1000l : 2000000000l, t_test_q8_extra};
+                   p->wait_limit_us ? p->wait_limit_us * 1000l : 2000000000l, t_test_q8_extra, t_test_q8_form};
     if (!launch_q8(a, (cudaStream_t)stream)) {
         cudaGetLastError();
         refuse("%s: the launch could not be set up", who);

@@ -26,7 +26,9 @@ struct Q8Args {
     int* status;                // or null: waits that ran out are noted there
     long wait_ns;               // their limit
     int test_extra;             // 1, 2, 3: an arrival that never comes is expected at a barrier (tests)
+    int test_form;              // 0: the form is chosen; kQ8Few, kQ8Any, or the tensor cores' columns a tile (tests)
 };
+constexpr int kQ8Few = 1, kQ8Any = 2;
 // false: a CUDA call before the launch failed
 bool launch_q8(const Q8Args& a, cudaStream_t s);
 bool q8_tc_fits(const Q8Args& a);

@@ -3,8 +3,8 @@
 //   out[m][n] = sum over blocks b of xs[m][b] * ws[n / 128][b] * (sum over the block of x[m][k] * w[n][k])
 //
 // Weights go from memory straight into the operand registers of mma.m16n8k32 (16 weight rows, 8 rows of x, 32 inner values):
-// the order of the inner values does not matter as long as both operands have the same, so a lane takes 32 neighbouring
-// bytes of its rows in every block of 128, two loads of 16 bytes a row, and no byte passes through shared memory.  A block's
+// the order of the inner values does not matter as long as both operands have the same, so a lane takes 16 neighbouring
+// bytes of its rows in each half of a block of 128 (four lanes a row, whole sectors), and no byte passes through shared memory.  A block's
 // sums are scaled and added in registers.  A block of threads has 16 weight rows (with SwiGLU 16 of gate and 16 of up), its
 // warps share the inner size; they add up through shared memory, in the order of the warps.  With SwiGLU eight blocks of
 // threads, a cluster, have the 128 columns that share a scale and exchange their rows' maxima through distributed shared memory.
@@ -43,7 +43,7 @@ __device__ __forceinline__ uint4 load_once(const uint8_t* p) {
     return v;
 }
 
-// 32 bytes of a row as eight operand words
+// a lane's 16 bytes in each half of a row's block, as eight operand words
 struct Bytes32 {
     uint32_t w[8];
     template <bool ONCE>
@@ -51,7 +51,7 @@ struct Bytes32 {
         uint4 u[2] = {};
 #pragma unroll
         for (int i = 0; i < 2; i++)
-            if (left > 16 * i) u[i] = ONCE ? load_once(p + 16 * i) : *reinterpret_cast<const uint4*>(p + 16 * i);
+            if (left > 64 * i) u[i] = ONCE ? load_once(p + 64 * i) : *reinterpret_cast<const uint4*>(p + 64 * i);
         w[0] = u[0].x, w[1] = u[0].y, w[2] = u[0].z, w[3] = u[0].w;
         w[4] = u[1].x, w[5] = u[1].y, w[6] = u[1].z, w[7] = u[1].w;
     }
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
     for (int p = 0; p < P; p++) {
         const int r = source(p * 8 + g);
         ok[p] = r >= 0;
-        px[p] = a.x + (size_t)max(r, 0) * a.x_row + 32 * t;
+        px[p] = a.x + (size_t)max(r, 0) * a.x_row + 16 * t;
 #pragma unroll
         for (int i = 0; i < 2; i++) ps[p][i] = a.xs + (long)max(source(p * 8 + 2 * t + i), 0) * a.xs_row;
     }
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
     for (int i = 0; i < MATS; i++) {
         const size_t mat = (size_t)at.group * MATS + i;
 #pragma unroll
-        for (int j = 0; j < 2; j++) pw[i][j] = a.w + (mat * a.n + min(n0 + g + 8 * j, a.n - 1)) * a.k + 32 * t;
+        for (int j = 0; j < 2; j++) pw[i][j] = a.w + (mat * a.n + min(n0 + g + 8 * j, a.n - 1)) * a.k + 16 * t;
         pws[i] = a.ws + (mat * nb + min(n0, a.n - 1) / kQ8Block) * kb;
     }
     float acc[MATS][P][4] = {};
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
             const int b = b0 + u, k0 = b * kQ8Block;
-            const int left = b < end ? a.k - k0 - 32 * t : 0;
+            const int left = b < end ? a.k - k0 - 16 * t : 0;
 #pragma unroll
             for (int i = 0; i < MATS; i++)
 #pragma unroll
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
             const int b = b0 + u, k0 = b * kQ8Block, bs = min(b, kb - 1);
-            const int left = b < end ? a.k - k0 - 32 * t : 0;
+            const int left = b < end ? a.k - k0 - 16 * t : 0;
 #pragma unroll
             for (int p = 0; p < P; p++) {
                 x[u][p].template load<false>(px[p] + k0, ok[p] ? left : 0);

@@ -29,7 +29,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
 
 namespace draco {
 namespace {
@@ -778,8 +777,9 @@ bool launch_k(const Q8Args& a, cudaStream_t s) {
 
 template <int MT, bool SW>
 bool launch_n(const Q8Args& a, int nt, cudaStream_t s) {
-    return nt == 256 ? launch_k<MT, 256, SW>(a, s) : nt == 128 ? launch_k<MT, 128, SW>(a, s)
-           : nt == 64 ? launch_k<MT, 64, SW>(a, s) : launch_k<MT, 32, SW>(a, s);
+    if constexpr (!SW)
+        if (nt == 32) return launch_k<MT, 32, SW>(a, s);
+    return nt == 256 ? launch_k<MT, 256, SW>(a, s) : nt == 128 ? launch_k<MT, 128, SW>(a, s) : launch_k<MT, 64, SW>(a, s);
 }
 
 }  // namespace
@@ -788,24 +788,37 @@ bool q8_tc_fits(const Q8Args& a) {
     return a.n_x > 0 && a.k % 16 == 0 && aligned16(a.x) && aligned16(a.w) && (a.n_x == 1 || (a.x_row % 16 == 0 && a.x_row >= a.k));
 }
 
+// The widest tile is not the fastest where it leaves SMs without one: the narrower ones make more tiles.  A tile takes about
+// as long as its blocks of inner values (us a block and for the rest, measured: rows of 128, inner sizes 512 to 7168; a block
+// of a narrow tile takes what its copies' and products' hand-over takes), and tiles run in rounds of as many as there is room for.
 bool launch_q8_tc(const Q8Args& a, cudaStream_t s) {
+    static const struct { int nt; float block, rest; } kTiles[] = {{256, 0.50f, 3.0f}, {128, 0.39f, 1.5f}, {64, 0.30f, 1.0f}, {32, 0.29f, 0.8f}};
     const bool few = a.offsets ? (long)a.n_rows <= 16l * a.groups : a.n_rows <= 32;
     const int mt = few ? 32 : 128;
     const long row_tiles = (a.n_rows + mt - 1) / mt + (a.offsets ? std::min(a.groups, a.n_rows) - 1 : 0);
-    // the widest tile that gives every SM one
-    const long cols = a.swiglu ? 2l * a.n : a.n;
+    const int kb = (a.k + kQ8Block - 1) / kQ8Block;
     int nt = 256;
-    if (const char* f = getenv("Q8_NT")) nt = atoi(f);
-    else while (nt > 32 && row_tiles * ((cols + nt - 1) / nt) < 148) nt >>= 1;
+    float best = 0.f;
+    for (const auto& t : kTiles) {
+        if (a.swiglu && t.nt == 32) continue;
+        const long tiles = row_tiles * (a.swiglu ? (a.n + kQ8Block - 1) / kQ8Block : (a.n + t.nt - 1) / t.nt);
+        const long room = 148 / (a.swiglu ? 256 / t.nt : 1);
+        const float time = (float)((tiles + room - 1) / room) * (kb * t.block + t.rest);
+        if (t.nt == 256 || time < best) best = time, nt = t.nt;
+    }
+    if (a.test_form >= 32) nt = a.swiglu && a.test_form == 32 ? 64 : a.test_form;
     if (a.swiglu) return few ? launch_n<32, true>(a, nt, s) : launch_n<128, true>(a, nt, s);
     return few ? launch_n<32, false>(a, nt, s) : launch_n<128, false>(a, nt, s);
 }
 
+// Few rows: the form whose weights go straight to registers (7 us against 16 for 16 rows, 2048 x 7168; 12 against 8 for 32
+// rows, 7168 x 2048; by expert 56 against 76 for 16 rows of 2048 x 7168, 97 against 90 for 32).
 bool launch_q8(const Q8Args& a, cudaStream_t s) {
-    if (!q8_tc_fits(a)) return launch_q8_any(a, s);
-    const char* few = getenv("Q8_FEW");
-    if (few ? atoi(few) >= a.n_rows : a.n_rows <= 16) return launch_q8_few(a, s);
-    return launch_q8_tc(a, s);
+    if (!q8_tc_fits(a) || a.test_form == kQ8Any) return launch_q8_any(a, s);
+    const double cost = (double)q8_slots(a, 8) * (a.swiglu ? 2 : 1) * a.n * a.k;
+    bool few = a.offsets ? a.n_rows <= 16 || cost <= 60e6 : a.n_rows <= 8 || cost <= 30e6;
+    if (a.test_form) few = a.test_form == kQ8Few;
+    return few ? launch_q8_few(a, s) : launch_q8_tc(a, s);
 }
 
 }  // namespace draco

@@ -19,7 +19,12 @@ DEV = "cuda"
 
 @pytest.fixture(autouse=True)
 def _gpu(dlib):
-    pass
+    yield
+    dlib.draco_b200_test_q8_form(0)
+
+
+# the forms that a call can take: chosen by sizes, for few rows, for any address, on the tensor cores by columns a tile
+FORMS = [0, 1, 2, 32, 64, 128, 256]
 
 
 def gen_of(seed):
@@ -84,6 +89,16 @@ def test_linear(rows, k, n, kind):
     same(out, want, bound, kind)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("form", FORMS[1:])
+@pytest.mark.parametrize("rows,k,n", [(1, 128, 16), (9, 1040, 130), (33, 2064, 257), (130, 640, 1001), (500, 512, 768)])
+def test_linear_forms(rows, k, n, form, kind, dlib):
+    """Every form on sizes that it would not be chosen for."""
+    x, xs, w, ws = operands(rows, k, n, gen_of(rows + k + n))
+    dlib.draco_b200_test_q8_form(form)
+    same(decoder.linear_q8(x, xs, w, ws, torch.full((rows, n), float("nan"), dtype=TYPES[kind], device=DEV)), *plain(x, xs, w, ws), kind)
+
+
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("off", [16, 3])
 def test_linear_strides(kind, off):
@@ -111,10 +126,12 @@ def test_linear_one_row_for_all():
     same(out, *plain(x.expand(9, 128), xs.expand(9, 1), w, ws), "f32")
 
 
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("rows,k,n", [(1, 128, 64), (40, 256, 300), (200, 512, 256)])
-def test_not_finite_stays_in_its_row(rows, k, n):
+def test_not_finite_stays_in_its_row(rows, k, n, form, dlib):
     """A NaN code or scale, or an infinite scale, reaches its own row, or its own column, alone."""
     gen = gen_of(rows)
+    dlib.draco_b200_test_q8_form(form)
     x, xs, w, ws = operands(rows, k, n, gen)
     clean = decoder.linear_q8(x, xs, w, ws, torch.empty(rows, n, device=DEV)).clone()
     bad = rows // 2
@@ -156,7 +173,9 @@ def of_row(x, rows, a, b):
 @pytest.mark.parametrize("gather", [False, True])
 @pytest.mark.parametrize("k,n", [(512, 256), (272, 1001), (40, 33), (128, 2048)])
 @pytest.mark.parametrize("counts", COUNTS)
-def test_grouped(counts, k, n, gather, kind):
+@pytest.mark.parametrize("form", FORMS)
+def test_grouped(counts, k, n, gather, kind, form, dlib):
+    dlib.draco_b200_test_q8_form(form)
     counts = COUNTS[counts]
     x, xs, w, ws, offsets, rows = group_args(counts, k, n, gather, k + n)
     total, behind = sum(counts), 3
@@ -176,7 +195,9 @@ def test_grouped(counts, k, n, gather, kind):
 
 
 @pytest.mark.parametrize("k", [256, 40])
-def test_rows_outside_x_give_zeros(k):
+@pytest.mark.parametrize("form", FORMS)
+def test_rows_outside_x_give_zeros(k, form, dlib):
+    dlib.draco_b200_test_q8_form(form)
     x, xs, w, ws = operands(4, k, 130, gen_of(3))
     x.view(torch.uint8)[0, 0] = 127       # the row that a careless kernel would read instead
     rows = ints(1, -1, 4, 2, -2147483648, 2147483647, 3)
@@ -199,10 +220,12 @@ def test_no_rows_of_x():
     assert decoder.linear_q8(x, xs, w, ws, torch.empty(0, 64, device=DEV)).numel() == 0
 
 
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("values", [(0, 40, 20, 60), (-5, 10, 20, 30), (0, 1000, 10, 5000), (50, 40, 30, 20), (7, 7, 7, 7)])
-def test_offsets_out_of_order_stay_inside(values):
+def test_offsets_out_of_order_stay_inside(values, form, dlib):
     """Such rows mean nothing, but nothing outside the output is touched."""
     x, xs, w, ws = operands(64, 128, 64, gen_of(5), (3,))
+    dlib.draco_b200_test_q8_form(form)
     buf = torch.full((66, 64), 3.0, device=DEV)
     decoder.linear_q8(x, xs, w, ws, buf[1:65], offsets=ints(*values))
     assert bool((buf[0] == 3).all() and (buf[65] == 3).all())
@@ -238,9 +261,11 @@ def check_swiglu(codes, scales, x, xs, w, ws):
         assert bool((codes[:, part].double().abs().amax(1) == 448).all())
 
 
+@pytest.mark.parametrize("form", [0, 1, 64, 128, 256])
 @pytest.mark.parametrize("rows,k,f", [(1, 7168, 2048), (1, 128, 128), (2, 256, 200), (7, 144, 16), (33, 512, 512), (3, 40, 33),
                                       (130, 2048, 768), (500, 1024, 129), (1000, 272, 640)])
-def test_swiglu(rows, k, f):
+def test_swiglu(rows, k, f, form, dlib):
+    dlib.draco_b200_test_q8_form(form)
     x, xs, w, ws = operands(rows, k, f, gen_of(rows + f), (2,))
     ws /= 500 * k ** 0.5
     codes, scales = torch.zeros(rows, f, device=DEV).to(E4M3), torch.full((rows, cdiv(f, 128)), 9.0, device=DEV)
@@ -251,7 +276,9 @@ def test_swiglu(rows, k, f):
 @pytest.mark.parametrize("gather", [False, True])
 @pytest.mark.parametrize("k,f", [(512, 256), (272, 200), (40, 33), (128, 1024)])
 @pytest.mark.parametrize("counts", COUNTS)
-def test_swiglu_grouped(counts, k, f, gather):
+@pytest.mark.parametrize("form", [0, 1, 64, 128, 256])
+def test_swiglu_grouped(counts, k, f, gather, form, dlib):
+    dlib.draco_b200_test_q8_form(form)
     counts = COUNTS[counts]
     x, xs, w, ws, offsets, rows = group_args(counts, k, f, gather, k + f, (2,))
     ws /= 500 * k ** 0.5
@@ -267,8 +294,10 @@ def test_swiglu_grouped(counts, k, f, gather):
     assert bool((buf[total:].float() == 7).all() and (buf[:, f:].float() == 7).all() and (sbuf[total:] == 7).all() and (sbuf[:, -1] == 7).all())
 
 
-def test_swiglu_extremes():
+@pytest.mark.parametrize("form", [0, 1, 2, 64, 128, 256])
+def test_swiglu_extremes(form, dlib):
     """Gates of both signs beyond exp's range, products of nothing, of tiny and of infinite size."""
+    dlib.draco_b200_test_q8_form(form)
     k, f = 128, 128
     x, w = torch.zeros(6, k, device=DEV), torch.zeros(2, f, k, device=DEV)
     x[:, 0], x[0, 0] = 1, 0
@@ -474,8 +503,8 @@ def test_stream_argument():
 
 @pytest.mark.parametrize("swiglu", [False, True])
 @pytest.mark.parametrize("which,bits", [(1, 0x101), (2, 0x102), (3, 0x104)])
-@pytest.mark.parametrize("rows,n", [(20, 256), (300, 512)])
-def test_waits_that_run_out(rows, n, which, bits, swiglu):
+@pytest.mark.parametrize("rows,n,form", [(20, 256, 64), (20, 256, 256), (300, 512, 32), (300, 512, 64), (300, 512, 128), (300, 512, 256)])
+def test_waits_that_run_out(rows, n, form, which, bits, swiglu):
     """Barriers of the tensor-core form that expect an arrival which never comes: the call ends, its rows are NaN, the status
     says which wait it was (others may have run out with it), and the next call is right."""
     if which == 3 and not swiglu:
@@ -488,6 +517,7 @@ def test_waits_that_run_out(rows, n, which, bits, swiglu):
     a.out, a.out_scales, a.out_scales_stride = out.data_ptr(), scales.data_ptr(), scales.shape[1]
     L = dm.lib()
     torch.cuda.synchronize()
+    L.draco_b200_test_q8_form(form)
     assert L.draco_b200_test_q8_barrier_extra(which) == 0
     try:
         assert L.draco_b200_linear_q8(a, None) == 0
