@@ -29,6 +29,7 @@ struct Q8Args {
     int test_form;              // 0: the form is chosen; kQ8Few, kQ8Any, or the tensor cores' columns a tile (tests)
 };
 constexpr int kQ8Few = 1, kQ8Any = 2;
+constexpr int kQ8FewMost = 1 << 16;     // inner size that the form for few rows has room for (its scales are in shared memory)
 // false: a CUDA call before the launch failed
 bool launch_q8(const Q8Args& a, cudaStream_t s);
 bool q8_tc_fits(const Q8Args& a);

@@ -2,12 +2,14 @@
 //
 //   out[m][n] = sum over blocks b of xs[m][b] * ws[n / 128][b] * (sum over the block of x[m][k] * w[n][k])
 //
-// Weights go from memory straight into the operand registers of mma.m16n8k32 (16 weight rows, 8 rows of x, 32 inner values):
-// the order of the inner values does not matter as long as both operands have the same, so a lane takes 16 neighbouring
-// bytes of its rows in each half of a block of 128 (four lanes a row, whole sectors), and no byte passes through shared memory.  A block's
-// sums are scaled and added in registers.  A block of threads has 16 weight rows (with SwiGLU 16 of gate and 16 of up), its
-// warps share the inner size; they add up through shared memory, in the order of the warps.  With SwiGLU eight blocks of
-// threads, a cluster, have the 128 columns that share a scale and exchange their rows' maxima through distributed shared memory.
+// Operands of mma.m16n8k32 (16 weight rows, 8 rows of x, 32 inner values).  The order of the inner values does not matter as
+// long as both operands have the same, so a lane takes 16 neighbouring bytes of its rows in each half of a block of 128 (four
+// lanes a row, whole sectors), by asynchronous copies into places of its own in shared memory: it reads only what it copied,
+// and no warp waits for another.  What is in flight is then bounded by shared memory, not by registers (a ring of registers
+// reached 64 KB an SM, too little for the memory's latency under load).  A block's sums are scaled and added in registers.  A
+// block of threads has 16 weight rows (with SwiGLU 16 of gate and 16 of up), its warps share the inner size; they add up
+// through shared memory, in the order of the warps.  With SwiGLU eight blocks of threads, a cluster, have the 128 columns that
+// share a scale and exchange their rows' maxima through distributed shared memory.
 #include "q8.cuh"
 
 #include <cooperative_groups.h>
@@ -22,14 +24,16 @@ namespace cg = cooperative_groups;
 
 constexpr float kTiny = 7.888609e-31f;   // 2^-100
 constexpr int kRows = 16;                // weight rows of a block of threads
-// blocks of 128 whose loads a warp has in flight: 16 loads of 16 bytes a lane, fewer where the rows of x take more registers
-template <int TOK, bool SW>
-constexpr int few_ahead() { return TOK == 8 && !SW ? 4 : 2; }
+constexpr int kFewSmem = 224 * 1024;
+// blocks of 128 that a warp has in flight
+template <bool SW>
+constexpr int few_ahead() { return SW ? 4 : 6; }
 
 struct Call {
     Q8Args a;
     int n_tiles;            // tiles of 16 weight rows (with SwiGLU whole clusters)
     int per_warp;           // blocks of a warp
+    int x_rows;             // rows of x that a tile has at most
 };
 
 __device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -37,33 +41,19 @@ __device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 load_once(const uint8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+// 16 bytes, or 16 zeros (bytes 0)
+__device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
-
-// a lane's 16 bytes in each half of a row's block, as eight operand words
-struct Bytes32 {
-    uint32_t w[8];
-    template <bool ONCE>
-    __device__ __forceinline__ void load(const uint8_t* p, int left) {      // bytes left in the row from p on
-        uint4 u[2] = {};
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            if (left > 64 * i) u[i] = ONCE ? load_once(p + 64 * i) : *reinterpret_cast<const uint4*>(p + 64 * i);
-        w[0] = u[0].x, w[1] = u[0].y, w[2] = u[0].z, w[3] = u[0].w;
-        w[4] = u[1].x, w[5] = u[1].y, w[6] = u[1].z, w[7] = u[1].w;
-    }
-};
 
 // TOK: rows of x of a tile, 8 or 16
 template <int TOK, bool SW>
 __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
     early_launch();
     wait_for_inputs();
-    constexpr int P = TOK / 8, MATS = SW ? 2 : 1, kAhead = few_ahead<TOK, SW>();
-    extern __shared__ float s_sum[];                // [warps][MATS][16][TOK]
+    constexpr int P = TOK / 8, MATS = SW ? 2 : 1, kAhead = few_ahead<SW>(), kScale = TOK + 2;     // a block's scales: rows of x, matrices
+    extern __shared__ __align__(16) uint8_t s_raw[];            // [warps][kAhead] blocks, later the sums; the warps' scales
+    float* const s_sum = (float*)s_raw;                         // [warps][MATS][16][TOK]
     __shared__ float s_h[kRows][TOK];
     __shared__ float s_top[8][TOK];
     const Q8Args& a = c.a;
@@ -80,70 +70,90 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
         return r >= 0 && r < a.n_x ? r : -1;
     };
     const uint8_t* px[P];                           // operand rows: g and g + 8
-    const float* ps[P][2];                          // rows of this lane's sums: 2 t, 2 t + 1 (and + 8)
     bool ok[P];
 #pragma unroll
     for (int p = 0; p < P; p++) {
         const int r = source(p * 8 + g);
         ok[p] = r >= 0;
         px[p] = a.x + (size_t)max(r, 0) * a.x_row + 16 * t;
-#pragma unroll
-        for (int i = 0; i < 2; i++) ps[p][i] = a.xs + (long)max(source(p * 8 + 2 * t + i), 0) * a.xs_row;
     }
-    const uint8_t* pw[MATS][2];
-    const float* pws[MATS];
+    const int begin = warp * c.per_warp, end = min(kb, begin + c.per_warp);
+    const uint8_t* pw = a.w + ((size_t)at.group * MATS * a.n + min(n0 + g, a.n - 1)) * a.k + 16 * t;       // weight row g; g + 8; those of up
+    const size_t below = (size_t)(min(n0 + g + 8, a.n - 1) - min(n0 + g, a.n - 1)) * a.k, up = (size_t)a.n * a.k;
+
+    // a block in shared memory: [matrix][row g, g + 8][half] 512 bytes, 16 a lane; then [half][row of x] 64 bytes
+    const int block = MATS * 2048 + c.x_rows * 128;
+    uint8_t* const ring = s_raw + (size_t)warp * kAhead * block;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    float* const scales = (float*)(s_raw + (size_t)warps * kAhead * block) + warp * c.per_warp * kScale;    // [block][rows of x, matrices]
+    auto fetch = [&](int u, int b) {
+        if (b < end) {
+            const int k0 = b * kQ8Block, left = a.k - k0 - 16 * t;
+            const uint32_t to = ring_at + u * block;
 #pragma unroll
-    for (int i = 0; i < MATS; i++) {
-        const size_t mat = (size_t)at.group * MATS + i;
+            for (int h = 0; h < 2; h++) {
+                const int bytes = left > 64 * h ? 16 : 0, o = bytes ? k0 + 64 * h : 0;
 #pragma unroll
-        for (int j = 0; j < 2; j++) pw[i][j] = a.w + (mat * a.n + min(n0 + g + 8 * j, a.n - 1)) * a.k + 16 * t;
-        pws[i] = a.ws + (mat * nb + min(n0, a.n - 1) / kQ8Block) * kb;
-    }
-    float acc[MATS][P][4] = {};
-    const int end = min(kb, (warp + 1) * c.per_warp);
-    for (int b0 = warp * c.per_warp; b0 < end; b0 += kAhead) {
-        Bytes32 w[kAhead][MATS][2], x[kAhead][P];
-        float sx[kAhead][P][2], sw[kAhead][MATS];
+                for (int i = 0; i < MATS; i++)
 #pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-            const int b = b0 + u, k0 = b * kQ8Block;
-            const int left = b < end ? a.k - k0 - 16 * t : 0;
+                    for (int j = 0; j < 2; j++)
+                        copy16(to + ((i * 2 + j) * 2 + h) * 512 + lane * 16, pw + (i ? up : 0) + (j ? below : 0) + o, bytes);
 #pragma unroll
-            for (int i = 0; i < MATS; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) w[u][i][j].template load<true>(pw[i][j] + k0, left);
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-            const int b = b0 + u, k0 = b * kQ8Block, bs = min(b, kb - 1);
-            const int left = b < end ? a.k - k0 - 16 * t : 0;
-#pragma unroll
-            for (int p = 0; p < P; p++) {
-                x[u][p].template load<false>(px[p] + k0, ok[p] ? left : 0);
-#pragma unroll
-                for (int i = 0; i < 2; i++) sx[u][p][i] = ps[p][i][bs];
+                for (int p = 0; p < P; p++)
+                    if (ok[p]) copy16(to + MATS * 2048 + (h * c.x_rows + p * 8 + g) * 64 + t * 16, px[p] + o, bytes);
             }
-#pragma unroll
-            for (int i = 0; i < MATS; i++) sw[u][i] = pws[i][bs];
         }
+        cp_commit();
+    };
+    for (int e = lane; e < (end - begin) * kScale; e += 32) {       // with the first block's copies
+        const int b = begin + e / kScale, m = e % kScale;
+        if (m >= TOK + MATS) continue;
+        const float* from = m < TOK ? a.xs + (long)max(source(m), 0) * a.xs_row
+                                    : a.ws + (((size_t)at.group * MATS + m - TOK) * nb + min(n0, a.n - 1) / kQ8Block) * kb;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(scales + e)), "l"(from + b) : "memory");
+    }
 #pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-            if (b0 + u >= end) break;
+    for (int u = 0; u < kAhead; u++) fetch(u, begin + u);
+    float acc[MATS][P][4] = {};
+    for (int b = begin, u = 0; b < end; b++) {
+        cp_wait<kAhead - 1>();
+        if (b == begin) __syncwarp();       // scales that other lanes copied
+        const float* const sc = scales + (b - begin) * kScale;
+        const uint8_t* const here = ring + u * block;
+        uint4 x[P][2];
 #pragma unroll
-            for (int i = 0; i < MATS; i++)
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                x[p][h] = ok[p] ? *reinterpret_cast<const uint4*>(here + MATS * 2048 + (h * c.x_rows + p * 8 + g) * 64 + t * 16)
+                                : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < MATS; i++) {
+            float d[P][4] = {};
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint4 lo = *reinterpret_cast<const uint4*>(here + ((i * 2 + 0) * 2 + h) * 512 + lane * 16),
+                            hi = *reinterpret_cast<const uint4*>(here + ((i * 2 + 1) * 2 + h) * 512 + lane * 16);
+                const uint32_t op0[4] = {lo.x, hi.x, lo.y, hi.y}, op1[4] = {lo.z, hi.z, lo.w, hi.w};
 #pragma unroll
                 for (int p = 0; p < P; p++) {
-                    float d[4] = {};
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t op[4] = {w[u][i][0].w[2 * j], w[u][i][1].w[2 * j], w[u][i][0].w[2 * j + 1], w[u][i][1].w[2 * j + 1]};
-                        mma_e4m3(d, op, x[u][p].w[2 * j], x[u][p].w[2 * j + 1]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[i][p][j] = fmaf(d[j], sx[u][p][j & 1] * sw[u][i], acc[i][p][j]);
+                    mma_e4m3(d[p], op0, x[p][h].x, x[p][h].y);
+                    mma_e4m3(d[p], op1, x[p][h].z, x[p][h].w);
                 }
+            }
+            const float sw = sc[TOK + i];
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+                const float2 sx = *reinterpret_cast<const float2*>(sc + p * 8 + 2 * t);
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[i][p][j] = fmaf(d[p][j], (j & 1 ? sx.y : sx.x) * sw, acc[i][p][j]);
+            }
         }
+        fetch(u, b + kAhead);
+        if (++u == kAhead) u = 0;
     }
+    cp_wait<0>();
+    __syncthreads();                                // the sums take the ring's place
     // [weight row][row of x]
 #pragma unroll
     for (int i = 0; i < MATS; i++)
@@ -200,18 +210,25 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
 
 template <int TOK, bool SW>
 bool launch_k(const Q8Args& a, cudaStream_t s) {
-    constexpr int kAhead = few_ahead<TOK, SW>();
-    Call c{a, 0, 0};
+    constexpr int kAhead = few_ahead<SW>(), MATS = SW ? 2 : 1;
+    Call c{a, 0, 0, a.offsets ? TOK : std::min(TOK, a.n_rows)};
     c.n_tiles = (a.n + kRows - 1) / kRows;
     if (SW) c.n_tiles = (c.n_tiles + 7) / 8 * 8;
     const int kb = (a.k + kQ8Block - 1) / kQ8Block;
     const long blocks = q8_slots(a, TOK) * c.n_tiles;
-    // 16 warps an SM have enough loads in flight; a warp has at least what it fetches at once
-    const int warps = (int)std::clamp<long>((148l * 16 + blocks - 1) / blocks, 1, std::min(16, (kb + kAhead - 1) / kAhead));
+    // As many warps as an SM's shared memory has room for, over the blocks of threads that it gets, which run at once where they
+    // can.  With SwiGLU two blocks of threads fit an SM: eight free SMs of one part of the GPU, which a cluster otherwise takes,
+    // may be hard to find (a last cluster that had to wait cost as much as all others together).
+    const int ring = kAhead * (MATS * 2048 + c.x_rows * 128);
+    const long room = std::min<long>(SW ? 8 : 16, (SW ? 104 : 208) * 1024 / (ring + (long)kb * (TOK + 2) * 4 / 8));
+    const int warps = (int)std::clamp<long>(room / ((blocks + 147) / 148), 1, std::min(16, (kb + 1) / 2));
     c.per_warp = (kb + warps - 1) / warps;
-    c.per_warp = (c.per_warp + kAhead - 1) / kAhead * kAhead;
     const int used = (kb + c.per_warp - 1) / c.per_warp;
-    const size_t smem = sizeof(float) * (size_t)used * (SW ? 2 : 1) * kRows * TOK;
+    const size_t sums = sizeof(float) * (size_t)MATS * kRows * TOK;
+    const size_t smem = (size_t)used * std::max<size_t>(ring, sums) + (size_t)used * c.per_warp * (TOK + 2) * sizeof(float);
+    if (smem > 40 * 1024 &&
+        cudaFuncSetAttribute(q8_few_kernel<TOK, SW>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) != cudaSuccess)
+        return false;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(used * 32);
@@ -231,7 +248,7 @@ bool launch_k(const Q8Args& a, cudaStream_t s) {
 
 bool launch_q8_few(const Q8Args& a, cudaStream_t s) {
     const bool eight = a.offsets || a.n_rows <= 8;
-    if (a.swiglu) return eight ? launch_k<8, true>(a, s) : launch_k<16, true>(a, s);
+    if (a.swiglu) return launch_k<8, true>(a, s);      // two matrices' weights leave no registers for more rows
     return eight ? launch_k<8, false>(a, s) : launch_k<16, false>(a, s);
 }
 

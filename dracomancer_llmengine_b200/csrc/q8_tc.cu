@@ -818,6 +818,7 @@ bool launch_q8(const Q8Args& a, cudaStream_t s) {
     const double cost = (double)q8_slots(a, 8) * (a.swiglu ? 2 : 1) * a.n * a.k;
     bool few = a.offsets ? a.n_rows <= 16 || cost <= 60e6 : a.n_rows <= 8 || cost <= 30e6;
     if (a.test_form) few = a.test_form == kQ8Few;
+    few = few && a.k <= kQ8FewMost;
     return few ? launch_q8_few(a, s) : launch_q8_tc(a, s);
 }
 
