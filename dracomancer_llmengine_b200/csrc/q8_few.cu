@@ -3,9 +3,8 @@
 //   out[m][n] = sum over blocks b of xs[m][b] * ws[n / 128][b] * (sum over the block of x[m][k] * w[n][k])
 //
 // Operands of mma.m16n8k32 (16 weight rows, 8 rows of x, 32 inner values).  The order of the inner values does not matter as
-// long as both operands have the same, so a lane takes 16 neighbouring bytes of its rows in each half of a block of 128 (four
-// lanes a row, whole sectors), by asynchronous copies into places of its own in shared memory: it reads only what it copied,
-// and no warp waits for another.  What is in flight is then bounded by shared memory, not by registers (a ring of registers
+// long as both operands have the same, so a lane takes 16 neighbouring bytes of its rows in each half of a block of 128.  They
+// come by asynchronous copies into a ring of the warp's own in shared memory: no warp waits for another.  What is in flight is then bounded by shared memory, not by registers (a ring of registers
 // reached 64 KB an SM, too little for the memory's latency under load).  A block's sums are scaled and added in registers.  A
 // block of threads has 16 weight rows (with SwiGLU 16 of gate and 16 of up), its warps share the inner size; they add up
 // through shared memory, in the order of the warps.  With SwiGLU eight blocks of threads, a cluster, have the 128 columns that
@@ -50,7 +49,6 @@ __device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from, int byt
 template <int TOK, bool SW>
 __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
     early_launch();
-    wait_for_inputs();
     constexpr int P = TOK / 8, MATS = SW ? 2 : 1, kAhead = few_ahead<SW>(), kScale = TOK + 2;     // a block's scales: rows of x, matrices
     extern __shared__ __align__(16) uint8_t s_raw[];            // [warps][kAhead] blocks, later the sums; the warps' scales
     float* const s_sum = (float*)s_raw;                         // [warps][MATS][16][TOK]
@@ -59,49 +57,58 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
     const Q8Args& a = c.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
     const int slot = blockIdx.x / c.n_tiles, tile = blockIdx.x % c.n_tiles;
+    const int kb = (a.k + kQ8Block - 1) / kQ8Block, nb = (a.n + kQ8Block - 1) / kQ8Block, n0 = tile * kRows, n_in = min(n0, a.n - 1);
+    const int begin = warp * c.per_warp, end = min(kb, begin + c.per_warp);
+    // The first weights' way into the L2 cache begins while the kernel before this one ends (a hint: what they are is read later,
+    // and the L2 cache holds what that kernel writes).
+    if (!a.offsets)
+        for (int e = lane; e < kAhead * MATS * kRows; e += 32) {
+            const int b = begin + e / (MATS * kRows), r = e % (MATS * kRows);
+            if (b < end)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(a.w + ((size_t)(r / kRows) * a.n + min(n0 + r % kRows, a.n - 1)) * a.k + b * kQ8Block));
+        }
+    wait_for_inputs();
     const Q8Where at = q8_locate<TOK>(a, slot);
     if (!at.count) return;                          // the same for a whole cluster
-    const int g = lane >> 2, t = lane & 3, n0 = tile * kRows;
-    const int kb = (a.k + kQ8Block - 1) / kQ8Block, nb = (a.n + kQ8Block - 1) / kQ8Block;
+    const int g = lane >> 2, t = lane & 3;
 
     auto source = [&](int m) {                      // row m's row of x, -1: none
         if (m >= at.count) return -1;
         const int r = a.rows ? a.rows[at.first + m] : at.first + m;
         return r >= 0 && r < a.n_x ? r : -1;
     };
-    const uint8_t* px[P];                           // operand rows: g and g + 8
-    bool ok[P];
+    // copies: eight lanes a row, so that a row's 128 bytes are one request; four rows a step
+    const int sub = lane >> 3, piece = lane & 7;
+    const uint8_t* px[TOK / 4];
+    bool there[TOK / 4];
 #pragma unroll
-    for (int p = 0; p < P; p++) {
-        const int r = source(p * 8 + g);
-        ok[p] = r >= 0;
-        px[p] = a.x + (size_t)max(r, 0) * a.x_row + 16 * t;
+    for (int i = 0; i < TOK / 4; i++) {
+        const int r = source(4 * i + sub);
+        there[i] = r >= 0;
+        px[i] = a.x + (size_t)max(r, 0) * a.x_row + 16 * piece;
     }
-    const int begin = warp * c.per_warp, end = min(kb, begin + c.per_warp);
-    const uint8_t* pw = a.w + ((size_t)at.group * MATS * a.n + min(n0 + g, a.n - 1)) * a.k + 16 * t;       // weight row g; g + 8; those of up
-    const size_t below = (size_t)(min(n0 + g + 8, a.n - 1) - min(n0 + g, a.n - 1)) * a.k, up = (size_t)a.n * a.k;
+    const uint8_t* const pw = a.w + ((size_t)at.group * MATS * a.n + n_in) * a.k + 16 * piece;
+    const size_t up = (size_t)a.n * a.k;
 
-    // a block in shared memory: [matrix][row g, g + 8][half] 512 bytes, 16 a lane; then [half][row of x] 64 bytes
-    const int block = MATS * 2048 + c.x_rows * 128;
+    // a block in shared memory: the weight's rows [matrix][16], then those of x, 128 bytes each; a row's pieces of 16 bytes are
+    // turned by it, so that the eight lanes that read two rows' halves at a time meet no bank twice
+    const int block = (MATS * kRows + c.x_rows) * 128;
     uint8_t* const ring = s_raw + (size_t)warp * kAhead * block;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    auto place = [](int row, int piece) { return row * 128 + ((piece ^ (row & 1) << 2) << 4); };
     float* const scales = (float*)(s_raw + (size_t)warps * kAhead * block) + warp * c.per_warp * kScale;    // [block][rows of x, matrices]
     auto fetch = [&](int u, int b) {
         if (b < end) {
-            const int k0 = b * kQ8Block, left = a.k - k0 - 16 * t;
+            const int k0 = b * kQ8Block, bytes = k0 + 16 * piece < a.k ? 16 : 0, o = bytes ? k0 : -16 * piece;     // behind a row: zeros
             const uint32_t to = ring_at + u * block;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int bytes = left > 64 * h ? 16 : 0, o = bytes ? k0 + 64 * h : 0;
-#pragma unroll
-                for (int i = 0; i < MATS; i++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++)
-                        copy16(to + ((i * 2 + j) * 2 + h) * 512 + lane * 16, pw + (i ? up : 0) + (j ? below : 0) + o, bytes);
-#pragma unroll
-                for (int p = 0; p < P; p++)
-                    if (ok[p]) copy16(to + MATS * 2048 + (h * c.x_rows + p * 8 + g) * 64 + t * 16, px[p] + o, bytes);
+            for (int i = 0; i < MATS * 4; i++) {
+                const int r = i % 4 * 4 + sub;
+                copy16(to + place(i * 4 + sub, piece), pw + (i / 4 ? up : 0) + (size_t)(min(n0 + r, a.n - 1) - n_in) * a.k + o, bytes);
             }
+#pragma unroll
+            for (int i = 0; i < TOK / 4; i++)
+                if (4 * i + sub < c.x_rows) copy16(to + place(MATS * kRows + 4 * i + sub, piece), px[i] + o, there[i] ? bytes : 0);
         }
         cp_commit();
     };
@@ -109,7 +116,7 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
         const int b = begin + e / kScale, m = e % kScale;
         if (m >= TOK + MATS) continue;
         const float* from = m < TOK ? a.xs + (long)max(source(m), 0) * a.xs_row
-                                    : a.ws + (((size_t)at.group * MATS + m - TOK) * nb + min(n0, a.n - 1) / kQ8Block) * kb;
+                                    : a.ws + (((size_t)at.group * MATS + m - TOK) * nb + n_in / kQ8Block) * kb;
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(scales + e)), "l"(from + b) : "memory");
     }
 #pragma unroll
@@ -117,7 +124,7 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
     float acc[MATS][P][4] = {};
     for (int b = begin, u = 0; b < end; b++) {
         cp_wait<kAhead - 1>();
-        if (b == begin) __syncwarp();       // scales that other lanes copied
+        __syncwarp();                       // what other lanes copied
         const float* const sc = scales + (b - begin) * kScale;
         const uint8_t* const here = ring + u * block;
         uint4 x[P][2];
@@ -125,15 +132,15 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
         for (int p = 0; p < P; p++)
 #pragma unroll
             for (int h = 0; h < 2; h++)
-                x[p][h] = ok[p] ? *reinterpret_cast<const uint4*>(here + MATS * 2048 + (h * c.x_rows + p * 8 + g) * 64 + t * 16)
-                                : make_uint4(0, 0, 0, 0);
+                x[p][h] = p * 8 + g < c.x_rows ? *reinterpret_cast<const uint4*>(here + place(MATS * kRows + p * 8 + g, 4 * h + t))
+                                               : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < MATS; i++) {
             float d[P][4] = {};
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const uint4 lo = *reinterpret_cast<const uint4*>(here + ((i * 2 + 0) * 2 + h) * 512 + lane * 16),
-                            hi = *reinterpret_cast<const uint4*>(here + ((i * 2 + 1) * 2 + h) * 512 + lane * 16);
+                const uint4 lo = *reinterpret_cast<const uint4*>(here + place(i * kRows + g, 4 * h + t)),
+                            hi = *reinterpret_cast<const uint4*>(here + place(i * kRows + g + 8, 4 * h + t));
                 const uint32_t op0[4] = {lo.x, hi.x, lo.y, hi.y}, op1[4] = {lo.z, hi.z, lo.w, hi.w};
 #pragma unroll
                 for (int p = 0; p < P; p++) {
@@ -149,6 +156,7 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
                 for (int j = 0; j < 4; j++) acc[i][p][j] = fmaf(d[p][j], (j & 1 ? sx.y : sx.x) * sw, acc[i][p][j]);
             }
         }
+        __syncwarp();                       // before the place is written again
         fetch(u, b + kAhead);
         if (++u == kAhead) u = 0;
     }

@@ -346,6 +346,15 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    const int kb = (a.k + kQ8Block - 1) / kQ8Block;
+    if (warp == 0 && !a.offsets && elect_one()) {
+        // the first weights' way into the L2 cache begins while the kernel before this one ends (a hint: what they are is read
+        // later, and the L2 cache holds what that kernel writes)
+        const int col = (int)blockIdx.x / CL / ((a.n_rows + MT - 1) / MT), n0 = SW ? col * kQ8Block + rank * (NT / 2) : col * NT;
+        for (int b = 0; b < min(kb, S * C::kPer); b++)
+            asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(&c.w), "r"(b * kQ8Block), "r"(n0), "r"(0), "r"(0)
+                         : "memory");
+    }
     wait_for_inputs();
     if (warp == 3) {        // row tiles before each group
         int before = 0;
@@ -375,7 +384,6 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
     const Groups groups(s_pre, s_off, a.groups, c.n_tiles, MT, (int)gridDim.x / CL, (int)blockIdx.x / CL);
-    const int kb = (a.k + kQ8Block - 1) / kQ8Block;
     volatile int* const fail = s_fail;
 
     if (warp < 4) {
