@@ -19,8 +19,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 
+constexpr int kKept = 8;
+
 struct PlanCall {
     PlanExpertsArgs a;
+    Div used;
     int per_warp;       // assignments of a warp
 };
 
@@ -47,12 +50,18 @@ __global__ void __launch_bounds__(1024) plan_experts_kernel(const PlanCall c) {
         const uint32_t d = (uint32_t)e - (uint32_t)a.first;      // the difference may pass 31 bits
         return e >= a.first && d < (uint32_t)E ? (int)d : -1;
     };
-    for (long i = lo; i < hi; i += 32) {
-        const int e = expert_of(i + lane);
+    int kept[kKept];        // the first steps' experts: their loads are in flight together, and serve both passes
+#pragma unroll
+    for (int s = 0; s < kKept; s++) kept[s] = expert_of(lo + 32 * s + lane);
+    auto count = [&](int e) {
         const uint32_t same = __match_any_sync(0xffffffffu, e);
         if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
         __syncwarp();
-    }
+    };
+#pragma unroll
+    for (int s = 0; s < kKept; s++)
+        if (lo + 32 * s < hi) count(kept[s]);
+    for (long i = lo + 32 * kKept; i < hi; i += 32) count(expert_of(i + lane));
     __syncthreads();
     for (int e = tid; e < E; e += blockDim.x) {     // the counts of the warps before, in place
         int sum = 0;
@@ -106,37 +115,41 @@ __global__ void __launch_bounds__(1024) plan_experts_kernel(const PlanCall c) {
         s_total[tid] = sum - all + before;
     }
     __syncthreads();
-    for (long i = lo; i < hi; i += 32) {
-        const int e = expert_of(i + lane);
+    auto put = [&](long i, int e) {
         const uint32_t same = __match_any_sync(0xffffffffu, e);
         int place = -1;
         if (e >= 0) {
-            const int at = s_total[e] + mine[e];
-            place = at + __popc(same & ((1u << lane) - 1));
-            a.rows[place] = (int)((i + lane) / a.used);
+            place = s_total[e] + mine[e] + __popc(same & ((1u << lane) - 1));
+            a.rows[place] = (int)(i + lane) / c.used;
         }
         __syncwarp();
         if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
         if (i + lane < hi) a.pos[i + lane] = place;
         __syncwarp();
-    }
+    };
+#pragma unroll
+    for (int s = 0; s < kKept; s++)
+        if (lo + 32 * s < hi) put(lo + 32 * s, kept[s]);
+    for (long i = lo + 32 * kKept; i < hi; i += 32) put(i, expert_of(i + lane));
 }
 
 struct CombineCall {
     CombineArgs a;
-    Div cols;           // threads of a token
+    int threads;        // of a token
     int wide;           // 8 columns a thread in 16-byte pieces; else one column a thread
+    int split;          // blocks of threads of a token
 };
 
+// a block of threads has 256 threads' columns of one token
 template <typename T>
 __global__ void __launch_bounds__(256) combine_experts_kernel(const CombineCall c) {
     early_launch();
     wait_for_inputs();
     const CombineArgs& a = c.a;
-    const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
-    const long t = i / c.cols.d;
-    if (t >= a.tokens) return;
-    const int col = (int)(i - t * c.cols.d) * (c.wide ? 8 : 1);
+    const long t = blockIdx.x / c.split;
+    const int i = (int)(blockIdx.x % c.split) * 256 + threadIdx.x;
+    if (i >= c.threads) return;
+    const int col = i * (c.wide ? 8 : 1);
     const int* pos = a.pos + t * a.pos_row;
     const float* w = a.weights + t * a.w_row;
     const T* y = (const T*)a.y + col;
@@ -149,25 +162,31 @@ __global__ void __launch_bounds__(256) combine_experts_kernel(const CombineCall 
         *out = from_f<T>(acc);
         return;
     }
+    constexpr int WORDS = 2 * sizeof(T), AT_ONCE = sizeof(T) == 4 ? 4 : 8;      // 16 KB to 32 KB of a token's rows in flight a block
     float acc[8] = {};
     if (add) load8<T>(add, true, acc);
-    for (int k0 = 0; k0 < a.used; k0 += 4) {        // four rows' loads in flight
-        float v[4][8], f[4];
-        bool some[4];
+    for (int k0 = 0; k0 < a.used; k0 += AT_ONCE) {
+        uint4 v[AT_ONCE][WORDS / 4];
+        float f[AT_ONCE];
+        bool some[AT_ONCE];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < AT_ONCE; j++) {
             const int p = k0 + j < a.used ? pos[k0 + j] : -1;
             some[j] = p >= 0 && p < a.n_y;
             if (some[j]) {
                 f[j] = w[k0 + j];
-                load8<T>(y + p * a.y_row, true, v[j]);
+#pragma unroll
+                for (int q = 0; q < WORDS / 4; q++) v[j][q] = __ldcs(reinterpret_cast<const uint4*>(y + p * a.y_row) + q);
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (some[j])
+        for (int j = 0; j < AT_ONCE; j++) {
+            if (!some[j]) continue;
+            float e[8];
+            load8<T>(reinterpret_cast<const T*>(v[j]), true, e);
 #pragma unroll
-                for (int q = 0; q < 8; q++) acc[q] = fmaf(f[j], v[j][q], acc[q]);
+            for (int q = 0; q < 8; q++) acc[q] = fmaf(f[j], e[q], acc[q]);
+        }
     }
     store8<T>(out, true, acc);
 }
@@ -179,7 +198,7 @@ bool launch_plan_experts(const PlanExpertsArgs& a, cudaStream_t s) {
     const int blocks = many ? 8 : 1;
     // a warp walks 32 assignments a step; a block has no more warps than that gives work for, and enough threads for the experts
     int warps = std::min<long>(32, std::max<long>((a.experts + 31) / 32, ((long)a.n + 32l * blocks - 1) / (32l * blocks)));
-    PlanCall c{a, 0};
+    PlanCall c{a, make_div(a.used), 0};
     c.per_warp = (int)((((long)a.n + (long)blocks * warps - 1) / ((long)blocks * warps) + 31) / 32 * 32);
     const size_t smem = sizeof(int) * (size_t)(warps + 1) * a.experts;
     auto kernel = many ? plan_experts_kernel<8> : plan_experts_kernel<1>;
@@ -203,12 +222,12 @@ bool launch_plan_experts(const PlanExpertsArgs& a, cudaStream_t s) {
 
 void launch_combine_experts(const CombineArgs& a, cudaStream_t s) {
     const int b = dtype_bytes(a.dtype);
-    CombineCall c{a, Div{}, 0};
+    CombineCall c{a, 0, 0, 0};
     c.wide = a.hidden % 8 == 0 && aligned16(a.y, a.y_row, 0, b) && aligned16(a.add, a.add ? a.add_row : 0, 0, b) &&
              aligned16(a.out, a.out_row, 0, b);
-    c.cols.d = c.wide ? a.hidden / 8 : a.hidden;
-    const long threads = (long)a.tokens * c.cols.d;
-    const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
+    c.threads = c.wide ? a.hidden / 8 : a.hidden;
+    c.split = (c.threads + 255) / 256;
+    const dim3 grid((unsigned)((long)a.tokens * c.split)), block(std::min(256, (c.threads + 31) / 32 * 32));
     if (a.dtype == kF32) launch(combine_experts_kernel<float>, grid, block, 0, s, c);
     else if (a.dtype == kF16) launch(combine_experts_kernel<__half>, grid, block, 0, s, c);
     else launch(combine_experts_kernel<__nv_bfloat16>, grid, block, 0, s, c);

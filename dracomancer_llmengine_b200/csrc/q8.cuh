@@ -47,6 +47,19 @@ __device__ __forceinline__ Q8Span q8_span(const int* offsets, int g, int n_rows)
     return Q8Span{a, b - a};
 }
 
+// g / (1 + exp(-g)) * u within 2^-21.  exp(-g) as a power of two whose exponent's rounding is put back to first order
+// (2^(t + d) = 2^t (1 + d ln 2)): the exponent is rounded at its own size, up to 2^-17 where exp still fits, which alone would
+// cost the result as much.  Beyond exp's range the quotient is 0.
+__device__ __forceinline__ float q8_silu_mul(float g, float u) {
+    const float log2e = 1.44269504f, t = -g * log2e, d = fmaf(-g, log2e, -t) - g * 1.925963033e-8f;      // log2(e) - log2e
+    float p, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(t));
+    p = fmaf(p, d * 0.693147181f, p);
+    if (t >= 128.f) p = __int_as_float(0x7f800000);        // not infinity times d
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + p));
+    return g * r * u;
+}
+
 // the group and rows of the row tile `slot` of tiles of M rows; count 0: there is no such tile.  By a whole warp.
 struct Q8Where {
     int group, first, count;

@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kN) q8_any_kernel(const Call c) {
             float h[4], top = 0.f;
             for (int i = 0; i < 4; i++) {
                 const float g = s_h[m][lane + 32 * i], u = s_h[m][128 + lane + 32 * i];
-                h[i] = tile * kQ8Block + lane + 32 * i < a.n ? g / (1.f + expf(-g)) * u : 0.f;
+                h[i] = tile * kQ8Block + lane + 32 * i < a.n ? q8_silu_mul(g, u) : 0.f;
                 top = max_nan(top, fabsf(h[i]));
             }
             top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));   // NaN is above infinity

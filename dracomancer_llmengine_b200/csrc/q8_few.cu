@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
             else if (a.dtype == kF16) ((__half*)a.out)[o] = __float2half_rn(v);
             else ((__nv_bfloat16*)a.out)[o] = __float2bfloat16_rn(v);
         } else {
-            s_h[r][m] = there && !zero ? __fdividef(sum[0], 1.f + expf(-sum[0])) * sum[MATS - 1] : 0.f;
+            s_h[r][m] = there && !zero ? q8_silu_mul(sum[0], sum[MATS - 1]) : 0.f;
         }
     }
     if constexpr (SW) {

@@ -41,6 +41,7 @@ constexpr int kStagingWarp = 2048;
 #endif
 constexpr int kStatusOperands = 1, kStatusProduct = 2, kStatusJoin = 4, kStatusBuffer = 8, kStatusStage = 16;
 constexpr float kTiny = 7.888609e-31f;   // 2^-100
+constexpr int kPrefetch = 64;            // blocks of a dense call's first tile that are prefetched
 constexpr int kSmemMost = 227 * 1024;
 
 struct Call {
@@ -347,11 +348,11 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     const int kb = (a.k + kQ8Block - 1) / kQ8Block;
-    if (warp == 0 && !a.offsets && elect_one()) {
-        // the first weights' way into the L2 cache begins while the kernel before this one ends (a hint: what they are is read
+    if (warp == 4 && !a.offsets && elect_one()) {
+        // the first tile's weights' way into the L2 cache begins while the kernel before this one ends (a hint: what they are is read
         // later, and the L2 cache holds what that kernel writes)
         const int col = (int)blockIdx.x / CL / ((a.n_rows + MT - 1) / MT), n0 = SW ? col * kQ8Block + rank * (NT / 2) : col * NT;
-        for (int b = 0; b < min(kb, S * C::kPer); b++)
+        for (int b = 0; b < min(kb, kPrefetch); b++)
             asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(&c.w), "r"(b * kQ8Block), "r"(n0), "r"(0), "r"(0)
                          : "memory");
     }
@@ -615,8 +616,8 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
 #pragma unroll
                     for (int j = 0; j < H / 2; j++) {
                         const float2 gate = acc[j], up = acc_u[j];
-                        h[2 * j] = __fdividef(gate.x, 1.f + expf(-gate.x)) * up.x;
-                        h[2 * j + 1] = __fdividef(gate.y, 1.f + expf(-gate.y)) * up.y;
+                        h[2 * j] = q8_silu_mul(gate.x, up.x);
+                        h[2 * j + 1] = q8_silu_mul(gate.y, up.y);
                     }
 #pragma unroll
                     for (int j = 0; j < H; j++) {
