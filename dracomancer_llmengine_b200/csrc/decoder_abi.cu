@@ -121,11 +121,12 @@ int draco_b200_test_q8_barrier_extra(int which) {
     return old;
 }
 // for tests, of this thread's next calls of the 8-bit products: 1 the form for few rows, 2 the one for any address, 32 to 256 the
-// tensor cores with so many columns a tile, 0 (the default) the one that is chosen; returns the old value
+// tensor cores with so many columns a tile, 0 (the default) the one that is chosen; from 1024 on, 1024 times 1, 2, 4 or 8 is
+// added: blocks of threads that share a tile's inner size.  Returns the old value.
 int draco_b200_test_q8_form(int form) {
-    const int old = t_test_q8_form;
-    if (form >= 0 && form <= 2) t_test_q8_form = form;
-    if (form == 32 || form == 64 || form == 128 || form == 256) t_test_q8_form = form;
+    const int old = t_test_q8_form, nt = form & 1023, split = form >> 10;
+    const bool known = (nt >= 0 && nt <= 2) || nt == 32 || nt == 64 || nt == 128 || nt == 256;
+    if (form >= 0 && known && (split == 0 || split == 1 || split == 2 || split == 4 || split == 8)) t_test_q8_form = form;
     return old;
 }
 // the id of the graph capture that the stream is in, 0: none
@@ -276,7 +277,7 @@ int draco_b200_linear_q8(const DracoLinearQ8* p, void* stream) {
     const Q8Args a{(const uint8_t*)p->x, p->x_scales, (const uint8_t*)p->w, p->w_scales, p->offsets, p->rows, p->out,
                    p->out_scales, p->x_stride, p->x_scales_stride, p->out_stride, p->out_scales_stride, p->n_x, p->n_rows,
                    p->n, p->k, p->n_groups, p->dtype, p->swiglu != 0, p->status,
-                   p->wait_limit_us ? p->wait_limit_us * 1000l : 2000000000l, t_test_q8_extra, t_test_q8_form};
+                   p->wait_limit_us ? p->wait_limit_us * 1000l : 2000000000l, t_test_q8_extra, t_test_q8_form & 1023, t_test_q8_form >> 10};
     if (!launch_q8(a, (cudaStream_t)stream)) {
         cudaGetLastError();
         refuse("%s: the launch could not be set up", who);

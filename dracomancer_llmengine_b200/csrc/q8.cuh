@@ -27,6 +27,7 @@ struct Q8Args {
     long wait_ns;               // their limit
     int test_extra;             // 1, 2, 3: an arrival that never comes is expected at a barrier (tests)
     int test_form;              // 0: the form is chosen; kQ8Few, kQ8Any, or the tensor cores' columns a tile (tests)
+    int test_split;             // 0: chosen; blocks of threads that share a tile's inner size (tests)
 };
 constexpr int kQ8Few = 1, kQ8Any = 2;
 constexpr int kQ8FewMost = 1 << 16;     // inner size that the form for few rows has room for (its scales are in shared memory)

@@ -41,6 +41,7 @@ constexpr int kStagingWarp = 2048;
 #endif
 constexpr int kStatusOperands = 1, kStatusProduct = 2, kStatusJoin = 4, kStatusBuffer = 8, kStatusStage = 16;
 constexpr float kTiny = 7.888609e-31f;   // 2^-100
+constexpr float kJoin = 2.f;             // us that the parts of a tile take to join
 constexpr int kPrefetch = 64;            // blocks of a dense call's first tile that are prefetched
 constexpr int kSmemMost = 227 * 1024;
 
@@ -49,6 +50,7 @@ struct Call {
     Q8Args a;
     int n_tiles;        // column tiles (with SwiGLU: of 128 columns)
     int vec;            // rows of the output start on 16 bytes
+    int split, per;     // blocks of threads that share a tile's inner size, blocks of 128 of each
 };
 
 template <int MT, int NT, bool SW>
@@ -299,6 +301,89 @@ __device__ __forceinline__ void store_product(uint8_t* staging, int lane, const 
     }
 }
 
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address of this block's shared memory `at` in block p of the cluster
+__device__ __forceinline__ uint32_t in_block(uint32_t at, int p) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(p));
+    return r;
+}
+
+// Where blocks of threads share a tile's inner size: each adds up the sums of an equal part of the rows, in the order of the
+// blocks, and writes them.  If a wait ran out in one of them the rows are NaN.
+template <int MT, int NT, bool SW>
+__device__ void join_parts(const Call& c, const Tile& now, const uint8_t* ring, const int* fail, int rank) {
+    const Q8Args& a = c.a;
+    const int per = MT / c.split, r0 = rank * per, rows = min(max(now.rows - r0, 0), per), tid = threadIdx.x;
+    const uint32_t base = smem_addr(ring);
+    bool bad = false;
+    for (int p = 0; p < c.split; p++) {
+        uint32_t f;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(f) : "r"(in_block(smem_addr(fail), p)));
+        bad |= f != 0;
+    }
+    auto sum = [&](int r, int piece) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p = 0; p < c.split; p++) {
+            float4 u;
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(u.x), "=f"(u.y), "=f"(u.z), "=f"(u.w)
+                         : "r"(in_block(base + r * (NT * 4) + ((piece ^ (r & 7)) << 4), p)));
+            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        }
+        const int src = a.rows ? a.rows[now.first + r] : 0;
+        if (src < 0 || src >= a.n_x) v = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float nan = __int_as_float(0x7fc00000);
+        return bad ? make_float4(nan, nan, nan, nan) : v;
+    };
+    if constexpr (!SW) {
+        for (int e = tid; e < rows * (NT / 4); e += Cfg<MT, NT, SW>::kThreads) {
+            const int r = r0 + e / (NT / 4), piece = e % (NT / 4), n = now.col * NT + piece * 4;
+            const float4 v = sum(r, piece);
+            const float f[4] = {v.x, v.y, v.z, v.w};
+            auto put = [&](auto kind) {
+                using T = decltype(kind);
+                T* out = (T*)a.out + (long)(now.first + r) * a.out_row + n;
+                if (c.vec && n + 4 <= a.n) {
+                    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = v;
+                    else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+                } else {
+                    for (int i = 0; i < 4; i++)
+                        if (n + i < a.n) out[i] = from_f<T>(f[i]);
+                }
+            };
+            if (a.dtype == kF32) put(0.f);
+            else if (a.dtype == kF16) put(__half());
+            else put(__nv_bfloat16());
+        }
+    } else {
+        const int lane = tid & 31;
+        for (int r = r0 + (tid >> 5); r < r0 + rows; r += Cfg<MT, NT, SW>::kThreads / 32) {     // a warp has a row's 128 columns
+            const float4 g = sum(r, lane), u = sum(r, NT / 8 + lane);
+            const float h[4] = {q8_silu_mul(g.x, u.x), q8_silu_mul(g.y, u.y), q8_silu_mul(g.z, u.z), q8_silu_mul(g.w, u.w)};
+            float top = max_nan(max_nan(fabsf(h[0]), fabsf(h[1])), max_nan(fabsf(h[2]), fabsf(h[3])));
+            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));       // NaN is above infinity
+            const float inv = top < kTiny ? 0.f : __fdiv_rn(448.f, top);
+            const int n = now.col * kQ8Block + lane * 4;
+            uint8_t* out = (uint8_t*)a.out + (long)(now.first + r) * a.out_row + n;
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(h[0] * inv, h[1] * inv), __NV_SATFINITE, __NV_E4M3),
+                           hi = __nv_cvt_float2_to_fp8x2(make_float2(h[2] * inv, h[3] * inv), __NV_SATFINITE, __NV_E4M3);
+            if (c.vec && n + 4 <= a.n) {
+                *reinterpret_cast<uint32_t*>(out) = lo | hi << 16;
+            } else {
+                for (int i = 0; i < 4; i++)
+                    if (n + i < a.n) out[i] = (uint8_t)((lo | hi << 16) >> (8 * i));
+            }
+            if (lane == 0)
+                a.out_scales[(long)(now.first + r) * a.os_row + now.col] =
+                    top < kTiny ? 0.f : top <= 3.402823466e38f ? __fdiv_rn(top, 448.f) : __int_as_float(0x7fc00000);
+        }
+    }
+}
+
 template <int MT, int NT, bool SW>
 __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(const __grid_constant__ Call c) {
     using C = Cfg<MT, NT, SW>;
@@ -347,13 +432,14 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const int kb = (a.k + kQ8Block - 1) / kQ8Block;
+    const int k_blocks = (a.k + kQ8Block - 1) / kQ8Block, split = CL == 1 ? c.split : 1, k_rank = (int)(blockIdx.x % split);
+    const int k_first = k_rank * c.per, kb = min(k_blocks - k_first, c.per);       // of this block of threads
     if (warp == 4 && !a.offsets && elect_one()) {
         // the first tile's weights' way into the L2 cache begins while the kernel before this one ends (a hint: what they are is read
         // later, and the L2 cache holds what that kernel writes)
-        const int col = (int)blockIdx.x / CL / ((a.n_rows + MT - 1) / MT), n0 = SW ? col * kQ8Block + rank * (NT / 2) : col * NT;
+        const int col = (int)blockIdx.x / CL / split / ((a.n_rows + MT - 1) / MT), n0 = SW ? col * kQ8Block + rank * (NT / 2) : col * NT;
         for (int b = 0; b < min(kb, kPrefetch); b++)
-            asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(&c.w), "r"(b * kQ8Block), "r"(n0), "r"(0), "r"(0)
+            asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(&c.w), "r"((k_first + b) * kQ8Block), "r"(n0), "r"(0), "r"(0)
                          : "memory");
     }
     wait_for_inputs();
@@ -379,12 +465,11 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
     tc_fence_before();
     __syncthreads();
     if constexpr (CL > 1) {     // the others' barriers are ready
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster_barrier();
     }
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
-    const Groups groups(s_pre, s_off, a.groups, c.n_tiles, MT, (int)gridDim.x / CL, (int)blockIdx.x / CL);
+    const Groups groups(s_pre, s_off, a.groups, c.n_tiles, MT, (int)gridDim.x / CL / split, (int)blockIdx.x / CL / split);
     volatile int* const fail = s_fail;
 
     if (warp < 4) {
@@ -406,11 +491,11 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
 #pragma unroll
                     for (int i = 0; i < MT / 32; i++) {
                         const int r = tile.first + min(lane + 32 * i, tile.rows - 1), src = a.rows ? a.rows[r] : r;
-                        scales[i] = a.xs + (long)(src >= 0 && src < a.n_x ? src : 0) * a.xs_row;
+                        scales[i] = a.xs + (long)(src >= 0 && src < a.n_x ? src : 0) * a.xs_row + k_first;
                     }
                     const int nb = (a.n + kQ8Block - 1) / kQ8Block, second = lane & 1;
                     const int block = SW ? tile.col : min(tile.col * NT + second * (NT / 2), a.n - 1) / kQ8Block;
-                    wscale = a.ws + ((long)tile.group * (SW ? 2 * nb : nb) + block + (SW ? second * nb : 0)) * kb;
+                    wscale = a.ws + ((long)tile.group * (SW ? 2 * nb : nb) + block + (SW ? second * nb : 0)) * k_blocks + k_first;
                 }
                 if (of_x && a.rows) {
                     __syncwarp();
@@ -430,7 +515,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                         // a row's 128 bytes by eight lanes; the 16-byte pieces lie where the 128-byte swizzle of the operand has them
                         const int sub = lane >> 3, piece = lane & 7;
                         for (int j = 0; j < here; j++) {
-                            const int k0 = (b + j) * kQ8Block + piece * 16;
+                            const int k0 = (k_first + b + j) * kQ8Block + piece * 16;
                             const int bytes = k0 < a.k ? 16 : 0;                // behind the row: zeros
                             const int from = bytes ? k0 : 0;
                             const uint32_t even = smem_addr(pa + j * C::kA) + sub * 128 + ((piece ^ sub) << 4), odd = even ^ 64;
@@ -449,7 +534,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
 #pragma unroll
                         for (int j = 0; j < C::kPer; j++) {
                             if (j >= here) break;
-                            const int k0 = (b + j) * kQ8Block;
+                            const int k0 = (k_first + b + j) * kQ8Block;
                             if (!of_x) {
                                 tma_4d(pb + j * C::kB, &c.w, k0, n0, 0, tile.group, full + stage);
                                 if constexpr (SW && C::kPer == 1)
@@ -587,6 +672,23 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                         add_block<COLS>(acc, at + j * NT, sx * (part * COLS < NT / 2 ? sw.x : sw.y), read);
                     }
                 }
+                if (CL == 1 && split > 1 && go) {
+                    // the sums of this part of the inner size go to the ring's memory, which no product reads any more: rows of NT
+                    // values, a row's pieces of 16 bytes turned by the row
+                    asm volatile("bar.sync 1, %0;" ::"n"(C::kActive * 32) : "memory");
+                    const int r = quarter * 32 + lane;
+                    auto put = [&](int piece, const float2& lo, const float2& hi) {
+                        *reinterpret_cast<float4*>(ring + r * (NT * 4) + ((piece ^ (r & 7)) << 4)) = make_float4(lo.x, lo.y, hi.x, hi.y);
+                    };
+                    constexpr int Q = SW ? COLS / 8 : COLS / 4;         // pieces of this warp (SwiGLU: of each matrix)
+#pragma unroll
+                    for (int i = 0; i < Q; i++) {
+                        put(part * Q + i, acc[2 * i], acc[2 * i + 1]);
+                        if constexpr (SW) put(NT / 8 + part * Q + i, acc_u[2 * i], acc_u[2 * i + 1]);
+                    }
+                    left = false;
+                    break;
+                }
                 bool zero = false;      // a row that takes none of x's
                 if (a.rows && quarter * 32 + lane < now.rows) {
                     const int src = a.rows[now.first + quarter * 32 + lane];
@@ -670,7 +772,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                 }
             }
             // a wait ran out: what this block had not finished becomes NaN
-            for (; left; left = walk.next()) {
+            for (; left && split == 1; left = walk.next()) {
                 const Tile tile = groups.at(walk.t);
                 const int r = quarter * 32 + lane;
                 if (r >= tile.rows) continue;
@@ -697,10 +799,13 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kColumns) : "memory");
     }
-    if constexpr (CL > 1) {     // the others may still write here
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if constexpr (CL == 1) {
+        if (split > 1) {
+            cluster_barrier();
+            join_parts<MT, NT, SW>(c, groups.at(groups.me), ring, s_fail, k_rank);
+        }
     }
+    if (CL > 1 || split > 1) cluster_barrier();     // the others may still read or write here
 }
 
 // ---------------------------------------------------------------- host
@@ -743,8 +848,14 @@ int resident_clusters(cudaLaunchConfig_t cfg) {
     return n;
 }
 
+// blocks of 128 inner values of each of `split` parts, which are whole stages; 0 where one of them would have none
+int part_blocks(int kb, int nt, int split) {
+    const int stage = nt <= 64 ? 2 : 1, per = ((kb + split - 1) / split + stage - 1) / stage * stage;
+    return per * (split - 1) < kb ? per : 0;
+}
+
 template <int MT, int NT, bool SW>
-bool launch_k(const Q8Args& a, cudaStream_t s) {
+bool launch_k(const Q8Args& a, int split, cudaStream_t s) {
     using C = Cfg<MT, NT, SW>;
     static_assert(C::kSmem <= kSmemMost && C::kStages >= 3 && C::kColumns <= 512, "the block's memory");
     Call c;
@@ -763,6 +874,9 @@ bool launch_k(const Q8Args& a, cudaStream_t s) {
     const cuuint32_t tbox[2] = {128, 128};
     if (MT == 128 && !a.rows && !map_bytes(&c.xt, 2, a.x, xd, xst, tbox)) return false;
 
+    const int kb = (a.k + kQ8Block - 1) / kQ8Block;
+    c.split = C::kCluster == 1 ? split : 1;
+    while (!(c.per = part_blocks(kb, NT, c.split))) c.split >>= 1;
     auto kernel = q8_tc_kernel<MT, NT, SW>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return false;
     cudaLaunchConfig_t cfg{};
@@ -771,24 +885,26 @@ bool launch_k(const Q8Args& a, cudaStream_t s) {
     cfg.stream = s;
     cudaLaunchAttribute at[2] = {};
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = C::kCluster, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[0].val.clusterDim.x = C::kCluster * c.split, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    const int room = resident_clusters<MT, NT, SW>(cfg);
+    const int room = c.split > 1 ? 1 : resident_clusters<MT, NT, SW>(cfg);
     if (room <= 0) return false;
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 2;
     const long tiles = ((long)(a.n_rows + MT - 1) / MT + (a.offsets ? std::min(a.groups, a.n_rows) : 0)) * c.n_tiles;
-    cfg.gridDim = dim3((unsigned)(std::min<long>(room, tiles) * C::kCluster));
+    cfg.gridDim = dim3((unsigned)(c.split > 1 ? tiles * c.split : std::min<long>(room, tiles) * C::kCluster));
     return cudaLaunchKernelEx(&cfg, kernel, c) == cudaSuccess;
 }
 
 template <int MT, bool SW>
-bool launch_n(const Q8Args& a, int nt, cudaStream_t s) {
+bool launch_n(const Q8Args& a, int nt, int split, cudaStream_t s) {
     if constexpr (!SW)
-        if (nt == 32) return launch_k<MT, 32, SW>(a, s);
-    return nt == 256 ? launch_k<MT, 256, SW>(a, s) : nt == 128 ? launch_k<MT, 128, SW>(a, s) : launch_k<MT, 64, SW>(a, s);
+        if (nt == 32) return launch_k<MT, 32, SW>(a, split, s);
+    return nt == 256   ? launch_k<MT, 256, SW>(a, split, s)
+           : nt == 128 ? launch_k<MT, 128, SW>(a, split, s)
+                       : launch_k<MT, 64, SW>(a, split, s);
 }
 
 }  // namespace
@@ -797,27 +913,36 @@ bool q8_tc_fits(const Q8Args& a) {
     return a.n_x > 0 && a.k % 16 == 0 && aligned16(a.x) && aligned16(a.w) && (a.n_x == 1 || (a.x_row % 16 == 0 && a.x_row >= a.k));
 }
 
-// The widest tile is not the fastest where it leaves SMs without one: the narrower ones make more tiles.  A tile takes about
-// as long as its blocks of inner values (us a block and for the rest, measured: rows of 128, inner sizes 512 to 7168; a block
-// of a narrow tile takes what its copies' and products' hand-over takes), and tiles run in rounds of as many as there is room for.
+// The widest tile is not the fastest where it leaves SMs without one: narrower ones make more tiles, and where one group has
+// few, several blocks of threads share a tile's inner size.  A tile takes about as long as its blocks of inner values (us a
+// block and for the rest, measured: rows of 128, inner sizes 512 to 7168; a block of a narrow tile takes what the hand-over of
+// its copies and products takes), and tiles run in rounds of as many as there is room for.
 bool launch_q8_tc(const Q8Args& a, cudaStream_t s) {
     static const struct { int nt; float block, rest; } kTiles[] = {{256, 0.50f, 3.0f}, {128, 0.39f, 1.5f}, {64, 0.30f, 1.0f}, {32, 0.29f, 0.8f}};
     const bool few = a.offsets ? (long)a.n_rows <= 16l * a.groups : a.n_rows <= 32;
     const int mt = few ? 32 : 128;
     const long row_tiles = (a.n_rows + mt - 1) / mt + (a.offsets ? std::min(a.groups, a.n_rows) - 1 : 0);
     const int kb = (a.k + kQ8Block - 1) / kQ8Block;
-    int nt = 256;
+    int nt = 256, split = 1;
     float best = 0.f;
     for (const auto& t : kTiles) {
         if (a.swiglu && t.nt == 32) continue;
+        if (a.test_form >= 32 && t.nt != (a.swiglu ? std::max(a.test_form, 64) : a.test_form)) continue;
+        const int cluster = a.swiglu ? 256 / t.nt : 1;
         const long tiles = row_tiles * (a.swiglu ? (a.n + kQ8Block - 1) / kQ8Block : (a.n + t.nt - 1) / t.nt);
-        const long room = 148 / (a.swiglu ? 256 / t.nt : 1);
-        const float time = (float)((tiles + room - 1) / room) * (kb * t.block + t.rest);
-        if (t.nt == 256 || time < best) best = time, nt = t.nt;
+        for (int parts = 1; parts <= 8; parts *= 2) {
+            // clusters that find room at once, of blocks of threads that have an SM each
+            static const int kRoom[4] = {148, 72, 34, 14};
+            const long room = parts > 1 ? kRoom[parts == 2 ? 1 : parts == 4 ? 2 : 3] : 148 / cluster;
+            const int per = part_blocks(kb, t.nt, parts);
+            if (parts > 1 && (a.offsets || cluster > 1 || tiles > room || per < 4)) continue;
+            const float time = (float)((tiles + room - 1) / room) * ((float)per * t.block + t.rest) + (parts > 1 ? kJoin : 0.f);
+            if (best == 0.f || time < best) best = time, nt = t.nt, split = parts;
+        }
     }
-    if (a.test_form >= 32) nt = a.swiglu && a.test_form == 32 ? 64 : a.test_form;
-    if (a.swiglu) return few ? launch_n<32, true>(a, nt, s) : launch_n<128, true>(a, nt, s);
-    return few ? launch_n<32, false>(a, nt, s) : launch_n<128, false>(a, nt, s);
+    if (a.test_split) split = a.offsets ? 1 : a.test_split;
+    if (a.swiglu) return few ? launch_n<32, true>(a, nt, split, s) : launch_n<128, true>(a, nt, split, s);
+    return few ? launch_n<32, false>(a, nt, split, s) : launch_n<128, false>(a, nt, split, s);
 }
 
 // Few rows: the form whose weights go straight to registers (7 us against 16 for 16 rows, 2048 x 7168; 12 against 8 for 32
@@ -825,7 +950,7 @@ bool launch_q8_tc(const Q8Args& a, cudaStream_t s) {
 bool launch_q8(const Q8Args& a, cudaStream_t s) {
     if (!q8_tc_fits(a) || a.test_form == kQ8Any) return launch_q8_any(a, s);
     const double cost = (double)q8_slots(a, 8) * (a.swiglu ? 2 : 1) * a.n * a.k;
-    bool few = a.offsets ? a.n_rows <= 16 || cost <= 60e6 : a.n_rows <= 8 || cost <= 30e6;
+    bool few = a.offsets ? a.n_rows <= 16 || cost <= 60e6 : a.n_rows <= 8 || cost <= (a.swiglu ? 15e6 : 30e6);
     if (a.test_form) few = a.test_form == kQ8Few;
     few = few && a.k <= kQ8FewMost;
     return few ? launch_q8_few(a, s) : launch_q8_tc(a, s);
