@@ -384,7 +384,7 @@ __device__ void join_parts(const Call& c, const Tile& now, const uint8_t* ring, 
     }
 }
 
-template <int MT, int NT, bool SW>
+template <int MT, int NT, bool SW, bool SPLIT>
 __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(const __grid_constant__ Call c) {
     using C = Cfg<MT, NT, SW>;
     constexpr int S = C::kStages, B = C::kBuffers, CL = C::kCluster;
@@ -432,8 +432,8 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const int k_blocks = (a.k + kQ8Block - 1) / kQ8Block, split = CL == 1 ? c.split : 1, k_rank = (int)(blockIdx.x % split);
-    const int k_first = k_rank * c.per, kb = min(k_blocks - k_first, c.per);       // of this block of threads
+    const int k_blocks = (a.k + kQ8Block - 1) / kQ8Block, split = SPLIT ? c.split : 1, k_rank = SPLIT ? (int)(blockIdx.x % split) : 0;
+    const int k_first = SPLIT ? k_rank * c.per : 0, kb = SPLIT ? min(k_blocks - k_first, c.per) : k_blocks;     // of this block of threads
     if (warp == 4 && !a.offsets && elect_one()) {
         // the first tile's weights' way into the L2 cache begins while the kernel before this one ends (a hint: what they are is read
         // later, and the L2 cache holds what that kernel writes)
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                     __syncwarp();
                     for (int r = lane; r < tile.rows; r += 32) {
                         const int src = a.rows[tile.first + r];
-                        s_src[r] = a.x + (src >= 0 && src < a.n_x ? src : 0) * a.x_row;     // not used where it is none: the row becomes zero
+                        s_src[r] = a.x + (src >= 0 && src < a.n_x ? src : 0) * a.x_row + k_first * kQ8Block;     // not used where it is none: the row becomes zero
                     }
                     __syncwarp();
                 }
@@ -512,11 +512,12 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                     uint8_t* const pb = pa + C::kPer * C::kA;
                     const int here = C::kPer == 1 ? 1 : min(C::kPer, kb - b);
                     if (of_x && a.rows) {
+                        const int k_left = a.k - k_first * kQ8Block;
                         // a row's 128 bytes by eight lanes; the 16-byte pieces lie where the 128-byte swizzle of the operand has them
                         const int sub = lane >> 3, piece = lane & 7;
                         for (int j = 0; j < here; j++) {
-                            const int k0 = (k_first + b + j) * kQ8Block + piece * 16;
-                            const int bytes = k0 < a.k ? 16 : 0;                // behind the row: zeros
+                            const int k0 = (b + j) * kQ8Block + piece * 16;
+                            const int bytes = k0 < k_left ? 16 : 0;             // behind the row: zeros
                             const int from = bytes ? k0 : 0;
                             const uint32_t even = smem_addr(pa + j * C::kA) + sub * 128 + ((piece ^ sub) << 4), odd = even ^ 64;
                             int r = sub;
@@ -672,7 +673,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                         add_block<COLS>(acc, at + j * NT, sx * (part * COLS < NT / 2 ? sw.x : sw.y), read);
                     }
                 }
-                if (CL == 1 && split > 1 && go) {
+                if (SPLIT && go) {
                     // the sums of this part of the inner size go to the ring's memory, which no product reads any more: rows of NT
                     // values, a row's pieces of 16 bytes turned by the row
                     asm volatile("bar.sync 1, %0;" ::"n"(C::kActive * 32) : "memory");
@@ -772,7 +773,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                 }
             }
             // a wait ran out: what this block had not finished becomes NaN
-            for (; left && split == 1; left = walk.next()) {
+            for (; left && !SPLIT; left = walk.next()) {
                 const Tile tile = groups.at(walk.t);
                 const int r = quarter * 32 + lane;
                 if (r >= tile.rows) continue;
@@ -799,13 +800,11 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kColumns) : "memory");
     }
-    if constexpr (CL == 1) {
-        if (split > 1) {
-            cluster_barrier();
-            join_parts<MT, NT, SW>(c, groups.at(groups.me), ring, s_fail, k_rank);
-        }
+    if constexpr (SPLIT) {
+        cluster_barrier();
+        join_parts<MT, NT, SW>(c, groups.at(groups.me), ring, s_fail, k_rank);
     }
-    if (CL > 1 || split > 1) cluster_barrier();     // the others may still read or write here
+    if constexpr (CL > 1 || SPLIT) cluster_barrier();     // the others may still read or write here
 }
 
 // ---------------------------------------------------------------- host
@@ -842,7 +841,7 @@ int resident_clusters(cudaLaunchConfig_t cfg) {
         if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
     } else {
         cfg.gridDim = dim3(Cfg<MT, NT, SW>::kCluster);
-        if (cudaOccupancyMaxActiveClusters(&n, q8_tc_kernel<MT, NT, SW>, &cfg) != cudaSuccess) return 0;
+        if (cudaOccupancyMaxActiveClusters(&n, q8_tc_kernel<MT, NT, SW, false>, &cfg) != cudaSuccess) return 0;
     }
     known.store(n, std::memory_order_relaxed);
     return n;
@@ -877,7 +876,9 @@ bool launch_k(const Q8Args& a, int split, cudaStream_t s) {
     const int kb = (a.k + kQ8Block - 1) / kQ8Block;
     c.split = C::kCluster == 1 ? split : 1;
     while (!(c.per = part_blocks(kb, NT, c.split))) c.split >>= 1;
-    auto kernel = q8_tc_kernel<MT, NT, SW>;
+    auto kernel = q8_tc_kernel<MT, NT, SW, false>;
+    if constexpr (C::kCluster == 1)
+        if (c.split > 1) kernel = q8_tc_kernel<MT, NT, SW, true>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return false;
     cudaLaunchConfig_t cfg{};
     cfg.blockDim = dim3(C::kThreads);
