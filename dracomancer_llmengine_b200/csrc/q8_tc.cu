@@ -274,10 +274,23 @@ __device__ __forceinline__ void store_rows(uint8_t* staging, int lane, const uin
                 for (int i = 0; i < P; i++)
                     *reinterpret_cast<uint4*>(staging + place(lane, i)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             __syncwarp();
+            if (vec) {
 #pragma unroll
-            for (int i = 0; i < ROWS * P / 32; i++) {
-                const int r = r0 + (i * 32 + lane) / P, c = lane % P;
-                if (r < rows) store_piece(out + r * row_bytes + c * 16, staging + place(r, c), left - c * 16, vec, elem);
+                for (int i = 0; i < ROWS * P / 32; i++) {
+                    const int r = r0 + (i * 32 + lane) / P, c = lane % P;
+                    if (r < rows) store_piece(out + r * row_bytes + c * 16, staging + place(r, c), left - c * 16, true, elem);
+                }
+            } else {        // element by element, neighbouring lanes neighbouring elements
+                const int per = BYTES / elem, inside = (int)min((long)BYTES, left);
+                for (int e = lane; e < min(rows - r0, ROWS) * per; e += 32) {
+                    const int r = r0 + e / per, at = e % per * elem;
+                    const uint8_t* src = staging + place(r, at / 16) + at % 16;
+                    uint8_t* p = out + r * row_bytes + at;
+                    if (at >= inside) continue;
+                    if (elem == 4) *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(src);
+                    else if (elem == 2) *reinterpret_cast<uint16_t*>(p) = *reinterpret_cast<const uint16_t*>(src);
+                    else *p = *src;
+                }
             }
         }
     }
