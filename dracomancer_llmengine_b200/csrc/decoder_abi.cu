@@ -274,6 +274,8 @@ int draco_b200_linear_q8(const DracoLinearQ8* p, void* stream) {
     if (!aligned_to(p->out, b) || !aligned_to(p->x_scales, 4) || !aligned_to(p->w_scales, 4) || !aligned_to(p->offsets, 4) ||
         !aligned_to(p->rows, 4) || !aligned_to(p->out_scales, 4) || !aligned_to(p->status, 4))
         return refuse("%s: buffers must be aligned to their elements", who);
+    if (p->out == p->x || p->out == p->w || (p->swiglu && p->out_scales == p->x_scales))
+        return refuse("%s: outputs must not overlap inputs", who);
     const Q8Args a{(const uint8_t*)p->x, p->x_scales, (const uint8_t*)p->w, p->w_scales, p->offsets, p->rows, p->out,
                    p->out_scales, p->x_stride, p->x_scales_stride, p->out_stride, p->out_scales_stride, p->n_x, p->n_rows,
                    p->n, p->k, p->n_groups, p->dtype, p->swiglu != 0, p->status,
@@ -323,6 +325,7 @@ int draco_b200_combine_experts(const DracoCombineExperts* p, void* stream) {
     if (!aligned_to(p->y, b) || !aligned_to(p->add, b) || !aligned_to(p->out, b) || !aligned_to(p->pos, 4) ||
         !aligned_to(p->weights, 4))
         return refuse("%s: buffers must be aligned to their elements", who);
+    if (p->out == p->y) return refuse("%s: out must not overlap y", who);
     const CombineArgs a{p->y, p->pos, p->weights, p->add, p->out, p->y_stride, p->add_stride, p->out_stride, p->pos_stride,
                         p->weights_stride, p->n_y, p->n_tokens, p->n_used, p->hidden, p->dtype};
     launch_combine_experts(a, (cudaStream_t)stream);

@@ -70,6 +70,7 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
     wait_for_inputs();
     const Q8Where at = q8_locate<TOK>(a, slot);
     if (!at.count) return;                          // the same for a whole cluster
+    if constexpr (SW) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");     // this block has begun
     const int g = lane >> 2, t = lane & 3;
 
     auto source = [&](int m) {                      // row m's row of x, -1: none
@@ -194,6 +195,7 @@ __global__ void __launch_bounds__(512, 1) q8_few_kernel(const Call c) {
         cg::cluster_group cluster = cg::this_cluster();
         const int rank = (int)cluster.block_rank();
         __syncthreads();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // all have: their memory may be written
         if (tid < TOK) {
             float top = 0.f;
             for (int r = 0; r < kRows; r++) top = max_nan(top, fabsf(s_h[r][tid]));

@@ -445,7 +445,7 @@ int draco_b200_rmsnorm_q8(const DracoNormQ8* args, void* stream);
  * with h = gate / (1 + exp(-gate)) * up and a the largest |h| of a row's 128 columns, out is e4m3(h * (448 / a)) and
  * out_scales [n_rows][ceil(n / 128)] a / 448: rows for the next product.  a < 2^-100: code and scale 0; an infinity or NaN
  * in the block: the scale is NaN.
- * At most 1024 groups, n, k, n_rows and n_x at most 2^24.  x, its rows' stride and w in whole 16 bytes (k % 16 == 0) take the tensor cores,
+ * No output may overlap an input.  At most 1024 groups, n, k, n_rows and n_x at most 2^24.  x, its rows' stride and w in whole 16 bytes (k % 16 == 0) take the tensor cores,
  * anything else a slow form.  status, wait_limit_us: as in draco_b200_kv4_attention_checked (rows of a block whose waits
  * ran out are NaN). */
 typedef struct DracoLinearQ8 {
@@ -473,7 +473,7 @@ int draco_b200_plan_experts(const int* order, int n_tokens, int n_used, int firs
                             int* pos, void* stream);
 
 /* out[t] = add[t] + sum over k ascending of weights[t][k] * y[pos[t][k]] (hidden values each, fp32 sums, one rounding to
- * dtype; add may be null and may be out; pos entries outside 0 .. n_y count as nothing). */
+ * dtype; add may be null and may be out, which overlaps nothing else; pos entries outside 0 .. n_y count as nothing). */
 typedef struct DracoCombineExperts {
     const void* y;
     const int* pos;

@@ -491,6 +491,52 @@ def test_experts_in_a_graph_and_on_streams():
     torch.cuda.synchronize()
 
 
+def test_outputs_that_are_inputs_are_refused():
+    x, xs, w, ws = operands(8, 128, 128, gen_of(1), (2,))
+    with pytest.raises(dm.DracoError, match="overlap"):
+        decoder.swiglu_q8(x, xs, w, ws, x, torch.empty(8, 1, device=DEV))
+    with pytest.raises(dm.DracoError, match="overlap"):
+        decoder.swiglu_q8(x, xs, w, ws, torch.empty_like(x), xs)
+    y = torch.zeros(4, 8, device=DEV)
+    with pytest.raises(dm.DracoError, match="overlap"):
+        decoder.combine_experts(y, ints(0, 0, 0, 0).view(4, 1), torch.ones(4, 1, device=DEV), y)
+
+
+def test_larger_plan_and_buffers_than_tokens():
+    """A server's buffers for its largest batch: places behind the batch's last are left as they were."""
+    gen = gen_of(11)
+    plan = decoder.plan_experts(torch.randint(6, (10, 2), device=DEV, generator=gen).int(), decoder.ExpertPlan(50, 2, 6))
+    x, xs, w, ws = operands(10, 256, 128, gen, (6,))
+    out = torch.full((100, 128), 3.0, device=DEV)
+    decoder.linear_q8(x, xs, w, ws, out, offsets=plan.offsets, rows=plan.rows)
+    assert bool((out[20:] == 3).all())
+    for e in range(6):
+        a, b = plan.offsets[e:e + 2].tolist()
+        same(out[a:b], *plain(of_row(x, plan.rows, a, b), of_row(xs, plan.rows, a, b), w[e], ws[e]), "f32") if b > a else None
+
+
+def test_offsets_past_32_bits():
+    """Weights of more than 2^32 bytes, and a row of x beyond 2^32 bytes: the last group's and the last row's products are right."""
+    gen = gen_of(12)
+    k, n, groups = 4096, 4096, 260
+    w = torch.zeros(groups, n, k, dtype=torch.uint8, device=DEV).view(E4M3)
+    ws = torch.ones(groups, n // 128, k // 128, device=DEV)
+    last = codes_of((n, k), gen)
+    w[-1] = last
+    big = torch.zeros(1 << 20, 4112, dtype=torch.uint8, device=DEV).view(E4M3)      # 4.3 GB of rows, of which the last are used
+    x, xs = big[:, :k], torch.ones(1 << 20, k // 128, device=DEV)
+    x[-40:] = codes_of((40, k), gen)
+    rows = torch.arange((1 << 20) - 40, 1 << 20, device=DEV).int()
+    offsets = torch.zeros(groups + 1, dtype=torch.int32, device=DEV)
+    offsets[-1] = 40
+    for form in (0, 1, 2, 64, 256):
+        dm.lib().draco_b200_test_q8_form(form)
+        out = decoder.linear_q8(x, xs, w, ws, torch.zeros(40, n, device=DEV), offsets=offsets, rows=rows)
+        same(out, *plain(x[-40:], xs[-40:], last, ws[-1]), "f32")
+    dense = decoder.linear_q8(x[-40:], xs[-40:], last, ws[-1], torch.zeros(40, n, device=DEV))
+    same(dense, *plain(x[-40:], xs[-40:], last, ws[-1]), "f32")
+
+
 def test_stream_argument():
     x, xs, w, ws = operands(20, 256, 256, gen_of(8))
     want = decoder.linear_q8(x, xs, w, ws, torch.empty(20, 256, device=DEV)).clone()
