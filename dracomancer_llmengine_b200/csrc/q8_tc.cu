@@ -4,19 +4,32 @@
 //
 // The scales are any fp32 numbers, one for 128 inner values, so the tensor cores' sums cannot run on from block to block:
 // each block's product goes to its own TMEM buffer, and consumer warps add it, times its scale, to sums in their
-// registers (fma, two values an instruction).  A row's scale is one register of its thread (a thread is a TMEM lane, a
-// lane a row of x), a weight's scale the same for a warp's columns.
+// registers (fma, two values an instruction).  A thread is a TMEM lane, a lane a row of x, so that a row's scale is one value
+// of its thread and a weight's the same for a warp's columns.  Codes' products are exact in fp32; on B200 the sums of a block
+// came out as exact as fp32's (results are within 1.4e-7 of 64 bits, relative in the 2-norm).
 //
-// A block of threads is persistent over tiles of MT rows of one group and NT rows of its weight:
-//   warp 0      copies: per 128 inner values MT x 128 codes of x (by TMA boxes of 32 rows, or row by row with gather4 where
-//               the rows are given by index) and NT x 128 of the weight, 128-byte swizzle, a ring of stages
-//   warp 1      products: 4 instructions of K 32 a stage, into a ring of TMEM buffers; frees the stage
-//   warps 4-11  sums: two warps for each quarter of the TMEM lanes, each half of the columns
+// A block of threads is persistent over tiles of MT rows of one group and NT rows of its weight.  A stage has one block of 128
+// inner values (two where NT <= 64: there a stage costs its hand-overs, not its bytes):
+//   warp 0      copies of the weight: TMA boxes of NT rows x 128 bytes, 128-byte swizzle, a ring of stages
+//   warp 2      copies of x: a TMA box, or 16 bytes at a time where rows are given by index (gather4 boxes took 75 cycles for
+//               four rows), and the block's scales, which would wait 2 us behind the copies in flight if each consumer
+//               asked for its own
+//   warps 1, 3  products of every second stage, each in two parts that are handed on alone: of each half of the weight's rows
+//               (so that one half's sums are added while the other's product runs: TMEM holds two stages' products of 256
+//               columns), or of each of the stage's blocks
+//   warps 4-11  sums: two warps for each quarter of the TMEM lanes, each half of the columns; 32 columns on their way while 32
+//               are added (16 took as long, twice the warps with half the columns each half as long again)
 // With SwiGLU the NT weight rows are NT / 2 of gate and the same of up, a thread holds both products of its columns, and
 // 256 / NT blocks of threads that share a scale group of 128 columns exchange their rows' maxima through distributed
-// shared memory.
+// shared memory.  Where a dense call has few tiles, up to eight blocks of threads, a cluster, share a tile's inner size and
+// add their sums up through distributed shared memory, each an equal part of the rows.
 //
-// Tiles run through a group's rows first, so that a weight's tile is read from memory once.
+// Tiles run through a group's rows first, so that a weight's tile is read from memory once.  Wide tiles: a block of 128 x 256
+// takes 512 cycles of the tensor cores and 48 KB from the L2 cache.
+//
+// Measured: 8192 rows, 7168 x 7168, bf16: 435 to 500 us by the GPU's power (1.74 to 1.93 PFLOP/s; at 1000 W its clock is 1.45
+// GHz; the products alone take 275 us, the copies alone 264, adding up alone 317).  384 experts of 2048 x 7168, 512 rows: 650 to
+// 710 us (5.8 to 6.3 TB/s); gate and up of 7168 x 2048: 1352 us (6.1 TB/s).
 //
 // Every wait is bounded; one that runs out ends the block's work, its rows (those it had not finished) become NaN and the
 // status word says which wait it was.
@@ -36,9 +49,6 @@ namespace {
 using sync::smem_addr;
 
 constexpr int kStagingWarp = 2048;
-#ifndef Q8_WIDE
-#define Q8_WIDE 512
-#endif
 constexpr int kStatusOperands = 1, kStatusProduct = 2, kStatusJoin = 4, kStatusBuffer = 8, kStatusStage = 16;
 constexpr float kTiny = 7.888609e-31f;   // 2^-100
 constexpr float kJoin = 2.f;             // us that the parts of a tile take to join
@@ -46,7 +56,7 @@ constexpr int kPrefetch = 64;            // blocks of a dense call's first tile 
 constexpr int kSmemMost = 227 * 1024;
 
 struct Call {
-    CUtensorMap x, xt, w;       // x in boxes of 32 rows (of one, where rows are given by index) and of 128
+    CUtensorMap x, xt, w;       // x in boxes of 32 rows and of 128
     Q8Args a;
     int n_tiles;        // column tiles (with SwiGLU: of 128 columns)
     int vec;            // rows of the output start on 16 bytes
@@ -61,10 +71,10 @@ struct Cfg {
     static constexpr int kSets = kPer == 1 ? 2 : 1;                     // parts of a stage's products that are handed on alone
     static constexpr int kBuffers = NT == 256 ? 2 : NT == 32 ? 8 : 4;   // a stage's products each
     static constexpr int kColumns = kPer * NT * kBuffers;               // 512
-    static constexpr int kParts = NT >= Q8_WIDE ? 4 : 2;                // warps that share a row's columns
+    static constexpr int kParts = 2;                                    // warps that share a row's columns
     static constexpr int kThreads = 128 + 128 * kParts;
     static constexpr int kActive = MT / 32 * kParts;                    // consumer warps that have rows
-    static constexpr int kStaging = kActive * kStagingWarp / (kParts / 2);
+    static constexpr int kStaging = kActive * kStagingWarp;
     static constexpr int kTops = SW ? 2 * kCluster * kParts * MT * 4 : 0;   // two tiles' maxima, of each part of each block
     // a block's scales: of MT rows of x, and two of the weight (of the halves of the columns, or of gate and up).  They stay until
     // the block's product has been added: the copies of a stage wait for the product S stages before, which waited for its
@@ -196,12 +206,9 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&v)[N]) {
 
 // acc += scale * the block's product, for COLS columns from `addr`; the next piece is on its way while one is added.  `read`
 // is called when the last one has arrived.
-#ifndef Q8_PIECE
-#define Q8_PIECE 32
-#endif
 template <int COLS, typename F>
 __device__ __forceinline__ void add_block(float2 (&acc)[COLS / 2], uint32_t addr, float scale, F&& read) {
-    constexpr int C = COLS < Q8_PIECE ? COLS : Q8_PIECE, N = COLS / C;
+    constexpr int C = COLS < 32 ? COLS : 32, N = COLS / C;
     const float2 s = make_float2(scale, scale);
     uint32_t v[2][C];
     tmem_load<C>(addr, v[0]);
@@ -234,7 +241,7 @@ __device__ __forceinline__ void store_piece(uint8_t* p, const uint8_t* src, long
 // 32 rows of BYTES bytes, one a lane, to memory in pieces of 16 bytes side by side, through the warp's staging buffer (2 KB; a
 // piece's place is turned by its row, so that eight rows' pieces lie in different banks).  A few rows go directly: the lanes
 // that have one need no other's.
-template <int BYTES, int STAGING>
+template <int BYTES>
 __device__ __forceinline__ void store_rows(uint8_t* staging, int lane, const uint32_t (&v)[BYTES / 4], uint8_t* out, long row_bytes,
                                            int rows, long left, bool vec, int elem) {
     if constexpr (BYTES < 16) {
@@ -264,39 +271,34 @@ __device__ __forceinline__ void store_rows(uint8_t* staging, int lane, const uin
             }
             return;
         }
-        constexpr int ROWS = STAGING / BYTES < 32 ? STAGING / BYTES : 32;       // at a time
-        auto place = [](int r, int i) { return r % ROWS * BYTES + (P == 4 ? i ^ ((r >> 1) & 3) : P == 2 ? i ^ ((r >> 2) & 1) : i) * 16; };
+                auto place = [](int r, int i) { return r * BYTES + (P == 4 ? i ^ ((r >> 1) & 3) : P == 2 ? i ^ ((r >> 2) & 1) : i) * 16; };
+        __syncwarp();
 #pragma unroll
-        for (int r0 = 0; r0 < 32; r0 += ROWS) {
-            __syncwarp();
-            if (ROWS == 32 || (lane >= r0 && lane < r0 + ROWS))
+        for (int i = 0; i < P; i++)
+            *reinterpret_cast<uint4*>(staging + place(lane, i)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        __syncwarp();
+        if (vec) {
 #pragma unroll
-                for (int i = 0; i < P; i++)
-                    *reinterpret_cast<uint4*>(staging + place(lane, i)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-            __syncwarp();
-            if (vec) {
-#pragma unroll
-                for (int i = 0; i < ROWS * P / 32; i++) {
-                    const int r = r0 + (i * 32 + lane) / P, c = lane % P;
-                    if (r < rows) store_piece(out + r * row_bytes + c * 16, staging + place(r, c), left - c * 16, true, elem);
-                }
-            } else {        // element by element, neighbouring lanes neighbouring elements
-                const int per = BYTES / elem, inside = (int)min((long)BYTES, left);
-                for (int e = lane; e < min(rows - r0, ROWS) * per; e += 32) {
-                    const int r = r0 + e / per, at = e % per * elem;
-                    const uint8_t* src = staging + place(r, at / 16) + at % 16;
-                    uint8_t* p = out + r * row_bytes + at;
-                    if (at >= inside) continue;
-                    if (elem == 4) *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(src);
-                    else if (elem == 2) *reinterpret_cast<uint16_t*>(p) = *reinterpret_cast<const uint16_t*>(src);
-                    else *p = *src;
-                }
+            for (int i = 0; i < P; i++) {
+                const int r = (i * 32 + lane) / P, c = lane % P;
+                if (r < rows) store_piece(out + r * row_bytes + c * 16, staging + place(r, c), left - c * 16, true, elem);
+            }
+        } else {        // element by element, neighbouring lanes neighbouring elements
+            const int per = BYTES / elem, inside = (int)min((long)BYTES, left);
+            for (int e = lane; e < min(rows, 32) * per; e += 32) {
+                const int r = e / per, at = e % per * elem;
+                const uint8_t* src = staging + place(r, at / 16) + at % 16;
+                uint8_t* p = out + r * row_bytes + at;
+                if (at >= inside) continue;
+                if (elem == 4) *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(src);
+                else if (elem == 2) *reinterpret_cast<uint16_t*>(p) = *reinterpret_cast<const uint16_t*>(src);
+                else *p = *src;
             }
         }
     }
 }
 
-template <typename T, int COLS, int STAGING>
+template <typename T, int COLS>
 __device__ __forceinline__ void store_product(uint8_t* staging, int lane, const float2 (&acc)[COLS / 2], bool zero, uint8_t* out,
                                               long row_bytes, int rows, long left, bool vec) {
     constexpr int S = sizeof(T), C = COLS * S < 64 ? COLS : 64 / S;     // columns of a piece
@@ -310,7 +312,7 @@ __device__ __forceinline__ void store_product(uint8_t* staging, int lane, const 
             if constexpr (S == 4) v[2 * j] = __float_as_uint(f.x), v[2 * j + 1] = __float_as_uint(f.y);
             else v[j] = pack2<T>(f.x, f.y);
         }
-        store_rows<C * S, STAGING>(staging, lane, v, out + i * C * S, row_bytes, rows, left - (long)i * C * S, vec, S);
+        store_rows<C * S>(staging, lane, v, out + i * C * S, row_bytes, rows, left - (long)i * C * S, vec, S);
     }
 }
 
@@ -486,7 +488,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
     volatile int* const fail = s_fail;
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kParts == 2 ? 72 : 32));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");     // 4 x 72 + 8 x 216 = 12 x 168 registers of 32 threads
         int stage = 0;
         bool go = true;
         Walk walk(groups);
@@ -627,7 +629,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             while (!sync::mbar_try(drain, 0) && sync::global_ns() - t0 < sync::kWaitLimitNs) {}
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kParts == 2 ? 216 : 112));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int quarter = warp & 3, part = (warp - 4) >> 2;
         if (quarter * 32 < MT) {
             constexpr int COLS = NT / C::kParts;            // of this warp; with SwiGLU half of them gate, half up
@@ -636,7 +638,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             const uint32_t columns = tmem + ((uint32_t)(quarter * 32) << 16) + set * (NT / 2) +
                                      (C::kSets == 2 ? part % (C::kParts / 2) : part) * (SW ? COLS / 2 : COLS);
             constexpr uint32_t to_up = C::kSets == 1 ? NT / 2 : NT / 4;
-            uint8_t* const mine = staging + (part * (MT / 32) + quarter) * (kStagingWarp / (C::kParts / 2));
+            uint8_t* const mine = staging + (part * (MT / 32) + quarter) * kStagingWarp;
             uint64_t* const my_full = tfull + set * B;
             uint64_t* const my_empty = tempty + set * B;
             int buf = 0, turn = 0, joins = 0, slot = 0;
@@ -718,7 +720,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                             using T = decltype(kind);
                             const long rb = a.out_row * (long)sizeof(T);
                             if (n0 < a.n)
-                                store_product<T, COLS, kStagingWarp / (C::kParts / 2)>(mine, lane, acc, zero, (uint8_t*)a.out + row * rb + (long)n0 * sizeof(T), rb,
+                                store_product<T, COLS>(mine, lane, acc, zero, (uint8_t*)a.out + row * rb + (long)n0 * sizeof(T), rb,
                                                        rows, (long)(a.n - n0) * sizeof(T), c.vec);
                         };
                         if (a.dtype == kF32) put(0.f);
@@ -778,7 +780,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                             v[j] = (uint32_t)lo | (uint32_t)hi << 16;
                         }
                         if (n0 < a.n)
-                            store_rows<H, kStagingWarp / (C::kParts / 2)>(mine, lane, v, (uint8_t*)a.out + row * a.out_row + n0, a.out_row, rows, a.n - n0, c.vec, 1);
+                            store_rows<H>(mine, lane, v, (uint8_t*)a.out + row * a.out_row + n0, a.out_row, rows, a.n - n0, c.vec, 1);
                         if (rank == 0 && part == 0 && lane < rows)
                             a.out_scales[(row + lane) * a.os_row + now.col] =
                                 top < kTiny ? 0.f : top <= 3.402823466e38f ? __fdiv_rn(top, 448.f) : __int_as_float(0x7fc00000);
