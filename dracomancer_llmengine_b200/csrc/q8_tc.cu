@@ -67,7 +67,11 @@ template <int MT, int NT, bool SW>
 struct Cfg {
     static constexpr int kCluster = SW ? 256 / NT : 1;
     static constexpr int kPer = NT <= 64 ? 2 : 1;                       // blocks of 128 inner values of a stage
-    static constexpr int kA = MT * 128, kB = NT * 128, kStage = kPer * (kA + kB);
+    // the product takes 128 rows of x: with MT 32 the others are zeros that stay in the wide tiles' stages (of which fewer fit, but
+    // products of whatever lies there take power, which a memory-bound call shares with the memory: 384 experts of 2048 x
+    // 7168, call after call, 790 us without, 755 with them), in narrow ones whatever lies there
+    static constexpr bool kZeros = MT == 32 && NT >= 128;
+    static constexpr int kA = (kZeros ? 128 : MT) * 128, kB = NT * 128, kStage = kPer * (kA + kB);
     static constexpr int kSets = kPer == 1 ? 2 : 1;                     // parts of a stage's products that are handed on alone
     static constexpr int kBuffers = NT == 256 ? 2 : NT == 32 ? 8 : 4;   // a stage's products each
     static constexpr int kColumns = kPer * NT * kBuffers;               // 512
@@ -81,8 +85,8 @@ struct Cfg {
     // buffer, so that S + B stages' scales are in use at most.
     static constexpr int kScale = MT + 4;
     static constexpr int kMiscBut = 640 + 2 * 4 * (kQ8MaxGroups + 1) + 8 * 128;
-    // the product reads 128 rows from a stage of MT: what lies behind the ring has to be there
-    static constexpr int kPad = kStaging + kTops + kMiscBut >= 16384 ? 0 : 16384;
+    // where the product reads 128 rows from a stage of MT, what lies behind the ring has to be there
+    static constexpr int kPad = kA == 128 * 128 || kStaging + kTops + kMiscBut >= 16384 ? 0 : 16384;
     static constexpr int kFixed = 1024 + kStaging + kTops + kMiscBut + kPad;
     static constexpr int turns(int stages) { return stages + kBuffers <= 8 ? 8 : stages + kBuffers <= 16 ? 16 : 32; }
     static constexpr int bytes(int stages) { return kFixed + stages * kStage + turns(stages) * kPer * kScale * 4; }
@@ -215,6 +219,8 @@ __device__ __forceinline__ void add_block(float2 (&acc)[COLS / 2], uint32_t addr
 #pragma unroll
     for (int i = 0; i < N; i++) {
         tc_wait_ld();
+#pragma unroll
+        for (int j = 0; j < C; j++) asm volatile("" : "+r"(v[i & 1][j]));      // used behind the wait only
         if (i + 1 < N) tmem_load<C>(addr + (i + 1) * C, v[(i + 1) & 1]);
         else read();
 #pragma unroll
@@ -476,6 +482,12 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             }
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
+    }
+    if constexpr (C::kZeros) {
+        constexpr int P = (C::kA - MT * 128) / 16;
+        for (int i = tid; i < S * P; i += C::kThreads)
+            *reinterpret_cast<uint4*>(ring + i / P * C::kStage + MT * 128 + i % P * 16) = make_uint4(0, 0, 0, 0);
+        sync::fence_proxy_async();
     }
     tc_fence_before();
     __syncthreads();
