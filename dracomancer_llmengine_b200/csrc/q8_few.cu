@@ -4,11 +4,18 @@
 //
 // Operands of mma.m16n8k32 (16 weight rows, 8 rows of x, 32 inner values).  The order of the inner values does not matter as
 // long as both operands have the same, so a lane takes 16 neighbouring bytes of its rows in each half of a block of 128.  They
-// come by asynchronous copies into a ring of the warp's own in shared memory: no warp waits for another.  What is in flight is then bounded by shared memory, not by registers (a ring of registers
-// reached 64 KB an SM, too little for the memory's latency under load).  A block's sums are scaled and added in registers.  A
-// block of threads has 16 weight rows (with SwiGLU 16 of gate and 16 of up), its warps share the inner size; they add up
-// through shared memory, in the order of the warps.  With SwiGLU eight blocks of threads, a cluster, have the 128 columns that
-// share a scale and exchange their rows' maxima through distributed shared memory.
+// come by asynchronous copies into a ring of the warp's own in shared memory: no warp waits for another.  What is in flight is
+// then bounded by shared memory, not by registers (a ring of registers reached 64 KB an SM, too little for the memory's latency
+// under load).  A block's sums are scaled and added in registers.  A block of threads has 16 weight rows (with SwiGLU 16 of gate
+// and 16 of up), its warps share the inner size; they add up through shared memory, in the order of the warps.  With SwiGLU eight
+// blocks of threads, a cluster, have the 128 columns that share a scale and exchange their rows' maxima through distributed
+// shared memory.
+//
+// Why not tcgen05: its products take 128 rows or columns at least, and a tile's hand-over from copies to products to sums takes
+// 0.3 us a block of 128 inner values, which a call of a few us cannot hide.
+//
+// Measured: one row, 2048 x 5120 5.1 us, 7168 x 7168 14.7 us (3.5 TB/s: 3 us pass before the first weights are there); gate and
+// up of 7168 x 2048 10.9 to 16 us by how the GPU's parts have room for clusters (4.5 us are its bytes at the copy rate).
 #include "q8.cuh"
 
 #include <cooperative_groups.h>
