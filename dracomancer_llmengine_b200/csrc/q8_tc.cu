@@ -67,17 +67,20 @@ template <int MT, int NT, bool SW>
 struct Cfg {
     static constexpr int kCluster = SW ? 256 / NT : 1;
     static constexpr int kPer = NT <= 64 ? 2 : 1;                       // blocks of 128 inner values of a stage
-    // the product takes 128 rows of x: with MT 32 the others are zeros that stay in the wide tiles' stages (of which fewer fit, but
-    // products of whatever lies there take power, which a memory-bound call shares with the memory: 384 experts of 2048 x
-    // 7168, call after call, 790 us without, 755 with them), in narrow ones whatever lies there
-    static constexpr bool kZeros = MT == 32 && NT >= 128;
-    static constexpr int kA = (kZeros ? 128 : MT) * 128, kB = NT * 128, kStage = kPer * (kA + kB);
+    // With MT 32 the wide tiles take products of 64 rows, of which 32 are zeros that stay in the stages: products of rows that are
+    // not there take power, which a memory-bound call shares with the memory (384 experts of 2048 x 7168, call after call: 790 us
+    // with 128 rows of whatever lies there, 770 with 96 of zeros, 707 with 64 rows).  Such a product has 16 rows in each quarter of
+    // the TMEM lanes.
+    static constexpr bool kHalf = MT == 32 && NT >= 128;
+    static constexpr int kRows = kHalf ? 64 : 128;                      // of a product
+    static constexpr int kLanes = kHalf ? 16 : 32;                      // rows of x of a quarter of the lanes
+    static constexpr int kA = (kHalf ? 64 : MT) * 128, kB = NT * 128, kStage = kPer * (kA + kB);
     static constexpr int kSets = kPer == 1 ? 2 : 1;                     // parts of a stage's products that are handed on alone
     static constexpr int kBuffers = NT == 256 ? 2 : NT == 32 ? 8 : 4;   // a stage's products each
     static constexpr int kColumns = kPer * NT * kBuffers;               // 512
     static constexpr int kParts = 2;                                    // warps that share a row's columns
     static constexpr int kThreads = 128 + 128 * kParts;
-    static constexpr int kActive = MT / 32 * kParts;                    // consumer warps that have rows
+    static constexpr int kActive = MT / kLanes * kParts;                // consumer warps that have rows
     static constexpr int kStaging = kActive * kStagingWarp;
     static constexpr int kTops = SW ? 2 * kCluster * kParts * MT * 4 : 0;   // two tiles' maxima, of each part of each block
     // a block's scales: of MT rows of x, and two of the weight (of the halves of the columns, or of gate and up).  They stay until
@@ -85,8 +88,8 @@ struct Cfg {
     // buffer, so that S + B stages' scales are in use at most.
     static constexpr int kScale = MT + 4;
     static constexpr int kMiscBut = 640 + 2 * 4 * (kQ8MaxGroups + 1) + 8 * 128;
-    // where the product reads 128 rows from a stage of MT, what lies behind the ring has to be there
-    static constexpr int kPad = kA == 128 * 128 || kStaging + kTops + kMiscBut >= 16384 ? 0 : 16384;
+    // where the product reads more rows than a stage has, what lies behind the ring has to be there
+    static constexpr int kPad = kA == kRows * 128 || kStaging + kTops + kMiscBut >= 16384 ? 0 : 16384;
     static constexpr int kFixed = 1024 + kStaging + kTops + kMiscBut + kPad;
     static constexpr int turns(int stages) { return stages + kBuffers <= 8 ? 8 : stages + kBuffers <= 16 ? 16 : 32; }
     static constexpr int bytes(int stages) { return kFixed + stages * kStage + turns(stages) * kPer * kScale * 4; }
@@ -483,7 +486,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
     }
-    if constexpr (C::kZeros) {
+    if constexpr (C::kHalf) {
         constexpr int P = (C::kA - MT * 128) / 16;
         for (int i = tid; i < S * P; i += C::kThreads)
             *reinterpret_cast<uint4*>(ring + i / P * C::kStage + MT * 128 + i % P * 16) = make_uint4(0, 0, 0, 0);
@@ -596,7 +599,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             }
         } else {        // products of every second stage, in two parts: halves of the weight's rows, or the stage's two blocks
             constexpr int N = NT / C::kSets;
-            constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+            constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(C::kRows >> 4) << 24);
             constexpr uint32_t step_a = C::kSets == 2 ? 0 : C::kA, step_b = C::kSets == 2 ? C::kB / 2 : C::kB;
             const int which = warp >> 1, per_tile = (kb + C::kPer - 1) / C::kPer;
             const long tiles = groups.total > groups.me ? (groups.total - groups.me + groups.at_once - 1) / groups.at_once : 0;
@@ -643,14 +646,16 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int quarter = warp & 3, part = (warp - 4) >> 2;
-        if (quarter * 32 < MT) {
+        if (quarter * C::kLanes < MT) {
             constexpr int COLS = NT / C::kParts;            // of this warp; with SwiGLU half of them gate, half up
             // this warp's columns of a buffer (with SwiGLU those of gate, and those of up behind)
             const int set = C::kSets == 2 ? part / (C::kParts / 2) : 0;
             const uint32_t columns = tmem + ((uint32_t)(quarter * 32) << 16) + set * (NT / 2) +
                                      (C::kSets == 2 ? part % (C::kParts / 2) : part) * (SW ? COLS / 2 : COLS);
             constexpr uint32_t to_up = C::kSets == 1 ? NT / 2 : NT / 4;
-            uint8_t* const mine = staging + (part * (MT / 32) + quarter) * kStagingWarp;
+            const int in_tile = quarter * C::kLanes + lane;        // this lane's row of the tile, if it has one
+            const bool has = C::kLanes == 32 || lane < C::kLanes;
+            uint8_t* const mine = staging + (part * (MT / C::kLanes) + quarter) * kStagingWarp;
             uint64_t* const my_full = tfull + set * B;
             uint64_t* const my_empty = tempty + set * B;
             int buf = 0, turn = 0, joins = 0, slot = 0;
@@ -662,7 +667,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             for (; left; left = walk.next()) {
                 const Tile now = groups.at(walk.t);
                 float2 acc[SW ? COLS / 4 : COLS / 2] = {}, acc_u[SW ? COLS / 4 : 1] = {};
-                const bool idle = quarter * 32 >= now.rows;
+                const bool idle = quarter * C::kLanes >= now.rows;
                 uint64_t* done = nullptr;
                 uint32_t at = 0;
                 // one copy of the code: the instruction cache is too small for several
@@ -680,7 +685,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                         if (++buf == B) buf = 0, parity ^= 1;
                     }
                     const float* const sc = s_scales + (slot * C::kPer + j) * C::kScale;
-                    const float sx = sc[quarter * 32 + lane];
+                    const float sx = sc[has ? in_tile : 0];
                     const float2 sw = *reinterpret_cast<const float2*>(sc + MT);
                     const bool last = C::kPer == 1 || j == C::kPer - 1 || b + 1 == kb;
                     if (last && ++slot == C::kTurns) slot = 0;
@@ -704,9 +709,9 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                     // the sums of this part of the inner size go to the ring's memory, which no product reads any more: rows of NT
                     // values, a row's pieces of 16 bytes turned by the row
                     asm volatile("bar.sync 1, %0;" ::"n"(C::kActive * 32) : "memory");
-                    const int r = quarter * 32 + lane;
+                    const int r = in_tile;
                     auto put = [&](int piece, const float2& lo, const float2& hi) {
-                        *reinterpret_cast<float4*>(ring + r * (NT * 4) + ((piece ^ (r & 7)) << 4)) = make_float4(lo.x, lo.y, hi.x, hi.y);
+                        if (has) *reinterpret_cast<float4*>(ring + r * (NT * 4) + ((piece ^ (r & 7)) << 4)) = make_float4(lo.x, lo.y, hi.x, hi.y);
                     };
                     constexpr int Q = SW ? COLS / 8 : COLS / 4;         // pieces of this warp (SwiGLU: of each matrix)
 #pragma unroll
@@ -718,13 +723,13 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                     break;
                 }
                 bool zero = false;      // a row that takes none of x's
-                if (a.rows && quarter * 32 + lane < now.rows) {
-                    const int src = a.rows[now.first + quarter * 32 + lane];
+                if (a.rows && has && in_tile < now.rows) {
+                    const int src = a.rows[now.first + in_tile];
                     zero = src < 0 || src >= a.n_x;
                 }
                 if (!go) break;
-                const int rows = min(now.rows - quarter * 32, 32);
-                const long row = now.first + quarter * 32;
+                const int rows = min(now.rows - quarter * C::kLanes, C::kLanes);
+                const long row = now.first + quarter * C::kLanes;
                 if constexpr (!SW) {
                     if (!idle) {
                         const int n0 = now.col * NT + part * COLS;
@@ -756,9 +761,10 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                     }
                     // the row's maximum over all 128 columns
                     float* const slots = tops + turn * (CL * C::kParts * MT);
-                    const uint32_t slot = smem_addr(slots + (rank * C::kParts + part) * MT + quarter * 32 + lane), bar = smem_addr(join + turn);
+                    const uint32_t slot = smem_addr(slots + (rank * C::kParts + part) * MT + in_tile), bar = smem_addr(join + turn);
 #pragma unroll
                     for (int p = 0; p < CL; p++) {
+                        if (!has) continue;
                         uint32_t to, at;
                         asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(slot), "r"(p));
                         asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(bar), "r"(p));
@@ -780,7 +786,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                     go = __all_sync(0xffffffffu, ok);
                     if (!go) break;
 #pragma unroll
-                    for (int p = 0; p < CL * C::kParts; p++) top = max_nan(top, slots[p * MT + quarter * 32 + lane]);
+                    for (int p = 0; p < CL * C::kParts; p++) top = max_nan(top, slots[p * MT + (has ? in_tile : 0)]);
                     turn ^= 1;
                     if (!idle) {
                         const float inv = top < kTiny ? 0.f : __fdiv_rn(448.f, top);
@@ -802,8 +808,8 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             // a wait ran out: what this block had not finished becomes NaN
             for (; left && !SPLIT; left = walk.next()) {
                 const Tile tile = groups.at(walk.t);
-                const int r = quarter * 32 + lane;
-                if (r >= tile.rows) continue;
+                const int r = in_tile;
+                if (!has || r >= tile.rows) continue;
                 const long row = tile.first + r;
                 if constexpr (SW) {
                     constexpr int H = COLS / 2;
