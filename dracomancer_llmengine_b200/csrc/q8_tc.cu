@@ -28,8 +28,8 @@
 // takes 512 cycles of the tensor cores and 48 KB from the L2 cache.
 //
 // Measured: 8192 rows, 7168 x 7168, bf16: 435 to 500 us by the GPU's power (1.74 to 1.93 PFLOP/s; at 1000 W its clock is 1.45
-// GHz; the products alone take 275 us, the copies alone 264, adding up alone 317).  384 experts of 2048 x 7168, 512 rows: 650 to
-// 710 us (5.8 to 6.3 TB/s); gate and up of 7168 x 2048: 1352 us (6.1 TB/s).
+// GHz; the products alone take 275 us, the copies alone 264, adding up alone 317).  384 experts of 2048 x 7168, 512 rows: 636 us
+// cool, 725 call after call (6.5 to 5.7 TB/s); gate and up of 7168 x 2048: 1254 and 1380 us (6.6 to 6.0 TB/s).
 //
 // Every wait is bounded; one that runs out ends the block's work, its rows (those it had not finished) become NaN and the
 // status word says which wait it was.
@@ -56,7 +56,7 @@ constexpr int kPrefetch = 64;            // blocks of a dense call's first tile 
 constexpr int kSmemMost = 227 * 1024;
 
 struct Call {
-    CUtensorMap x, xt, w;       // x in boxes of 32 rows and of 128
+    CUtensorMap x, xt, w;       // x in boxes of 32 rows and of the tile's
     Q8Args a;
     int n_tiles;        // column tiles (with SwiGLU: of 128 columns)
     int vec;            // rows of the output start on 16 bytes
@@ -67,11 +67,11 @@ template <int MT, int NT, bool SW>
 struct Cfg {
     static constexpr int kCluster = SW ? 256 / NT : 1;
     static constexpr int kPer = NT <= 64 ? 2 : 1;                       // blocks of 128 inner values of a stage
-    // With MT 32 the wide tiles take products of 64 rows, of which 32 are zeros that stay in the stages: products of rows that are
-    // not there take power, which a memory-bound call shares with the memory (384 experts of 2048 x 7168, call after call: 790 us
-    // with 128 rows of whatever lies there, 770 with 96 of zeros, 707 with 64 rows).  Such a product has 16 rows in each quarter of
-    // the TMEM lanes.
-    static constexpr bool kHalf = MT == 32 && NT >= 128;
+    // With MT 64, and 32 in wide tiles, products are of 64 rows, in the latter 32 of them zeros that stay in the stages: products
+    // of rows that are not there take power, which a memory-bound call shares with the memory (384 experts of 2048 x 7168, call
+    // after call: 790 us with 128 rows of whatever lies there, 770 with 96 of zeros, 707 to 725 with 64 rows).  Such a product has
+    // 16 rows in each quarter of the TMEM lanes.
+    static constexpr bool kHalf = MT == 64 || (MT == 32 && NT >= 128);
     static constexpr int kRows = kHalf ? 64 : 128;                      // of a product
     static constexpr int kLanes = kHalf ? 16 : 32;                      // rows of x of a quarter of the lanes
     static constexpr int kA = (kHalf ? 64 : MT) * 128, kB = NT * 128, kStage = kPer * (kA + kB);
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
         *s_fail = 0;
         sync::fence_init();
         if (!a.rows) asm volatile("prefetch.tensormap [%0];" ::"l"(&c.x) : "memory");
-        if (!a.rows && MT == 128) asm volatile("prefetch.tensormap [%0];" ::"l"(&c.xt) : "memory");
+        if (!a.rows && MT > 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&c.xt) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&c.w) : "memory");
     }
     if (warp == 1) {
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
     }
-    if constexpr (C::kHalf) {
+    if constexpr (C::kHalf && C::kA > MT * 128) {
         constexpr int P = (C::kA - MT * 128) / 16;
         for (int i = tid; i < S * P; i += C::kThreads)
             *reinterpret_cast<uint4*>(ring + i / P * C::kStage + MT * 128 + i % P * 16) = make_uint4(0, 0, 0, 0);
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             while (go && walk.next()) {
                 const Tile tile = groups.at(walk.t);
                 const int n0 = SW ? tile.col * kQ8Block + rank * (NT / 2) : tile.col * NT;
-                const bool tall = MT == 128 && tile.rows > 32;      // one box of 128 rows, else of 32
+                const bool tall = MT > 32 && tile.rows > 32;        // one box of MT rows, else of 32
                 const float* scales[MT / 32];                       // of x's rows lane, lane + 32, ..
                 const float* wscale = nullptr;                      // lanes 0 and 1
                 if (of_x) {
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                             for (; r < tile.rows; r += 4) copy16(((r - sub) & 4 ? odd : even) + (r - sub) * 128, s_src[r] + from, bytes);
                         }
                     } else if (elect_one()) {
-                        sync::mbar_expect_tx(full + stage, (uint32_t)here * (!of_x ? C::kB : tall ? 16384 : 4096));
+                        sync::mbar_expect_tx(full + stage, (uint32_t)here * (!of_x ? C::kB : tall ? MT * 128 : 4096));
 #pragma unroll
                         for (int j = 0; j < C::kPer; j++) {
                             if (j >= here) break;
@@ -903,8 +903,8 @@ bool launch_k(const Q8Args& a, int split, cudaStream_t s) {
     const cuuint64_t wst[3] = {(cuuint64_t)a.k, (cuuint64_t)a.n * a.k, (cuuint64_t)a.n * a.k * mats};
     const cuuint32_t wbox[4] = {128, (cuuint32_t)(!SW ? NT : C::kPer == 1 ? NT / 4 : NT / 2), (cuuint32_t)mats, 1};
     if ((!a.rows && !map_bytes(&c.x, 2, a.x, xd, xst, xbox)) || !map_bytes(&c.w, 4, a.w, wd, wst, wbox)) return false;
-    const cuuint32_t tbox[2] = {128, 128};
-    if (MT == 128 && !a.rows && !map_bytes(&c.xt, 2, a.x, xd, xst, tbox)) return false;
+    const cuuint32_t tbox[2] = {128, MT};
+    if (MT > 32 && !a.rows && !map_bytes(&c.xt, 2, a.x, xd, xst, tbox)) return false;
 
     const int kb = (a.k + kQ8Block - 1) / kQ8Block;
     c.split = C::kCluster == 1 ? split : 1;
@@ -941,6 +941,13 @@ bool launch_n(const Q8Args& a, int nt, int split, cudaStream_t s) {
                        : launch_k<MT, 64, SW>(a, split, s);
 }
 
+template <bool SW>
+bool launch_m(const Q8Args& a, int mt, int nt, int split, cudaStream_t s) {
+    return mt == 32   ? launch_n<32, SW>(a, nt, split, s)
+           : mt == 64 ? launch_n<64, SW>(a, nt, split, s)
+                      : launch_n<128, SW>(a, nt, split, s);
+}
+
 }  // namespace
 
 bool q8_tc_fits(const Q8Args& a) {
@@ -951,10 +958,16 @@ bool q8_tc_fits(const Q8Args& a) {
 // few, several blocks of threads share a tile's inner size.  A tile takes about as long as its blocks of inner values (us a
 // block and for the rest, measured: rows of 128, inner sizes 512 to 7168; a block of a narrow tile takes what the hand-over of
 // its copies and products takes), and tiles run in rounds of as many as there is room for.
+//
+// The rows of a tile: one group's are as many as they need.  By expert, where they differ, tiles of 32 hold most experts' rows up
+// to 16 on average and those of 64 up to 40; with more, more experts need a second tile and with it the weights once more, and
+// tall tiles take power for rows that are not there.  128 experts of 7168 x 2048, call after call, us with tiles of 32, 64 and
+// 128 rows: 16 rows on average 340, 350, 397; 24: 358, 361, 404; 32: 454, 369, 415; 40: 550, 377, 426; 64: 690, 495, 437.  With
+// uneven loads (expert i's share as (i + 1)^-1.2) 16: 402, 373, 406; 40: 537, 449, 446.
 bool launch_q8_tc(const Q8Args& a, cudaStream_t s) {
     static const struct { int nt; float block, rest; } kTiles[] = {{256, 0.50f, 3.0f}, {128, 0.39f, 1.5f}, {64, 0.30f, 1.0f}, {32, 0.29f, 0.8f}};
-    const bool few = a.offsets ? (long)a.n_rows <= 16l * a.groups : a.n_rows <= 32;
-    const int mt = few ? 32 : 128;
+    const long sets = a.offsets ? a.groups : 1;
+    const int mt = a.n_rows <= sets * (a.offsets ? 16 : 32) ? 32 : a.n_rows <= sets * (a.offsets ? 40 : 64) ? 64 : 128;
     const long row_tiles = (a.n_rows + mt - 1) / mt + (a.offsets ? std::min(a.groups, a.n_rows) - 1 : 0);
     const int kb = (a.k + kQ8Block - 1) / kQ8Block;
     int nt = 256, split = 1;
@@ -975,8 +988,8 @@ bool launch_q8_tc(const Q8Args& a, cudaStream_t s) {
         }
     }
     if (a.test_split) split = a.offsets ? 1 : a.test_split;
-    if (a.swiglu) return few ? launch_n<32, true>(a, nt, split, s) : launch_n<128, true>(a, nt, split, s);
-    return few ? launch_n<32, false>(a, nt, split, s) : launch_n<128, false>(a, nt, split, s);
+    if (a.swiglu) return launch_m<true>(a, mt, nt, split, s);
+    return launch_m<false>(a, mt, nt, split, s);
 }
 
 // Few rows: the form whose weights go straight to registers (7 us against 16 for 16 rows, 2048 x 7168; 12 against 8 for 32

@@ -73,7 +73,7 @@ def same(got, want, bound, kind):
 
 
 SHAPES = [(1, 128, 16), (1, 2048, 130), (1, 7168, 2048), (3, 16, 1), (2, 1, 1), (5, 40, 33), (17, 272, 257), (32, 4096, 640),
-          (33, 512, 100), (64, 2048, 2048), (128, 1024, 128), (129, 144, 255), (257, 2064, 513), (1000, 384, 1536), (700, 7168, 384)]
+          (48, 7168, 1040), (33, 512, 100), (64, 2048, 2048), (128, 1024, 128), (129, 144, 255), (257, 2064, 513), (1000, 384, 1536), (700, 7168, 384)]
 
 
 @pytest.mark.parametrize("kind", TYPES)
@@ -154,7 +154,8 @@ def test_not_finite_stays_in_its_row(rows, k, n, form, dlib):
 
 
 COUNTS = {"mixed": [5, 0, 1, 128, 129, 0, 300, 31, 32, 33, 0], "empty ends": [0, 0, 7, 0], "one": [64], "nothing": [0, 0, 0],
-          "decode": [1, 2, 0, 1, 1, 3, 0, 0, 1, 1, 2, 1] * 4, "large": [700, 3, 1025, 0, 257]}
+          "decode": [1, 2, 0, 1, 1, 3, 0, 0, 1, 1, 2, 1] * 4, "large": [700, 3, 1025, 0, 257],
+          "few and some": [33, 0, 1, 0, 64, 2, 0, 17, 0, 0, 65], "tens": [20, 64, 0, 65, 33, 70, 31, 1, 16]}
 
 
 def group_args(counts, k, n, gather, seed, lead=()):
@@ -552,7 +553,8 @@ def test_stream_argument():
 @pytest.mark.parametrize("swiglu", [False, True])
 @pytest.mark.parametrize("which,bits", [(1, 0x101), (2, 0x102), (3, 0x104)])
 @pytest.mark.parametrize("rows,n,form", [(20, 256, 64), (20, 256, 256), (300, 512, 32), (300, 512, 64), (300, 512, 128), (300, 512, 256),
-                                         (300, 512, 2048 + 64), (20, 512, 2048 + 256)])
+                                         (300, 512, 2048 + 64), (20, 512, 2048 + 256), (50, 512, 64), (50, 512, 128), (50, 512, 256),
+                                         (50, 512, 4096 + 256)])
 def test_waits_that_run_out(rows, n, form, which, bits, swiglu):
     """Barriers of the tensor-core form that expect an arrival which never comes: the call ends, its rows are NaN, the status
     says which wait it was (others may have run out with it), and the next call is right."""
