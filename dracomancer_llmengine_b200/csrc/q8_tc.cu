@@ -12,8 +12,8 @@
 // inner values (two where NT <= 64: there a stage costs its hand-overs, not its bytes):
 //   warp 0      copies of the weight: TMA boxes of NT rows x 128 bytes, 128-byte swizzle, a ring of stages
 //   warp 2      copies of x: a TMA box, or 16 bytes at a time where rows are given by index (gather4 boxes took 75 cycles for
-//               four rows), and the block's scales, which would wait 2 us behind the copies in flight if each consumer
-//               asked for its own
+//               four rows; of tall tiles warp 0 copies half), and the block's scales, which would wait 2 us behind the copies in
+//               flight if each consumer asked for its own
 //   warps 1, 3  products of every second stage, each in two parts that are handed on alone: of each half of the weight's rows
 //               (so that one half's sums are added while the other's product runs: TMEM holds two stages' products of 256
 //               columns), or of each of the stage's blocks
@@ -75,6 +75,11 @@ struct Cfg {
     static constexpr int kRows = kHalf ? 64 : 128;                      // of a product
     static constexpr int kLanes = kHalf ? 16 : 32;                      // rows of x of a quarter of the lanes
     static constexpr int kA = (kHalf ? 64 : MT) * 128, kB = NT * 128, kStage = kPer * (kA + kB);
+    // rows by index: in tall tiles the warp that copies the weight copies half of them (4096 tokens, 8 of 256 experts, gate and up of
+    // 2048 x 512: 187 us alone, 177 with it; 8192 tokens, 7168 x 2048: 4310, 4060); in lower ones the weight would wait for it
+    // (tiles of 64: 89 us alone, 92 with it)
+    static constexpr bool kBoth = MT == 128;
+    static constexpr int kApart = kBoth ? 8 : 4;                        // rows between a lane's
     static constexpr int kSets = kPer == 1 ? 2 : 1;                     // parts of a stage's products that are handed on alone
     static constexpr int kBuffers = NT == 256 ? 2 : NT == 32 ? 8 : 4;   // a stage's products each
     static constexpr int kColumns = kPer * NT * kBuffers;               // 512
@@ -436,7 +441,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
     early_launch();
     if (warp == 0 && lane == 0) {
         for (int i = 0; i < S; i++) {
-            sync::mbar_init(full + i, 1 + (a.rows ? 0 : 1) + 32 + (a.test_extra == 1));
+            sync::mbar_init(full + i, (!a.rows ? 2 : C::kBoth ? 33 : 1) + 32 + (a.test_extra == 1));
             sync::mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 2 * B; i++) {
@@ -527,9 +532,13 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                     const int block = SW ? tile.col : min(tile.col * NT + second * (NT / 2), a.n - 1) / kQ8Block;
                     wscale = a.ws + ((long)tile.group * (SW ? 2 * nb : nb) + block + (SW ? second * nb : 0)) * k_blocks + k_first;
                 }
-                if (of_x && a.rows) {
+                const bool copies_rows = a.rows && (C::kBoth || of_x);
+                const int sub = lane >> 3, piece = lane & 7, mine = sub + (C::kBoth && !of_x ? 4 : 0);      // rows by index: mine, mine + kApart, ..
+                if (copies_rows) {
                     __syncwarp();
-                    for (int r = lane; r < tile.rows; r += 32) {
+                    for (int i = lane; i < MT * 4 / C::kApart; i += 32) {
+                        const int r = C::kBoth ? (i & ~3) * 2 + (i & 3) + (of_x ? 0 : 4) : i;
+                        if (r >= tile.rows) break;
                         const int src = a.rows[tile.first + r];
                         s_src[r] = a.x + (src >= 0 && src < a.n_x ? src : 0) * a.x_row + k_first * kQ8Block;     // not used where it is none: the row becomes zero
                     }
@@ -541,26 +550,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                     uint8_t* const pa = ring + stage * C::kStage;
                     uint8_t* const pb = pa + C::kPer * C::kA;
                     const int here = C::kPer == 1 ? 1 : min(C::kPer, kb - b);
-                    if (of_x && a.rows) {
-                        const int k_left = a.k - k_first * kQ8Block;
-                        // a row's 128 bytes by eight lanes; the 16-byte pieces lie where the 128-byte swizzle of the operand has them
-                        const int sub = lane >> 3, piece = lane & 7;
-                        for (int j = 0; j < here; j++) {
-                            const int k0 = (b + j) * kQ8Block + piece * 16;
-                            const int bytes = k0 < k_left ? 16 : 0;             // behind the row: zeros
-                            const int from = bytes ? k0 : 0;
-                            const uint32_t even = smem_addr(pa + j * C::kA) + sub * 128 + ((piece ^ sub) << 4), odd = even ^ 64;
-                            int r = sub;
-                            for (; r + 28 < tile.rows; r += 32) {
-                                const uint8_t* src[8];
-#pragma unroll
-                                for (int i = 0; i < 8; i++) src[i] = s_src[r + 4 * i];
-#pragma unroll
-                                for (int i = 0; i < 8; i++) copy16((i & 1 ? odd : even) + (r - sub + 4 * i) * 128, src[i] + from, bytes);
-                            }
-                            for (; r < tile.rows; r += 4) copy16(((r - sub) & 4 ? odd : even) + (r - sub) * 128, s_src[r] + from, bytes);
-                        }
-                    } else if (elect_one()) {
+                    if ((!of_x || !a.rows) && elect_one()) {
                         sync::mbar_expect_tx(full + stage, (uint32_t)here * (!of_x ? C::kB : tall ? MT * 128 : 4096));
 #pragma unroll
                         for (int j = 0; j < C::kPer; j++) {
@@ -574,6 +564,28 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                                 tma_2d(pa + j * C::kA, tall ? &c.xt : &c.x, k0, tile.first, full + stage);
                             }
                         }
+                    }
+                    __syncwarp();       // the lanes' copies go together (215 us without in the case at kBoth)
+                    if (copies_rows) {
+                        const int k_left = a.k - k_first * kQ8Block;
+                        // a row's 128 bytes by eight lanes; the 16-byte pieces lie where the 128-byte swizzle of the operand has them
+                        for (int j = 0; j < here; j++) {
+                            const int k0 = (b + j) * kQ8Block + piece * 16;
+                            const int bytes = k0 < k_left ? 16 : 0;             // behind the row: zeros
+                            const int from = bytes ? k0 : 0;
+                            const uint32_t to = smem_addr(pa + j * C::kA) + ((piece ^ mine) << 4);
+                            constexpr int A = C::kApart;
+                            int r = mine;
+                            for (; r + A * 7 < tile.rows; r += A * 8) {
+                                const uint8_t* src[8];
+#pragma unroll
+                                for (int i = 0; i < 8; i++) src[i] = s_src[r + A * i];
+#pragma unroll
+                                for (int i = 0; i < 8; i++) copy16((A == 4 && (i & 1) ? to ^ 64 : to) + (r + A * i) * 128, src[i] + from, bytes);
+                            }
+                            for (; r < tile.rows; r += A) copy16((A == 4 && ((r - mine) & 4) ? to ^ 64 : to) + r * 128, s_src[r] + from, bytes);
+                        }
+                        if (!of_x) asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(full + stage)) : "memory");
                     }
                     if (of_x) {
                         for (int j = 0; j < here; j++) {
