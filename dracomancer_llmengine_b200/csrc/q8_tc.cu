@@ -1004,8 +1004,8 @@ bool launch_q8_tc(const Q8Args& a, cudaStream_t s) {
     return launch_m<false>(a, mt, nt, split, s);
 }
 
-// Few rows: the form whose weights go straight to registers (7 us against 16 for 16 rows, 2048 x 7168; 12 against 8 for 32
-// rows, 7168 x 2048; by expert 56 against 76 for 16 rows of 2048 x 7168, 97 against 90 for 32).
+// Few rows: the form whose weights go straight to registers (7 us against 10 for 16 rows, 2048 x 7168; 13 against 8.5 for 32
+// rows, 7168 x 2048; by expert 53 against 58 for 16 rows of 2048 x 7168, 96 against 83 for 32).
 bool launch_q8(const Q8Args& a, cudaStream_t s) {
     if (!q8_tc_fits(a) || a.test_form == kQ8Any) return launch_q8_any(a, s);
     const double cost = (double)q8_slots(a, 8) * (a.swiglu ? 2 : 1) * a.n * a.k;
