@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             sync::mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 2 * B; i++) {
-            sync::mbar_init(tfull + i, 1 + (a.test_extra == 2));
+            sync::mbar_init(tfull + i, 1 + (a.test_extra == 2 || (a.test_extra == 4 && i >= B)));
             sync::mbar_init(tempty + i, C::kActive / C::kSets);
         }
         for (int i = 0; i < 2; i++) sync::mbar_init(join + i, CL * C::kParts * MT + (a.test_extra == 3));
@@ -717,10 +717,13 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                         add_block<COLS>(acc, at + j * NT, sx * (part * COLS < NT / 2 ? sw.x : sw.y), read);
                     }
                 }
-                if (SPLIT && go) {
+                if constexpr (SPLIT) {
                     // the sums of this part of the inner size go to the ring's memory, which no product reads any more: rows of NT
-                    // values, a row's pieces of 16 bytes turned by the row
+                    // values, a row's pieces of 16 bytes turned by the row.  A warp whose wait ran out comes here too, for the others
+                    // wait for it: a wait can run out in one warp and end in time in the next.
                     asm volatile("bar.sync 1, %0;" ::"n"(C::kActive * 32) : "memory");
+                    left = false;
+                    if (!go) break;
                     const int r = in_tile;
                     auto put = [&](int piece, const float2& lo, const float2& hi) {
                         if (has) *reinterpret_cast<float4*>(ring + r * (NT * 4) + ((piece ^ (r & 7)) << 4)) = make_float4(lo.x, lo.y, hi.x, hi.y);
@@ -731,7 +734,6 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                         put(part * Q + i, acc[2 * i], acc[2 * i + 1]);
                         if constexpr (SW) put(NT / 8 + part * Q + i, acc_u[2 * i], acc_u[2 * i + 1]);
                     }
-                    left = false;
                     break;
                 }
                 bool zero = false;      // a row that takes none of x's
