@@ -25,7 +25,7 @@ struct Q8Args {
     bool swiglu;
     int* status;                // or null: waits that ran out are noted there
     long wait_ns;               // their limit
-    int test_extra;             // 1 to 4: an arrival that never comes is expected at a barrier (tests)
+    int test_extra;             // 1 to 4: an arrival that never comes is expected at a barrier, 5: a late copy (tests)
     int test_form;              // 0: the form is chosen; kQ8Few, kQ8Any, or the tensor cores' columns a tile (tests)
     int test_split;             // 0: chosen; blocks of threads that share a tile's inner size (tests)
 };

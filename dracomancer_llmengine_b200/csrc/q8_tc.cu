@@ -100,6 +100,11 @@ struct Cfg {
     static constexpr int bytes(int stages) { return kFixed + stages * kStage + turns(stages) * kPer * kScale * 4; }
     static constexpr int most(int stages) { return stages <= 2 || bytes(stages) <= kSmemMost ? stages : most(stages - 1); }
     static constexpr int kStages = most(16), kTurns = turns(kStages);   // kTurns: stages whose scales are kept
+    // Whether a product warp could take a stage's phase before for the one that it waits for (a phase is known by its parity only).
+    // It has every second step, so with an odd number of stages the phase before is the other warp's step, S before its own.  That
+    // its own step before, i - 2, had a buffer shows that step i - 2 - B has been added; where S < B + 2 step i - S may still be on
+    // its way: copies land in any order.
+    static constexpr bool kAlias = kStages % 2 == 1 && kStages < kBuffers + 2;
     static constexpr int kSmem = bytes(kStages);
 };
 
@@ -185,6 +190,12 @@ __device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x,
             smem_addr(dst)),
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(smem_addr(bar))
         : "memory");
+}
+// a block's NT weight rows from n0 on, with SwiGLU NT / 2 of each matrix
+template <bool SW, int NT, int PER, int BYTES>
+__device__ __forceinline__ void copy_weight(uint8_t* to, const Call& c, int k0, int n0, int group, uint64_t* bar) {
+    tma_4d(to, &c.w, k0, n0, 0, group, bar);
+    if constexpr (SW && PER == 1) tma_4d(to + BYTES / 2, &c.w, k0, n0 + NT / 4, 0, group, bar);
 }
 __device__ __forceinline__ void copy4(uint32_t to, const float* from) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
@@ -557,9 +568,8 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                             if (j >= here) break;
                             const int k0 = (k_first + b + j) * kQ8Block;
                             if (!of_x) {
-                                tma_4d(pb + j * C::kB, &c.w, k0, n0, 0, tile.group, full + stage);
-                                if constexpr (SW && C::kPer == 1)
-                                    tma_4d(pb + C::kB / 2, &c.w, k0, n0 + NT / 4, 0, tile.group, full + stage);
+                                if (a.test_extra == 5 && filled == 0) continue;     // a consumer warp copies it, later
+                                copy_weight<SW, NT, C::kPer, C::kB>(pb + j * C::kB, c, k0, n0, tile.group, full + stage);
                             } else {
                                 tma_2d(pa + j * C::kA, tall ? &c.xt : &c.x, k0, tile.first, full + stage);
                             }
@@ -620,6 +630,10 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             uint32_t parity = 0, bparity = 1;
             const uint64_t desc_a = sdesc_sw128(smem_addr(ring)), desc_b = sdesc_sw128(smem_addr(ring + C::kPer * C::kA));
             for (long i = which; i < tiles * per_tile; i += 2) {
+                if constexpr (C::kAlias) {      // the product S steps before is over: its stage is this step's, or about to be
+                    go = __all_sync(0xffffffffu, wait_bar(empty + stage, parity ^ 1, fail, a.wait_ns, kStatusStage));
+                    if (!go) break;
+                }
                 go = __all_sync(0xffffffffu, wait_bar(full + stage, parity, fail, a.wait_ns, kStatusOperands));
                 if (!go) break;
                 if (a.rows) sync::fence_proxy_async();      // rows came by copies of the generic proxy
@@ -676,6 +690,14 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             bool go = true, ready = false;
             Walk walk(groups);
             bool left = walk.next();
+            if (a.test_extra == 5 && warp == 4 && left && elect_one()) {        // tests: the first step's weight lands last
+                const Tile tile = groups.at(walk.t);
+                const int n0 = SW ? tile.col * kQ8Block + rank * (NT / 2) : tile.col * NT;
+                for (const uint64_t t0 = sync::global_ns(); sync::global_ns() - t0 < 20000;) {}
+                for (int j = 0; j < min(C::kPer, kb); j++)
+                    copy_weight<SW, NT, C::kPer, C::kB>(ring + C::kPer * C::kA + j * C::kB, c, (k_first + j) * kQ8Block, n0, tile.group, full);
+            }
+            __syncwarp();
             for (; left; left = walk.next()) {
                 const Tile now = groups.at(walk.t);
                 float2 acc[SW ? COLS / 4 : COLS / 2] = {}, acc_u[SW ? COLS / 4 : 1] = {};

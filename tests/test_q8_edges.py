@@ -1,9 +1,10 @@
-"""The 8-bit products where they could go wrong: waits of which some run out and some do not."""
+"""The 8-bit products where they could go wrong: waits of which some run out and some do not, copies that land in any order."""
 import pytest
 import torch
 
 import dracomancer_llmengine_b200 as dm
-from test_q8_ops import DEV, cdiv, gen_of, ints, operands, plain, same
+from dracomancer_llmengine_b200 import decoder
+from test_q8_ops import DEV, E4M3, cdiv, check_swiglu, gen_of, ints, of_row, operands, plain, same
 
 pytestmark = pytest.mark.gpu
 
@@ -18,6 +19,8 @@ def _gpu(dlib):
 def c_call(rows, k, n, seed, swiglu):
     """(arguments of a C call, its tensors: x, x_scales, w, w_scales, out, scales, status)"""
     x, xs, w, ws = operands(rows, k, n, gen_of(seed), (2,) if swiglu else ())
+    if swiglu:
+        ws /= 500 * k ** 0.5
     out = torch.zeros(rows, n, dtype=torch.uint8 if swiglu else torch.float32, device=DEV)
     scales, status = torch.zeros(rows, cdiv(n, 128), device=DEV), ints(0)
     a = dm.DracoLinearQ8(x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), n_x=rows, n_rows=rows, n=n, k=k, n_groups=1,
@@ -48,3 +51,45 @@ def test_waits_that_run_out_in_some_warps(swiglu, rows, split, columns, dlib):
     assert int(status) == 0 and not (scales if swiglu else out).isnan().any()
     if not swiglu:
         same(out, *plain(x, xs, w, ws), "f32")
+
+
+@pytest.mark.parametrize("swiglu,form", [(False, f) for f in (32, 64, 128, 256, 2048 + 64, 2048 + 256)] +
+                         [(True, f) for f in (64, 128, 256, 2048 + 256)])
+@pytest.mark.parametrize("rows,k,n", [(20, 4096, 256), (50, 4096, 384), (64, 7168, 130), (300, 4096, 640), (1000, 2064, 1001)])
+def test_copies_that_land_in_another_order(rows, k, n, form, swiglu, dlib):
+    """Every block's first weights land after all its other copies: the same bits."""
+    a, (x, xs, w, ws, out, scales, status) = c_call(rows, k, n, rows + n, swiglu)
+    torch.cuda.synchronize()
+    dlib.draco_b200_test_q8_form(form)
+    assert dlib.draco_b200_linear_q8(a, None) == 0
+    torch.cuda.synchronize()
+    want, want_scales = out.clone(), scales.clone()
+    out.zero_(), scales.zero_()
+    dlib.draco_b200_test_q8_barrier_extra(5)
+    a.wait_limit_us = 0
+    for _ in range(3):
+        assert dlib.draco_b200_linear_q8(a, None) == 0
+    torch.cuda.synchronize()
+    assert int(status) == 0 and torch.equal(out, want) and torch.equal(scales, want_scales)
+    if not swiglu:
+        same(out, *plain(x, xs, w, ws), "f32")
+    else:
+        check_swiglu(out.view(E4M3), scales, x, xs, w, ws)
+
+
+@pytest.mark.parametrize("form", [64, 128, 256])
+@pytest.mark.parametrize("each", [10, 30, 100])
+def test_copies_that_land_in_another_order_by_expert(each, form, dlib):
+    """The same with rows by index, where rows come by other copies, and with many tiles a block."""
+    gen, k, n, groups = gen_of(each), 2048, 2048, 12
+    x, xs, w, ws = operands(100, k, n, gen, (groups,))
+    offsets = torch.arange(groups + 1, device=DEV).int() * each
+    rows = torch.randint(100, (groups * each,), device=DEV, generator=gen).int()
+    dlib.draco_b200_test_q8_form(form)
+    want = decoder.linear_q8(x, xs, w, ws, torch.zeros(groups * each, n, device=DEV), offsets=offsets, rows=rows)
+    dlib.draco_b200_test_q8_barrier_extra(5)
+    status = ints(0)
+    for _ in range(3):
+        got = decoder.linear_q8(x, xs, w, ws, torch.zeros(groups * each, n, device=DEV), offsets=offsets, rows=rows, status=status)
+        assert int(status) == 0 and torch.equal(got, want)
+    same(got[:each], *plain(of_row(x, rows, 0, each), xs[rows[:each].long()], w[0], ws[0]), "f32")
