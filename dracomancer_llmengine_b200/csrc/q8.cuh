@@ -48,17 +48,32 @@ __device__ __forceinline__ Q8Span q8_span(const int* offsets, int g, int n_rows)
     return Q8Span{a, b - a};
 }
 
-// g / (1 + exp(-g)) * u within 2^-21.  exp(-g) as a power of two whose exponent's rounding is put back to first order
-// (2^(t + d) = 2^t (1 + d ln 2)): the exponent is rounded at its own size, up to 2^-17 where exp still fits, which alone would
-// cost the result as much.  Beyond exp's range the quotient is 0.
-__device__ __forceinline__ float q8_silu_mul(float g, float u) {
-    const float log2e = 1.44269504f, t = -g * log2e, d = fmaf(-g, log2e, -t) - g * 1.925963033e-8f;      // log2(e) - log2e
-    float p, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(t));
-    p = fmaf(p, d * 0.693147181f, p);
-    if (t >= 128.f) p = __int_as_float(0x7f800000);        // not infinity times d
+// 2^t within 2^-22, where t is the rounded value of v * log2(e), d what its rounding took away: put back to first order
+// (2^(t + d) = 2^t (1 + d ln 2)).  t is rounded at its own size, up to 2^-18, which alone would cost the result as much.
+__device__ __forceinline__ float q8_exp2(float v, float t, float at) {
+    const float log2e = 1.44269504f, low = (float)(1.4426950408889634 - (double)log2e);
+    const float d = fmaf(v, log2e, -t) + v * low;
+    float p;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(at));
+    return fmaf(p, d * 0.693147181f, p);
+}
+
+// silu(g) * u = g / (1 + exp(-g)) * u within 2^-21 of its value.  Up to |g| = kSiluNear nothing in it leaves fp32's normal range.
+constexpr float kSiluNear = 80.f;
+__device__ __forceinline__ float q8_silu_near(float g, float u) {
+    const float t = -g * 1.44269504f, p = q8_exp2(-g, t, t);
+    float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + p));
     return g * r * u;
+}
+// Farther out silu(g) is g, or g exp(g), which a large u brings back: exp(g) is kept 2^110 times as large, so that what it loses
+// is below 2^-100 of anything.
+__device__ __forceinline__ float q8_silu_mul(float g, float u) {
+    if (fabsf(g) <= kSiluNear) return q8_silu_near(g, u);
+    if (g > 0.f) return g * u;
+    const float t = g * 1.44269504f;
+    const float p = g > -1000.f ? q8_exp2(g, t, t + 110.f) : 0.f;      // NaN: g below
+    return g * p * (u * 7.703719778e-34f);                             // 2^-110
 }
 
 // the group and rows of the row tile `slot` of tiles of M rows; count 0: there is no such tile.  By a whole warp.

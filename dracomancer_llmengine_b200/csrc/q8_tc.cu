@@ -784,11 +784,21 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                     constexpr int H = COLS / 2;             // columns of the result
                     float h[H], top = 0.f;
                     const int n0 = now.col * kQ8Block + rank * (NT / 2) + part * H;
+                    float most = 0.f;
 #pragma unroll
-                    for (int j = 0; j < H / 2; j++) {
-                        const float2 gate = acc[j], up = acc_u[j];
-                        h[2 * j] = q8_silu_mul(gate.x, up.x);
-                        h[2 * j + 1] = q8_silu_mul(gate.y, up.y);
+                    for (int j = 0; j < H / 2; j++) most = fmaxf(most, fmaxf(fabsf(acc[j].x), fabsf(acc[j].y)));    // without NaN, which any form keeps
+                    if (__any_sync(0xffffffffu, most > kSiluNear)) {
+#pragma unroll
+                        for (int j = 0; j < H / 2; j++) {
+                            h[2 * j] = q8_silu_mul(acc[j].x, acc_u[j].x);
+                            h[2 * j + 1] = q8_silu_mul(acc[j].y, acc_u[j].y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < H / 2; j++) {
+                            h[2 * j] = q8_silu_near(acc[j].x, acc_u[j].x);
+                            h[2 * j + 1] = q8_silu_near(acc[j].y, acc_u[j].y);
+                        }
                     }
 #pragma unroll
                     for (int j = 0; j < H; j++) {

@@ -1,4 +1,5 @@
-"""The 8-bit products where they could go wrong: waits of which some run out and some do not, copies that land in any order."""
+"""The 8-bit products where they could go wrong: waits of which some run out and some do not, copies that land in any order,
+gates beyond the range of exp."""
 import pytest
 import torch
 
@@ -93,3 +94,53 @@ def test_copies_that_land_in_another_order_by_expert(each, form, dlib):
         got = decoder.linear_q8(x, xs, w, ws, torch.zeros(groups * each, n, device=DEV), offsets=offsets, rows=rows, status=status)
         assert int(status) == 0 and torch.equal(got, want)
     same(got[:each], *plain(of_row(x, rows, 0, each), xs[rows[:each].long()], w[0], ws[0]), "f32")
+
+
+FAR = [3e38, 2.4e38, 1e30, 1000.5, 999.0, 400.0, 163.0, 104.0, 90.0, 88.7, 87.4, 80.1, 79.9, 20.0, 1.0]
+
+
+@pytest.mark.parametrize("rows", [3, 40, 300])
+@pytest.mark.parametrize("form", [0, 1, 2, 64, 128, 256, 2048 + 256])
+def test_swiglu_of_far_gates(rows, form, dlib):
+    """Gates to the ends of fp32, with ups that bring the product back into its range.  The products are exact here (one value,
+    powers of two); silu and the product are within 2^-21, the scale's quotient is rounded once more; codes are off by half a step
+    (2^-4 of the value, 2^-10 below the normal range) and by what value and scale are off (2^-20 together)."""
+    dlib.draco_b200_test_q8_form(form)
+    k, f = 256, 128
+    x, w = torch.zeros(rows, k, device=DEV), torch.zeros(2, f, k, device=DEV)
+    x[:, 0] = 1
+    sign = torch.tensor([1.0, -1.0, 0.5, -0.5, 0.25, -0.25, 2.0 ** -6, -2.0 ** -6], device=DEV)
+    w[0, :, 0], w[1, :, 0] = sign.repeat(f // 8), sign.repeat_interleave(f // 8)
+    x, w = x.to(E4M3), w.to(E4M3)
+    for gate in FAR + [-g for g in FAR]:
+        for up in (3e38, 1e30, 1e18, 1e9, 1.0, 1e-6, 1e-30, 0.0):
+            ws = torch.ones(2, 1, 2, device=DEV)
+            ws[0], ws[1] = gate, up
+            codes, scales = torch.empty(rows, f, device=DEV).to(E4M3), torch.empty(rows, 1, device=DEV)
+            decoder.swiglu_q8(x, torch.ones(rows, 2, device=DEV), w, ws, codes, scales)
+            g, u = (ws[i, 0, 0].double() * w[i, :, 0].double() for i in (0, 1))
+            h = g / (1 + torch.exp(-g)) * u
+            a, got = float(h.abs().max()), scales.double()
+            assert bool((codes.view(torch.uint8) == codes.view(torch.uint8)[0]).all() and (got == got[0]).all() or got.isnan().all())
+            if a > 3.41e38:
+                assert got.isnan().all()
+            elif a < 2.0 ** -101:
+                assert not got.any() and not codes.float().any()
+            elif a > 2.0 ** -99 and a < 3.4e38:
+                assert bool(((got - a / 448).abs() <= a / 448 * 2.0 ** -20).all())
+                v = h / a * 448
+                assert bool(((codes.double() - v).abs() <= v.abs() * (2.0 ** -4 + 1.1 * 2.0 ** -20) + 2.0 ** -10).all())
+
+
+@pytest.mark.parametrize("form", [0, 1, 2, 64, 128, 256])
+def test_swiglu_of_infinite_gates(form, dlib):
+    """silu(infinity) = infinity and silu(-infinity) = -infinity / infinity: the block's scale is NaN, other blocks' are not."""
+    dlib.draco_b200_test_q8_form(form)
+    x, w = torch.zeros(5, 128, device=DEV), torch.ones(2, 256, 128, device=DEV)
+    x[:, 0] = 1
+    for gate in (float("inf"), -float("inf"), float("nan")):
+        ws = torch.ones(2, 2, 1, device=DEV)
+        ws[0, 1] = gate
+        codes, scales = torch.empty(5, 256, device=DEV).to(E4M3), torch.empty(5, 2, device=DEV)
+        decoder.swiglu_q8(x.to(E4M3), torch.ones(5, 1, device=DEV), w.to(E4M3), ws, codes, scales)
+        assert scales[:, 1].isnan().all() and bool((scales[:, 0] > 0).all() and (codes.float()[:, :128] == 448).all())
