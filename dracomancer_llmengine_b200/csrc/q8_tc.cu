@@ -784,21 +784,23 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                     constexpr int H = COLS / 2;             // columns of the result
                     float h[H], top = 0.f;
                     const int n0 = now.col * kQ8Block + rank * (NT / 2) + part * H;
-                    float most = 0.f;
+                    // A gate far out, which is rare, becomes one of 64 whose up product gives the same (silu(64) is 64): one copy of the code
+                    // that all gates take (4096 tokens, 8 of 256 experts, 2048 x 512: 176.9 us, 178.1 with two, 174.8 without far gates).
+                    float most[4] = {};
 #pragma unroll
-                    for (int j = 0; j < H / 2; j++) most = fmaxf(most, fmaxf(fabsf(acc[j].x), fabsf(acc[j].y)));    // without NaN, which any form keeps
-                    if (__any_sync(0xffffffffu, most > kSiluNear)) {
-#pragma unroll
-                        for (int j = 0; j < H / 2; j++) {
-                            h[2 * j] = q8_silu_mul(acc[j].x, acc_u[j].x);
-                            h[2 * j + 1] = q8_silu_mul(acc[j].y, acc_u[j].y);
-                        }
-                    } else {
+                    for (int j = 0; j < H / 2; j++) most[j & 3] = fmaxf(most[j & 3], fmaxf(fabsf(acc[j].x), fabsf(acc[j].y)));
+                    const bool far = __any_sync(0xffffffffu, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) > kSiluNear);
+                    if (far) {
 #pragma unroll
                         for (int j = 0; j < H / 2; j++) {
-                            h[2 * j] = q8_silu_near(acc[j].x, acc_u[j].x);
-                            h[2 * j + 1] = q8_silu_near(acc[j].y, acc_u[j].y);
+                            if (fabsf(acc[j].x) > kSiluNear) acc_u[j].x = q8_silu_mul(acc[j].x, acc_u[j].x) * (1.f / 64.f), acc[j].x = 64.f;
+                            if (fabsf(acc[j].y) > kSiluNear) acc_u[j].y = q8_silu_mul(acc[j].y, acc_u[j].y) * (1.f / 64.f), acc[j].y = 64.f;
                         }
+                    }
+#pragma unroll
+                    for (int j = 0; j < H / 2; j++) {
+                        h[2 * j] = q8_silu_near(acc[j].x, acc_u[j].x);
+                        h[2 * j + 1] = q8_silu_near(acc[j].y, acc_u[j].y);
                     }
 #pragma unroll
                     for (int j = 0; j < H; j++) {
