@@ -48,6 +48,42 @@ bool on_device(std::initializer_list<const void*> ps) {
         if (p && !abi_device_ptr(p)) return false;
     return true;
 }
+
+// `rows` rows of `bytes` bytes each, `stride` bytes apart; all of them lie in at .. end
+struct View {
+    using Wide = __int128;
+    long at, end, rows, stride, bytes;
+    View(const void* p, long rows_, long stride_, long bytes_)
+        : at((long)(uintptr_t)p), end(at), rows(p && bytes_ > 0 ? rows_ : 0), stride(stride_), bytes(bytes_) {
+        if (stride == 0 && rows > 1) rows = 1;
+        if (rows > 0) end = (long)std::min<Wide>(at + (Wide)(rows - 1) * stride + bytes, 0x7fffffffffffffffl);
+    }
+    View(const void* p, long bytes_) : View(p, 1, 0, bytes_) {}
+};
+// whether a row of one has a byte of a row of the other, where the two are interleaved
+bool rows_meet(const View& a, const View& b) {
+    using Wide = View::Wide;
+    if (a.rows > b.rows) return rows_meet(b, a);
+    // whether a row of b, counted from `first` on, has a byte in from .. from + a.bytes: the first that ends behind `from`
+    auto row_in = [&](Wide from, Wide first) {
+        const Wide past = from - b.bytes - (b.at + first * b.stride);
+        const Wide j = first + (b.rows > 1 && past >= 0 ? past / b.stride + 1 : 0), at = b.at + j * b.stride;
+        return j < b.rows && at + b.bytes > from && at < from + a.bytes;
+    };
+    // with one stride, row j of b lies to row i of a as row j - i would to a's first
+    if (a.rows == 1 || a.stride == b.stride) return row_in(a.at, 1 - a.rows);
+    for (long i = 0; i < a.rows; i++)
+        if (row_in(a.at + (Wide)i * a.stride, 0)) return true;
+    return false;
+}
+// whether the two share a byte; parts of one wider buffer, side by side, do not
+inline bool meet(const View& a, const View& b) { return a.end > b.at && b.end > a.at && a.rows > 0 && b.rows > 0 && rows_meet(a, b); }
+template <size_t N>
+inline bool meets_any(const View& a, const View (&others)[N]) {
+    for (const View& b : others)
+        if (meet(a, b)) return true;
+    return false;
+}
 bool aligned_to(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
 
 const char* cache_fault(const DracoKV4Cache* c) {
@@ -275,8 +311,15 @@ int draco_b200_linear_q8(const DracoLinearQ8* p, void* stream) {
     if (!aligned_to(p->out, b) || !aligned_to(p->x_scales, 4) || !aligned_to(p->w_scales, 4) || !aligned_to(p->offsets, 4) ||
         !aligned_to(p->rows, 4) || !aligned_to(p->out_scales, 4) || !aligned_to(p->status, 4))
         return refuse("%s: buffers must be aligned to their elements", who);
-    if (p->out == p->x || p->out == p->w || (p->swiglu && p->out_scales == p->x_scales))
-        return refuse("%s: outputs must not overlap inputs", who);
+    const long kb = (p->k + kQ8Block - 1) / kQ8Block, mats = (long)p->n_groups * (p->swiglu ? 2 : 1);
+    const View out(p->out, p->n_rows, p->out_stride * (long)b, p->n * (long)b), status(p->status, 4),
+        scales(p->swiglu ? p->out_scales : nullptr, p->n_rows, p->out_scales_stride * 4, nb * 4);
+    const View inputs[] = {View(p->x, p->n_x, p->x_stride, p->k), View(p->x_scales, p->n_x, p->x_scales_stride * 4, kb * 4),
+                           View(p->w, mats * p->n * p->k), View(p->w_scales, mats * nb * kb * 4),
+                           View(p->offsets, (p->n_groups + 1l) * 4), View(p->rows, p->n_rows * 4l)};
+    if (meets_any(out, inputs) || meets_any(scales, inputs) || meets_any(status, inputs) || meet(out, scales) || meet(out, status) ||
+        meet(scales, status))
+        return refuse("%s: outputs must not overlap inputs or one another", who);
     const Q8Args a{(const uint8_t*)p->x, p->x_scales, (const uint8_t*)p->w, p->w_scales, p->offsets, p->rows, p->out,
                    p->out_scales, p->x_stride, p->x_scales_stride, p->out_stride, p->out_scales_stride, p->n_x, p->n_rows,
                    p->n, p->k, p->n_groups, p->dtype, p->swiglu != 0, p->status,
@@ -300,7 +343,9 @@ int draco_b200_plan_experts(const int* order, int n_tokens, int n_used, int firs
     if (!on_device({order, offsets, rows, pos})) return refuse("%s: buffers must be device memory", who);
     if (!aligned_to(order, 4) || !aligned_to(offsets, 4) || !aligned_to(rows, 4) || !aligned_to(pos, 4))
         return refuse("%s: buffers must be aligned to their elements", who);
-    if (n && (order == pos || order == rows || rows == pos)) return refuse("%s: outputs must not overlap inputs", who);
+    const View in(order, n * 4l), o(offsets, (n_experts + 1l) * 4), r(rows, n * 4l), at(pos, n * 4l);
+    if (meet(in, o) || meet(in, r) || meet(in, at) || meet(o, r) || meet(o, at) || meet(r, at))
+        return refuse("%s: outputs must not overlap inputs or one another", who);
     if (!launch_plan_experts(PlanExpertsArgs{order, offsets, rows, pos, n, n_used, n_experts, first}, (cudaStream_t)stream)) {
         const cudaError_t e = cudaGetLastError();
         refuse("%s: launch failed: %s", who, cudaGetErrorString(e));
@@ -326,7 +371,14 @@ int draco_b200_combine_experts(const DracoCombineExperts* p, void* stream) {
     if (!aligned_to(p->y, b) || !aligned_to(p->add, b) || !aligned_to(p->out, b) || !aligned_to(p->pos, 4) ||
         !aligned_to(p->weights, 4))
         return refuse("%s: buffers must be aligned to their elements", who);
-    if (p->out == p->y) return refuse("%s: out must not overlap y", who);
+    const long row = p->hidden * (long)b, used = p->n_used * 4l;
+    const View out(p->out, p->n_tokens, p->out_stride * (long)b, row), add(p->add, p->n_tokens, p->add_stride * (long)b, row);
+    const View inputs[] = {View(p->y, p->n_used ? p->n_y : 0, p->y_stride * (long)b, row),
+                           View(p->pos, p->n_tokens, p->pos_stride * 4, used), View(p->weights, p->n_tokens, p->weights_stride * 4, used)};
+    if (meets_any(out, inputs))
+        return refuse("%s: out must not overlap y, pos or weights", who);
+    if ((p->add != p->out || (p->n_tokens > 1 && p->add_stride != p->out_stride)) && meet(out, add))
+        return refuse("%s: add must be out itself or not overlap it", who);
     const CombineArgs a{p->y, p->pos, p->weights, p->add, p->out, p->y_stride, p->add_stride, p->out_stride, p->pos_stride,
                         p->weights_stride, p->n_y, p->n_tokens, p->n_used, p->hidden, p->dtype};
     launch_combine_experts(a, (cudaStream_t)stream);

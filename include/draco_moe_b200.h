@@ -445,7 +445,7 @@ int draco_b200_rmsnorm_q8(const DracoNormQ8* args, void* stream);
  * with h = gate / (1 + exp(-gate)) * up and a the largest |h| of a row's 128 columns, out is e4m3(h * (448 / a)) and
  * out_scales [n_rows][ceil(n / 128)] a / 448: rows for the next product.  a < 2^-100: code and scale 0; an infinity or NaN
  * in the block: the scale is NaN.
- * No output may overlap an input.  At most 1024 groups, n, k, n_rows and n_x at most 2^24.  x, its rows' stride and w in whole 16 bytes (k % 16 == 0) take the tensor cores,
+ * No output may share a byte with an input or another output (refused; parts of one wider buffer side by side do not).  At most 1024 groups, n, k, n_rows and n_x at most 2^24.  x, its rows' stride and w in whole 16 bytes (k % 16 == 0) take the tensor cores,
  * anything else a slow form.  status, wait_limit_us: as in draco_b200_kv4_attention_checked (rows of a block whose waits
  * ran out are NaN). */
 typedef struct DracoLinearQ8 {
@@ -468,12 +468,12 @@ int draco_b200_linear_q8(const DracoLinearQ8* args, void* stream);
  *   offsets[n_experts + 1]   where each expert's rows start
  *   rows[n_tokens * n_used]  the token of each sorted assignment; entries from offsets[n_experts] on are left as they were
  *   pos[n_tokens * n_used]   where each assignment went, -1 for experts outside the slice
- * At most 1024 experts and 2^24 assignments.  One launch, no workspace. */
+ * None of the four may share a byte with another (refused).  At most 1024 experts and 2^24 assignments.  One launch, no workspace. */
 int draco_b200_plan_experts(const int* order, int n_tokens, int n_used, int first, int n_experts, int* offsets, int* rows,
                             int* pos, void* stream);
 
 /* out[t] = add[t] + sum over k ascending of weights[t][k] * y[pos[t][k]] (hidden values each, fp32 sums, one rounding to
- * dtype; add may be null and may be out, which overlaps nothing else; pos entries outside 0 .. n_y count as nothing). */
+ * dtype; add may be null and may be out, with its stride; out shares no byte with anything else, which is refused; pos entries outside 0 .. n_y count as nothing). */
 typedef struct DracoCombineExperts {
     const void* y;
     const int* pos;

@@ -1,5 +1,5 @@
 """The 8-bit products where they could go wrong: waits of which some run out and some do not, copies that land in any order,
-gates beyond the range of exp."""
+gates beyond the range of exp, inputs and outputs in one buffer."""
 import pytest
 import torch
 
@@ -144,3 +144,52 @@ def test_swiglu_of_infinite_gates(form, dlib):
         codes, scales = torch.empty(5, 256, device=DEV).to(E4M3), torch.empty(5, 2, device=DEV)
         decoder.swiglu_q8(x.to(E4M3), torch.ones(5, 1, device=DEV), w.to(E4M3), ws, codes, scales)
         assert scales[:, 1].isnan().all() and bool((scales[:, 0] > 0).all() and (codes.float()[:, :128] == 448).all())
+
+
+def test_parts_of_one_buffer():
+    """Inputs and outputs side by side in the rows of one buffer are apart; ones that share a byte are refused, with nothing written."""
+    buf = torch.zeros(40, 512, device=DEV).to(E4M3)
+    x, xs, w, ws = operands(40, 256, 128, gen_of(2), (2,))
+    buf[:, :256] = x
+    want = decoder.swiglu_q8(x, xs, w, ws, torch.empty(40, 128, device=DEV).to(E4M3), torch.empty(40, 1, device=DEV))
+    wide_s = torch.cat([xs, xs.new_zeros(40, 1)], 1)
+    got = decoder.swiglu_q8(buf[:, :256], wide_s[:, :2], w, ws, buf[:, 256:384], wide_s[:, 2:])
+    assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(got[1], want[1])
+    before = buf.view(torch.uint8).clone()
+    for codes, scales in ((buf[:, 255:383], wide_s[:, 2:]), (buf[:, 256:384], wide_s[:, 1:2]), (buf[:, 384:], ws.view(-1)[:1].expand(40, 1)),
+                          (buf[:, 384:], buf.view(torch.float32)[:, 100:101])):
+        with pytest.raises(dm.DracoError, match="overlap|strides"):
+            decoder.swiglu_q8(buf[:, :256], wide_s[:, :2], w, ws, codes, scales)
+    flat = torch.zeros(8192, device=DEV)
+    with pytest.raises(dm.DracoError, match="overlap"):
+        decoder.linear_q8(x, flat[:80].view(40, 2), w[0], ws[0], flat[79:79 + 40 * 128].view(40, 128))
+    order = torch.zeros(65, 2, dtype=torch.int32, device=DEV)
+    plan = decoder.ExpertPlan(64, 2, 4)
+    plan.pos = order[1:]
+    with pytest.raises(dm.DracoError, match="overlap"):
+        decoder.plan_experts(order[:64], plan)
+    y = torch.zeros(9, 16, device=DEV)
+    with pytest.raises(dm.DracoError, match="overlap"):
+        decoder.combine_experts(y[:8], ints(0, 1).view(2, 1), torch.ones(2, 1, device=DEV), y[7:9])
+    torch.cuda.synchronize()
+    assert torch.equal(buf.view(torch.uint8), before) and not flat.any() and not order.any()
+
+
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("rows,form", [(20, 128), (20, 256), (50, 128), (300, 128), (300, 256)])
+def test_waits_that_run_out_leave_nothing_wrong(rows, form, swiglu, dlib):
+    """Without shared tiles: what is not NaN is right, what has no product is NaN."""
+    a, (x, xs, w, ws, out, scales, status) = c_call(rows, 512, 512, rows, swiglu)
+    dlib.draco_b200_test_q8_form(form)
+    dlib.draco_b200_test_q8_barrier_extra(4)
+    torch.cuda.synchronize()
+    assert dlib.draco_b200_linear_q8(a, None) == 0
+    torch.cuda.synchronize()
+    assert int(status) & 0x102 == 0x102
+    if swiglu:
+        assert scales.isnan().all()
+    else:
+        want, bound = plain(x, xs, w, ws)
+        bad = out.isnan()
+        assert bad.any() and not bad.all()
+        same(torch.where(bad, 0.0, out), torch.where(bad, 0.0, want), bound, "f32")
