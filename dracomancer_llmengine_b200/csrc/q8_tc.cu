@@ -214,17 +214,9 @@ __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint3
 
 template <int N>
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&v)[N]) {
-    if constexpr (N == 32) {
-        tc_ld32(addr, v);
-    } else if constexpr (N == 16) {
-        tc_ld16(addr, v);
-    } else {
-        static_assert(N == 8, "8, 16 or 32 columns");
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                     : "r"(addr)
-                     : "memory");
-    }
+    static_assert(N == 16 || N == 32, "16 or 32 columns");
+    if constexpr (N == 32) tc_ld32(addr, v);
+    else tc_ld16(addr, v);
 }
 
 // acc += scale * the block's product, for COLS columns from `addr`; the next piece is on its way while one is added.  `read`
@@ -269,56 +261,40 @@ __device__ __forceinline__ void store_piece(uint8_t* p, const uint8_t* src, long
 template <int BYTES>
 __device__ __forceinline__ void store_rows(uint8_t* staging, int lane, const uint32_t (&v)[BYTES / 4], uint8_t* out, long row_bytes,
                                            int rows, long left, bool vec, int elem) {
-    if constexpr (BYTES < 16) {
+    static_assert(BYTES % 16 == 0, "whole pieces");
+    constexpr int P = BYTES / 16;       // pieces of a row
+    if (rows <= 4) {
         if (lane >= rows) return;
-        uint8_t* p = out + lane * row_bytes;
-        if (vec && left >= BYTES) {
 #pragma unroll
-            for (int i = 0; i < BYTES / 4; i++) reinterpret_cast<uint32_t*>(p)[i] = v[i];
-        } else if (elem == 1) {
-#pragma unroll
-            for (int i = 0; i < BYTES; i++)
-                if (i < left) p[i] = (uint8_t)(v[i / 4] >> (8 * (i & 3)));
-        } else {
-#pragma unroll
-            for (int i = 0; i < BYTES / 2; i++)
-                if (2 * i < left) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+        for (int i = 0; i < P; i++) {
+            const uint4 u = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            if (vec && left >= 16 * i + 16) *reinterpret_cast<uint4*>(out + lane * row_bytes + i * 16) = u;
+            else store_piece(out + lane * row_bytes + i * 16, reinterpret_cast<const uint8_t*>(&u), left - i * 16, false, elem);
         }
-    } else {
-        constexpr int P = BYTES / 16;       // pieces of a row
-        if (rows <= 4) {
-            if (lane >= rows) return;
+        return;
+    }
+    auto place = [](int r, int i) { return r * BYTES + (P == 4 ? i ^ ((r >> 1) & 3) : P == 2 ? i ^ ((r >> 2) & 1) : i) * 16; };
+    __syncwarp();
 #pragma unroll
-            for (int i = 0; i < P; i++) {
-                const uint4 u = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                if (vec && left >= 16 * i + 16) *reinterpret_cast<uint4*>(out + lane * row_bytes + i * 16) = u;
-                else store_piece(out + lane * row_bytes + i * 16, reinterpret_cast<const uint8_t*>(&u), left - i * 16, false, elem);
-            }
-            return;
+    for (int i = 0; i < P; i++)
+        *reinterpret_cast<uint4*>(staging + place(lane, i)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    __syncwarp();
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < P; i++) {
+            const int r = (i * 32 + lane) / P, c = lane % P;
+            if (r < rows) store_piece(out + r * row_bytes + c * 16, staging + place(r, c), left - c * 16, true, elem);
         }
-                auto place = [](int r, int i) { return r * BYTES + (P == 4 ? i ^ ((r >> 1) & 3) : P == 2 ? i ^ ((r >> 2) & 1) : i) * 16; };
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < P; i++)
-            *reinterpret_cast<uint4*>(staging + place(lane, i)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        __syncwarp();
-        if (vec) {
-#pragma unroll
-            for (int i = 0; i < P; i++) {
-                const int r = (i * 32 + lane) / P, c = lane % P;
-                if (r < rows) store_piece(out + r * row_bytes + c * 16, staging + place(r, c), left - c * 16, true, elem);
-            }
-        } else {        // element by element, neighbouring lanes neighbouring elements
-            const int per = BYTES / elem, inside = (int)min((long)BYTES, left);
-            for (int e = lane; e < min(rows, 32) * per; e += 32) {
-                const int r = e / per, at = e % per * elem;
-                const uint8_t* src = staging + place(r, at / 16) + at % 16;
-                uint8_t* p = out + r * row_bytes + at;
-                if (at >= inside) continue;
-                if (elem == 4) *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(src);
-                else if (elem == 2) *reinterpret_cast<uint16_t*>(p) = *reinterpret_cast<const uint16_t*>(src);
-                else *p = *src;
-            }
+    } else {        // element by element, neighbouring lanes neighbouring elements
+        const int per = BYTES / elem, inside = (int)min((long)BYTES, left);
+        for (int e = lane; e < min(rows, 32) * per; e += 32) {
+            const int r = e / per, at = e % per * elem;
+            const uint8_t* src = staging + place(r, at / 16) + at % 16;
+            uint8_t* p = out + r * row_bytes + at;
+            if (at >= inside) continue;
+            if (elem == 4) *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(src);
+            else if (elem == 2) *reinterpret_cast<uint16_t*>(p) = *reinterpret_cast<const uint16_t*>(src);
+            else *p = *src;
         }
     }
 }
