@@ -68,13 +68,13 @@ __device__ __forceinline__ float q8_silu_near(float g, float u) {
 }
 // Farther out silu(g) is g, or g exp(g), which a large u brings back: exp(g) is kept 2^110 times as large, so that what it loses
 // is below 2^-100 of anything.
-__device__ __forceinline__ float q8_silu_mul(float g, float u) {
-    if (fabsf(g) <= kSiluNear) return q8_silu_near(g, u);
+__device__ __forceinline__ float q8_silu_far(float g, float u) {
     if (g > 0.f) return g * u;
     const float t = g * 1.44269504f;
     const float p = g > -1000.f ? q8_exp2(g, t, t + 110.f) : 0.f;      // NaN: g below
     return g * p * (u * 7.703719778e-34f);                             // 2^-110
 }
+__device__ __forceinline__ float q8_silu_mul(float g, float u) { return fabsf(g) <= kSiluNear ? q8_silu_near(g, u) : q8_silu_far(g, u); }
 
 // the group and rows of the row tile `slot` of tiles of M rows; count 0: there is no such tile.  By a whole warp.
 struct Q8Where {

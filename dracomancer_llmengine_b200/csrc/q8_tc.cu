@@ -379,7 +379,9 @@ __device__ void join_parts(const Call& c, const Tile& now, const uint8_t* ring, 
         const int lane = tid & 31;
         for (int r = r0 + (tid >> 5); r < r0 + rows; r += Cfg<MT, NT, SW>::kThreads / 32) {     // a warp has a row's 128 columns
             const float4 g = sum(r, lane), u = sum(r, NT / 8 + lane);
-            const float h[4] = {q8_silu_mul(g.x, u.x), q8_silu_mul(g.y, u.y), q8_silu_mul(g.z, u.z), q8_silu_mul(g.w, u.w)};
+            float h[4] = {q8_silu_near(g.x, u.x), q8_silu_near(g.y, u.y), q8_silu_near(g.z, u.z), q8_silu_near(g.w, u.w)};
+            if (fmaxf(fmaxf(fabsf(g.x), fabsf(g.y)), fmaxf(fabsf(g.z), fabsf(g.w))) > kSiluNear)
+                h[0] = q8_silu_mul(g.x, u.x), h[1] = q8_silu_mul(g.y, u.y), h[2] = q8_silu_mul(g.z, u.z), h[3] = q8_silu_mul(g.w, u.w);
             float top = max_nan(max_nan(fabsf(h[0]), fabsf(h[1])), max_nan(fabsf(h[2]), fabsf(h[3])));
             top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));       // NaN is above infinity
             const float inv = top < kTiny ? 0.f : __fdiv_rn(448.f, top);
@@ -761,7 +763,8 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                     float h[H], top = 0.f;
                     const int n0 = now.col * kQ8Block + rank * (NT / 2) + part * H;
                     // A gate far out, which is rare, becomes one of 64 whose up product gives the same (silu(64) is 64): one copy of the code
-                    // that all gates take (4096 tokens, 8 of 256 experts, 2048 x 512: 176.9 us, 178.1 with two, 174.8 without far gates).
+                    // that all gates take (4096 tokens, 8 of 256 experts, 2048 x 512, call after call: 203 us, 205 with two, 202 without
+                    // far gates).
                     float most[4] = {};
 #pragma unroll
                     for (int j = 0; j < H / 2; j++) most[j & 3] = fmaxf(most[j & 3], fmaxf(fabsf(acc[j].x), fabsf(acc[j].y)));
@@ -769,8 +772,8 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                     if (far) {
 #pragma unroll
                         for (int j = 0; j < H / 2; j++) {
-                            if (fabsf(acc[j].x) > kSiluNear) acc_u[j].x = q8_silu_mul(acc[j].x, acc_u[j].x) * (1.f / 64.f), acc[j].x = 64.f;
-                            if (fabsf(acc[j].y) > kSiluNear) acc_u[j].y = q8_silu_mul(acc[j].y, acc_u[j].y) * (1.f / 64.f), acc[j].y = 64.f;
+                            if (fabsf(acc[j].x) > kSiluNear) acc_u[j].x = q8_silu_far(acc[j].x, acc_u[j].x) * (1.f / 64.f), acc[j].x = 64.f;
+                            if (fabsf(acc[j].y) > kSiluNear) acc_u[j].y = q8_silu_far(acc[j].y, acc_u[j].y) * (1.f / 64.f), acc[j].y = 64.f;
                         }
                     }
 #pragma unroll
