@@ -151,7 +151,7 @@ int draco_b200_test_kv4_barrier_extra(int which) {
     return old;
 }
 // the same for the 8-bit products' tensor-core form (1: a step's operands, 2: its product, 3: a join of a block's column maxima,
-// 4: the product of the second half of a tile's columns alone, in tiles of 128 and 256 columns); 5: the copy of each block's first weights comes 20 us late, all else as it is
+// 4: the product of the second half of a tile's columns alone, in tiles of 128 and 256 columns); 5: each block's first operands come 20 us late, all else as it is
 int draco_b200_test_q8_barrier_extra(int which) {
     const int old = t_test_q8_extra;
     if (which >= 0 && which <= 5) t_test_q8_extra = which;

@@ -265,7 +265,9 @@ bool launch_k(const Q8Args& a, cudaStream_t s) {
 
 bool launch_q8_few(const Q8Args& a, cudaStream_t s) {
     const bool eight = a.offsets || a.n_rows <= 8;
-    if (a.swiglu) return launch_k<8, true>(a, s);      // two matrices' weights leave no registers for more rows
+    // gate/up takes eight at a time: with 16 their sums leave the registers (16 rows of 2048 x 768: 5.3 us with two tiles of 8, 7.3
+    // with one of 16; 32 rows, which are rarely few, 9.6 and 7.7)
+    if (a.swiglu) return launch_k<8, true>(a, s);
     return eight ? launch_k<8, false>(a, s) : launch_k<16, false>(a, s);
 }
 

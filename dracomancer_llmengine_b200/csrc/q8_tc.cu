@@ -191,12 +191,6 @@ __device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x,
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(smem_addr(bar))
         : "memory");
 }
-// a block's NT weight rows from n0 on, with SwiGLU NT / 2 of each matrix
-template <bool SW, int NT, int PER, int BYTES>
-__device__ __forceinline__ void copy_weight(uint8_t* to, const Call& c, int k0, int n0, int group, uint64_t* bar) {
-    tma_4d(to, &c.w, k0, n0, 0, group, bar);
-    if constexpr (SW && PER == 1) tma_4d(to + BYTES / 2, &c.w, k0, n0 + NT / 4, 0, group, bar);
-}
 __device__ __forceinline__ void copy4(uint32_t to, const float* from) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
@@ -439,6 +433,8 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
         }
         for (int i = 0; i < 2; i++) sync::mbar_init(join + i, CL * C::kParts * MT + (a.test_extra == 3));
         sync::mbar_init(drain, 2);
+        if (a.test_extra == 5)      // tests: the first step's operands are there when warp 1 says so
+            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], 16;" ::"r"(smem_addr(full)) : "memory");
         *s_fail = 0;
         sync::fence_init();
         if (!a.rows) asm volatile("prefetch.tensormap [%0];" ::"l"(&c.x) : "memory");
@@ -546,8 +542,9 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
                             if (j >= here) break;
                             const int k0 = (k_first + b + j) * kQ8Block;
                             if (!of_x) {
-                                if (a.test_extra == 5 && filled == 0) continue;     // a consumer warp copies it, later
-                                copy_weight<SW, NT, C::kPer, C::kB>(pb + j * C::kB, c, k0, n0, tile.group, full + stage);
+                                tma_4d(pb + j * C::kB, &c.w, k0, n0, 0, tile.group, full + stage);
+                                if constexpr (SW && C::kPer == 1)
+                                    tma_4d(pb + C::kB / 2, &c.w, k0, n0 + NT / 4, 0, tile.group, full + stage);
                             } else {
                                 tma_2d(pa + j * C::kA, tall ? &c.xt : &c.x, k0, tile.first, full + stage);
                             }
@@ -607,6 +604,11 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             stage = which;
             uint32_t parity = 0, bparity = 1;
             const uint64_t desc_a = sdesc_sw128(smem_addr(ring)), desc_b = sdesc_sw128(smem_addr(ring + C::kPer * C::kA));
+            if (a.test_extra == 5 && which == 0 && lane == 0) {
+                for (const uint64_t t0 = sync::global_ns(); sync::global_ns() - t0 < 20000;) {}
+                asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], 16;" ::"r"(smem_addr(full)) : "memory");
+            }
+            __syncwarp();
             for (long i = which; i < tiles * per_tile; i += 2) {
                 if constexpr (C::kAlias) {      // the product S steps before is over: its stage is this step's, or about to be
                     go = __all_sync(0xffffffffu, wait_bar(empty + stage, parity ^ 1, fail, a.wait_ns, kStatusStage));
@@ -668,14 +670,6 @@ __global__ void __launch_bounds__(Cfg<MT, NT, SW>::kThreads, 1) q8_tc_kernel(con
             bool go = true, ready = false;
             Walk walk(groups);
             bool left = walk.next();
-            if (a.test_extra == 5 && warp == 4 && left && elect_one()) {        // tests: the first step's weight lands last
-                const Tile tile = groups.at(walk.t);
-                const int n0 = SW ? tile.col * kQ8Block + rank * (NT / 2) : tile.col * NT;
-                for (const uint64_t t0 = sync::global_ns(); sync::global_ns() - t0 < 20000;) {}
-                for (int j = 0; j < min(C::kPer, kb); j++)
-                    copy_weight<SW, NT, C::kPer, C::kB>(ring + C::kPer * C::kA + j * C::kB, c, (k_first + j) * kQ8Block, n0, tile.group, full);
-            }
-            __syncwarp();
             for (; left; left = walk.next()) {
                 const Tile now = groups.at(walk.t);
                 float2 acc[SW ? COLS / 4 : COLS / 2] = {}, acc_u[SW ? COLS / 4 : 1] = {};
@@ -1019,8 +1013,13 @@ bool launch_q8_tc(const Q8Args& a, cudaStream_t s) {
     return launch_m<false>(a, mt, nt, split, s);
 }
 
-// Few rows: the form whose weights go straight to registers (7 us against 10 for 16 rows, 2048 x 7168; 13 against 8.5 for 32
-// rows, 7168 x 2048; by expert 53 against 58 for 16 rows of 2048 x 7168, 96 against 83 for 32).
+// Few rows: the form in which every warp reads weights through a ring of its own.  It is as fast as its bytes come for a tile of rows
+// (8, dense products up to 16), and takes the weights again for each further tile; the tensor cores' start costs 4 to 5 us more.  So
+// what counts is the number of tiles times the weight.  By expert that is an upper bound, not the load, which the host does not
+// know: a tile for every 8 rows and one more for every expert that can have any.  Measured, us, few rows / tensor cores: 1 row,
+// 7168 x 2048 5.3 / 10.1; 16 rows 6.9 / 10.4; 32 rows 10.8 / 10.5; 64 rows of 2048 x 2048 7.5 / 7.6; gate/up of 8 rows, 7168 x 2048
+// 12.6 / 15.1; 16 rows 21.3 / 15.2; 32 rows of 2048 x 768 9.6 / 9.3; by expert, of 128, products of 16 rows, 2048 x 7168 47 / 45; 32 rows
+// 85 / 78; 32 rows of 768 x 2048 16.1 / 18.6; gate/up of 16 rows, 2048 x 768 15.6 / 21.9.
 bool launch_q8(const Q8Args& a, cudaStream_t s) {
     if (!q8_tc_fits(a) || a.test_form == kQ8Any) return launch_q8_any(a, s);
     const double cost = (double)q8_slots(a, 8) * (a.swiglu ? 2 : 1) * a.n * a.k;

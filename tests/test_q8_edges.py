@@ -58,7 +58,7 @@ def test_waits_that_run_out_in_some_warps(swiglu, rows, split, columns, dlib):
                          [(True, f) for f in (64, 128, 256, 2048 + 256)])
 @pytest.mark.parametrize("rows,k,n", [(20, 4096, 256), (50, 4096, 384), (64, 7168, 130), (300, 4096, 640), (1000, 2064, 1001)])
 def test_copies_that_land_in_another_order(rows, k, n, form, swiglu, dlib):
-    """Every block's first weights land after all its other copies: the same bits."""
+    """Every block's first operands come after all its other copies: the same bits."""
     a, (x, xs, w, ws, out, scales, status) = c_call(rows, k, n, rows + n, swiglu)
     torch.cuda.synchronize()
     dlib.draco_b200_test_q8_form(form)
