@@ -10,8 +10,8 @@
 //
 // combine: out[t] = add[t] + sum over k ascending of weights[t][k] * y[pos[t][k]], fused multiply-adds in fp32, one rounding.
 // Bound by memory: a thread takes 8 neighbouring columns of a token and has eight rows' loads in flight (four in fp32).
-// Measured: 4096 tokens of 8 rows of 7168 bf16 and one more: 99 us, 5.9 TB/s; with four in flight and an index division a
-// thread it was 152.
+// Measured: 4096 tokens of 8 rows of 7168 bf16 and one more: 102 us call after call, 5.8 TB/s; with four in flight and an index
+// division a thread it was 152.
 #include "q8.cuh"
 
 #include <cooperative_groups.h>

@@ -11,11 +11,12 @@
 // blocks of threads, a cluster, have the 128 columns that share a scale and exchange their rows' maxima through distributed
 // shared memory.
 //
-// Why not tcgen05: its products take 128 rows or columns at least, and a tile's hand-over from copies to products to sums takes
+// Why not tcgen05: its products take 64 rows at least, and a tile's hand-over from copies to products to sums takes
 // 0.3 us a block of 128 inner values, which a call of a few us cannot hide.
 //
-// Measured: one row, 2048 x 5120 5.1 us, 7168 x 7168 14.7 us (3.5 TB/s: 3 us pass before the first weights are there); gate and
-// up of 7168 x 2048 10.9 to 16 us by how the GPU's parts have room for clusters (4.5 us are its bytes at the copy rate).
+// Measured, call after call: one row, 2048 x 5120 5.3 us, 7168 x 7168 14.7 us (3.5 TB/s: 3 us pass before the first weights are
+// there); gate and up of 7168 x 2048 11.4 us, 10.9 to 16 by how the GPU's parts have room for clusters (4.5 us are its bytes at the
+// copy rate).
 #include "q8.cuh"
 
 #include <cooperative_groups.h>

@@ -27,9 +27,9 @@
 // Tiles run through a group's rows first, so that a weight's tile is read from memory once.  Wide tiles: a block of 128 x 256
 // takes 512 cycles of the tensor cores and 48 KB from the L2 cache.
 //
-// Measured: 8192 rows, 7168 x 7168, bf16: 435 to 500 us by the GPU's power (1.74 to 1.93 PFLOP/s; at 1000 W its clock is 1.45
-// GHz; the products alone take 275 us, the copies alone 264, adding up alone 317).  384 experts of 2048 x 7168, 512 rows: 636 us
-// cool, 725 call after call (6.5 to 5.7 TB/s); gate and up of 7168 x 2048: 1254 and 1380 us (6.6 to 6.0 TB/s).
+// Measured, call after call for a second (after a rest in brackets; at 1000 W the clock falls to 1.45 GHz): 8192 rows, 7168 x 7168,
+// bf16: 507 us, 1.66 PFLOP/s (468 to 517; the products alone take 275 us, the copies alone 264, adding up alone 317).  384 experts of
+// 2048 x 7168, 512 rows: 704 us, 5.8 TB/s (634 to 697); gate and up of 7168 x 2048: 1340 us, 6.1 TB/s (1242 to 1295).
 //
 // Every wait is bounded; one that runs out ends the block's work, its rows (those it had not finished) become NaN and the
 // status word says which wait it was.
@@ -76,8 +76,8 @@ struct Cfg {
     static constexpr int kLanes = kHalf ? 16 : 32;                      // rows of x of a quarter of the lanes
     static constexpr int kA = (kHalf ? 64 : MT) * 128, kB = NT * 128, kStage = kPer * (kA + kB);
     // rows by index: in tall tiles the warp that copies the weight copies half of them (4096 tokens, 8 of 256 experts, gate and up of
-    // 2048 x 512: 187 us alone, 177 with it; 8192 tokens, 7168 x 2048: 4310, 4060); in lower ones the weight would wait for it
-    // (tiles of 64: 89 us alone, 92 with it)
+    // 2048 x 512, call after call: 212 us alone, 202 with it; 8192 tokens, 7168 x 2048: 4464, 4235); in lower ones the weight would
+    // wait for it (tiles of 64: 89 us alone, 92 with it)
     static constexpr bool kBoth = MT == 128;
     static constexpr int kApart = kBoth ? 8 : 4;                        // rows between a lane's
     static constexpr int kSets = kPer == 1 ? 2 : 1;                     // parts of a stage's products that are handed on alone
