@@ -542,7 +542,7 @@ bool dev_kind(const void* p) { return is_device_ptr(p); }
 // Resolve a [3n] (gate, up, down) pointer table to device addresses; cached per table
 // address and validated against its current contents on every call.
 Table* get_table(Ctx* c, const uint64_t* ptrs, const int* codes, int n, int inter, int n_in, int n_out,
-                 uintptr_t key_addr = 0) {
+                 uintptr_t key_addr = 0, int attempts = 4) {
     auto key = std::make_tuple(key_addr ? key_addr : (uintptr_t)ptrs, n, inter, n_in, n_out);
     auto it = c->tables.find(key);
     if (it != c->tables.end()) {
@@ -636,11 +636,13 @@ Table* get_table(Ctx* c, const uint64_t* ptrs, const int* codes, int n, int inte
         }
         if (dptr[e] % 16) t.aligned16 = false;
     }
-    // an upload made while building this table may have dropped cached tables; the matrices
-    // resolved above must still resolve to the same device bytes
+    // an upload made while building this table may have dropped cached tables, or the copy that an earlier matrix was
+    // found in (an older range of other contents at these addresses): the matrices resolved above must still resolve to
+    // the same device bytes, else the table is resolved again, now without that copy
     for (auto& m : t.mats) {
         size_t dp = 0;
         if (dev_matrix(c, (const void*)m.host, m.code, m.rows, m.n_in, m.n_mats, m.host_per, &dp) != m.dev) {
+            if (attempts > 1) return get_table(c, ptrs, codes, n, inter, n_in, n_out, key_addr, attempts - 1);
             set_err("weight ranges moved while resolving the expert table");
             return nullptr;
         }

@@ -67,3 +67,25 @@ def test_changed_weights_are_copied_again(reg, port):
     second = dm.forward(layer, X)
     assert not np.array_equal(first, second)
     assert rel_l2(second, port.layer_forward(layer, X)) <= 1e-3
+
+
+@pytest.mark.parametrize("routed", [False, True])
+def test_a_copy_that_is_replaced_while_a_table_is_resolved(reg, port, routed):
+    """New weights in memory of which an older copy is still known: down (Q6_K, which has a copy of its own kind) starts where that
+    copy does, gate and up lie inside it.  Resolving down drops the copy that gate and up were found in."""
+    layer = synth.make_layer(hidden=1024, n_exp=4, n_used=2, inter=512, shared_inter=512, seed=96)
+    X = synth.make_tokens(layer, 5, 97)
+    want = port.layer_forward(layer, X)
+    names = ("down", "gate", "up") if routed else ("sh_down", "sh_gate", "sh_up")
+    assert layer.code_d != layer.code_gu
+    old = np.zeros(sum(getattr(layer, n).nbytes + 256 for n in names), np.uint8)
+    assert reg.draco_b200_register(old.ctypes.data, old.nbytes) == 0
+    at = 0
+    for n in names:
+        a = getattr(layer, n)
+        new = old[at:at + a.nbytes].view(a.dtype).reshape(a.shape)
+        new[...] = a
+        setattr(layer, n, new)
+        at += (a.nbytes + 255) // 256 * 256
+    for _ in range(2):
+        assert rel_l2(dm.forward(layer, X), want) <= 1e-3
