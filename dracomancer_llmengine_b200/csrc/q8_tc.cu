@@ -27,9 +27,10 @@
 // Tiles run through a group's rows first, so that a weight's tile is read from memory once.  Wide tiles: a block of 128 x 256
 // takes 512 cycles of the tensor cores and 48 KB from the L2 cache.
 //
-// Measured, call after call for a second (after a rest in brackets; at 1000 W the clock falls to 1.45 GHz): 8192 rows, 7168 x 7168,
-// bf16: 507 us, 1.66 PFLOP/s (468 to 517; the products alone take 275 us, the copies alone 264, adding up alone 317).  384 experts of
-// 2048 x 7168, 512 rows: 704 us, 5.8 TB/s (634 to 697); gate and up of 7168 x 2048: 1340 us, 6.1 TB/s (1242 to 1295).
+// Measured on several cards, call after call for a second (after a rest in brackets; at 1000 W the clock falls to 1.45 GHz): 8192
+// rows, 7168 x 7168, bf16: 498 to 510 us, 1.65 to 1.69 PFLOP/s (468 to 517; the products alone take 275 us, the copies alone 264,
+// adding up alone 317).  384 experts of 2048 x 7168, 512 rows: 650 to 710 us, 6.3 to 5.8 TB/s (634 to 697); gate and up of
+// 7168 x 2048: 1263 to 1365 us, 6.5 to 6.0 TB/s (1242 to 1295).
 //
 // Every wait is bounded; one that runs out ends the block's work, its rows (those it had not finished) become NaN and the
 // status word says which wait it was.
